@@ -465,6 +465,8 @@ const void *qw35_hip_runtime_store(void *runtime);
  * activations, 2^29 for fp32. */
 #define QW35_HIP_DTYPE_F32 0u
 #define QW35_HIP_DTYPE_BF16 1u
+#define QW35_HIP_DTYPE_F16 2u
+#define QW35_HIP_DTYPE_E4M3 3u /* 8-bit float (OCP e4m3), key/value caches only */
 /* workspace: NULL, or device memory of
  * qw35_hip_matmul_prefill_workspace_size(w, n_tokens) bytes (256-byte
  * aligned, owned by the caller, not shared by concurrent calls).
@@ -539,6 +541,137 @@ int qw35_hip_matmul_prefill_epilogue(const qw35_hip_weight *w, const void *a, ui
  * has none (it reads those types through gguf-py).  src must be finite. */
 int qw35_hip_quantize(uint32_t type_id, const float *src, uint64_t rows, uint64_t k, const float *col_scale,
                       void *dst, void *stream, char *err, uintptr_t err_len);
+
+/* ---- Attention between the projections -----------------------------------
+ * Rotary positions, a paged key/value cache and attention over it.  They take
+ * the place of the reference's QK-norm + MRoPE + cache write and flash kernels
+ * (qw35_attention.metal:29-930) between its projections
+ * (Qw35MetalRuntime+Attention.m:35-113).  All are asynchronous on `stream`,
+ * allocate nothing and may be recorded into a graph. */
+
+/* A device view [n_tokens][heads][dim] with unit column stride; strides in
+ * elements (a head's half of a wider row is a view: the queries of a gated
+ * projection have head_stride 2 * dim).  Rows that start 16-byte aligned are
+ * read and written 16 bytes a lane, others element by element. */
+typedef struct qw35_hip_heads {
+    void *data;
+    int64_t token_stride;
+    int64_t head_stride;
+    uint32_t dtype; /* QW35_HIP_DTYPE_F32 / BF16 / F16 */
+    uint32_t reserved;
+} qw35_hip_heads;
+
+/* Rotary positions.  The first rot_dim columns (a multiple of 16) turn in
+ * pairs (i, i + rot_dim / 2) by position * base^(-2 i / rot_dim).  With
+ * sections (time, height, width, extra: pairs of each axis, together
+ * rot_dim / 2) a pair's position is that of its axis: sections in a row, or,
+ * interleaved, pairs 3 j + 1 and 3 j + 2 take height and width while j is
+ * within those sections and every other pair time (qw35_hip_hparams'
+ * rope_sections).  All sections zero: one axis. */
+typedef struct qw35_hip_rope {
+    const uint64_t *freq; /* device [rot_dim / 2], from qw35_hip_rope_freq */
+    uint32_t rot_dim;
+    uint32_t interleaved;
+    uint32_t sections[4];
+} qw35_hip_rope;
+
+/* The frequencies of a qw35_hip_rope into host memory freq[rot_dim / 2]:
+ * base^(-2 i / rot_dim) in turns per position, as 64-bit fixed-point fractions
+ * (so that an angle stays exact at any position).  base > 1. */
+int qw35_hip_rope_freq(uint32_t rot_dim, double base, uint64_t *freq, char *err, uintptr_t err_len);
+
+/* y = rotated RMS norm of x, rows [n_tokens][heads][dim], dim a multiple of 8
+ * up to 512; y may be x itself.  norm: device fp32 [dim], nullable (no norm:
+ * x * norm / sqrt(mean(x^2) + eps)).  rope: nullable (no rotation).
+ * positions: device int32 [n_axes][n_tokens], n_axes 1 (every section the same
+ * position) or the number of sections up to the last that is not zero.
+ * n_tokens 0 does nothing. */
+int qw35_hip_rotate(const qw35_hip_heads *x, const qw35_hip_heads *y, uint32_t n_tokens, uint32_t heads, uint32_t dim,
+                    const qw35_hip_rope *rope, const int32_t *positions, uint32_t n_axes, const float *norm, float eps,
+                    void *stream, char *err, uintptr_t err_len);
+
+/* A paged key/value cache of one layer: n_pages pages of page_size tokens (a
+ * multiple of 32).  Token at % page_size of page at / page_size has slot `at`.
+ * k, v: device, 16-byte aligned, [n_pages][kv_heads] pages of a head, laid out
+ * for the attention's matrix operands:
+ *   keys   [page_size / 32][head_dim / 8][32 tokens][8 columns]
+ *   values [page_size / 8][head_dim][8 tokens]
+ * dtype QW35_HIP_DTYPE_F16, BF16 or E4M3; for E4M3 a stored element stands for
+ * itself times the head's scale (k_scale, v_scale: device fp32 [kv_heads],
+ * nullable = 1), and appended elements past 448 scales become 448.
+ * head_dim 64, 128 or 256. */
+typedef struct qw35_hip_kv_cache {
+    void *k;
+    void *v;
+    const float *k_scale;
+    const float *v_scale;
+    uint32_t n_pages;
+    uint32_t page_size;
+    uint32_t kv_heads;
+    uint32_t head_dim;
+    uint32_t dtype;
+    uint32_t reserved;
+} qw35_hip_kv_cache;
+
+/* Appends n_tokens tokens: keys k (normed and rotated as qw35_hip_rotate does)
+ * and values v, [n_tokens][kv_heads][head_dim] of one type, to the slots
+ * slots[n_tokens] (device int64).  A token whose slot is negative or past the
+ * cache is left out (padding).  Slots of a call should differ. */
+int qw35_hip_kv_append(const qw35_hip_kv_cache *cache, const qw35_hip_heads *k, const qw35_hip_heads *v,
+                       uint32_t n_tokens, const int64_t *slots, const qw35_hip_rope *rope, const int32_t *positions,
+                       uint32_t n_axes, const float *norm, float eps, void *stream, char *err, uintptr_t err_len);
+
+/* Attention of a ragged batch whose sequences share a prefix of prefix_len
+ * tokens, which is read once for all of them.
+ *   Sequence s has new tokens starts[s] .. starts[s + 1] - 1 of q (device int32
+ * [n_seqs + 1]; NULL: one each, n_tokens = n_seqs), the last of its lengths[s]
+ * own tokens (device int32, the new ones among them, already appended).
+ * Positions 0 .. prefix_len - 1 are the shared tokens, in prefix_pages (device
+ * int32 [n_prefix_pages]); own token j stands at prefix_len + j, in page
+ * pages[s * pages_per_seq + j / page_size] (device int32).
+ *   A token at position p sees positions <= p; with window > 0 of these only
+ * those > p - window and those < sink.  out = softmax(scale * q . k) v over
+ * what it sees, zero where it sees nothing, times 1 / (1 + exp(-gate)) with a
+ * gate (data NULL: none).  What a token does not see does not reach its row,
+ * infinities and NaN included.
+ *   q: F16 or BF16, the cache's type (either for an E4M3 cache); out and gate:
+ * F32, BF16 or F16.  n_heads a multiple of the cache's kv_heads: query head h
+ * reads kv head h / (n_heads / kv_heads).
+ *   max_new: the most new tokens of a sequence (0: n_tokens); it only chooses
+ * how rows are divided.  workspace: device, 256-byte aligned, of
+ * qw35_hip_prefix_attention_workspace_size bytes for this or a larger batch;
+ * its contents do not matter, and calls that overlap need one each.
+ *   Bad device data is kept in bounds, not reported: lengths past the page
+ * table count as its capacity, tokens of a page number outside the cache as
+ * not there, and rows of q outside every sequence give zero. */
+typedef struct qw35_hip_attention {
+    qw35_hip_heads q;
+    qw35_hip_heads out;
+    qw35_hip_heads gate;
+    uint32_t n_tokens;
+    uint32_t n_heads;
+    uint32_t n_seqs;
+    uint32_t max_new;
+    const int32_t *starts;
+    const int32_t *lengths;
+    const int32_t *pages;
+    const int32_t *prefix_pages;
+    uint32_t pages_per_seq;
+    uint32_t n_prefix_pages;
+    uint32_t prefix_len;
+    uint32_t window;
+    uint32_t sink;
+    float scale;
+    void *workspace;
+    uint64_t workspace_bytes;
+} qw35_hip_attention;
+
+/* Bytes for a batch of n_seqs sequences and n_tokens new tokens, whatever its
+ * max_new and prefix (0: a cache or batch that the call refuses). */
+uint64_t qw35_hip_prefix_attention_workspace_size(const qw35_hip_kv_cache *cache, uint32_t n_heads, uint32_t n_seqs,
+                                                  uint32_t n_tokens);
+int qw35_hip_prefix_attention(const qw35_hip_attention *op, const qw35_hip_kv_cache *cache, void *stream, char *err,
+                              uintptr_t err_len);
 
 /* Streaming-read probe: reads every byte of the device buffer `buf` once
  * (`bytes` a multiple of 16, 16-byte aligned) and writes one XOR digest per

@@ -22,6 +22,8 @@ TYPE_GF4 = 100
 MAX_BATCH = 8
 DTYPE_F32 = 0
 DTYPE_BF16 = 1
+DTYPE_F16 = 2
+DTYPE_E4M3 = 3
 
 
 class TensorDesc(C.Structure):
@@ -122,6 +124,72 @@ class Hparams(C.Structure):
     ]
 
 
+class Heads(C.Structure):
+    """``qw35_hip_heads``."""
+
+    _fields_ = [
+        ("data", C.c_void_p),
+        ("token_stride", C.c_int64),
+        ("head_stride", C.c_int64),
+        ("dtype", C.c_uint32),
+        ("reserved", C.c_uint32),
+    ]
+
+
+class Rope(C.Structure):
+    """``qw35_hip_rope``."""
+
+    _fields_ = [
+        ("freq", C.c_void_p),
+        ("rot_dim", C.c_uint32),
+        ("interleaved", C.c_uint32),
+        ("sections", C.c_uint32 * 4),
+    ]
+
+
+class KvCache(C.Structure):
+    """``qw35_hip_kv_cache``."""
+
+    _fields_ = [
+        ("k", C.c_void_p),
+        ("v", C.c_void_p),
+        ("k_scale", C.c_void_p),
+        ("v_scale", C.c_void_p),
+        ("n_pages", C.c_uint32),
+        ("page_size", C.c_uint32),
+        ("kv_heads", C.c_uint32),
+        ("head_dim", C.c_uint32),
+        ("dtype", C.c_uint32),
+        ("reserved", C.c_uint32),
+    ]
+
+
+class Attention(C.Structure):
+    """``qw35_hip_attention``."""
+
+    _fields_ = [
+        ("q", Heads),
+        ("out", Heads),
+        ("gate", Heads),
+        ("n_tokens", C.c_uint32),
+        ("n_heads", C.c_uint32),
+        ("n_seqs", C.c_uint32),
+        ("max_new", C.c_uint32),
+        ("starts", C.c_void_p),
+        ("lengths", C.c_void_p),
+        ("pages", C.c_void_p),
+        ("prefix_pages", C.c_void_p),
+        ("pages_per_seq", C.c_uint32),
+        ("n_prefix_pages", C.c_uint32),
+        ("prefix_len", C.c_uint32),
+        ("window", C.c_uint32),
+        ("sink", C.c_uint32),
+        ("scale", C.c_float),
+        ("workspace", C.c_void_p),
+        ("workspace_bytes", C.c_uint64),
+    ]
+
+
 # name -> (restype, argtypes); every symbol declared in include/qw35_hip.h.
 PROTOTYPES: dict[str, tuple] = {
     "qw35_hip_gguf_parse": (
@@ -217,6 +285,22 @@ PROTOTYPES: dict[str, tuple] = {
         [C.c_uint32, C.c_void_p, C.c_uint64, C.c_uint64, C.c_void_p, C.c_void_p, C.c_void_p, C.c_char_p,
          C.c_size_t],
     ),
+    "qw35_hip_rope_freq": (
+        C.c_int, [C.c_uint32, C.c_double, C.c_void_p, C.c_char_p, C.c_size_t]),
+    "qw35_hip_rotate": (
+        C.c_int,
+        [C.POINTER(Heads), C.POINTER(Heads), C.c_uint32, C.c_uint32, C.c_uint32, C.POINTER(Rope), C.c_void_p,
+         C.c_uint32, C.c_void_p, C.c_float, C.c_void_p, C.c_char_p, C.c_size_t],
+    ),
+    "qw35_hip_kv_append": (
+        C.c_int,
+        [C.POINTER(KvCache), C.POINTER(Heads), C.POINTER(Heads), C.c_uint32, C.c_void_p, C.POINTER(Rope), C.c_void_p,
+         C.c_uint32, C.c_void_p, C.c_float, C.c_void_p, C.c_char_p, C.c_size_t],
+    ),
+    "qw35_hip_prefix_attention_workspace_size": (
+        C.c_uint64, [C.POINTER(KvCache), C.c_uint32, C.c_uint32, C.c_uint32]),
+    "qw35_hip_prefix_attention": (
+        C.c_int, [C.POINTER(Attention), C.POINTER(KvCache), C.c_void_p, C.c_char_p, C.c_size_t]),
     "qw35_hip_stream_read_sink_len": (C.c_uint32, [C.c_uint64]),
     "qw35_hip_stream_read": (C.c_int, [C.c_void_p, C.c_uint64, C.c_void_p, C.c_void_p, C.c_char_p, C.c_size_t]),
     "qw35_hip_mfma_probe": (C.c_int, [C.c_uint32, C.c_uint32, C.c_void_p, C.c_void_p, C.c_char_p, C.c_size_t]),

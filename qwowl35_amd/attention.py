@@ -1,0 +1,256 @@
+"""Attention between the projections: rotary positions, a paged key/value cache
+and attention of a batch that shares a prefix, over the C ABI.
+
+An attention layer of the reference runs its q / k / v projections, one kernel
+that norms, rotates and caches, flash attention and the output projection
+(qw35-server/src/metal/bridge/Qw35MetalRuntime+Attention.m:35-113).  Here:
+
+* ``rotate``            RMS norm and multi-axis rotary of the queries
+* ``kv_append``         the same of the keys, and keys and values into the cache
+* ``prefix_attention``  softmax attention of one or more new tokens of each
+  sequence over the shared prefix (read once for the batch) and their own pages
+
+``GatedAttention`` runs a whole layer of them with the projections.
+
+Device memory and streams come from torch; every computation is a call into
+``libqw35_hip.so``, asynchronous on ``stream`` (default: the current one).
+Tensors made on another stream than that must be synchronised with it first.
+"""
+from __future__ import annotations
+
+import ctypes as C
+import math
+
+import torch
+
+from . import _ffi
+from . import runtime as rt
+from ._ffi import Qw35Error
+
+_DTYPE = {torch.float32: _ffi.DTYPE_F32, torch.bfloat16: _ffi.DTYPE_BF16, torch.float16: _ffi.DTYPE_F16,
+          torch.float8_e4m3fn: _ffi.DTYPE_E4M3}
+_ptr, _stream = rt._ptr, rt._stream
+
+
+def _heads(x: torch.Tensor, name: str) -> _ffi.Heads:
+    """``qw35_hip_heads`` of a [n_tokens, heads, dim] tensor with unit column stride."""
+    if x.dim() != 3 or not x.is_cuda or x.dtype not in _DTYPE:
+        raise Qw35Error(f"{name} must be an fp32, bf16 or fp16 [n_tokens, heads, dim] device tensor")
+    if x.stride(2) != 1 and x.shape[2] > 1:
+        raise Qw35Error(f"{name} must have unit column stride, got strides {x.stride()}")
+    return _ffi.Heads(x.data_ptr(), x.stride(0), x.stride(1), _DTYPE[x.dtype], 0)
+
+
+def _index(x: torch.Tensor, dtype: torch.dtype, shape: tuple, like: torch.Tensor, name: str) -> None:
+    if x.dtype != dtype or tuple(x.shape) != shape or not x.is_contiguous() or x.device != like.device:
+        raise Qw35Error(f"{name} must be a contiguous {dtype} {list(shape)} tensor on {like.device}, got "
+                        f"{x.dtype} {list(x.shape)} on {x.device}")
+
+
+def _vector(x: torch.Tensor | None, n: int, like: torch.Tensor, name: str) -> None:
+    if x is not None:
+        _index(x, torch.float32, (n,), like, name)
+
+
+class Rotary:
+    """Rotary positions: ``rot_dim`` columns (a multiple of 16) of a head turn by
+    ``position * base^(-2 i / rot_dim)``, pair i being columns i and i + rot_dim / 2.
+
+    ``sections`` gives the pairs of each axis (time, height, width, extra:
+    ``rope_sections``), in a row or ``interleaved``; without it there is one axis."""
+
+    def __init__(self, rot_dim: int, base: float, sections=None, interleaved: bool = False, device="cuda"):
+        sections = [int(s) for s in (sections or [])]
+        if len(sections) > 4 or any(s < 0 for s in sections):
+            raise Qw35Error(f"rotary sections must be up to four counts, got {sections}")
+        if rot_dim <= 0 or rot_dim % 16 or (sum(sections) and sum(sections) != rot_dim // 2):
+            raise Qw35Error(f"rot_dim={rot_dim} must be a positive multiple of 16 and twice the sections {sections}")
+        host = torch.empty(rot_dim // 2, dtype=torch.int64)
+        _ffi.call("qw35_hip_rope_freq", rot_dim, float(base), C.c_void_p(host.data_ptr()))
+        self.freq = host.to(device)  # 64-bit fixed-point turns per position
+        self.rot_dim, self.sections, self.interleaved = rot_dim, sections, bool(interleaved)
+        self.axes = max([i + 1 for i, s in enumerate(sections) if s], default=1)
+        self.view = _ffi.Rope(self.freq.data_ptr(), rot_dim, int(interleaved),
+                              (C.c_uint32 * 4)(*(sections + [0] * (4 - len(sections)))))
+
+
+def _turn(rope: Rotary | None, positions, n: int, like: torch.Tensor) -> tuple:
+    """The rope, positions and n_axes arguments of a call."""
+    if rope is None:
+        return None, None, 0
+    if positions is None:
+        raise Qw35Error("positions are needed with a rope")
+    if rope.freq.device != like.device:
+        raise Qw35Error(f"the rope lives on {rope.freq.device}, the input on {like.device}")
+    axes = 1 if positions.dim() == 1 else int(positions.shape[0])
+    _index(positions, torch.int32, (n,) if positions.dim() == 1 else (axes, n), like, "positions")
+    if axes not in (1, rope.axes):
+        raise Qw35Error(f"positions have {axes} axes, the sections 1 or {rope.axes}")
+    return C.byref(rope.view), _ptr(positions), axes
+
+
+def rotate(x: torch.Tensor, rope: Rotary | None, positions: torch.Tensor | None = None, norm: torch.Tensor | None = None,
+           eps: float = 1e-6, out: torch.Tensor | None = None, out_dtype: torch.dtype | None = None,
+           stream=None) -> torch.Tensor:
+    """RMS norm (with ``norm``, fp32 [dim]) and rotation of x [n_tokens, heads, dim].
+
+    x: fp32, bf16 or fp16, any token and head stride; ``positions`` int32
+    [n_tokens], or [axes, n_tokens] for the rope's sections.  Statistics and
+    rotation in fp32, rounded once to ``out_dtype`` (default: ``out``'s or x's
+    type).  ``out`` may be x."""
+    hx = _heads(x, "x")
+    n, heads, dim = x.shape
+    if out is None:
+        out = torch.empty((n, heads, dim), dtype=out_dtype or x.dtype, device=x.device)
+    elif out.shape != x.shape or out.device != x.device or (out_dtype or out.dtype) != out.dtype:
+        raise Qw35Error(f"out must be a {list(x.shape)} tensor of out_dtype on {x.device}")
+    hy = _heads(out, "out")
+    _vector(norm, dim, x, "norm")
+    turn, pos, axes = _turn(rope, positions, n, x)
+    if n == 0:
+        return out
+    _ffi.call("qw35_hip_rotate", C.byref(hx), C.byref(hy), n, heads, dim, turn, pos, axes, _ptr(norm), eps,
+              _stream(stream))
+    return out
+
+
+class PagedCache:
+    """A paged key/value cache of one layer (``qw35_hip_kv_cache``) over two tensors:
+
+    k [n_pages, kv_heads, page_size / 32, dim / 8, 32, 8] and
+    v [n_pages, kv_heads, page_size / 8, dim, 8], fp16, bf16 or float8_e4m3fn
+    (then with an fp32 scale per kv head, default 1).  Slot ``s`` is token
+    ``s % page_size`` of page ``s // page_size``."""
+
+    def __init__(self, k: torch.Tensor, v: torch.Tensor, k_scale: torch.Tensor | None = None,
+                 v_scale: torch.Tensor | None = None):
+        if k.dim() != 6 or tuple(k.shape[4:]) != (32, 8) or not k.is_cuda or not k.is_contiguous():
+            raise Qw35Error("cache keys must be a contiguous [n_pages, kv_heads, page_size / 32, dim / 8, 32, 8] device "
+                            f"tensor, got {list(k.shape)}")
+        pages, heads, blocks, octets = (int(s) for s in k.shape[:4])
+        want = (pages, heads, blocks * 4, octets * 8, 8)
+        if tuple(v.shape) != want or v.dtype != k.dtype or v.device != k.device or not v.is_contiguous():
+            raise Qw35Error(f"cache values must be a contiguous {k.dtype} {list(want)} tensor on {k.device}")
+        if k.dtype not in _DTYPE or k.dtype == torch.float32:
+            raise Qw35Error(f"a cache is float16, bfloat16 or float8_e4m3fn, got {k.dtype}")
+        if k.dtype != torch.float8_e4m3fn and (k_scale is not None or v_scale is not None):
+            raise Qw35Error("only a float8_e4m3fn cache has scales")
+        _vector(k_scale, heads, k, "k_scale")
+        _vector(v_scale, heads, k, "v_scale")
+        self.k, self.v, self.k_scale, self.v_scale = k, v, k_scale, v_scale
+        self.n_pages, self.kv_heads, self.page_size, self.head_dim = pages, heads, blocks * 32, octets * 8
+        at = lambda t: t.data_ptr() if t is not None else None  # noqa: E731
+        self.view = _ffi.KvCache(at(k), at(v), at(k_scale), at(v_scale), pages, self.page_size, heads, self.head_dim,
+                                 _DTYPE[k.dtype], 0)
+
+    @classmethod
+    def empty(cls, n_pages: int, kv_heads: int, page_size: int, head_dim: int, dtype: torch.dtype = torch.float16,
+              k_scale: torch.Tensor | None = None, v_scale: torch.Tensor | None = None, device="cuda") -> "PagedCache":
+        if page_size <= 0 or page_size % 32 or head_dim not in (64, 128, 256):
+            raise Qw35Error(f"page_size={page_size} must be a multiple of 32 and head_dim={head_dim} 64, 128 or 256")
+        k = torch.empty((n_pages, kv_heads, page_size // 32, head_dim // 8, 32, 8), dtype=dtype, device=device)
+        v = torch.empty((n_pages, kv_heads, page_size // 8, head_dim, 8), dtype=dtype, device=device)
+        return cls(k, v, k_scale, v_scale)
+
+    def slots(self, pages: torch.Tensor, at: torch.Tensor) -> torch.Tensor:
+        """Slots of the tokens ``at`` (int tensor) of a sequence with page list ``pages``."""
+        at = at.long()
+        return pages.long()[at // self.page_size] * self.page_size + at % self.page_size
+
+
+def kv_append(cache: PagedCache, k: torch.Tensor, v: torch.Tensor, slots: torch.Tensor, rope: Rotary | None = None,
+              positions: torch.Tensor | None = None, norm: torch.Tensor | None = None, eps: float = 1e-6,
+              stream=None) -> None:
+    """Keys (normed and rotated as ``rotate`` does) and values [n_tokens, kv_heads,
+    head_dim] into ``slots`` (int64 [n_tokens]; a negative one leaves its token out).
+
+    Into an e4m3 cache go the values over the head's scale, rounded to nearest
+    even, past +-448 to +-448."""
+    hk, hv = _heads(k, "k"), _heads(v, "v")
+    n = int(k.shape[0])
+    if tuple(k.shape) != (n, cache.kv_heads, cache.head_dim) or v.shape != k.shape or k.dtype != v.dtype:
+        raise Qw35Error(f"k and v must be [n_tokens, {cache.kv_heads}, {cache.head_dim}] of one type, got "
+                        f"{list(k.shape)} {k.dtype} and {list(v.shape)} {v.dtype}")
+    if k.device != cache.k.device or v.device != cache.k.device:
+        raise Qw35Error(f"k and v must be on the cache's {cache.k.device}")
+    _index(slots, torch.int64, (n,), k, "slots")
+    _vector(norm, cache.head_dim, k, "norm")
+    turn, pos, axes = _turn(rope, positions, n, k)
+    if n == 0:
+        return
+    _ffi.call("qw35_hip_kv_append", C.byref(cache.view), C.byref(hk), C.byref(hv), n, _ptr(slots), turn, pos, axes,
+              _ptr(norm), eps, _stream(stream))
+
+
+def prefix_attention_workspace(cache: PagedCache, n_heads: int, n_seqs: int, n_tokens: int, device="cuda") -> torch.Tensor:
+    """A workspace for ``prefix_attention`` of up to this batch (its contents do not
+    matter; calls that overlap need one each)."""
+    size = int(_ffi.load().qw35_hip_prefix_attention_workspace_size(C.byref(cache.view), n_heads, n_seqs, n_tokens))
+    if size == 0:
+        raise Qw35Error(f"prefix_attention: no workspace for n_heads={n_heads}, n_seqs={n_seqs}, n_tokens={n_tokens}")
+    return torch.empty(size, dtype=torch.uint8, device=device)
+
+
+def prefix_attention(q: torch.Tensor, cache: PagedCache, pages: torch.Tensor, lengths: torch.Tensor,
+                     starts: torch.Tensor | None = None, max_new: int = 0, prefix_pages: torch.Tensor | None = None,
+                     prefix_len: int = 0, scale: float | None = None, window: int = 0, sink: int = 0,
+                     gate: torch.Tensor | None = None, out: torch.Tensor | None = None,
+                     out_dtype: torch.dtype | None = None, workspace: torch.Tensor | None = None,
+                     stream=None) -> torch.Tensor:
+    """Attention of the new tokens q [n_tokens, n_heads, head_dim] of a batch of sequences.
+
+    Sequence s has the new tokens ``starts[s]:starts[s + 1]`` (int32 [n_seqs + 1];
+    None: one each), the last of its ``lengths[s]`` own tokens (int32), which lie in
+    the pages ``pages[s]`` (int32 [n_seqs, pages_per_seq]) after the ``prefix_len``
+    tokens in ``prefix_pages`` that all sequences share.  A token sees the
+    positions up to its own, with ``window`` only the last ``window`` of them and
+    the first ``sink``.  Result: softmax(scale q k) v (scale default
+    1 / sqrt(head_dim)), zeros where nothing is seen, times sigmoid(``gate``), in
+    ``out_dtype`` (default q's type).
+
+    ``max_new``: the most new tokens of a sequence, where it is known: it chooses
+    how rows are divided, not what is computed.  All lengths live on the device, so
+    a recorded call serves every later step."""
+    hq = _heads(q, "q")
+    n, heads, dim = q.shape
+    if dim != cache.head_dim or q.device != cache.k.device:
+        raise Qw35Error(f"q must be [n_tokens, n_heads, {cache.head_dim}] on {cache.k.device}, got {list(q.shape)}")
+    seqs = int(lengths.shape[0])
+    _index(lengths, torch.int32, (seqs,), q, "lengths")
+    if pages.dim() != 2:
+        raise Qw35Error("pages must be int32 [n_seqs, pages_per_seq]")
+    _index(pages, torch.int32, (seqs, int(pages.shape[1])), q, "pages")
+    if starts is not None:
+        _index(starts, torch.int32, (seqs + 1,), q, "starts")
+    if prefix_len and prefix_pages is None:
+        raise Qw35Error("prefix_len needs prefix_pages")
+    if prefix_pages is not None:
+        _index(prefix_pages, torch.int32, (int(prefix_pages.numel()),), q, "prefix_pages")
+    if min(max_new, prefix_len, window, sink) < 0:
+        raise Qw35Error("max_new, prefix_len, window and sink cannot be negative")
+    if out is None:
+        out = torch.empty((n, heads, dim), dtype=out_dtype or q.dtype, device=q.device)
+    elif out.shape != q.shape or out.device != q.device or (out_dtype or out.dtype) != out.dtype:
+        raise Qw35Error(f"out must be a {list(q.shape)} tensor of out_dtype on {q.device}")
+    op = _ffi.Attention()
+    op.q, op.out = hq, _heads(out, "out")
+    if gate is not None:
+        if gate.shape != q.shape or gate.device != q.device:
+            raise Qw35Error(f"gate must be a {list(q.shape)} tensor on {q.device}")
+        op.gate = _heads(gate, "gate")
+    if n == 0:
+        return out
+    if workspace is None:  # this call's own
+        workspace = prefix_attention_workspace(cache, heads, seqs, n, device=q.device)
+    if workspace.device != q.device or not workspace.is_contiguous():
+        raise Qw35Error(f"workspace must be a contiguous tensor on {q.device}")
+    op.n_tokens, op.n_heads, op.n_seqs, op.max_new = n, heads, seqs, max_new
+    op.starts = starts.data_ptr() if starts is not None else None
+    op.lengths, op.pages, op.pages_per_seq = lengths.data_ptr(), pages.data_ptr(), int(pages.shape[1])
+    if prefix_len:
+        op.prefix_pages, op.n_prefix_pages = prefix_pages.data_ptr(), prefix_pages.numel()
+    op.prefix_len, op.window, op.sink = prefix_len, window, sink
+    op.scale = 1.0 / math.sqrt(dim) if scale is None else scale
+    op.workspace, op.workspace_bytes = workspace.data_ptr(), workspace.numel() * workspace.element_size()
+    _ffi.call("qw35_hip_prefix_attention", C.byref(op), C.byref(cache.view), _stream(stream))
+    return out

@@ -3,24 +3,19 @@
 // (qw35-server/src/metal/bridge/Qw35MetalRuntime+FFN.m:184-256), the greedy
 // head of encodeOutputHead (Qw35MetalRuntime+Output.m:11-65) and the
 // 0 + err[err_len] error convention of Qw35FFI.m:15-22.
-#include <stdarg.h>
 #include <stdio.h>
 #include <string.h>
 
 #include <mutex>
 
 #include "../../include/qw35_hip.h"
+#include "abi_error.h"
 #include "qw35_kernels.h"
 
 namespace {
 
-void set_err(char* err, uintptr_t err_len, const char* fmt, ...) {
-    if (!err || err_len == 0) return;
-    va_list ap;
-    va_start(ap, fmt);
-    vsnprintf(err, (size_t)err_len, fmt, ap);
-    va_end(ap);
-}
+using qw35::check_hip;
+using qw35::set_err;
 
 bool type_supported(uint32_t t) {
     return t == qw35::kTypeGF4 || t == qw35::kTypeGF2 || t == qw35::kTypeQ8_0 || t == qw35::kTypeQ4_K ||
@@ -114,12 +109,6 @@ bool check_chunked_k(const qw35_hip_weight* w, const char* what, char* err, uint
     if (w->k % 256 == 0) return true;
     set_err(err, err_len, "%s: needs k %% 256 == 0, got k=%llu (a q8_0 weight of such k runs the decode GEMV only)",
             what, (unsigned long long)w->k);
-    return false;
-}
-
-bool check_hip(hipError_t e, const char* what, char* err, uintptr_t err_len) {
-    if (e == hipSuccess) return true;
-    set_err(err, err_len, "%s: %s", what, hipGetErrorString(e));
     return false;
 }
 

@@ -1,0 +1,94 @@
+// Host-side launch interface of the attention operators (rope_kv.hip,
+// prefix_attention.hip): internal to the library, the public C ABI is
+// include/qw35_hip.h.
+#pragma once
+
+#include <hip/hip_runtime.h>
+#include <stdint.h>
+
+#include "../../include/qw35_hip.h"
+
+namespace qw35 {
+
+// [n_tokens][heads][dim] with unit column stride; strides in elements.
+struct HeadsView {
+    void* data;
+    int64_t token_stride;
+    int64_t head_stride;
+    uint32_t dtype;  // QW35_HIP_DTYPE_*
+    int vec;         // rows start 16-byte aligned: vector loads and stores
+};
+
+struct RopeArgs {
+    const uint64_t* freq;      // nullptr: no rotation
+    const int32_t* positions;  // [n_axes][n_tokens]
+    const float* norm;         // [dim] or nullptr: no RMS norm
+    float eps;
+    int rot_dim;
+    int n_axes;
+    int interleaved;
+    int sections[4];
+};
+
+hipError_t launch_rotate(const HeadsView& x, const HeadsView& y, int n_tokens, int heads, int dim, const RopeArgs& rope,
+                         hipStream_t stream);
+hipError_t launch_kv_append(const qw35_hip_kv_cache& cache, const HeadsView& k, const HeadsView& v, int n_tokens,
+                            const int64_t* slots, const RopeArgs& rope, hipStream_t stream);
+
+// How a launch divides the rows (new token x head of a group) of a kind of
+// unit: workgroups of four waves, RG groups of waves with 16 R rows each, the
+// 4 / RG waves of a group on different 32-token tiles.
+struct RowSplit {
+    int log2_rg;
+    int rows;  // rows of a unit: 16 R RG
+    int cost;  // cost of a step (4 / RG tiles)
+};
+
+struct AttnPlan {
+    int r;             // 16-row tiles per wave
+    RowSplit prefix, own;
+    int workgroups;
+    int prefix_entries;  // row tiles of the prefix, of every kv head
+    int max_entries;     // bound of prefix and own row tiles together
+    int slot_rows;       // rows of a partial result's slot
+    uint64_t slots;
+    uint64_t meta_bytes;
+    uint64_t workspace_bytes;
+};
+
+struct AttnArgs {
+    HeadsView q, out, gate;
+    const void* ck;
+    const void* cv;
+    const float* k_scale;
+    const float* v_scale;
+    uint32_t n_pages;
+    uint32_t page_blocks;  // 32-token blocks of a page
+    int kv_heads;
+    int group;
+    int n_tokens;
+    int n_seqs;
+    const int32_t* starts;
+    const int32_t* lengths;
+    const int32_t* pages;
+    uint32_t pages_per_seq;
+    const int32_t* prefix_pages;
+    int prefix_len;
+    float scale_log2;  // softmax scale times log2(e)
+    int window;
+    int sink;
+    uint8_t* meta;
+    float* part;
+    AttnPlan plan;
+};
+
+AttnPlan plan_attention(int dim, int kv_heads, int group, int n_seqs, int n_tokens, int max_new, bool prefix);
+hipError_t launch_prefix_attention(const AttnArgs& a, int dim, uint32_t q_dtype, uint32_t cache_dtype,
+                                   hipStream_t stream);
+
+// One translation unit per head dimension (attn_d<dim>.hip).
+hipError_t launch_attn_d64(const AttnArgs& a, bool bf16, bool f8, hipStream_t stream);
+hipError_t launch_attn_d128(const AttnArgs& a, bool bf16, bool f8, hipStream_t stream);
+hipError_t launch_attn_d256(const AttnArgs& a, bool bf16, bool f8, hipStream_t stream);
+
+}  // namespace qw35
