@@ -36,16 +36,19 @@ hipError_t launch_kv_append(const qw35_hip_kv_cache& cache, const HeadsView& k, 
                             const int64_t* slots, const RopeArgs& rope, hipStream_t stream);
 
 // How a launch divides the rows (new token x head of a group) of a kind of
-// unit: workgroups of four waves, RG groups of waves with 16 R rows each, the
-// 4 / RG waves of a group on different 32-token tiles.
+// unit among a workgroup's four waves.  Up to 64 rows: 32 rows a wave, the
+// waves of a row group on different 32-token tiles (a step is 4 or 2 tiles).
+// More: 32 or 64 rows a wave, all four on the same tile (a step is one).
 struct RowSplit {
-    int log2_rg;
-    int rows;  // rows of a unit: 16 R RG
-    int cost;  // cost of a step (4 / RG tiles)
+    int log2_rg;  // row groups
+    int rows;     // rows of a unit
+    int cost;     // cost of a step
+    int shared;   // the waves share their tiles
+    __host__ __device__ int step() const { return 4 >> log2_rg; }
 };
 
 struct AttnPlan {
-    int r;             // 16-row tiles per wave
+    int shared_r;  // 32-row tiles of a wave where waves share tiles (0: no unit does)
     RowSplit prefix, own;
     int workgroups;
     int prefix_entries;  // row tiles of the prefix, of every kv head
@@ -54,6 +57,7 @@ struct AttnPlan {
     uint64_t slots;
     uint64_t meta_bytes;
     uint64_t workspace_bytes;
+    uint64_t lds_bytes;
 };
 
 struct AttnArgs {

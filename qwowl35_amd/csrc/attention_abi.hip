@@ -15,7 +15,7 @@ using qw35::set_err;
 constexpr uint32_t kMaxTokens = 1u << 22;   // rows of a call and their heads stay within 32 bits
 constexpr uint32_t kMaxHeads = 256;
 constexpr uint64_t kMaxLength = 1u << 30;   // positions
-constexpr int kMaxEntries = 4096;           // row tiles of a call, in LDS
+constexpr uint64_t kMaxLds = 160 * 1024;    // of a compute unit: a call's row tiles are listed there
 
 size_t dtype_size(uint32_t t) { return t == QW35_HIP_DTYPE_F32 ? 4 : t == QW35_HIP_DTYPE_E4M3 ? 1 : 2; }
 
@@ -244,12 +244,12 @@ uint64_t qw35_hip_prefix_attention_workspace_size(const qw35_hip_kv_cache* cache
                                                   uint32_t n_tokens) {
     if (!check_batch(cache, n_heads, n_seqs, n_tokens, nullptr, 0)) return 0;
     const uint32_t group = n_heads / cache->kv_heads;
-    // every division of the rows that a call of this batch may take
+    // every division of the rows that a call of this batch may take: the most rows of a sequence that each has
+    const uint32_t most[] = {1, 32 / group, 64 / group, 128 / group, 128 / group + 1, n_tokens};
     uint64_t need = 256;
     for (int prefix = 0; prefix < 2; ++prefix)
-        for (uint32_t rows = 16; rows <= 256; rows *= 2) {
-            uint32_t max_new = rows / group ? rows / group : 1;
-            if (max_new > n_tokens) max_new = n_tokens;
+        for (uint32_t max_new : most) {
+            if (max_new == 0 || max_new > n_tokens) continue;
             const qw35::AttnPlan p = plan_of(cache, n_heads, n_seqs, n_tokens, max_new, prefix != 0);
             if (p.workspace_bytes > need) need = p.workspace_bytes;
         }
@@ -306,9 +306,9 @@ int qw35_hip_prefix_attention(const qw35_hip_attention* op, const qw35_hip_kv_ca
     }
     const uint32_t max_new = op->max_new == 0 || op->max_new > op->n_tokens ? op->n_tokens : op->max_new;
     a.plan = plan_of(cache, op->n_heads, op->n_seqs, op->n_tokens, max_new, op->prefix_len != 0);
-    if (a.plan.max_entries > kMaxEntries) {
-        set_err(err, err_len, "%s: %d row tiles in a call are over %d; give it fewer tokens or sequences", what,
-                a.plan.max_entries, kMaxEntries);
+    if (a.plan.lds_bytes > kMaxLds) {
+        set_err(err, err_len, "%s: %d row tiles in a call are %llu over the list's room; give it fewer tokens or sequences",
+                what, a.plan.max_entries, (unsigned long long)((a.plan.lds_bytes - kMaxLds + 11) / 12));
         return 0;
     }
     if (!op->workspace || ((uintptr_t)op->workspace & 255u) || op->workspace_bytes < a.plan.workspace_bytes) {

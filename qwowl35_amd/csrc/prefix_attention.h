@@ -20,14 +20,19 @@
 // piece has; the combine kernel finds a row's slots by the same arithmetic.
 //
 // Operands.  A tile's scores are S^T = K Q^T and the output O^T = V^T P^T, on
-// v_mfma_f32_16x16x32: lane l holds query row l % 16 in S, P and O alike, so
-// maximum, sum and rescaling stay in a lane (and its three others of the same
-// row).  The cache's granules are the A operands: 16 bytes are eight columns of
-// a key, or eight tokens of a value column, and a wave's load is 1 KB in a
-// piece, straight from HBM to registers.  Key row i of half b of a tile is
-// token 8 (i / 4) + 4 b + i % 4, which leaves the four scores a lane holds of
-// either half as the eight tokens 8 (l / 16) .. + 7 of its value granule: P
-// needs no exchange between lanes.
+// v_mfma_f32_32x32x16: lane l holds query row l % 32 in S, P and O alike, so
+// maximum, sum and rescaling stay in a lane (and its other one of the same
+// row).  The cache's granules are the A operands: eight columns of a key, or
+// eight tokens of a value column.  Row i of a tile's scores is the token whose
+// number is i with bits 2 and 3 exchanged, which leaves the scores a lane holds
+// as the tokens of its two value granules: P needs no exchange between lanes.
+//
+// Data.  Tiles go from HBM to LDS by copies that take no registers, as far
+// ahead as the ring has room (128 KB for 256 columns), and from there to the
+// matrix instructions: 16 bytes a lane, a wave's reads consecutive.  With up to
+// 64 rows in a unit each wave (or pair) has its own tiles, since then a compute
+// unit only waits for HBM; more rows share a tile among the four waves, which
+// reads it once for 128 or 256 rows.
 //
 // Rounding.  Scores, maxima, sums and O are fp32.  P is rounded once to the
 // cache's 16-bit type for the second product (relative 2^-12 fp16, 2^-9 bf16
@@ -42,16 +47,19 @@ namespace attn {
 
 constexpr int kThreads = 256;
 constexpr int kWaves = 4;
+constexpr int kSeqs = 256;  // sequences kept in LDS
 constexpr uint32_t kNoBlock = 0xffffffffu;
+
+typedef float acc_t __attribute__((ext_vector_type(16)));
 
 // Element type of queries and 16-bit caches, and its matrix instruction.
 struct Half {
     typedef _Float16 elem;
     typedef half8_t vec8;
-    static __device__ __forceinline__ float4_t mfma(vec8 a, vec8 b, float4_t c) {
-        return __builtin_amdgcn_mfma_f32_16x16x32_f16(a, b, c, 0, 0, 0);
+    static __device__ __forceinline__ acc_t mfma(vec8 a, vec8 b, acc_t c) {
+        return __builtin_amdgcn_mfma_f32_32x32x16_f16(a, b, c, 0, 0, 0);
     }
-    static constexpr uint32_t kInf2 = 0x7c007c00u;
+    static constexpr short kInf = 0x7c00;  // bits of +inf
     static __device__ __forceinline__ vec8 from_e4m3(uint2 w) {
         uint4_t r;
         r[0] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(w.x, 1.0f, false));
@@ -65,10 +73,10 @@ struct Half {
 struct Bf16 {
     typedef __bf16 elem;
     typedef bf16x8_t vec8;
-    static __device__ __forceinline__ float4_t mfma(vec8 a, vec8 b, float4_t c) {
-        return __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b, c, 0, 0, 0);
+    static __device__ __forceinline__ acc_t mfma(vec8 a, vec8 b, acc_t c) {
+        return __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, b, c, 0, 0, 0);
     }
-    static constexpr uint32_t kInf2 = 0x7f807f80u;
+    static constexpr short kInf = 0x7f80, kUp = 0x3f80, kDown = 0x4280, kBoth = 0x4282;
     static __device__ __forceinline__ vec8 from_e4m3(uint2 w) {
         uint4_t r;
         r[0] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(w.x, 1.0f, false));
@@ -103,6 +111,20 @@ struct Seq {
     int length;  // its own tokens in the cache
 };
 
+// A value that all lanes hold alike, as one the compiler knows to be.
+__device__ __forceinline__ int uniform(int v) { return __builtin_amdgcn_readfirstlane(v); }
+__device__ __forceinline__ int64_t uniform(int64_t v) {
+    return (int64_t)((uint64_t)(uint32_t)uniform((int)(v >> 32)) << 32 | (uint32_t)uniform((int)v));
+}
+__device__ __forceinline__ uint64_t uniform(uint64_t v) { return (uint64_t)uniform((int64_t)v); }
+
+// x / d of whole numbers below 2^52.
+__device__ __forceinline__ uint64_t quotient(uint64_t x, uint64_t d) {
+    uint64_t q = (uint64_t)((double)x / (double)d);
+    if (q * d > x) --q;
+    return q;
+}
+
 __device__ __forceinline__ int clampi(int v, int lo, int hi) { return v < lo ? lo : v > hi ? hi : v; }
 
 __device__ __forceinline__ Seq seq_at(const AttnArgs& a, int s) {
@@ -114,16 +136,33 @@ __device__ __forceinline__ Seq seq_at(const AttnArgs& a, int s) {
     return q;
 }
 
-// The sequence of new token t: the last whose start is at or before it (-1: none).
-__device__ __forceinline__ int seq_of(const AttnArgs& a, int t) {
-    if (!a.starts) return t;
-    int lo = 0, hi = a.n_seqs;  // starts[0..lo) <= t < starts[hi..)
+// The last of n ascending numbers that is at most t (-1: none).
+__device__ __forceinline__ int last_at(const int* starts, int n, int t) {
+    int lo = 0, hi = n;  // starts[0..lo) <= t < starts[hi..)
     while (lo < hi) {
         const int mid = (lo + hi) / 2;
-        if (a.starts[mid] <= t) lo = mid + 1;
+        if (starts[mid] <= t) lo = mid + 1;
         else hi = mid;
     }
     return lo - 1;
+}
+
+// The sequence of new token t: the last whose start is at or before it (-1: none).
+__device__ __forceinline__ int seq_of(const AttnArgs& a, int t) {
+    return a.starts ? last_at(a.starts, a.n_seqs, t) : t;
+}
+
+// The same of a token that the wave's lanes have alike: 64 starts a load.
+__device__ __forceinline__ int seq_of_wave(const AttnArgs& a, int t, int lane) {
+    if (!a.starts) return t;
+    int s = -1;
+    for (int s0 = 0; s0 < a.n_seqs; s0 += 64) {
+        const bool at = s0 + lane < a.n_seqs && a.starts[s0 + lane] <= t;
+        const uint64_t votes = __ballot(at);
+        if (votes) s = s0 + 63 - __builtin_clzll(votes);
+        if (votes != ~0ull) break;
+    }
+    return s;
 }
 
 // Tokens [lo, hi) and [0, sink) of a unit's n are seen.
@@ -219,7 +258,9 @@ struct Line {
 
 // Fills cost[0..entries] (cost before an entry) and info[entry] (sequence << 16
 // | row tile) in LDS; the first workgroup also leaves them for the combine kernel.
-__device__ __forceinline__ Line build_line(const AttnArgs& a, uint64_t* cost, uint32_t* info, uint64_t* scratch) {
+template <class S>
+__device__ __forceinline__ Line build_line(const AttnArgs& a, uint64_t* cost, uint32_t* info, S& sh) {
+    uint64_t* const scratch = sh.scratch;
     const int tid = threadIdx.x;
     const AttnPlan& p = a.plan;
     int* const meta_first = reinterpret_cast<int*>(a.meta + meta_first_at());
@@ -237,6 +278,11 @@ __device__ __forceinline__ Line build_line(const AttnArgs& a, uint64_t* cost, ui
             const int before = q.n - q.length;  // (> -2^31: the earliest position is prefix_len - this)
             const uint32_t b = (uint32_t)(before + 0x40000000);
             if (q.n && b > back) back = b;
+            if (s < kSeqs) {
+                sh.start[s] = a.starts ? a.starts[s] : s;
+                sh.end[s] = q.q0 + q.n;
+                sh.ahead[s] = q.length - q.n - q.q0;
+            }
         }
         uint32_t total;
         const uint32_t at = base + block_scan<uint32_t>(n, reinterpret_cast<uint32_t*>(scratch), total) - n;
@@ -265,10 +311,10 @@ __device__ __forceinline__ Line build_line(const AttnArgs& a, uint64_t* cost, ui
         const int e = e0 + tid;
         uint64_t c = 0;
         if (e < p.prefix_entries) {
-            const int step = kWaves >> p.prefix.log2_rg;
+            const int step = p.prefix.step();
             c = (uint64_t)((prefix_tiles(a, line.min_pos).count() + step - 1) / step) * p.prefix.cost;
         } else if (e < line.entries) {
-            const int step = kWaves >> p.own.log2_rg;
+            const int step = p.own.step();
             const Seq q = seq_at(a, (int)(info[e] >> 16));
             c = (uint64_t)((own_tiles(a, q, (int)(info[e] & 0xffff)).count() + step - 1) / step) * p.own.cost;
         }
@@ -283,7 +329,7 @@ __device__ __forceinline__ Line build_line(const AttnArgs& a, uint64_t* cost, ui
     if (tid == 0) cost[line.entries] = sum;
     line.head_cost = sum;
     const uint64_t all = sum * (uint64_t)a.kv_heads;
-    uint64_t per = (all + p.workgroups - 1) / p.workgroups;
+    uint64_t per = quotient(all + p.workgroups - 1, p.workgroups);
     const uint64_t least = p.prefix.cost > p.own.cost ? p.prefix.cost : p.own.cost;  // a piece has a step of any unit
     line.per = per < least ? least : per;
     if (blockIdx.x == 0 && tid == 0) {
@@ -294,6 +340,10 @@ __device__ __forceinline__ Line build_line(const AttnArgs& a, uint64_t* cost, ui
         m->entries = line.entries;
     }
     __syncthreads();
+    line.head_cost = uniform(line.head_cost);
+    line.per = uniform(line.per);
+    line.min_pos = uniform(line.min_pos);
+    line.entries = uniform(line.entries);
     return line;
 }
 
@@ -350,49 +400,86 @@ __device__ __forceinline__ void finish(const AttnArgs& a, int t, int head, int c
 
 // ---- the kernel ----------------------------------------------------------------------------------------------------
 
-// Lanes l and l ^ 16, l and l ^ 32: both values, in either.  (Elements of the
-// builtins' results are copied before their bits are read as a float: a
+// Lanes l and l ^ 32: both values, in either.  (Elements of the builtin's
+// result are copied before their bits are read as a float: a
 // __builtin_bit_cast of an element itself reads element 0.)
 struct Pair {
     float a, b;
 };
-__device__ __forceinline__ Pair pair_xor16(float v) {
-    const uint32_t u = __builtin_bit_cast(uint32_t, v);
-    const auto p = __builtin_amdgcn_permlane16_swap(u, u, false, false);
-    const uint32_t a = p[0], b = p[1];
-    return {__builtin_bit_cast(float, a), __builtin_bit_cast(float, b)};
-}
 __device__ __forceinline__ Pair pair_xor32(float v) {
     const uint32_t u = __builtin_bit_cast(uint32_t, v);
     const auto p = __builtin_amdgcn_permlane32_swap(u, u, false, false);
     const uint32_t a = p[0], b = p[1];
     return {__builtin_bit_cast(float, a), __builtin_bit_cast(float, b)};
 }
-// Over the four lanes of a row.
+// Over the two lanes of a row.
 __device__ __forceinline__ float row_max(float v) {
-    const Pair p = pair_xor16(v);
-    const Pair q = pair_xor32(fmaxf(p.a, p.b));
-    return fmaxf(q.a, q.b);
+    const Pair p = pair_xor32(v);
+    return fmaxf(p.a, p.b);
 }
 __device__ __forceinline__ float row_sum(float v) {
-    const Pair p = pair_xor16(v);
-    const Pair q = pair_xor32(p.a + p.b);
-    return q.a + q.b;
+    const Pair p = pair_xor32(v);
+    return p.a + p.b;
 }
 
-// A part of a row whose maximum is m, seen from the maximum `top` of several: exp2(m - top), 0 for a part with nothing.
+// v *= f in v's own registers (the compiler's products would go to others,
+// with a copy of every accumulator where the paths meet).
+__device__ __forceinline__ void scale_in_place(acc_t& v, float f) {
+#pragma unroll
+    for (int i = 0; i < 16; ++i) {
+        float x = v[i];
+        asm("v_mul_f32 %0, %1, %0" : "+v"(x) : "v"(f));
+        v[i] = x;
+    }
+}
+
+// A part of a row whose exponents count from m, seen from the largest `top` of several: exp2(m - top), 0 for a part
+// with nothing.
 __device__ __forceinline__ float part_weight(float m, float top) {
     return m == -__builtin_inff() ? 0.0f : __builtin_amdgcn_exp2f(m - top);
 }
 
+// Waits until at most n of this wave's vector memory operations are in flight.
+template <int N>
+__device__ __forceinline__ void wait_vm() {
+    static_assert(N >= 0 && N < 64, "vmcnt range");
+    __builtin_amdgcn_s_waitcnt((N & 0xF) | ((N >> 4) << 14) | (0x7 << 4) | (0xF << 8));
+    asm volatile("" ::: "memory");
+}
+// Waits until this wave's LDS reads have returned.
+__device__ __forceinline__ void wait_lds() {
+    asm volatile("" ::: "memory");
+    __builtin_amdgcn_s_waitcnt(0xF | (3 << 14) | (0x7 << 4));
+}
+
+// Copies kCount KB from global memory to LDS without registers: each
+// instruction moves 1 KB, lane i's 16 bytes to base + 16 i.
+template <int kCount>
+__device__ __forceinline__ void copy_kb(const uint8_t* from, uint8_t* to, int lane) {
+    typedef const __attribute__((address_space(1))) void global_t;
+    typedef __attribute__((address_space(3))) void lds_t;
+#pragma unroll
+    for (int i = 0; i < kCount; i += 4) {
+        const uint8_t* const g = from + i * 1024 + lane * 16;
+        uint8_t* const l = to + i * 1024;
+        __builtin_amdgcn_global_load_lds((global_t*)g, (lds_t*)l, 16, 0, 0);
+        if (i + 1 < kCount) __builtin_amdgcn_global_load_lds((global_t*)g, (lds_t*)l, 16, 1024, 0);
+        if (i + 2 < kCount) __builtin_amdgcn_global_load_lds((global_t*)g, (lds_t*)l, 16, 2048, 0);
+        if (i + 3 < kCount) __builtin_amdgcn_global_load_lds((global_t*)g, (lds_t*)l, 16, 3072, 0);
+    }
+}
+
 template <int D>
 struct Shared {
-    // Four waves' sums of 16 rows, rows padded by four floats: the 16 rows a
-    // wave stores at once start in 16 different 16-byte groups.
-    static constexpr int kRow = D + 4;
-    float o[kWaves][16][kRow];
-    float m[kWaves][16];
-    float l[kWaves][16];
+    static constexpr int kRing = D == 256 ? 128 * 1024 : 64 * 1024;
+    uint8_t ring[kRing];  // tiles on their way; at a unit's end the waves' sums
+    float m[kWaves][32];
+    float l[kWaves][32];
+    Limits all[kWaves];
+    // of the first sequences, for the rows of the prefix: starts[s], the end of its new tokens, and a new token's
+    // position less its index and prefix_len
+    int start[kSeqs], end[kSeqs], ahead[kSeqs];
+    uint32_t marks[kWaves][32 * D / 16];
     uint64_t scratch[kWaves];
 };
 
@@ -406,270 +493,512 @@ __device__ __forceinline__ typename E::vec8 operand(raw8<F8> w) {
     else return __builtin_bit_cast(typename E::vec8, w);
 }
 
-template <int D, class E, bool F8, int R>
+template <int D, class E, bool F8>
 struct Unit {
     typedef typename E::vec8 vec8;
     typedef raw8<F8> raw;
-    static constexpr int kM = D / 32;  // contraction steps of a score
-    static constexpr int kT = D / 16;  // 16-column tiles of the output
+    static constexpr int kM = D / 16;  // contraction steps of a score
+    static constexpr int kT = D / 32;  // 32-column tiles of the output
     static constexpr int kElem = F8 ? 1 : 2;
+    static constexpr int kTile = 32 * D * kElem;  // bytes of a tile's keys, and of its values
+    static constexpr int kKb = kTile / 1024;
+    static constexpr int kRing = Shared<D>::kRing;
+    // The exponents' reference follows the maximum only when that has risen by
+    // 2^8: sums then hold up to 2^8 times a row's largest term, which costs
+    // neither type precision, and most tiles rescale nothing.
+    static constexpr float kRise = 8.0f;
 
     const AttnArgs& a;
     Shared<D>& sh;
-    const int lane, wave, n, g;  // this lane's row of a 16-row tile, and its quarter
+    const int lane, wave, n, g;  // this lane's row of a 32-row tile, and its half
 
     __device__ Unit(const AttnArgs& a_, Shared<D>& sh_)
         : a(a_), sh(sh_), lane(threadIdx.x & 63), wave(__builtin_amdgcn_readfirstlane(threadIdx.x >> 6)),
-          n(threadIdx.x & 15), g((threadIdx.x & 63) >> 4) {}
+          n(threadIdx.x & 31), g((threadIdx.x & 63) >> 5) {}
 
-    __device__ __forceinline__ void load_keys(const uint8_t* tile, raw (&k)[2][kM]) const {
-        const uint8_t* p = tile + (g * 256 + (8 * (n >> 2) + (n & 3)) * 8) * kElem;
-#pragma unroll
-        for (int m = 0; m < kM; ++m)
-#pragma unroll
-            for (int b = 0; b < 2; ++b)
-                k[b][m] = *reinterpret_cast<const raw*>(p + (m * 1024 + b * 32) * kElem);
+    // What a wave carries through its tiles.
+    template <int R>
+    struct Rows {
+        vec8 q[R][kM];
+        acc_t o[R][kT];
+        float mx[R], l[R];
+        Limits lim[R];
+        int all_lo, all_hi, all_sink;  // what every row of the wave sees
+        float scale;
+        bool marked;  // infinities to add at the end
+    };
+
+    // The granule of step m / of column tile t and token step kk.
+    __device__ __forceinline__ vec8 key(const uint8_t* tile, int m) const {
+        // row i of the product is token i with bits 2 and 3 exchanged
+        const int tok = (n & 19) | (n & 4) << 1 | (n & 8) >> 1;
+        return operand<E, F8>(*reinterpret_cast<const raw*>(tile + ((2 * m + g) * 32 + tok) * 8 * kElem));
+    }
+    __device__ __forceinline__ vec8 value(const uint8_t* tile, int t, int kk) const {
+        return operand<E, F8>(*reinterpret_cast<const raw*>(tile + ((2 * kk + g) * D + t * 32 + n) * 8 * kElem));
     }
 
-    __device__ __forceinline__ void load_values(const uint8_t* tile, raw (&v)[kT]) const {
-        const uint8_t* p = tile + (g * 8 * D + n * 8) * kElem;
+    template <int R>
+    __device__ __forceinline__ void scores(const uint8_t* keys, const Rows<R>& w, acc_t (&s)[R]) const {
+        constexpr int kAhead = kM < 4 ? kM : 4;
+        vec8 k[kAhead];
 #pragma unroll
-        for (int t = 0; t < kT; ++t) v[t] = *reinterpret_cast<const raw*>(p + t * 128 * kElem);
+        for (int m = 0; m < kAhead; ++m) k[m] = key(keys, m);
+#pragma unroll
+        for (int r = 0; r < R; ++r) s[r] = acc_t{};
+#pragma unroll
+        for (int m = 0; m < kM; ++m) {
+            const vec8 kk = k[m % kAhead];
+            if (m + kAhead < kM) k[m % kAhead] = key(keys, m + kAhead);
+#pragma unroll
+            for (int r = 0; r < R; ++r) s[r] = E::mfma(kk, w.q[r][m], s[r]);
+        }
+        interleave<kM, R, kAhead>();
+    }
+
+    // LDS reads kAhead ahead of the matrix instructions that take them.
+    template <int kSteps, int R, int kAhead>
+    static __device__ __forceinline__ void interleave() {
+        __builtin_amdgcn_sched_group_barrier(0x100, kAhead, 0);
+#pragma unroll
+        for (int m = 0; m < kSteps; ++m) {
+            if (F8) __builtin_amdgcn_sched_group_barrier(0x002, 4, 0);
+            __builtin_amdgcn_sched_group_barrier(0x008, R, 0);
+            if (m + kAhead < kSteps) __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);
+        }
+    }
+
+    // Softmax of a tile's scores: its terms to p, the running reference, sum and output kept.
+    template <int R>
+    __device__ __forceinline__ void softmax(Rows<R>& w, acc_t (&s)[R], int t0, bool masked, bool there,
+                                            vec8 (&p)[R][2]) const {
+#pragma unroll
+        for (int r = 0; r < R; ++r) {
+            if (masked) {
+#pragma unroll
+                for (int j = 0; j < 16; ++j)
+                    s[r][j] = sees(w.lim[r], t0 + token(j), there) ? s[r][j] : -__builtin_inff();
+            }
+            float top = s[r][0];
+#pragma unroll
+            for (int j = 1; j < 16; ++j) top = fmaxf(top, s[r][j]);
+            top = row_max(top) * w.scale;
+            if (__builtin_expect(__any(top > w.mx[r] + kRise), 0)) {
+                const float m_new = fmaxf(w.mx[r], top);
+                const float shrink = m_new == w.mx[r] ? 1.0f : __builtin_amdgcn_exp2f(w.mx[r] - m_new);
+                w.l[r] *= shrink;
+#pragma unroll
+                for (int t = 0; t < kT; ++t) scale_in_place(w.o[r][t], shrink);
+                w.mx[r] = m_new;
+            }
+            const float ref = w.mx[r] == -__builtin_inff() ? 0.0f : w.mx[r];
+#pragma unroll
+            for (int j = 0; j < 16; ++j) {
+                const float e = __builtin_amdgcn_exp2f(fmaf(s[r][j], w.scale, -ref));
+                w.l[r] += e;
+                p[r][j / 8][j % 8] = (typename E::elem)e;
+            }
+        }
+    }
+
+    template <int R>
+    __device__ __forceinline__ void add_values(const uint8_t* values, Rows<R>& w, const vec8 (&p)[R][2]) const {
+        constexpr int kSteps = 2 * kT, kAhead = kSteps < 4 ? kSteps : 4;
+        vec8 v[kAhead];
+#pragma unroll
+        for (int i = 0; i < kAhead; ++i) v[i] = value(values, i / 2, i % 2);
+#pragma unroll
+        for (int i = 0; i < kSteps; ++i) {
+            const vec8 vv = v[i % kAhead];
+            if (i + kAhead < kSteps) v[i % kAhead] = value(values, (i + kAhead) / 2, i % 2);
+#pragma unroll
+            for (int r = 0; r < R; ++r) w.o[r][i / 2] = E::mfma(vv, p[r][i % 2], w.o[r][i / 2]);
+        }
+        interleave<kSteps, R, kAhead>();
+    }
+
+    // Keeps infinities and NaN of a tile's values, of which some rows see only
+    // a part, from the product (all waves of a shared tile come here together).
+    template <int R, bool kShared>
+    __device__ __forceinline__ void split_off_infinities(uint8_t* tile, Rows<R>& w, int t0, bool there,
+                                                         uint32_t* marks) const {
+        if (__builtin_expect(!__any(not_finite(tile)), 1)) return;
+        mark_infinities<R>(tile, w, t0, there, marks);
+        if (kShared) __syncthreads();
+        make_finite(tile, kShared ? wave : 0, kShared ? kWaves : 1);
+        if (kShared) __syncthreads();
+    }
+
+    // Every step-th granule from `first` on, without its infinities and NaN.
+    __device__ __forceinline__ void make_finite(uint8_t* tile, int first, int step) const {
+#pragma unroll 1
+        for (int i = first; i < 2 * kT; i += step) {
+            uint8_t* const at = tile + ((2 * (i & 1) + g) * D + (i >> 1) * 32 + n) * 8 * kElem;
+            typedef std::conditional_t<F8, uint8_t, short> part_t;
+            typedef part_t bits_t __attribute__((ext_vector_type(8)));
+            bits_t v = *reinterpret_cast<const bits_t*>(at);
+            constexpr part_t kSize = F8 ? 0x7f : 0x7fff, kFirst = F8 ? 0x7f : E::kInf;  // (e4m3 has a NaN, no infinities)
+#pragma unroll
+            for (int j = 0; j < 8; ++j) v[j] = (v[j] & kSize) >= kFirst ? part_t(0) : v[j];
+            *reinterpret_cast<bits_t*>(at) = v;
+        }
+        wait_lds();
+    }
+
+    // Token of a lane's score j.
+    __device__ __forceinline__ int token(int j) const { return (j & 8) * 2 + g * 8 + (j & 7); }
+
+    template <int R>
+    __device__ __forceinline__ bool partly(const Rows<R>& w, int t0, bool there) const {
+        return !there || !((t0 >= w.all_lo && t0 + 32 <= w.all_hi) || t0 + 32 <= w.all_sink);
+    }
+
+    // Where a unit's tiles lie: 64 of them are looked up at a time, one a lane.
+    struct Pages {
+        const int* table;
+        Tiles tiles;
+        int first, step, count;  // this wave's tiles: first, first + step, ...
+        int h;
+        uint32_t blocks;  // lane i: the cache block of tile 64 j + i
+    };
+
+    __device__ __forceinline__ uint32_t block_of(Pages& p, int i) const {
+        if ((i & 63) == 0) {
+            const int mine = i + lane < p.count ? i + lane : p.count - 1;
+            const uint32_t b = (uint32_t)p.tiles.at(p.first + mine * p.step);
+            const uint32_t pi = b / a.page_blocks;
+            const int id = p.table[pi];
+            // a page outside the cache holds nothing that a row sees
+            uint32_t block = ((uint32_t)id * (uint32_t)a.kv_heads + p.h) * a.page_blocks + (b - pi * a.page_blocks);
+            asm("" : "+v"(block));  // (a choice of two values, not of two paths)
+            p.blocks = (uint32_t)id < a.n_pages ? block : kNoBlock;
+        }
+        return (uint32_t)__builtin_amdgcn_readlane((int)p.blocks, i & 63);
+    }
+    static __device__ __forceinline__ int64_t bytes_at(uint32_t block) {
+        return (int64_t)(block == kNoBlock ? 0u : block) * kTile;
     }
 
     // Steps [s0, s1) of an entry for kv head h; the result to `slot`, or where
-    // this is all there is of the rows (slot < 0) to the output.
+    // this is all there is of the rows (slot < 0) to the output.  R: 32-row
+    // tiles of a wave; kShared: the waves share their tiles.
+    template <int R, bool kShared>
     __device__ __forceinline__ void run(int h, bool prefix, int seq, int tile, Tiles tiles, int s0, int s1, int64_t slot) {
         const RowSplit& split = prefix ? a.plan.prefix : a.plan.own;
-        const int rg = wave & ((1 << split.log2_rg) - 1), tg = wave >> split.log2_rg;
-        const int step = kWaves >> split.log2_rg;
+        const int rg = kShared ? wave : wave & ((1 << split.log2_rg) - 1), tg = kShared ? 0 : wave >> split.log2_rg;
+        const int step = kShared ? 1 : kWaves >> split.log2_rg;
         Seq sq = {0, a.n_tokens, a.prefix_len};
-        if (!prefix) sq = seq_at(a, seq);
+        if (!prefix) {
+            sq = seq_at(a, seq);
+            sq = {uniform(sq.q0), uniform(sq.n), uniform(sq.length)};
+        }
         const int base = prefix ? 0 : a.prefix_len;
         const int row_end = sq.n * a.group;
-        const int row0 = tile * split.rows + rg * 16 * R;  // this wave's first row
-        const int* const table = prefix ? a.prefix_pages : a.pages + (int64_t)seq * a.pages_per_seq;
+        const int row0 = tile * split.rows + rg * 32 * R;  // this wave's first row
 
-        // this lane's rows: queries and limits
-        vec8 q[R][kM];
-        Limits lim[R];
-        int all_lo = 0, all_hi = 0x7fffffff, all_sink = 0x7fffffff;  // what every row of the wave sees
+        // this wave's tiles: step * s0 + tg, and every step-th after it
+        Pages pages;
+        pages.table = prefix ? a.prefix_pages : a.pages + (int64_t)seq * a.pages_per_seq;
+        pages.tiles = tiles;
+        pages.first = s0 * step + tg;
+        pages.step = step;
+        pages.h = h;
+        const int end = s1 * step < tiles.count() ? s1 * step : tiles.count();
+        pages.count = (kShared || row0 < row_end) && pages.first < end ? (end - pages.first + step - 1) / step : 0;
+        const uint8_t* const kbase = static_cast<const uint8_t*>(a.ck);
+        const uint8_t* const vbase = static_cast<const uint8_t*>(a.cv);
+
+        __syncthreads();  // the ring is free
+        constexpr int kFit = kShared ? kRing / (2 * kTile) : kRing / kWaves / (2 * kTile);
+        constexpr int kMarks = R * 32 * D / 4;  // bytes of a wave's marks; shared tiles leave room for them in the ring
+        constexpr int kPairs = kFit < 4 ? kFit : 2 * kTile * 4 + kWaves * kMarks <= kRing ? 4 : 3;
+        static_assert(!kShared || 2 * kTile * kPairs + kWaves * kMarks <= kRing, "tiles and marks fit the ring");
+        uint32_t* const marks = kShared ? reinterpret_cast<uint32_t*>(sh.ring + 2 * kTile * kPairs + wave * kMarks)
+                                        : sh.marks[wave];
+        uint8_t* const ring = sh.ring + (kShared ? 0 : wave * (kRing / kWaves));
+        uint32_t there_bits = 0;  // of the tiles loaded last, the newest in bit 0
+        auto note = [&](uint32_t block) { there_bits = there_bits << 1 | (block != kNoBlock ? 1u : 0u); };
+        // shared: this wave's quarter of a pair of tiles
+        auto load_quarter = [&](int i) {
+            const uint32_t block = block_of(pages, i);
+            note(block);
+            const int64_t at = bytes_at(block);
+            uint8_t* const to = ring + (i % kPairs) * 2 * kTile;
+            if constexpr (kKb >= 2) {
+                const uint8_t* const from = wave < 2 ? kbase : vbase;
+                const int part = (wave & 1) * (kTile / 2);
+                copy_kb<kKb / 2>(from + at + part, to + (wave < 2 ? 0 : kTile) + part, lane);
+            }
+        };
+
+        Rows<R> w;
+        if (pages.count) block_of(pages, 0);
+        load_queries<R>(w, sq, h, row0, row_end);
+        int loaded = 0;
+        if constexpr (kShared) {
+            for (; loaded < kPairs - 1 && loaded < pages.count; ++loaded) load_quarter(loaded);
+        } else {
+            for (; loaded < kPairs && loaded < pages.count; ++loaded) {
+                const uint32_t block = block_of(pages, loaded);
+                note(block);
+                uint8_t* const to = ring + loaded * 2 * kTile;
+                copy_kb<kKb>(kbase + bytes_at(block), to, lane);
+                copy_kb<kKb>(vbase + bytes_at(block), to + kTile, lane);
+            }
+        }
+        start_rows<R, kShared>(w, sq, prefix, base, row0, row_end);
+        use_queries<R>(w);  // (here the queries are waited for, not in the tile loop)
+
+        if constexpr (kShared) {
+            constexpr int kEach = kKb / 2;  // a wave's copies of a pair
+            for (int i = 0; i < pages.count; ++i) {
+                if (i + kPairs - 2 < pages.count) wait_vm<(kPairs - 2) * kEach>();
+                else wait_vm<0>();
+                __builtin_amdgcn_s_barrier();  // tile i is there, and tile i - 1 read by all
+                asm volatile("" ::: "memory");
+                if (loaded < pages.count) load_quarter(loaded++);
+                uint8_t* const at = ring + (i % kPairs) * 2 * kTile;
+                const bool there = there_bits >> (loaded - 1 - i) & 1;
+                const int t0 = tiles.at(pages.first + i) * 32;
+                const bool masked = partly<R>(w, t0, there);
+                if (masked) split_off_infinities<R, true>(at + kTile, w, t0, there, marks);
+                acc_t s[R];
+                vec8 p[R][2];
+                scores<R>(at, w, s);
+                softmax<R>(w, s, t0, masked, there, p);
+                add_values<R>(at + kTile, w, p);
+                wait_lds();
+            }
+        } else {
+            constexpr int kLater = (2 * kPairs - 1) * kKb;  // copies issued after the keys of a tile, or after its values
+            for (int i = 0; i < pages.count; ++i) {
+                uint8_t* const at = ring + (i % kPairs) * 2 * kTile;
+                const bool there = there_bits >> (loaded - 1 - i) & 1;
+                const bool more = loaded < pages.count;
+                const int t0 = tiles.at(pages.first + i * step) * 32;
+                const bool masked = partly<R>(w, t0, there);
+                acc_t s[R];
+                vec8 p[R][2];
+                if (more) wait_vm<kLater>();
+                else wait_vm<0>();
+                scores<R>(at, w, s);
+                uint32_t block = 0;
+                if (more) {
+                    wait_lds();
+                    block = block_of(pages, loaded);
+                    note(block);
+                    ++loaded;
+                    copy_kb<kKb>(kbase + bytes_at(block), at, lane);
+                }
+                softmax<R>(w, s, t0, masked, there, p);
+                if (more) wait_vm<kLater>();
+                if (masked) split_off_infinities<R, false>(at + kTile, w, t0, there, marks);
+                add_values<R>(at + kTile, w, p);
+                if (more) {
+                    wait_lds();
+                    copy_kb<kKb>(vbase + bytes_at(block), at + kTile, lane);
+                }
+            }
+        }
+        if (__builtin_expect(w.marked, 0)) add_infinities<R>(w, marks);
+#pragma unroll
+        for (int r = 0; r < R; ++r) w.l[r] = row_sum(w.l[r]);
+
+        const float v_scale = F8 && a.v_scale ? a.v_scale[h] : 1.0f;
+        float* const part = a.part + (slot < 0 ? 0 : slot) * slot_floats(a.plan.slot_rows, D);
+        const int part_row0 = rg * 32 * R;
+        float4_t* const mine = reinterpret_cast<float4_t*>(sh.ring + wave * (kRing / kWaves)) + lane;
+        static_assert(32 * D * 4 <= kRing / kWaves, "a wave's sums of 32 rows fit its part of the ring");
+        auto leave = [&](int r) {  // 32 rows' sums, in lane order
+#pragma unroll
+            for (int t = 0; t < kT; ++t)
+#pragma unroll
+                for (int c = 0; c < 4; ++c) mine[(t * 4 + c) * 64] = quad(w.o[r][t], c);
+        };
+        if constexpr (kShared) {
+            if (slot >= 0) {
+#pragma unroll
+                for (int r = 0; r < R; ++r) {
+                    if (row0 + r * 32 + n < row_end) {
+                        float* const to = part + (int64_t)(part_row0 + r * 32 + n) * D + g * 4;
+#pragma unroll
+                        for (int t = 0; t < kT; ++t)
+#pragma unroll
+                            for (int c = 0; c < 4; ++c)
+                                *reinterpret_cast<float4_t*>(to + t * 32 + c * 8) = quad(w.o[r][t], c);
+                        if (g == 0) put_stats(part, part_row0 + r * 32 + n, w.mx[r], w.l[r]);
+                    }
+                }
+            } else {
+                __syncthreads();  // (the tiles are read)
+#pragma unroll
+                for (int r = 0; r < R; ++r) {
+                    leave(r);
+                    const int row = row0 + r * 32 + n;
+                    if (row < row_end) {
+#pragma unroll 1
+                        for (int i = 0; i < kT * 4; ++i)
+                            put(part, slot, sq.q0, row, 0, h, (i >> 2) * 32 + (i & 3) * 8 + g * 4, mine[i * 64], w.l[r],
+                                v_scale);
+                    }
+                    wait_lds();
+                }
+            }
+        } else {
+            // The waves of a row group join: each leaves its sums in LDS in
+            // lane order, then adds up every step-th of all of theirs.
+            static_assert(R == 1, "a wave of its own tiles has 32 rows");
+            if (g == 0) {
+                sh.m[wave][n] = w.mx[0];
+                sh.l[wave][n] = w.l[0];
+            }
+            leave(0);
+            __syncthreads();
+            const int row = row0 + n;
+            float top = -__builtin_inff();
+            for (int v = 0; v < step; ++v) top = fmaxf(top, sh.m[rg + (v << split.log2_rg)][n]);
+            float weight[kWaves], sum = 0.0f;
+#pragma unroll
+            for (int v = 0; v < kWaves; ++v) {
+                weight[v] = 0.0f;
+                if (v < step) {
+                    weight[v] = part_weight(sh.m[rg + (v << split.log2_rg)][n], top);
+                    sum += weight[v] * sh.l[rg + (v << split.log2_rg)][n];
+                }
+            }
+            if (row < row_end) {
+#pragma unroll 1
+                for (int i = tg; i < kT * 4; i += step) {
+                    float4_t acc = {0, 0, 0, 0};
+#pragma unroll
+                    for (int v = 0; v < kWaves; ++v)
+                        if (v < step && weight[v] != 0.0f)
+                            acc += weight[v] * reinterpret_cast<const float4_t*>(
+                                                   sh.ring + (rg + (v << split.log2_rg)) * (kRing / kWaves))[i * 64 + lane];
+                    put(part, slot, sq.q0, row, part_row0 + n, h, (i >> 2) * 32 + (i & 3) * 8 + g * 4, acc, sum, v_scale);
+                }
+                if (slot >= 0 && tg == 0 && g == 0) put_stats(part, part_row0 + n, top, sum);
+            }
+        }
+    }
+
+    // This lane's queries (asked for; use_queries waits).
+    template <int R>
+    __device__ __forceinline__ void load_queries(Rows<R>& w, const Seq& sq, int h, int row0, int row_end) const {
 #pragma unroll
         for (int r = 0; r < R; ++r) {
-            const int row = row0 + r * 16 + n;
+            const int row = row0 + r * 32 + n;
             const bool on = row < row_end;
             const int t = sq.q0 + (on ? row / a.group : 0), head = h * a.group + (on ? row % a.group : 0);
             const typename E::elem* p = static_cast<const typename E::elem*>(a.q.data) + t * a.q.token_stride +
                                         head * a.q.head_stride + g * 8;
 #pragma unroll
-            for (int m = 0; m < kM; ++m) {
-                vec8 w = {};
-                if (on) {
-                    if (a.q.vec) {
-                        w = *reinterpret_cast<const vec8*>(p + m * 32);
-                    } else {
+            for (int m = 0; m < kM; ++m) w.q[r][m] = vec8{};
+            if (on && a.q.vec) {
 #pragma unroll
-                        for (int j = 0; j < 8; ++j) w[j] = p[m * 32 + j];
-                    }
+                for (int m = 0; m < kM; ++m) w.q[r][m] = *reinterpret_cast<const vec8*>(p + m * 16);
+            } else if (on) {
+#pragma unroll
+                for (int m = 0; m < kM; ++m) {
+#pragma unroll
+                    for (int j = 0; j < 8; ++j) w.q[r][m][j] = p[m * 16 + j];
+                    asm volatile("" ::: "memory");  // (eight loads at a time)
                 }
-                q[r][m] = w;
             }
-            lim[r] = Limits{0, 0, 0};
+        }
+        w.scale = a.scale_log2 * (F8 && a.k_scale ? a.k_scale[h] : 1.0f);
+    }
+
+    template <int R>
+    __device__ __forceinline__ void use_queries(Rows<R>& w) const {
+        // a negative scale turns the queries' signs, so that the largest score has the largest product
+        const uint32_t flip = w.scale < 0.0f ? 0x80008000u : 0u;
+        w.scale = fabsf(w.scale);
+        if (w.scale < 2e-38f) w.scale = 2e-38f;  // (zero: every finite score alike, and a masked one still none)
+#pragma unroll
+        for (int r = 0; r < R; ++r)
+#pragma unroll
+            for (int m = 0; m < kM; ++m) {
+                uint4_t x = __builtin_bit_cast(uint4_t, w.q[r][m]) ^ flip;
+                asm volatile("" : "+v"(x));
+                w.q[r][m] = __builtin_bit_cast(vec8, x);
+            }
+    }
+
+    // What this lane's rows see.
+    template <int R, bool kShared>
+    __device__ __forceinline__ void start_rows(Rows<R>& w, const Seq& sq, bool prefix, int base, int row0,
+                                               int row_end) const {
+        w.marked = false;
+        w.all_lo = 0;
+        w.all_hi = w.all_sink = 0x7fffffff;
+#pragma unroll
+        for (int r = 0; r < R; ++r) {
+            const int row = row0 + r * 32 + n;
+            const bool on = row < row_end;
+            const int t = sq.q0 + (on ? row / a.group : 0);
+            w.lim[r] = Limits{0, 0, 0};
             if (on) {
                 if (!prefix) {
-                    lim[r] = limits_of(a, (int64_t)base + sq.length - sq.n + row / a.group, base, sq.length);
+                    w.lim[r] = limits_of(a, (int64_t)base + sq.length - sq.n + row / a.group, base, sq.length);
                 } else {
-                    const int s = seq_of(a, t);
-                    if (s >= 0) {
-                        const Seq mine = seq_at(a, s);
-                        if (t < mine.q0 + mine.n)
-                            lim[r] = limits_of(a, (int64_t)a.prefix_len + mine.length - mine.n + t - mine.q0, 0,
-                                               a.prefix_len);
+                    int s, stop = 0, ahead = 0;
+                    if (a.n_seqs <= kSeqs) {
+                        s = a.starts ? last_at(sh.start, a.n_seqs, t) : t;
+                        if (s >= 0) {
+                            stop = sh.end[s];
+                            ahead = sh.ahead[s];
+                        }
+                    } else {
+                        s = seq_of(a, t);
+                        if (s >= 0) {
+                            const Seq mine = seq_at(a, s);
+                            stop = mine.q0 + mine.n;
+                            ahead = mine.length - mine.n - mine.q0;
+                        }
                     }
+                    if (s >= 0 && t < stop)
+                        w.lim[r] = limits_of(a, (int64_t)a.prefix_len + ahead + t, 0, a.prefix_len);
                 }
-                all_lo = lim[r].lo > all_lo ? lim[r].lo : all_lo;
-                all_hi = lim[r].hi < all_hi ? lim[r].hi : all_hi;
-                all_sink = lim[r].sink < all_sink ? lim[r].sink : all_sink;
+                w.all_lo = w.lim[r].lo > w.all_lo ? w.lim[r].lo : w.all_lo;
+                w.all_hi = w.lim[r].hi < w.all_hi ? w.lim[r].hi : w.all_hi;
+                w.all_sink = w.lim[r].sink < w.all_sink ? w.lim[r].sink : w.all_sink;
             }
+            w.mx[r] = -__builtin_inff();
+            w.l[r] = 0.0f;
+#pragma unroll
+            for (int t2 = 0; t2 < kT; ++t2) w.o[r][t2] = acc_t{};
         }
 #pragma unroll
-        for (int o = 1; o < 16; o *= 2) {
-            const int lo = __shfl_xor(all_lo, o), hi = __shfl_xor(all_hi, o), sk = __shfl_xor(all_sink, o);
-            all_lo = lo > all_lo ? lo : all_lo;
-            all_hi = hi < all_hi ? hi : all_hi;
-            all_sink = sk < all_sink ? sk : all_sink;
+        for (int o = 1; o < 32; o *= 2) {
+            const int lo = __shfl_xor(w.all_lo, o), hi = __shfl_xor(w.all_hi, o), sk = __shfl_xor(w.all_sink, o);
+            w.all_lo = lo > w.all_lo ? lo : w.all_lo;
+            w.all_hi = hi < w.all_hi ? hi : w.all_hi;
+            w.all_sink = sk < w.all_sink ? sk : w.all_sink;
         }
-        all_lo = __builtin_amdgcn_readfirstlane(all_lo);
-        all_hi = __builtin_amdgcn_readfirstlane(all_hi);
-        all_sink = __builtin_amdgcn_readfirstlane(all_sink);
-
-        float4_t o[R][kT];
-        float mx[R], l[R];
+        w.all_lo = uniform(w.all_lo);
+        w.all_hi = uniform(w.all_hi);
+        w.all_sink = uniform(w.all_sink);
+        if constexpr (kShared) {
+            // what every row of the workgroup sees: its waves take a tile apart together or not at all
+            if (lane == 0) sh.all[wave] = Limits{w.all_lo, w.all_hi, w.all_sink};
+            __syncthreads();
 #pragma unroll
-        for (int r = 0; r < R; ++r) {
-            mx[r] = -__builtin_inff();
-            l[r] = 0.0f;
-#pragma unroll
-            for (int t = 0; t < kT; ++t) o[r][t] = float4_t{0, 0, 0, 0};
-        }
-        const float scale = a.scale_log2 * (F8 && a.k_scale ? a.k_scale[h] : 1.0f);
-
-        // this wave's tiles: step * s0 + tg, and every step-th after it
-        const int first = s0 * step + tg;
-        const int end = s1 * step < tiles.count() ? s1 * step : tiles.count();
-        const int mine = row0 < row_end && first < end ? (end - first + step - 1) / step : 0;
-        const uint8_t* const kbase = static_cast<const uint8_t*>(a.ck);
-        const uint8_t* const vbase = static_cast<const uint8_t*>(a.cv);
-        uint32_t blocks = kNoBlock;  // lane i: the cache block of tile 64 j + i
-        auto look_up = [&](int j) {
-            const int v = first + (j + lane) * step;
-            blocks = kNoBlock;
-            if (j + lane < mine) {
-                const uint32_t b = (uint32_t)tiles.at(v);
-                const uint32_t pi = b / a.page_blocks;
-                const int id = table[pi];
-                // a page outside the cache holds nothing that a row sees
-                if ((uint32_t)id < a.n_pages)
-                    blocks = ((uint32_t)id * (uint32_t)a.kv_heads + h) * a.page_blocks + (b - pi * a.page_blocks);
-            }
-        };
-        auto block_at = [&](int j) {
-            return (uint32_t)__builtin_amdgcn_readlane((int)blocks, j & 63);
-        };
-        auto bytes_at = [&](uint32_t block) {
-            return (int64_t)(block == kNoBlock ? 0u : block) * (32 * D * kElem);
-        };
-        raw k[2][kM];
-        uint32_t block = kNoBlock;
-        if (mine) {
-            look_up(0);
-            block = block_at(0);
-            load_keys(kbase + bytes_at(block), k);
-        }
-        for (int i = 0; i < mine; ++i) {
-            raw v[kT];
-            const uint8_t* const vtile = vbase + bytes_at(block);
-            load_values(vtile, v);
-            float4_t s[R][2];
-#pragma unroll
-            for (int r = 0; r < R; ++r) s[r][0] = s[r][1] = float4_t{0, 0, 0, 0};
-#pragma unroll
-            for (int m = 0; m < kM; ++m)
-#pragma unroll
-                for (int b = 0; b < 2; ++b) {
-                    const vec8 kk = operand<E, F8>(k[b][m]);
-#pragma unroll
-                    for (int r = 0; r < R; ++r) s[r][b] = E::mfma(kk, q[r][m], s[r][b]);
-                }
-            const int t0 = tiles.at(first + i * step) * 32;
-            const bool there = block != kNoBlock;
-            if (i + 1 < mine) {
-                if (((i + 1) & 63) == 0) look_up(i + 1);
-                block = block_at(i + 1);
-                load_keys(kbase + bytes_at(block), k);
-            }
-            const bool masked = !there || !((t0 >= all_lo && t0 + 32 <= all_hi) || t0 + 32 <= all_sink);
-            vec8 p[R];
-#pragma unroll
-            for (int r = 0; r < R; ++r) {
-                float x[8];
-#pragma unroll
-                for (int j = 0; j < 8; ++j) x[j] = s[r][j >> 2][j & 3] * scale;
-                if (masked) {
-#pragma unroll
-                    for (int j = 0; j < 8; ++j)
-                        if (!sees(lim[r], t0 + g * 8 + j, there)) x[j] = -__builtin_inff();
-                }
-                float top = x[0];
-#pragma unroll
-                for (int j = 1; j < 8; ++j) top = fmaxf(top, x[j]);
-                top = row_max(top);
-                const float m_new = fmaxf(mx[r], top);
-                const float ref = m_new == -__builtin_inff() ? 0.0f : m_new;
-                if (__any(m_new != mx[r])) {
-                    const float shrink = __builtin_amdgcn_exp2f(mx[r] - ref);
-                    l[r] *= shrink;
-#pragma unroll
-                    for (int t = 0; t < kT; ++t) o[r][t] *= shrink;
-                }
-                mx[r] = m_new;
-#pragma unroll
-                for (int j = 0; j < 8; ++j) {
-                    const float e2 = __builtin_amdgcn_exp2f(x[j] - ref);
-                    l[r] += e2;
-                    p[r][j] = (typename E::elem)e2;
-                }
-            }
-            if (masked && __any(not_finite(v))) {
-                add_values_seen(vtile, lim, t0, there, p, o);
-            } else {
-#pragma unroll
-                for (int t = 0; t < kT; ++t) {
-                    const vec8 vv = operand<E, F8>(v[t]);
-#pragma unroll
-                    for (int r = 0; r < R; ++r) o[r][t] = E::mfma(vv, p[r], o[r][t]);
-                }
-            }
-        }
-#pragma unroll
-        for (int r = 0; r < R; ++r) l[r] = row_sum(l[r]);
-
-        // the waves of a row group join, 16 rows at a time
-        const float v_scale = F8 && a.v_scale ? a.v_scale[h] : 1.0f;
-        float* const part = a.part + (slot < 0 ? 0 : slot) * slot_floats(a.plan.slot_rows, D);
-        const int part_row0 = rg * 16 * R;
-#pragma unroll
-        for (int r = 0; r < R; ++r) {
-            if (step > 1) {
-                __syncthreads();
-#pragma unroll
-                for (int t = 0; t < kT; ++t)
-                    *reinterpret_cast<float4_t*>(&sh.o[wave][n][t * 16 + g * 4]) = o[r][t];
-                if (g == 0) {
-                    sh.m[wave][n] = mx[r];
-                    sh.l[wave][n] = l[r];
-                }
-                __syncthreads();
-                // 64 lanes x step waves of a group: row n of lanes' 16, columns g * 4 + 16 * ...
-                float top = -__builtin_inff();
-                for (int w = 0; w < step; ++w) top = fmaxf(top, sh.m[rg + (w << split.log2_rg)][n]);
-                float weight[kWaves], sum = 0.0f;
-#pragma unroll
-                for (int w = 0; w < kWaves; ++w) {
-                    weight[w] = 0.0f;
-                    if (w < step) {
-                        weight[w] = part_weight(sh.m[rg + (w << split.log2_rg)][n], top);
-                        sum += weight[w] * sh.l[rg + (w << split.log2_rg)][n];
-                    }
-                }
-                const int row = row0 + r * 16 + n;
-                if (row < row_end) {
-                    for (int t = tg; t < kT; t += step) {
-                        float4_t acc = {0, 0, 0, 0};
-#pragma unroll
-                        for (int w = 0; w < kWaves; ++w)
-                            if (w < step && weight[w] != 0.0f)
-                                acc += weight[w] *
-                                       *reinterpret_cast<const float4_t*>(
-                                           &sh.o[rg + (w << split.log2_rg)][n][t * 16 + g * 4]);
-                        put(part, slot, sq.q0, row, part_row0 + r * 16 + n, h, t * 16 + g * 4, acc, sum, v_scale);
-                    }
-                    if (slot >= 0 && tg == 0 && g == 0) put_stats(part, part_row0 + r * 16 + n, top, sum);
-                }
-            } else {
-                const int row = row0 + r * 16 + n;
-                if (row < row_end) {
-#pragma unroll
-                    for (int t = 0; t < kT; ++t)
-                        put(part, slot, sq.q0, row, part_row0 + r * 16 + n, h, t * 16 + g * 4, o[r][t], l[r], v_scale);
-                    if (slot >= 0 && g == 0) put_stats(part, part_row0 + r * 16 + n, mx[r], l[r]);
-                }
+            for (int v = 0; v < kWaves; ++v) {
+                const Limits l = sh.all[v];
+                w.all_lo = uniform(l.lo > w.all_lo ? l.lo : w.all_lo);
+                w.all_hi = uniform(l.hi < w.all_hi ? l.hi : w.all_hi);
+                w.all_sink = uniform(l.sink < w.all_sink ? l.sink : w.all_sink);
             }
         }
     }
 
     static __device__ __forceinline__ bool sees(const Limits& l, int token, bool there) {
-        return there && token < l.hi && (token >= l.lo || token < l.sink);
+        return there & (token < l.hi) & ((token >= l.lo) | (token < l.sink));
+    }
+
+    static __device__ __forceinline__ float4_t quad(const acc_t& v, int c) {
+        return float4_t{v[4 * c], v[4 * c + 1], v[4 * c + 2], v[4 * c + 3]};
     }
 
     // Four columns of a row: sums into the partial slot, or the finished output.
@@ -680,8 +1009,8 @@ struct Unit {
             return;
         }
         const float inv = sum == 0.0f ? 0.0f : v_scale / sum;
-        float w[4] = {v[0] * inv, v[1] * inv, v[2] * inv, v[3] * inv};
-        finish<4>(a, q0 + row / a.group, h * a.group + row % a.group, col, w);
+        float x[4] = {v[0] * inv, v[1] * inv, v[2] * inv, v[3] * inv};
+        finish<4>(a, q0 + row / a.group, h * a.group + row % a.group, col, x);
     }
 
     __device__ __forceinline__ void put_stats(float* part, int part_row, float m, float l) const {
@@ -689,76 +1018,95 @@ struct Unit {
         part[(int64_t)a.plan.slot_rows * (D + 1) + part_row] = l;
     }
 
-    // Whether a granule of the tile holds an infinity or a NaN.
-    static __device__ __forceinline__ bool not_finite(const raw (&v)[kT]) {
-        typedef uint16_t u16x2 __attribute__((ext_vector_type(2)));
-        u16x2 top = {0, 0};
+    // Whether a granule of the tile of values holds an infinity or a NaN.
+    __device__ __forceinline__ bool not_finite(const uint8_t* tile) const {
+        typedef short bits_t __attribute__((ext_vector_type(8)));
+        bits_t top = {};
+#pragma unroll 4
+        for (int t = 0; t < 2 * kT; ++t)
+            top = __builtin_elementwise_max(
+                top, __builtin_bit_cast(bits_t, value(tile, t >> 1, t & 1)) & (short)0x7fff);
+        bool bad = false;
 #pragma unroll
-        for (int t = 0; t < kT; ++t) {
-            const uint4_t w = __builtin_bit_cast(uint4_t, operand<E, F8>(v[t]));
-#pragma unroll
-            for (int i = 0; i < 4; ++i)
-                top = __builtin_elementwise_max(top, __builtin_bit_cast(u16x2, w[i] & 0x7fff7fffu));
-        }
-        const u16x2 inf = __builtin_bit_cast(u16x2, E::kInf2);
-        return top[0] >= inf[0] || top[1] >= inf[1];
+        for (int j = 0; j < 8; ++j) bad |= top[j] >= E::kInf;
+        return bad;
     }
 
-    // O += V^T P^T token by token, for a tile with infinities or NaN among its
-    // values of which some rows see only a part: what a row does not see must
-    // not reach it even as 0 x NaN, which the matrix instruction would add.
-    __device__ __forceinline__ void add_values_seen(const uint8_t* vtile, const Limits (&lim)[R], int t0, bool there,
-                                                 const vec8 (&p)[R], float4_t (&o)[R][kT]) const {
+    // For a tile with infinities or NaN among its values of which some rows
+    // see only a part: what a row does not see must not reach it even as
+    // 0 x NaN, which the matrix instruction would add.  The product takes the
+    // finite values; which infinities (a NaN is both) a row saw in which column
+    // is kept, a bit each, and added when the unit's tiles are done.
+    //   marks: [r][t][sign][32 rows], bits of the tile's 32 columns; lane (n, g)
+    // keeps sign g of row n.  (No branch here or in the tile loop depends on the
+    // lane: the paths would keep copies of the accumulators where they meet.)
+    template <int R>
+    __device__ __forceinline__ void mark_infinities(const uint8_t* tile, Rows<R>& w, int t0, bool there,
+                                                    uint32_t* marks) const {
+        if (!w.marked) {
+            w.marked = true;
 #pragma unroll 1
-        for (int i = 0; i < 32; ++i) {
-            float w[R];
+            for (int i = 0; i < R * kT; ++i) marks[i * 64 + lane] = 0;
+        }
+#pragma unroll 1
+        for (int i = 0; i < 2 * kT; ++i) {
+            typedef short bits_t __attribute__((ext_vector_type(8)));
+            bits_t v = __builtin_bit_cast(bits_t, value(tile, i >> 1, i & 1));
+#pragma unroll 1
+            for (int j = 0; j < 8; ++j) {
+                const short mine = v[0], size = mine & 0x7fff;
+                v = __builtin_shufflevector(v, v, 1, 2, 3, 4, 5, 6, 7, 0);
+                const uint64_t up = __ballot(size > E::kInf || mine == E::kInf);
+                const uint64_t down = __ballot(size > E::kInf || (size == E::kInf && mine < 0));
+                if ((up | down) == 0) continue;
+                const uint64_t sign = g ? down : up;  // columns 32 (i / 2) ..: of token j, and of token 8 + j
+                const int at = t0 + (i & 1) * 16 + j;
 #pragma unroll
-            for (int r = 0; r < R; ++r) {
-                float mine = 0.0f;
-#pragma unroll
-                for (int j = 0; j < 8; ++j) mine = (i & 7) == j ? (float)p[r][j] : mine;
-                w[r] = __shfl(mine, (i >> 3) * 16 + n);
-            }
-            const uint8_t* const at = vtile + (int64_t)((i >> 3) * 8 * D + (i & 7)) * kElem;
-#pragma unroll
-            for (int t = 0; t < kT; ++t) {
-                __builtin_amdgcn_sched_barrier(0);  // four loads at a time: this path keeps no registers of its own
-#pragma unroll
-                for (int c = 0; c < 4; ++c) {
-                    const int col = t * 16 + g * 4 + c;
-                    float x;
-                    if constexpr (F8) {
-                        uint2 byte = {at[col * 8], 0u};
-                        x = (float)E::from_e4m3(byte)[0];
-                    } else {
-                        x = (float)*reinterpret_cast<const typename E::elem*>(at + col * 8 * kElem);
-                    }
-#pragma unroll
-                    for (int r = 0; r < R; ++r)
-                        if (sees(lim[r], t0 + i, there)) o[r][t][c] = fmaf(w[r], x, o[r][t][c]);
-                }
+                for (int r = 0; r < R; ++r)
+                    marks[(r * kT + (i >> 1)) * 64 + lane] |=
+                        (sees(w.lim[r], at, there) ? (uint32_t)sign : 0u) |
+                        (sees(w.lim[r], at + 8, there) ? (uint32_t)(sign >> 32) : 0u);
             }
         }
+    }
+
+    template <int R>
+    __device__ __forceinline__ void add_infinities(Rows<R>& w, const uint32_t* marks) const {
+        wait_lds();
+#pragma unroll
+        for (int r = 0; r < R; ++r)
+#pragma unroll
+            for (int t = 0; t < kT; ++t) {
+                const uint32_t up = marks[(r * kT + t) * 64 + n], down = marks[(r * kT + t) * 64 + 32 + n];
+#pragma unroll
+                for (int c = 0; c < 16; ++c) {
+                    const int col = (c >> 2) * 8 + g * 4 + (c & 3);
+                    const float inf = __builtin_inff();
+                    w.o[r][t][c] += (up >> col & 1 ? inf : 0.0f) - (down >> col & 1 ? inf : 0.0f);
+                }
+                __builtin_amdgcn_sched_barrier(0);
+            }
     }
 };
 
-template <int D, class E, bool F8, int R>
-__global__ __launch_bounds__(kThreads, D == 256 ? 1 : 2) void prefix_attention_kernel(AttnArgs a) {
+// kR: 32-row tiles of a wave where waves share their tiles; 0: no unit of the launch does.
+template <int D, class E, bool F8, int kR>
+__global__ __launch_bounds__(kThreads, D == 256 || kR == 2 ? 1 : 2) void prefix_attention_kernel(AttnArgs a) {
     extern __shared__ __align__(16) uint8_t lds[];
     Shared<D>& sh = *reinterpret_cast<Shared<D>*>(lds);
     uint64_t* const cost = reinterpret_cast<uint64_t*>(lds + sizeof(Shared<D>));
     uint32_t* const info = reinterpret_cast<uint32_t*>(cost + a.plan.max_entries + 1);
-    const Line line = build_line(a, cost, info, sh.scratch);
+    const Line line = build_line(a, cost, info, sh);
     // Pieces follow each other by XCD (workgroup b runs on XCD b % 8), so that
     // the row tiles of one kv head, which read the same keys, share an L2.
     const int grid = a.plan.workgroups;
     const int w = grid % 8 ? blockIdx.x : (blockIdx.x % 8) * (grid / 8) + blockIdx.x / 8;
     const uint64_t all = line.head_cost * (uint64_t)a.kv_heads;
-    uint64_t x = line.per * (uint64_t)w;
-    const uint64_t x1 = x + line.per < all ? x + line.per : all;
-    Unit<D, E, F8, R> unit(a, sh);
+    const uint64_t x0 = line.per * (uint64_t)w, x1 = x0 + line.per < all ? x0 + line.per : all;
+    uint64_t x = x0;
+    Unit<D, E, F8> unit(a, sh);
     while (x < x1) {
-        const int h = (int)(x / line.head_cost);
+        const int h = (int)quotient(x, line.head_cost);
         const uint64_t at = x - h * line.head_cost;  // within the head
         int lo = 0, hi = line.entries;               // the entry: cost[lo] <= at < cost[lo + 1]
         while (hi - lo > 1) {
@@ -766,36 +1114,51 @@ __global__ __launch_bounds__(kThreads, D == 256 ? 1 : 2) void prefix_attention_k
             if (cost[mid] <= at) lo = mid;
             else hi = mid;
         }
-        const int e = lo;
+        const int e = uniform(lo);
         const bool prefix = e < a.plan.prefix_entries;
-        const uint32_t c = (uint32_t)(prefix ? a.plan.prefix.cost : a.plan.own.cost);
-        const uint64_t e0 = cost[e], e1 = cost[e + 1];
-        const uint64_t stop = x1 - h * line.head_cost < e1 ? x1 - h * line.head_cost : e1;
-        // steps whose first point lies in the piece
-        const int s0 = (int)((at - e0 + c - 1) / c), s1 = (int)((stop - e0 + c - 1) / c);
-        const int seq = prefix ? 0 : (int)(info[e] >> 16), tile = prefix ? e : (int)(info[e] & 0xffff);
+        const RowSplit& split = prefix ? a.plan.prefix : a.plan.own;
+        const uint32_t c = (uint32_t)split.cost;
+        const uint64_t e0 = uniform(cost[e]), e1 = uniform(cost[e + 1]);
+        const uint64_t head0 = h * line.head_cost;
+        const uint64_t stop = x1 - head0 < e1 ? x1 - head0 : e1;
+        // steps whose first point lies in the piece (an entry has less than 2^32)
+        const int s0 = (int)(((uint32_t)(at - e0) + c - 1) / c), s1 = (int)(((uint32_t)(stop - e0) + c - 1) / c);
+        const uint32_t who = prefix ? e : uniform((int)info[e]);
+        const int seq = prefix ? 0 : (int)(who >> 16), tile = prefix ? e : (int)(who & 0xffff);
         Tiles tiles;
         if (prefix) tiles = prefix_tiles(a, line.min_pos);
         else tiles = own_tiles(a, seq_at(a, seq), tile);
-        const uint64_t head0 = h * line.head_cost;
-        const bool alone = !a.plan.prefix_entries && (head0 + e0) / line.per == (head0 + e1 - c) / line.per;
-        if (s0 < s1)
-            unit.run(h, prefix, seq, tile, tiles, s0, s1,
-                     alone ? -1 : (int64_t)w + (int64_t)h * line.entries + e);
+        tiles = {uniform(tiles.sink), uniform(tiles.lo), uniform(tiles.hi)};
+        // all of the entry's steps begin in this piece
+        const bool alone = !a.plan.prefix_entries && x - at + e0 >= x0 && head0 + e1 - c < x0 + line.per;
+        if (s0 < s1) {
+            const int64_t slot = alone ? -1 : (int64_t)w + (int64_t)h * line.entries + e;
+            if (kR == 0 || !split.shared) unit.template run<1, false>(h, prefix, seq, tile, tiles, s0, s1, slot);
+            else unit.template run<kR ? kR : 1, true>(h, prefix, seq, tile, tiles, s0, s1, slot);
+        }
         x = head0 + stop;
     }
 }
 
-template <int D, class E, bool F8, int R>
+// Dynamic LDS of a launch: the tiles and the line of entries.
+template <int D>
+size_t lds_bytes(int max_entries) {
+    return sizeof(Shared<D>) + 8 * ((size_t)max_entries + 1) + 4 * (size_t)max_entries;
+}
+
+template <int D, class E, bool F8, int kR>
 hipError_t launch_as(const AttnArgs& a, hipStream_t stream) {
-    const size_t lds = sizeof(Shared<D>) + 8 * ((size_t)a.plan.max_entries + 1) + 4 * (size_t)a.plan.max_entries;
-    prefix_attention_kernel<D, E, F8, R><<<dim3((unsigned)a.plan.workgroups), kThreads, lds, stream>>>(a);
+    prefix_attention_kernel<D, E, F8, kR><<<dim3((unsigned)a.plan.workgroups), kThreads, lds_bytes<D>(a.plan.max_entries), stream>>>(a);
     return hipGetLastError();
 }
 
 template <int D, class E, bool F8>
 hipError_t launch_rows(const AttnArgs& a, hipStream_t stream) {
-    return a.plan.r == 1 ? launch_as<D, E, F8, 1>(a, stream) : launch_as<D, E, F8, 2>(a, stream);
+    if (a.plan.shared_r == 0) return launch_as<D, E, F8, 0>(a, stream);
+    if constexpr (D < 256) {
+        if (a.plan.shared_r == 2) return launch_as<D, E, F8, 2>(a, stream);
+    }
+    return launch_as<D, E, F8, 1>(a, stream);
 }
 
 template <int D>

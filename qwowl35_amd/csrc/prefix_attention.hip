@@ -8,12 +8,10 @@ using attn::MetaHead;
 
 namespace {
 
-RowSplit split_rows(int64_t rows, int r, int cost) {
-    RowSplit s;
-    s.log2_rg = rows <= 16 * r ? 0 : rows <= 32 * r ? 1 : 2;
-    s.rows = 16 * r << s.log2_rg;
-    s.cost = cost;
-    return s;
+RowSplit split_rows(int64_t rows, int shared_r) {
+    if (rows <= 32) return {0, 32, 3, 0};
+    if (rows <= 64) return {1, 64, 2, 0};
+    return {2, 128 * shared_r, shared_r, 1};
 }
 
 // A unit's pieces: workgroups w0.., slots slot0...
@@ -55,12 +53,12 @@ __global__ __launch_bounds__(256) void prefix_attention_join(AttnArgs a, int wav
     const MetaHead m = *reinterpret_cast<const MetaHead*>(a.meta);
     const int* const first = reinterpret_cast<const int*>(a.meta + attn::meta_first_at());
     const uint64_t* const cost = reinterpret_cast<const uint64_t*>(a.meta + attn::meta_cost_at(a.n_seqs));
-    const int s = attn::seq_of(a, t);
+    const int s = attn::seq_of_wave(a, t, lane);
     Pieces own = {0, 0, 0}, pre = {0, 0, 0};
     bool on = false;
     if (s >= 0) {
         const attn::Seq q = attn::seq_at(a, s);
-        on = t < q.q0 + q.n;
+        on = t >= q.q0 && t < q.q0 + q.n;
         if (on) {
             const int row = (t - q.q0) * a.group + head % a.group;
             own = pieces_of(m, cost, h, first[s] + row / a.plan.own.rows, row, a.plan.own);
@@ -162,16 +160,19 @@ AttnPlan plan_attention(int dim, int kv_heads, int group, int n_seqs, int n_toke
     AttnPlan p = {};
     const int64_t rows_prefix = prefix ? (int64_t)n_tokens * group : 0, rows_own = (int64_t)max_new * group;
     const int64_t most = rows_prefix > rows_own ? rows_prefix : rows_own;
-    p.r = most <= 16 ? 1 : 2;
-    p.prefix = split_rows(rows_prefix, p.r, 1);
-    p.own = split_rows(rows_own, p.r, 1);
-    p.workgroups = dim == 256 ? 256 : 512;
+    p.shared_r = most <= 64 ? 0 : most <= 128 || dim == 256 ? 1 : 2;
+    p.prefix = split_rows(rows_prefix, p.shared_r);
+    p.own = split_rows(rows_own, p.shared_r);
+    p.workgroups = dim == 256 || p.shared_r == 2 ? 256 : 512;
     p.prefix_entries = (int)((rows_prefix + p.prefix.rows - 1) / p.prefix.rows);
     // every sequence's last row tile may be a part of one
     p.max_entries = p.prefix_entries + n_seqs + (int)((int64_t)n_tokens * group / p.own.rows);
     p.slot_rows = p.prefix.rows > p.own.rows && prefix ? p.prefix.rows : p.own.rows;
     p.slots = (uint64_t)p.workgroups + (uint64_t)kv_heads * p.max_entries;
     p.meta_bytes = (attn::meta_cost_at(n_seqs) + 8 * ((uint64_t)p.max_entries + 1) + 255) / 256 * 256;
+    p.lds_bytes = dim == 64    ? attn::lds_bytes<64>(p.max_entries)
+                  : dim == 128 ? attn::lds_bytes<128>(p.max_entries)
+                               : attn::lds_bytes<256>(p.max_entries);
     p.workspace_bytes = p.meta_bytes + 4 * p.slots * attn::slot_floats(p.slot_rows, dim);
     return p;
 }
