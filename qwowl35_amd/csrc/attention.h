@@ -35,26 +35,32 @@ hipError_t launch_rotate(const HeadsView& x, const HeadsView& y, int n_tokens, i
 hipError_t launch_kv_append(const qw35_hip_kv_cache& cache, const HeadsView& k, const HeadsView& v, int n_tokens,
                             const int64_t* slots, const RopeArgs& rope, hipStream_t stream);
 
-// How a launch divides the rows (new token x head of a group) of a kind of
-// unit among a workgroup's four waves.  Up to 64 rows: 32 rows a wave, the
-// waves of a row group on different 32-token tiles (a step is 4 or 2 tiles).
-// More: 32 or 64 rows a wave, all four on the same tile (a step is one).
+// How a launch divides the rows (new token x head of a group) of a kind of unit.
+//   Own units of up to 64 rows: a wave has 16 or 32 rows and goes through the
+// tokens by itself.
+//   Prefix units of up to 64 rows: a workgroup, 16 or 32 rows a wave, the waves
+// of a row group on different 32-token tiles (a step is 4 or 2 tiles).
+//   More rows: a workgroup, 32 or 64 rows a wave, all four on the same tile.
 struct RowSplit {
-    int log2_rg;  // row groups
-    int rows;     // rows of a unit
-    int cost;     // cost of a step
-    int shared;   // the waves share their tiles
-    __host__ __device__ int step() const { return 4 >> log2_rg; }
+    int log2_tiles;  // tiles of a step
+    int log2_rg;     // row groups of the workgroup's waves
+    int log2_rows;   // rows of a unit
+    int narrow;      // 16 rows a wave
+    int shared;      // the waves share their tiles
+    int lead;        // cost of a unit beside its steps
+    int log2_cost;   // cost of a step
+    __host__ __device__ int step() const { return 1 << log2_tiles; }
 };
 
 struct AttnPlan {
     int shared_r;  // 32-row tiles of a wave where waves share tiles (0: no unit does)
     RowSplit prefix, own;
-    int workgroups;
+    int log2_workgroups;
+    int lanes;           // up to 64 sequences whose costs fit 32 bits
+    uint32_t group_magic, page_magic;  // 2^32 / group and page_blocks, rounded up (0: they are 1)
     int prefix_entries;  // row tiles of the prefix, of every kv head
-    int max_entries;     // bound of prefix and own row tiles together
-    int slot_rows;       // rows of a partial result's slot
-    uint64_t slots;
+    int own_entries;     // bound of the sequences' row tiles together
+    uint64_t own_part;   // floats of the prefix' partial slots
     uint64_t meta_bytes;
     uint64_t workspace_bytes;
     uint64_t lds_bytes;
@@ -82,11 +88,17 @@ struct AttnArgs {
     int window;
     int sink;
     uint8_t* meta;
-    float* part;
+    float* part;      // partial slots: of the prefix
+    float* own_part;  // and of own units
     AttnPlan plan;
 };
 
-AttnPlan plan_attention(int dim, int kv_heads, int group, int n_seqs, int n_tokens, int max_new, bool prefix);
+// A batch as the plan sees it; `own_tokens`: the most own tokens that a sequence's page table holds.
+struct AttnShape {
+    int dim, kv_heads, group, n_seqs, n_tokens, max_new, page_blocks, prefix_len;
+    int64_t own_tokens;
+};
+AttnPlan plan_attention(const AttnShape& s);
 hipError_t launch_prefix_attention(const AttnArgs& a, int dim, uint32_t q_dtype, uint32_t cache_dtype,
                                    hipStream_t stream);
 

@@ -235,9 +235,10 @@ static bool check_batch(const qw35_hip_kv_cache* cache, uint32_t n_heads, uint32
 }
 
 static qw35::AttnPlan plan_of(const qw35_hip_kv_cache* c, uint32_t n_heads, uint32_t n_seqs, uint32_t n_tokens,
-                              uint32_t max_new, bool prefix) {
-    return qw35::plan_attention((int)c->head_dim, (int)c->kv_heads, (int)(n_heads / c->kv_heads), (int)n_seqs,
-                                (int)n_tokens, (int)max_new, prefix);
+                              uint32_t max_new, uint32_t prefix_len, uint32_t pages_per_seq) {
+    return qw35::plan_attention({(int)c->head_dim, (int)c->kv_heads, (int)(n_heads / c->kv_heads), (int)n_seqs,
+                                 (int)n_tokens, (int)max_new, (int)(c->page_size / 32), (int)prefix_len,
+                                 (int64_t)pages_per_seq * c->page_size});
 }
 
 uint64_t qw35_hip_prefix_attention_workspace_size(const qw35_hip_kv_cache* cache, uint32_t n_heads, uint32_t n_seqs,
@@ -245,12 +246,12 @@ uint64_t qw35_hip_prefix_attention_workspace_size(const qw35_hip_kv_cache* cache
     if (!check_batch(cache, n_heads, n_seqs, n_tokens, nullptr, 0)) return 0;
     const uint32_t group = n_heads / cache->kv_heads;
     // every division of the rows that a call of this batch may take: the most rows of a sequence that each has
-    const uint32_t most[] = {1, 32 / group, 64 / group, 128 / group, 128 / group + 1, n_tokens};
+    const uint32_t most[] = {1, 16 / group, 32 / group, 64 / group, 128 / group, 128 / group + 1, n_tokens};
     uint64_t need = 256;
-    for (int prefix = 0; prefix < 2; ++prefix)
+    for (uint32_t prefix = 0; prefix < 2; ++prefix)
         for (uint32_t max_new : most) {
             if (max_new == 0 || max_new > n_tokens) continue;
-            const qw35::AttnPlan p = plan_of(cache, n_heads, n_seqs, n_tokens, max_new, prefix != 0);
+            const qw35::AttnPlan p = plan_of(cache, n_heads, n_seqs, n_tokens, max_new, prefix, 1u << 15);
             if (p.workspace_bytes > need) need = p.workspace_bytes;
         }
     return need;
@@ -305,10 +306,10 @@ int qw35_hip_prefix_attention(const qw35_hip_attention* op, const qw35_hip_kv_ca
         return 0;
     }
     const uint32_t max_new = op->max_new == 0 || op->max_new > op->n_tokens ? op->n_tokens : op->max_new;
-    a.plan = plan_of(cache, op->n_heads, op->n_seqs, op->n_tokens, max_new, op->prefix_len != 0);
+    a.plan = plan_of(cache, op->n_heads, op->n_seqs, op->n_tokens, max_new, op->prefix_len, op->pages_per_seq);
     if (a.plan.lds_bytes > kMaxLds) {
         set_err(err, err_len, "%s: %d row tiles in a call are %llu over the list's room; give it fewer tokens or sequences",
-                what, a.plan.max_entries, (unsigned long long)((a.plan.lds_bytes - kMaxLds + 11) / 12));
+                what, a.plan.own_entries, (unsigned long long)((a.plan.lds_bytes - kMaxLds + 11) / 12));
         return 0;
     }
     if (!op->workspace || ((uintptr_t)op->workspace & 255u) || op->workspace_bytes < a.plan.workspace_bytes) {
@@ -338,6 +339,7 @@ int qw35_hip_prefix_attention(const qw35_hip_attention* op, const qw35_hip_kv_ca
     a.sink = (int)op->sink;
     a.meta = static_cast<uint8_t*>(op->workspace);
     a.part = reinterpret_cast<float*>(a.meta + a.plan.meta_bytes);
+    a.own_part = a.part + a.plan.own_part;
     return check_hip(qw35::launch_prefix_attention(a, (int)cache->head_dim, op->q.dtype, cache->dtype,
                                                    static_cast<hipStream_t>(stream)),
                      what, err, err_len);

@@ -3,29 +3,35 @@
 //
 // Mathematics.  For a row (new token t of sequence s, query head of group h):
 //   out = sum_i p_i v_i / sum_i p_i,  p_i = exp(scale q.k_i - m)
-// over the tokens i the row sees, in one pass: tiles of 32 tokens keep the
-// running maximum m, the sum of p and the sum of p v (fp32), rescaled when m
-// rises.  Parts of a row's tokens (the shared prefix, the sequence's own
-// pages, pieces of either) give (m, sum p, sum p v) each, joined at the end by
-// exp(m_part - m).
+// over the tokens i the row sees, in one pass: tiles of 32 tokens keep a
+// reference m close to the running maximum, the sum of p and the sum of p v
+// (fp32), rescaled when m rises.  Parts of a row's tokens (the shared prefix,
+// the sequence's own pages, pieces of either) give (m, sum p, sum p v) each,
+// joined at the end by exp(m_part - m).
 //
 // Units.  The rows of all sequences read the same prefix, so a prefix unit is
 // a kv head and a tile of rows out of the whole batch: the prefix is read once
 // for all of them.  An own unit is a kv head, a sequence and a tile of its
-// rows.  Every unit's steps of 32-token tiles lie behind each other on one
-// line, of which each workgroup takes an equal piece (weighted by what a
-// step costs), crossing units where it has to: lengths live on the device, and
-// whatever they are the load is even and the grid constant.  A workgroup's
-// piece of a unit goes to the partial slot (workgroup + unit), which no other
-// piece has; the combine kernel finds a row's slots by the same arithmetic.
+// rows.  The steps of all prefix units lie behind each other on one line, those
+// of all own units on another, and each workgroup (on the own line each wave,
+// unless units have over 64 rows) takes an equal piece of either, crossing
+// units where it has to: lengths live on the device, and whatever they are the
+// load is even and the grid constant.  A piece's part of a unit goes to the
+// partial slot (place of the piece + unit), which no other has; one workgroup
+// lists every unit's slots for the join.
+//
+// A call is often a few microseconds long, of which a wave alone on its SIMD
+// takes one for every 500 or so instructions that are not a tile's.  So up to
+// 64 sequences of one row tile each, the own line is kept a sequence a lane, in
+// 32 bits and without a barrier.
 //
 // Operands.  A tile's scores are S^T = K Q^T and the output O^T = V^T P^T, on
-// v_mfma_f32_32x32x16: lane l holds query row l % 32 in S, P and O alike, so
-// maximum, sum and rescaling stay in a lane (and its other one of the same
-// row).  The cache's granules are the A operands: eight columns of a key, or
-// eight tokens of a value column.  Row i of a tile's scores is the token whose
-// number is i with bits 2 and 3 exchanged, which leaves the scores a lane holds
-// as the tokens of its two value granules: P needs no exchange between lanes.
+// v_mfma_f32_32x32x16 (units of more than 16 rows) or 16x16x32: a lane holds one
+// query row in S, P and O alike, so maximum, sum and rescaling stay in a lane
+// and the one or three others of the same row.  The cache's granules are the A
+// operands: eight columns of a key, or eight tokens of a value column.  Which
+// token is which row of the scores is chosen so that a lane's scores are the
+// tokens of its own value granules: P needs no exchange between lanes.
 //
 // Data.  Tiles go from HBM to LDS by copies that take no registers, as far
 // ahead as the ring has room (128 KB for 256 columns), and from there to the
@@ -52,12 +58,15 @@ constexpr uint32_t kNoBlock = 0xffffffffu;
 
 typedef float acc_t __attribute__((ext_vector_type(16)));
 
-// Element type of queries and 16-bit caches, and its matrix instruction.
+// Element type of queries and 16-bit caches, and its matrix instructions.
 struct Half {
     typedef _Float16 elem;
     typedef half8_t vec8;
     static __device__ __forceinline__ acc_t mfma(vec8 a, vec8 b, acc_t c) {
         return __builtin_amdgcn_mfma_f32_32x32x16_f16(a, b, c, 0, 0, 0);
+    }
+    static __device__ __forceinline__ float4_t mfma(vec8 a, vec8 b, float4_t c) {
+        return __builtin_amdgcn_mfma_f32_16x16x32_f16(a, b, c, 0, 0, 0);
     }
     static constexpr short kInf = 0x7c00;  // bits of +inf
     static __device__ __forceinline__ vec8 from_e4m3(uint2 w) {
@@ -76,7 +85,10 @@ struct Bf16 {
     static __device__ __forceinline__ acc_t mfma(vec8 a, vec8 b, acc_t c) {
         return __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, b, c, 0, 0, 0);
     }
-    static constexpr short kInf = 0x7f80, kUp = 0x3f80, kDown = 0x4280, kBoth = 0x4282;
+    static __device__ __forceinline__ float4_t mfma(vec8 a, vec8 b, float4_t c) {
+        return __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b, c, 0, 0, 0);
+    }
+    static constexpr short kInf = 0x7f80;  // bits of +inf
     static __device__ __forceinline__ vec8 from_e4m3(uint2 w) {
         uint4_t r;
         r[0] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(w.x, 1.0f, false));
@@ -87,17 +99,20 @@ struct Bf16 {
     }
 };
 
-// What the combine kernel needs of a launch, at the start of the meta block:
-// this, then first[n_seqs] (a sequence's first entry), then cost[entries + 1].
+// What the join needs of a launch, at the start of the workspace: this, then
+// first[n_seqs] (a sequence's first own entry), then [kv_heads][prefix and own
+// entries] Pieces.
 struct MetaHead {
-    uint64_t head_cost;  // cost of one kv head's entries
-    uint64_t per;        // cost of a workgroup's piece
-    int entries;
-    int pad;
+    int own_entries;
+    int lanes;  // first[s] is s
+};
+struct Pieces {
+    uint32_t slot0;  // the first partial slot of an entry, and how many
+    uint32_t n;
 };
 
 __host__ __device__ inline size_t meta_first_at() { return sizeof(MetaHead); }
-__host__ __device__ inline size_t meta_cost_at(int n_seqs) {
+__host__ __device__ inline size_t meta_pieces_at(int n_seqs) {
     return (sizeof(MetaHead) + 4 * (size_t)n_seqs + 7) / 8 * 8;
 }
 
@@ -123,6 +138,37 @@ __device__ __forceinline__ uint64_t quotient(uint64_t x, uint64_t d) {
     uint64_t q = (uint64_t)((double)x / (double)d);
     if (q * d > x) --q;
     return q;
+}
+
+// x / d of numbers below 2^31, the quotient below 2^15.
+__device__ __forceinline__ uint32_t quotient(uint32_t x, uint32_t d) {
+    uint32_t q = (uint32_t)((float)x * __builtin_amdgcn_rcpf((float)d));
+    if ((int32_t)(x - q * d) < 0) --q;
+    if (x - q * d >= d) ++q;
+    return q;
+}
+
+// Over a wave's 64 lanes, by lane exchanges inside the vector unit.
+template <class Op>
+__device__ __forceinline__ int lane_scan(int v, int none, Op op) {
+    v = op(v, __builtin_amdgcn_update_dpp(none, v, 0x111, 0xf, 0xf, false));  // from 1, 2, 4, 8 lanes below in 16
+    v = op(v, __builtin_amdgcn_update_dpp(none, v, 0x112, 0xf, 0xf, false));
+    v = op(v, __builtin_amdgcn_update_dpp(none, v, 0x114, 0xf, 0xf, false));
+    v = op(v, __builtin_amdgcn_update_dpp(none, v, 0x118, 0xf, 0xf, false));
+    v = op(v, __builtin_amdgcn_update_dpp(none, v, 0x142, 0xa, 0xf, false));  // lane 15 to the next 16
+    v = op(v, __builtin_amdgcn_update_dpp(none, v, 0x143, 0xc, 0xf, false));  // lane 31 to the upper half
+    return v;
+}
+__device__ __forceinline__ int lane_max(int v, int none) {
+    return __builtin_amdgcn_readlane(lane_scan(v, none, [](int x, int y) { return x > y ? x : y; }), 63);
+}
+__device__ __forceinline__ int lane_min(int v, int none) {
+    return __builtin_amdgcn_readlane(lane_scan(v, none, [](int x, int y) { return x < y ? x : y; }), 63);
+}
+
+// row / group (a row stays below 2^24).
+__device__ __forceinline__ int token_of(const AttnArgs& a, int row) {
+    return a.plan.group_magic ? (int)__umulhi((uint32_t)row, a.plan.group_magic) : row;
 }
 
 __device__ __forceinline__ int clampi(int v, int lo, int hi) { return v < lo ? lo : v > hi ? hi : v; }
@@ -170,24 +216,32 @@ struct Limits {
     int lo, hi, sink;
 };
 
-// Of a unit whose first token stands at position `base`, by a token at `pos`.
-__device__ __forceinline__ Limits limits_of(const AttnArgs& a, int64_t pos, int base, int n) {
-    Limits l;
-    const int64_t hi = pos + 1 - base;
-    l.hi = hi < 0 ? 0 : hi > n ? n : (int)hi;
-    l.lo = 0;
-    l.sink = 0;
+// Of a unit of n tokens, from unclamped ends.
+__device__ __forceinline__ Limits limits_of(const AttnArgs& a, int hi, int lo, int sink, int n) {
+    Limits l = {0, clampi(hi, 0, n), 0};
     if (a.window) {
-        const int64_t lo = hi - a.window;
-        l.lo = lo < 0 ? 0 : lo > n ? n : (int)lo;
-        l.sink = clampi(a.sink - base, 0, l.hi);
+        l.lo = clampi(lo, 0, n);
+        l.sink = clampi(sink, 0, l.hi);
     }
     return l;
+}
+
+// What a new token sees of its own sequence's tokens and of the prefix, `upto`
+// of its own ones lying at or before it (up to 2^30, and 2^22 below zero, as
+// prefix_len and window: nothing here passes 32 bits).
+__device__ __forceinline__ int upto_of(const Seq& q, int tok) { return q.length - q.n + tok + 1; }
+__device__ __forceinline__ Limits own_limits(const AttnArgs& a, const Seq& q, int upto) {
+    return limits_of(a, upto, upto - a.window, a.sink - a.prefix_len, q.length);
+}
+__device__ __forceinline__ Limits prefix_limits(const AttnArgs& a, int upto) {
+    return limits_of(a, upto < 0 ? a.prefix_len + upto : a.prefix_len, a.prefix_len - a.window + upto, a.sink,
+                     a.prefix_len);
 }
 
 // The 32-token tiles a unit goes through: `sink` ones from 0, then lo..hi-1.
 struct Tiles {
     int sink, lo, hi;
+    __device__ __forceinline__ int steps(const RowSplit& s) const { return (count() + s.step() - 1) >> s.log2_tiles; }
     __device__ __forceinline__ int count() const { return sink + hi - lo; }
     __device__ __forceinline__ int at(int v) const { return v < sink ? v : v - sink + lo; }
 };
@@ -202,20 +256,18 @@ __device__ __forceinline__ Tiles tiles_of(Limits l) {
 
 // Tiles that any row of an own entry sees: up to the last row's position, from the first one's window.
 __device__ __forceinline__ Tiles own_tiles(const AttnArgs& a, const Seq& q, int tile) {
-    const int rows = q.n * a.group, r0 = tile * a.plan.own.rows;
-    const int last = (r0 + a.plan.own.rows < rows ? r0 + a.plan.own.rows : rows) - 1;
-    const int64_t pos0 = (int64_t)a.prefix_len + q.length - q.n;
-    Limits l = limits_of(a, pos0 + last / a.group, a.prefix_len, q.length);
-    const Limits first = limits_of(a, pos0 + r0 / a.group, a.prefix_len, q.length);
-    l.lo = first.lo;
+    const int rows = q.n * a.group, r0 = tile << a.plan.own.log2_rows, r1 = r0 + (1 << a.plan.own.log2_rows);
+    const int last = (r1 < rows ? r1 : rows) - 1;
+    Limits l = own_limits(a, q, upto_of(q, token_of(a, last)));
+    if (a.window) l.lo = own_limits(a, q, upto_of(q, token_of(a, r0))).lo;
     return tiles_of(l);
 }
 
 // Tiles of the prefix: from the window of the batch's first position.
-__device__ __forceinline__ Tiles prefix_tiles(const AttnArgs& a, int64_t min_pos) {
-    Limits l = limits_of(a, min_pos, 0, a.prefix_len);
+__device__ __forceinline__ Tiles prefix_tiles(const AttnArgs& a, int least_upto) {
+    Limits l = prefix_limits(a, least_upto);
     l.hi = a.prefix_len;
-    l.sink = a.window ? clampi(a.sink, 0, l.hi) : 0;
+    if (a.window) l.sink = clampi(a.sink, 0, l.hi);
     return tiles_of(l);
 }
 
@@ -249,148 +301,335 @@ __device__ __forceinline__ T block_scan(T v, T* shared, T& total) {
     return v + before;
 }
 
-struct Line {
-    int entries;         // prefix row tiles, then every sequence's
-    uint64_t head_cost;
-    uint64_t per;
-    int64_t min_pos;     // of the batch (with a window and a prefix)
+// Cost of an entry: its own, and its steps'.
+__device__ __forceinline__ uint32_t entry_cost(const RowSplit& s, int steps) {
+    return steps ? s.lead + ((uint32_t)steps << s.log2_cost) : 0u;
+}
+
+// A unit's part in a piece of a line.
+struct Job {
+    int h, seq, tile;
+    Seq sq;
+    Tiles tiles;
+    int s0, s1;   // its steps
+    float* part;  // where its sums go; null: these are all of the rows', they go to the output
 };
 
-// Fills cost[0..entries] (cost before an entry) and info[entry] (sequence << 16
-// | row tile) in LDS; the first workgroup also leaves them for the combine kernel.
+// What is left to a workgroup (or wave) of its piece: [x, x1), which began at x0.
+struct Piece {
+    uint64_t per, x0, x, x1;
+    int place;
+};
+
+struct Line {
+    Piece prefix, own;
+    uint64_t head_cost;    // of a kv head's own entries
+    int own_entries;       // of a kv head
+    uint32_t prefix_cost;  // of an entry of the prefix
+    Tiles prefix_tiles;
+    bool lanes;            // the own line is a sequence a lane
+    bool plain;            // every new token sees the whole prefix
+};
+
+__device__ __forceinline__ uint64_t line_quotient(const Line& l, uint64_t x, uint64_t d) {
+    return l.lanes ? quotient((uint32_t)x, (uint32_t)d) : quotient(x, d);
+}
+
+// A piece of a line of `all`, for one of 2^log2_places.
+__device__ __forceinline__ Piece piece_of(uint64_t all, int log2_places, int place, const RowSplit& s, uint64_t least) {
+    Piece p;
+    p.place = place;
+    p.per = (all + (1ull << log2_places) - 1) >> log2_places;
+    if (least < 1u << s.log2_cost) least = 1u << s.log2_cost;  // a step
+    if (p.per < least) p.per = least;
+    p.x = p.x0 = p.per * (uint64_t)place;
+    p.x1 = p.x0 + p.per < all ? p.x0 + p.per : all;
+    return p;
+}
+
+// The slots of an entry whose cost begins at x.
+__device__ __forceinline__ Pieces pieces_of(const Line& l, uint64_t per, const RowSplit& s, uint64_t x, uint32_t cost,
+                                            int unit) {
+    if (!cost) return {0, 0};
+    const uint32_t w0 = (uint32_t)line_quotient(l, x + s.lead, per);
+    const uint32_t w1 = (uint32_t)line_quotient(l, x + cost - (1u << s.log2_cost), per);
+    return {w0 + (uint32_t)unit, w1 - w0 + 1};
+}
+
+// Steps of an entry at x, cost c, whose first point, of x + lead + (step << log2_cost), lies in what is left of the
+// piece; moves on behind them.  True: all of the entry's steps begin in the piece.
+__device__ __forceinline__ bool take_steps(Piece& p, const RowSplit& s, uint64_t x, uint32_t c, Job& job) {
+    const uint32_t up = (1u << s.log2_cost) - 1;
+    const uint64_t stop = p.x1 < x + c ? p.x1 : x + c;
+    const uint32_t from = (uint32_t)(p.x - x), to = (uint32_t)(stop - x);
+    job.s0 = (int)((from > (uint32_t)s.lead ? from - s.lead + up : 0u) >> s.log2_cost);
+    job.s1 = (int)((to > (uint32_t)s.lead ? to - s.lead + up : 0u) >> s.log2_cost);
+    p.x = stop;
+    return x + s.lead >= p.x0 && x + c - (up + 1) < p.x0 + p.per;
+}
+
 template <class S>
-__device__ __forceinline__ Line build_line(const AttnArgs& a, uint64_t* cost, uint32_t* info, S& sh) {
+__device__ __forceinline__ void keep_seq(const AttnArgs& a, S& sh, int s, const Seq& q) {
+    if (s < kSeqs) {
+        sh.start[s] = a.starts ? a.starts[s] : s;
+        sh.end[s] = q.q0 + q.n;
+        sh.upto[s] = upto_of(q, -q.q0);
+    }
+}
+
+// (of a sequence without new tokens: more than any)
+__device__ __forceinline__ int least_upto_of(const Seq& q) { return q.n ? upto_of(q, 0) : 1 << 30; }
+
+__device__ __forceinline__ void set_prefix(const AttnArgs& a, Line& line, int least_upto) {
+    if (!a.plan.prefix_entries) return;
+    line.prefix_tiles = prefix_tiles(a, least_upto);
+    line.prefix_cost = entry_cost(a.plan.prefix, line.prefix_tiles.steps(a.plan.prefix));
+}
+
+// The own line of up to 64 sequences with a row tile each: sequence s in lane
+// s, kept in LDS, where all waves write the same.  False: one has more rows.
+template <class S>
+__device__ __forceinline__ bool line_in_lanes(const AttnArgs& a, S& sh, Line& line) {
+    const int lane = threadIdx.x & 63;
+    const AttnPlan& p = a.plan;
+    const bool on = lane < a.n_seqs;
+    Seq q = {0, 0, 0};
+    if (on) q = seq_at(a, lane);
+    if (__any(q.n * a.group > 1 << p.own.log2_rows)) return false;
+    line.plain = !a.window && !__any(q.length < q.n);
+    int least = 1 << 30;
+    if (p.prefix_entries && !line.plain) {
+        if (a.window) least = lane_min(least_upto_of(q), 1 << 30);
+        if (on) keep_seq(a, sh, lane, q);
+        __syncthreads();
+    }
+    set_prefix(a, line, least);
+    const uint32_t mine = q.n ? entry_cost(p.own, own_tiles(a, q, 0).steps(p.own)) : 0u;
+    const uint32_t upto = (uint32_t)lane_scan((int)mine, 0, [](int x, int y) { return x + y; });
+    sh.lane_line[0][lane] = on ? upto - mine : 0x7fffffffu;
+    sh.lane_line[1][lane] = mine;
+    sh.lane_line[2][lane] = q.q0;
+    sh.lane_line[3][lane] = q.n;
+    sh.lane_line[4][lane] = q.length;
+    line.head_cost = (uint32_t)__builtin_amdgcn_readlane((int)upto, 63);
+    line.own_entries = a.n_seqs;
+    return true;
+}
+
+// The own line of any batch: cost[0..entries] (cost before an entry) and
+// info[entry] (sequence << 16 | row tile) in LDS.
+template <class S>
+__device__ __forceinline__ void line_in_lds(const AttnArgs& a, uint64_t* cost, uint32_t* info, S& sh, Line& line,
+                                            bool writes) {
     uint64_t* const scratch = sh.scratch;
     const int tid = threadIdx.x;
     const AttnPlan& p = a.plan;
     int* const meta_first = reinterpret_cast<int*>(a.meta + meta_first_at());
-    uint64_t* const meta_cost = reinterpret_cast<uint64_t*>(a.meta + meta_cost_at(a.n_seqs));
-    Line line;
-    line.min_pos = 0;
-    int base = p.prefix_entries;
-    uint32_t back = 0;  // new tokens that reach furthest before their sequence's end
+    int base = 0, least = 1 << 30;
     for (int s0 = 0; s0 < a.n_seqs; s0 += kThreads) {
         const int s = s0 + tid;
         uint32_t n = 0;
         if (s < a.n_seqs) {
             const Seq q = seq_at(a, s);
-            n = (uint32_t)((q.n * a.group + p.own.rows - 1) / p.own.rows);
-            const int before = q.n - q.length;  // (> -2^31: the earliest position is prefix_len - this)
-            const uint32_t b = (uint32_t)(before + 0x40000000);
-            if (q.n && b > back) back = b;
-            if (s < kSeqs) {
-                sh.start[s] = a.starts ? a.starts[s] : s;
-                sh.end[s] = q.q0 + q.n;
-                sh.ahead[s] = q.length - q.n - q.q0;
-            }
+            n = (uint32_t)((q.n * a.group + (1 << p.own.log2_rows) - 1) >> p.own.log2_rows);
+            least = least_upto_of(q) < least ? least_upto_of(q) : least;
+            keep_seq(a, sh, s, q);
         }
         uint32_t total;
         const uint32_t at = base + block_scan<uint32_t>(n, reinterpret_cast<uint32_t*>(scratch), total) - n;
-        for (uint32_t r = 0; r < n && at + r < (uint32_t)p.max_entries; ++r) info[at + r] = (uint32_t)s << 16 | r;
-        if (blockIdx.x == 0 && s < a.n_seqs) meta_first[s] = (int)at;
+        for (uint32_t r = 0; r < n && at + r < (uint32_t)p.own_entries; ++r) info[at + r] = (uint32_t)s << 16 | r;
+        if (writes && s < a.n_seqs) meta_first[s] = (int)at;
         base += (int)total;
     }
-    line.entries = base < p.max_entries ? base : p.max_entries;
-    if (a.window && p.prefix_entries) {
-#pragma unroll
-        for (int o = 1; o < 64; o *= 2) {
-            const uint32_t other = (uint32_t)__shfl_xor((int)back, o);
-            back = other > back ? other : back;
-        }
-        uint32_t* const top = reinterpret_cast<uint32_t*>(scratch);
+    const int entries = base < p.own_entries ? base : p.own_entries;
+    line.plain = false;
+    if (p.prefix_entries && a.window) {
+        least = lane_min(least, 1 << 30);
+        int* const top = reinterpret_cast<int*>(scratch);
         __syncthreads();
-        if ((tid & 63) == 0) top[tid >> 6] = back;
+        if ((tid & 63) == 0) top[tid >> 6] = least;
         __syncthreads();
 #pragma unroll
-        for (int w = 0; w < kWaves; ++w) back = top[w] > back ? top[w] : back;
-        line.min_pos = back ? (int64_t)a.prefix_len - ((int64_t)back - 0x40000000) : a.prefix_len;
+        for (int w = 0; w < kWaves; ++w) least = top[w] < least ? top[w] : least;
+        least = uniform(least);
     }
+    set_prefix(a, line, least);
     __syncthreads();
     uint64_t sum = 0;
-    for (int e0 = 0; e0 < line.entries; e0 += kThreads) {
+    for (int e0 = 0; e0 < entries; e0 += kThreads) {
         const int e = e0 + tid;
         uint64_t c = 0;
-        if (e < p.prefix_entries) {
-            const int step = p.prefix.step();
-            c = (uint64_t)((prefix_tiles(a, line.min_pos).count() + step - 1) / step) * p.prefix.cost;
-        } else if (e < line.entries) {
-            const int step = p.own.step();
-            const Seq q = seq_at(a, (int)(info[e] >> 16));
-            c = (uint64_t)((own_tiles(a, q, (int)(info[e] & 0xffff)).count() + step - 1) / step) * p.own.cost;
-        }
+        if (e < entries)
+            c = entry_cost(p.own, own_tiles(a, seq_at(a, (int)(info[e] >> 16)), (int)(info[e] & 0xffff)).steps(p.own));
         uint64_t total;
         const uint64_t at = sum + block_scan<uint64_t>(c, scratch, total) - c;
-        if (e < line.entries) {
-            cost[e] = at;
-            if (blockIdx.x == 0) meta_cost[e] = at;
-        }
+        if (e < entries) cost[e] = at;
         sum += total;
     }
-    if (tid == 0) cost[line.entries] = sum;
-    line.head_cost = sum;
-    const uint64_t all = sum * (uint64_t)a.kv_heads;
-    uint64_t per = quotient(all + p.workgroups - 1, p.workgroups);
-    const uint64_t least = p.prefix.cost > p.own.cost ? p.prefix.cost : p.own.cost;  // a piece has a step of any unit
-    line.per = per < least ? least : per;
-    if (blockIdx.x == 0 && tid == 0) {
-        meta_cost[line.entries] = sum;
-        MetaHead* m = reinterpret_cast<MetaHead*>(a.meta);
-        m->head_cost = sum;
-        m->per = line.per;
-        m->entries = line.entries;
-    }
+    if (tid == 0) cost[entries] = sum;
+    line.head_cost = uniform(sum);
+    line.own_entries = uniform(entries);
     __syncthreads();
-    line.head_cost = uniform(line.head_cost);
-    line.per = uniform(line.per);
-    line.min_pos = uniform(line.min_pos);
-    line.entries = uniform(line.entries);
+}
+
+template <class S>
+__device__ __forceinline__ Line build_line(const AttnArgs& a, uint64_t* cost, uint32_t* info, S& sh) {
+    const AttnPlan& p = a.plan;
+    const int grid = 1 << p.log2_workgroups;
+    // Pieces follow each other by XCD (workgroup b runs on XCD b % 8), so that
+    // the row tiles of one kv head, which read the same keys, share an L2.
+    const int w = (int)((blockIdx.x & 7) << (p.log2_workgroups - 3) | blockIdx.x >> 3);
+    const bool writes = w == grid / 2;  // (in a small launch without a piece of its own)
+    Line line;
+    line.prefix_cost = 0;
+    line.prefix_tiles = {0, 0, 0};
+    line.lanes = p.lanes && line_in_lanes(a, sh, line);
+    if (!line.lanes) line_in_lds(a, cost, info, sh, line, writes);
+    // the own line from the other end, so that in a small launch a workgroup has a piece of one line only
+    line.prefix = piece_of((uint64_t)line.prefix_cost * (uint64_t)(p.prefix_entries * a.kv_heads), p.log2_workgroups, w,
+                           p.prefix, 0);
+    // (next to a long piece of the prefix, a piece of up to four steps rather than more parts to join)
+    const uint64_t beside = line.prefix.per >> 2, most = 4u << p.own.log2_cost;
+    line.own = piece_of(line.head_cost * (uint64_t)a.kv_heads, p.log2_workgroups + (p.own.shared ? 0 : 2),
+                        p.own.shared ? grid - 1 - w : (grid - 1 - w) * kWaves + uniform((int)(threadIdx.x >> 6)), p.own,
+                        !p.prefix_entries ? 0 : beside < most ? beside : most);
+    if (writes) {  // for the join
+        Pieces* const pieces = reinterpret_cast<Pieces*>(a.meta + meta_pieces_at(a.n_seqs));
+        if (threadIdx.x == 0) *reinterpret_cast<MetaHead*>(a.meta) = MetaHead{line.own_entries, line.lanes};
+        const int entries = p.prefix_entries + line.own_entries;
+        for (int h = threadIdx.x >> 6; h < a.kv_heads; h += kWaves)
+            for (int i = threadIdx.x & 63; i < entries; i += 64) {
+                Pieces c;
+                if (i < p.prefix_entries) {
+                    const int unit = h * p.prefix_entries + i;
+                    c = pieces_of(line, line.prefix.per, p.prefix, unit * (uint64_t)line.prefix_cost, line.prefix_cost,
+                                  unit);
+                } else {
+                    const int e = i - p.prefix_entries;
+                    const uint64_t e0 = line.lanes ? (uint64_t)(uint32_t)sh.lane_line[0][e & 63] : cost[e];
+                    const uint32_t c0 = line.lanes ? (uint32_t)sh.lane_line[1][e & 63] : (uint32_t)(cost[e + 1] - e0);
+                    c = pieces_of(line, line.own.per, p.own, h * line.head_cost + e0, c0, h * line.own_entries + e);
+                }
+                pieces[h * entries + i] = c;
+            }
+    }
     return line;
+}
+
+// The next unit of the piece of the prefix; false when there is none.
+__device__ __forceinline__ bool next_prefix(const AttnArgs& a, Line& line, Job& job, int dim) {
+    Piece& p = line.prefix;
+    if (p.x >= p.x1) return false;
+    const int unit = (int)line_quotient(line, p.x, line.prefix_cost), n = a.plan.prefix_entries;
+    job.h = n > 1 ? (int)quotient((uint32_t)unit, (uint32_t)n) : unit;
+    job.seq = 0;
+    job.tile = unit - job.h * n;
+    job.sq = {0, a.n_tokens, a.prefix_len};
+    job.tiles = line.prefix_tiles;
+    take_steps(p, a.plan.prefix, unit * (uint64_t)line.prefix_cost, line.prefix_cost, job);
+    job.part = a.part + (uint64_t)(p.place + unit) * slot_floats(1 << a.plan.prefix.log2_rows, dim);
+    return true;
+}
+
+// The next unit of the piece of the sequences' own tokens; false when there is none.
+template <class S>
+__device__ __forceinline__ bool next_own(const AttnArgs& a, Line& line, const uint64_t* cost, const uint32_t* info,
+                                         const S& sh, Job& job, int dim) {
+    Piece& p = line.own;
+    if (p.x >= p.x1) return false;
+    uint64_t x;  // where the entry begins
+    uint32_t c;
+    int e;
+    job.h = (int)line_quotient(line, p.x, line.head_cost);
+    const uint64_t head0 = job.h * line.head_cost, at = p.x - head0;
+    if (line.lanes) {
+        const int lane = threadIdx.x & 63;
+        const int first = sh.lane_line[0][lane], mine = sh.lane_line[1][lane];
+        const int q0 = sh.lane_line[2][lane], n = sh.lane_line[3][lane], length = sh.lane_line[4][lane];
+        e = 63 - __builtin_clzll(__ballot(first <= (int)at));
+        x = head0 + (uint32_t)__builtin_amdgcn_readlane(first, e);
+        c = (uint32_t)__builtin_amdgcn_readlane(mine, e);
+        job.sq = {__builtin_amdgcn_readlane(q0, e), __builtin_amdgcn_readlane(n, e),
+                  __builtin_amdgcn_readlane(length, e)};
+        job.seq = e;
+        job.tile = 0;
+    } else {
+        int lo = 0, hi = line.own_entries;  // the entry: cost[lo] <= at < cost[lo + 1]
+        while (hi - lo > 1) {
+            const int mid = (lo + hi) / 2;
+            if (cost[mid] <= at) lo = mid;
+            else hi = mid;
+        }
+        e = uniform(lo);
+        x = uniform(cost[e]);
+        c = (uint32_t)uniform((int)(cost[e + 1] - x));
+        x += head0;
+        const uint32_t who = (uint32_t)uniform((int)info[e]);
+        job.seq = (int)(who >> 16);
+        job.tile = (int)(who & 0xffff);
+        const Seq q = seq_at(a, job.seq);
+        job.sq = {uniform(q.q0), uniform(q.n), uniform(q.length)};
+    }
+    job.tiles = own_tiles(a, job.sq, job.tile);
+    const bool alone = take_steps(p, a.plan.own, x, c, job) && !a.plan.prefix_entries;
+    job.part = alone ? nullptr
+                     : a.own_part + (uint64_t)(p.place + job.h * line.own_entries + e) *
+                                        slot_floats(1 << a.plan.own.log2_rows, dim);
+    return true;
 }
 
 // ---- a row's result ------------------------------------------------------------------------------------------------
 
-__device__ __forceinline__ float load1(const HeadsView& v, int64_t at) {
-    if (v.dtype == QW35_HIP_DTYPE_F32) return static_cast<const float*>(v.data)[at];
-    if (v.dtype == QW35_HIP_DTYPE_F16) return (float)static_cast<const _Float16*>(v.data)[at];
-    return (float)static_cast<const __bf16*>(v.data)[at];
-}
-
-// N (4, 2 or 1) consecutive columns from `col`, gated, in the output's type.
-template <int N>
-__device__ __forceinline__ void finish(const AttnArgs& a, int t, int head, int col, float (&v)[N]) {
+// K groups of N (4, 2 or 1) consecutive columns, from `col` on and `stride`
+// apart, gated, in the output's type.
+template <int K, int N>
+__device__ __forceinline__ void finish(const AttnArgs& a, int t, int head, int col, int stride, float (&v)[K][N]) {
     if (a.gate.data) {
         const int64_t at = t * a.gate.token_stride + head * a.gate.head_stride + col;
-        float g[N];
-        bool done = false;
-        if constexpr (N > 1) {
-            if (a.gate.vec && a.gate.dtype == QW35_HIP_DTYPE_F32) {
-                typedef float vec_t __attribute__((ext_vector_type(N)));
-                const vec_t w = *reinterpret_cast<const vec_t*>(static_cast<const float*>(a.gate.data) + at);
+        float g[K][N];
+        auto get = [&](auto zero) {
+            typedef decltype(zero) T;
+            typedef T vec_t __attribute__((ext_vector_type(N > 1 ? N : 2)));
+            const T* const from = static_cast<const T*>(a.gate.data) + at;
+            if (N > 1 && a.gate.vec) {
+                vec_t w[K];
 #pragma unroll
-                for (int j = 0; j < N; ++j) g[j] = w[j];
-                done = true;
+                for (int k = 0; k < K; ++k) w[k] = *reinterpret_cast<const vec_t*>(from + k * stride);
+#pragma unroll
+                for (int k = 0; k < K; ++k)
+#pragma unroll
+                    for (int j = 0; j < N; ++j) g[k][j] = (float)w[k][j];
+            } else {
+#pragma unroll
+                for (int k = 0; k < K; ++k)
+#pragma unroll
+                    for (int j = 0; j < N; ++j) g[k][j] = (float)from[k * stride + j];
             }
-        }
-        if (!done) {
+        };
+        if (a.gate.dtype == QW35_HIP_DTYPE_F32) get(0.0f);
+        else if (a.gate.dtype == QW35_HIP_DTYPE_F16) get((_Float16)0.0f);
+        else get((__bf16)0.0f);
 #pragma unroll
-            for (int j = 0; j < N; ++j) g[j] = load1(a.gate, at + j);
-        }
+        for (int k = 0; k < K; ++k)
 #pragma unroll
-        for (int j = 0; j < N; ++j) v[j] /= 1.0f + __expf(-g[j]);
+            for (int j = 0; j < N; ++j) v[k][j] /= 1.0f + __expf(-g[k][j]);
     }
     const int64_t at = t * a.out.token_stride + head * a.out.head_stride + col;
     auto put = [&](auto zero) {
         typedef decltype(zero) T;
-        T* p = static_cast<T*>(a.out.data) + at;
-        if (a.out.vec && N > 1) {
-            typedef T vec_t __attribute__((ext_vector_type(N > 1 ? N : 2)));
-            vec_t w;
+        typedef T vec_t __attribute__((ext_vector_type(N > 1 ? N : 2)));
+        T* const to = static_cast<T*>(a.out.data) + at;
 #pragma unroll
-            for (int j = 0; j < N; ++j) w[j] = (T)v[j];
-            *reinterpret_cast<vec_t*>(p) = w;
-        } else {
+        for (int k = 0; k < K; ++k) {
+            if (N > 1 && a.out.vec) {
+                vec_t w;
 #pragma unroll
-            for (int j = 0; j < N; ++j) p[j] = (T)v[j];
+                for (int j = 0; j < N; ++j) w[j] = (T)v[k][j];
+                *reinterpret_cast<vec_t*>(to + k * stride) = w;
+            } else {
+#pragma unroll
+                for (int j = 0; j < N; ++j) to[k * stride + j] = (T)v[k][j];
+            }
         }
     };
     if (a.out.dtype == QW35_HIP_DTYPE_F32) put(0.0f);
@@ -400,7 +639,7 @@ __device__ __forceinline__ void finish(const AttnArgs& a, int t, int head, int c
 
 // ---- the kernel ----------------------------------------------------------------------------------------------------
 
-// Lanes l and l ^ 32: both values, in either.  (Elements of the builtin's
+// Lanes l and l ^ 32 (l ^ 16): both values, in either.  (Elements of the builtin's
 // result are copied before their bits are read as a float: a
 // __builtin_bit_cast of an element itself reads element 0.)
 struct Pair {
@@ -412,21 +651,38 @@ __device__ __forceinline__ Pair pair_xor32(float v) {
     const uint32_t a = p[0], b = p[1];
     return {__builtin_bit_cast(float, a), __builtin_bit_cast(float, b)};
 }
-// Over the two lanes of a row.
+__device__ __forceinline__ Pair pair_xor16(float v) {
+    const uint32_t u = __builtin_bit_cast(uint32_t, v);
+    const auto p = __builtin_amdgcn_permlane16_swap(u, u, false, false);
+    const uint32_t a = p[0], b = p[1];
+    return {__builtin_bit_cast(float, a), __builtin_bit_cast(float, b)};
+}
+// Over the lanes of a row: l, l ^ 32 and, of 16 rows, l ^ 16.
+template <int kRows>
 __device__ __forceinline__ float row_max(float v) {
+    if constexpr (kRows == 16) {
+        const Pair q = pair_xor16(v);
+        v = fmaxf(q.a, q.b);
+    }
     const Pair p = pair_xor32(v);
     return fmaxf(p.a, p.b);
 }
+template <int kRows>
 __device__ __forceinline__ float row_sum(float v) {
+    if constexpr (kRows == 16) {
+        const Pair q = pair_xor16(v);
+        v = q.a + q.b;
+    }
     const Pair p = pair_xor32(v);
     return p.a + p.b;
 }
 
 // v *= f in v's own registers (the compiler's products would go to others,
 // with a copy of every accumulator where the paths meet).
-__device__ __forceinline__ void scale_in_place(acc_t& v, float f) {
+template <class Acc>
+__device__ __forceinline__ void scale_in_place(Acc& v, float f) {
 #pragma unroll
-    for (int i = 0; i < 16; ++i) {
+    for (int i = 0; i < (int)(sizeof(Acc) / 4); ++i) {
         float x = v[i];
         asm("v_mul_f32 %0, %1, %0" : "+v"(x) : "v"(f));
         v[i] = x;
@@ -436,7 +692,8 @@ __device__ __forceinline__ void scale_in_place(acc_t& v, float f) {
 // A part of a row whose exponents count from m, seen from the largest `top` of several: exp2(m - top), 0 for a part
 // with nothing.
 __device__ __forceinline__ float part_weight(float m, float top) {
-    return m == -__builtin_inff() ? 0.0f : __builtin_amdgcn_exp2f(m - top);
+    // (never zero otherwise: an infinity in a part that hardly counts stays one)
+    return m == -__builtin_inff() ? 0.0f : fmaxf(__builtin_amdgcn_exp2f(m - top), 1e-37f);
 }
 
 // Waits until at most n of this wave's vector memory operations are in flight.
@@ -476,11 +733,12 @@ struct Shared {
     float m[kWaves][32];
     float l[kWaves][32];
     Limits all[kWaves];
-    // of the first sequences, for the rows of the prefix: starts[s], the end of its new tokens, and a new token's
-    // position less its index and prefix_len
-    int start[kSeqs], end[kSeqs], ahead[kSeqs];
+    // of the first sequences, for the rows of the prefix: starts[s], the end of its new tokens, and how many own
+    // tokens a new one sees, less its index
+    int start[kSeqs], end[kSeqs], upto[kSeqs];
     uint32_t marks[kWaves][32 * D / 16];
     uint64_t scratch[kWaves];
+    int lane_line[5][64];  // of a line in lanes: cost before, cost, and q0, n, length
 };
 
 // Raw granules of a tile: 16 bytes of a 16-bit cache, 8 of an e4m3 one.
@@ -493,12 +751,21 @@ __device__ __forceinline__ typename E::vec8 operand(raw8<F8> w) {
     else return __builtin_bit_cast(typename E::vec8, w);
 }
 
-template <int D, class E, bool F8>
+// kRows: rows of a wave's tile, 16 or 32.
+template <int D, class E, bool F8, int kRows>
 struct Unit {
     typedef typename E::vec8 vec8;
     typedef raw8<F8> raw;
-    static constexpr int kM = D / 16;  // contraction steps of a score
-    static constexpr int kT = D / 32;  // 32-column tiles of the output
+    typedef std::conditional_t<kRows == 32, acc_t, float4_t> acc;  // of a matrix instruction
+    static constexpr int kAcc = sizeof(acc) / 4;
+    static constexpr int kGroups = 64 / kRows;      // lanes of a row
+    static constexpr int kM = D / (8 * kGroups);    // contraction steps of a score
+    static constexpr int kB = 32 / kRows;           // matrix tiles of the scores
+    static constexpr int kT = D / kRows;            // column tiles of the output
+    static constexpr int kK = 4 / kGroups;          // token steps of the output
+    static constexpr int kScores = kB * kAcc;       // of a lane
+    static constexpr int kQuads = kT * kAcc / 4;    // 4-column groups of the output in a lane: group i holds columns
+    static constexpr int kQuadCols = 4 * kGroups;   // kQuadCols i + 4 g ..
     static constexpr int kElem = F8 ? 1 : 2;
     static constexpr int kTile = 32 * D * kElem;  // bytes of a tile's keys, and of its values
     static constexpr int kKb = kTile / 1024;
@@ -510,17 +777,17 @@ struct Unit {
 
     const AttnArgs& a;
     Shared<D>& sh;
-    const int lane, wave, n, g;  // this lane's row of a 32-row tile, and its half
+    const int lane, wave, n, g;  // this lane's row of a tile, and which of the row's lanes it is
 
     __device__ Unit(const AttnArgs& a_, Shared<D>& sh_)
         : a(a_), sh(sh_), lane(threadIdx.x & 63), wave(__builtin_amdgcn_readfirstlane(threadIdx.x >> 6)),
-          n(threadIdx.x & 31), g((threadIdx.x & 63) >> 5) {}
+          n(threadIdx.x & (kRows - 1)), g((threadIdx.x & 63) / kRows) {}
 
     // What a wave carries through its tiles.
     template <int R>
     struct Rows {
         vec8 q[R][kM];
-        acc_t o[R][kT];
+        acc o[R][kT];
         float mx[R], l[R];
         Limits lim[R];
         int all_lo, all_hi, all_sink;  // what every row of the wave sees
@@ -528,32 +795,37 @@ struct Unit {
         bool marked;  // infinities to add at the end
     };
 
-    // The granule of step m / of column tile t and token step kk.
-    __device__ __forceinline__ vec8 key(const uint8_t* tile, int m) const {
-        // row i of the product is token i with bits 2 and 3 exchanged
-        const int tok = (n & 19) | (n & 4) << 1 | (n & 8) >> 1;
-        return operand<E, F8>(*reinterpret_cast<const raw*>(tile + ((2 * m + g) * 32 + tok) * 8 * kElem));
+    // The granule of step m for score tile b / of column tile t and token step kk.
+    __device__ __forceinline__ vec8 key(const uint8_t* tile, int m, int b) const {
+        // which token is row n of the product: token(j) of the lane that gets it
+        const int tok = kRows == 32 ? (n & 19) | (n & 4) << 1 | (n & 8) >> 1 : (n >> 2) * 8 + b * 4 + (n & 3);
+        return operand<E, F8>(*reinterpret_cast<const raw*>(tile + ((kGroups * m + g) * 32 + tok) * 8 * kElem));
     }
     __device__ __forceinline__ vec8 value(const uint8_t* tile, int t, int kk) const {
-        return operand<E, F8>(*reinterpret_cast<const raw*>(tile + ((2 * kk + g) * D + t * 32 + n) * 8 * kElem));
+        return operand<E, F8>(
+            *reinterpret_cast<const raw*>(tile + ((kGroups * kk + g) * D + t * kRows + n) * 8 * kElem));
     }
+    // Token of a lane's score j.
+    __device__ __forceinline__ int token(int j) const { return kRows == 32 ? (j & 8) * 2 + g * 8 + (j & 7) : g * 8 + j; }
 
     template <int R>
-    __device__ __forceinline__ void scores(const uint8_t* keys, const Rows<R>& w, acc_t (&s)[R]) const {
-        constexpr int kAhead = kM < 4 ? kM : 4;
+    __device__ __forceinline__ void scores(const uint8_t* keys, const Rows<R>& w, acc (&s)[R][kB]) const {
+        constexpr int kSteps = kM * kB, kAhead = kSteps < 4 ? kSteps : 4;
         vec8 k[kAhead];
 #pragma unroll
-        for (int m = 0; m < kAhead; ++m) k[m] = key(keys, m);
+        for (int i = 0; i < kAhead; ++i) k[i] = key(keys, i / kB, i % kB);
 #pragma unroll
-        for (int r = 0; r < R; ++r) s[r] = acc_t{};
+        for (int r = 0; r < R; ++r)
 #pragma unroll
-        for (int m = 0; m < kM; ++m) {
-            const vec8 kk = k[m % kAhead];
-            if (m + kAhead < kM) k[m % kAhead] = key(keys, m + kAhead);
+            for (int b = 0; b < kB; ++b) s[r][b] = acc{};
 #pragma unroll
-            for (int r = 0; r < R; ++r) s[r] = E::mfma(kk, w.q[r][m], s[r]);
+        for (int i = 0; i < kSteps; ++i) {
+            const vec8 kk = k[i % kAhead];
+            if (i + kAhead < kSteps) k[i % kAhead] = key(keys, (i + kAhead) / kB, (i + kAhead) % kB);
+#pragma unroll
+            for (int r = 0; r < R; ++r) s[r][i % kB] = E::mfma(kk, w.q[r][i / kB], s[r][i % kB]);
         }
-        interleave<kM, R, kAhead>();
+        interleave<kSteps, R, kAhead>();
     }
 
     // LDS reads kAhead ahead of the matrix instructions that take them.
@@ -570,19 +842,22 @@ struct Unit {
 
     // Softmax of a tile's scores: its terms to p, the running reference, sum and output kept.
     template <int R>
-    __device__ __forceinline__ void softmax(Rows<R>& w, acc_t (&s)[R], int t0, bool masked, bool there,
-                                            vec8 (&p)[R][2]) const {
+    __device__ __forceinline__ void softmax(Rows<R>& w, acc (&s)[R][kB], int t0, bool masked, bool there,
+                                            vec8 (&p)[R][kK]) const {
 #pragma unroll
         for (int r = 0; r < R; ++r) {
+            float x[kScores];
+#pragma unroll
+            for (int j = 0; j < kScores; ++j) x[j] = s[r][j / kAcc][j % kAcc];
             if (masked) {
 #pragma unroll
-                for (int j = 0; j < 16; ++j)
-                    s[r][j] = sees(w.lim[r], t0 + token(j), there) ? s[r][j] : -__builtin_inff();
+                for (int j = 0; j < kScores; ++j)
+                    x[j] = sees(w.lim[r], t0 + token(j), there) ? x[j] : -__builtin_inff();
             }
-            float top = s[r][0];
+            float top = x[0];
 #pragma unroll
-            for (int j = 1; j < 16; ++j) top = fmaxf(top, s[r][j]);
-            top = row_max(top) * w.scale;
+            for (int j = 1; j < kScores; ++j) top = fmaxf(top, x[j]);
+            top = row_max<kRows>(top) * w.scale;
             if (__builtin_expect(__any(top > w.mx[r] + kRise), 0)) {
                 const float m_new = fmaxf(w.mx[r], top);
                 const float shrink = m_new == w.mx[r] ? 1.0f : __builtin_amdgcn_exp2f(w.mx[r] - m_new);
@@ -593,8 +868,8 @@ struct Unit {
             }
             const float ref = w.mx[r] == -__builtin_inff() ? 0.0f : w.mx[r];
 #pragma unroll
-            for (int j = 0; j < 16; ++j) {
-                const float e = __builtin_amdgcn_exp2f(fmaf(s[r][j], w.scale, -ref));
+            for (int j = 0; j < kScores; ++j) {
+                const float e = __builtin_amdgcn_exp2f(fmaf(x[j], w.scale, -ref));
                 w.l[r] += e;
                 p[r][j / 8][j % 8] = (typename E::elem)e;
             }
@@ -602,17 +877,17 @@ struct Unit {
     }
 
     template <int R>
-    __device__ __forceinline__ void add_values(const uint8_t* values, Rows<R>& w, const vec8 (&p)[R][2]) const {
-        constexpr int kSteps = 2 * kT, kAhead = kSteps < 4 ? kSteps : 4;
+    __device__ __forceinline__ void add_values(const uint8_t* values, Rows<R>& w, const vec8 (&p)[R][kK]) const {
+        constexpr int kSteps = kK * kT, kAhead = kSteps < 4 ? kSteps : 4;
         vec8 v[kAhead];
 #pragma unroll
-        for (int i = 0; i < kAhead; ++i) v[i] = value(values, i / 2, i % 2);
+        for (int i = 0; i < kAhead; ++i) v[i] = value(values, i / kK, i % kK);
 #pragma unroll
         for (int i = 0; i < kSteps; ++i) {
             const vec8 vv = v[i % kAhead];
-            if (i + kAhead < kSteps) v[i % kAhead] = value(values, (i + kAhead) / 2, i % 2);
+            if (i + kAhead < kSteps) v[i % kAhead] = value(values, (i + kAhead) / kK, (i + kAhead) % kK);
 #pragma unroll
-            for (int r = 0; r < R; ++r) w.o[r][i / 2] = E::mfma(vv, p[r][i % 2], w.o[r][i / 2]);
+            for (int r = 0; r < R; ++r) w.o[r][i / kK] = E::mfma(vv, p[r][i % kK], w.o[r][i / kK]);
         }
         interleave<kSteps, R, kAhead>();
     }
@@ -629,24 +904,100 @@ struct Unit {
         if (kShared) __syncthreads();
     }
 
-    // Every step-th granule from `first` on, without its infinities and NaN.
+    // 1 KB (512 bytes of e4m3) i of a tile's values, this lane's granule.
+    static constexpr int kParts = D / 16;
+    __device__ __forceinline__ uint8_t* granule(uint8_t* tile, int i) const { return tile + (i * 64 + lane) * 8 * kElem; }
+
+    // Whether the tile of values holds an infinity or a NaN.
+    __device__ __forceinline__ bool not_finite(uint8_t* tile) const {
+        typedef short bits_t __attribute__((ext_vector_type(8)));
+        bits_t top = {};
+#pragma unroll 4
+        for (int i = 0; i < kParts; ++i)
+            top = __builtin_elementwise_max(
+                top, __builtin_bit_cast(bits_t, operand<E, F8>(*reinterpret_cast<const raw*>(granule(tile, i)))) &
+                         (short)0x7fff);
+        bool bad = false;
+#pragma unroll
+        for (int j = 0; j < 8; ++j) bad |= top[j] >= E::kInf;
+        return bad;
+    }
+
+    // Every step-th part from `first` on, without its infinities and NaN.
     __device__ __forceinline__ void make_finite(uint8_t* tile, int first, int step) const {
 #pragma unroll 1
-        for (int i = first; i < 2 * kT; i += step) {
-            uint8_t* const at = tile + ((2 * (i & 1) + g) * D + (i >> 1) * 32 + n) * 8 * kElem;
+        for (int i = first; i < kParts; i += step) {
             typedef std::conditional_t<F8, uint8_t, short> part_t;
             typedef part_t bits_t __attribute__((ext_vector_type(8)));
-            bits_t v = *reinterpret_cast<const bits_t*>(at);
+            bits_t v = *reinterpret_cast<const bits_t*>(granule(tile, i));
             constexpr part_t kSize = F8 ? 0x7f : 0x7fff, kFirst = F8 ? 0x7f : E::kInf;  // (e4m3 has a NaN, no infinities)
 #pragma unroll
             for (int j = 0; j < 8; ++j) v[j] = (v[j] & kSize) >= kFirst ? part_t(0) : v[j];
-            *reinterpret_cast<bits_t*>(at) = v;
+            *reinterpret_cast<bits_t*>(granule(tile, i)) = v;
         }
         wait_lds();
     }
 
-    // Token of a lane's score j.
-    __device__ __forceinline__ int token(int j) const { return (j & 8) * 2 + g * 8 + (j & 7); }
+    // For a tile with infinities or NaN among its values of which some rows
+    // see only a part: what a row does not see must not reach it even as
+    // 0 x NaN, which the matrix instruction would add.  The product takes the
+    // finite values; which infinities (a NaN is both) a row saw in which column
+    // is kept, a bit each, and added when the unit's tiles are done.
+    //   marks: [r][t][sign][kRows], bits of the tile's kRows columns; a lane
+    // keeps sign g % 2 of row n.  (No branch here or in the tile loop depends on
+    // the lane: the paths would keep copies of the accumulators where they meet.)
+    template <int R>
+    __device__ __forceinline__ void mark_infinities(const uint8_t* tile, Rows<R>& w, int t0, bool there,
+                                                    uint32_t* marks) const {
+        const int mine = (g & 1) * kRows + n;
+        if (!w.marked) {
+            w.marked = true;
+#pragma unroll 1
+            for (int i = 0; i < R * kT; ++i) marks[i * 2 * kRows + mine] = 0;
+        }
+#pragma unroll 1
+        for (int i = 0; i < kK * kT; ++i) {
+            const int t = i / kK, kk = i % kK;
+            typedef short bits_t __attribute__((ext_vector_type(8)));
+            bits_t v = __builtin_bit_cast(bits_t, value(tile, t, kk));
+#pragma unroll 1
+            for (int j = 0; j < 8; ++j) {
+                const short x = v[0], size = x & 0x7fff;
+                v = __builtin_shufflevector(v, v, 1, 2, 3, 4, 5, 6, 7, 0);
+                const uint64_t up = __ballot(size > E::kInf || x == E::kInf);
+                const uint64_t down = __ballot(size > E::kInf || (size == E::kInf && x < 0));
+                if ((up | down) == 0) continue;
+                uint64_t sign = g & 1 ? down : up;  // kRows columns: of token j, 8 + j ...
+                const int at = t0 + kk * 16 + j;
+#pragma unroll
+                for (int r = 0; r < R; ++r) {
+                    uint32_t see = 0;
+#pragma unroll
+                    for (int k = 0; k < kGroups; ++k)
+                        see |= sees(w.lim[r], at + 8 * k, there) ? (uint32_t)(sign >> kRows * k) : 0u;
+                    marks[(r * kT + t) * 2 * kRows + mine] |= see;
+                }
+            }
+        }
+    }
+
+    template <int R>
+    __device__ __forceinline__ void add_infinities(Rows<R>& w, const uint32_t* marks) const {
+        wait_lds();
+#pragma unroll
+        for (int r = 0; r < R; ++r)
+#pragma unroll
+            for (int t = 0; t < kT; ++t) {
+                const uint32_t up = marks[(r * kT + t) * 2 * kRows + n], down = marks[(r * kT + t) * 2 * kRows + kRows + n];
+#pragma unroll
+                for (int c = 0; c < kAcc; ++c) {
+                    const int col = (c >> 2) * 8 + g * 4 + (c & 3);
+                    const float inf = __builtin_inff();
+                    w.o[r][t][c] += (up >> col & 1 ? inf : 0.0f) - (down >> col & 1 ? inf : 0.0f);
+                }
+                __builtin_amdgcn_sched_barrier(0);
+            }
+    }
 
     template <int R>
     __device__ __forceinline__ bool partly(const Rows<R>& w, int t0, bool there) const {
@@ -662,56 +1013,59 @@ struct Unit {
         uint32_t blocks;  // lane i: the cache block of tile 64 j + i
     };
 
+    // Tiles i .. i + 63 (below the count).
+    __device__ __forceinline__ void look_up(Pages& p, int i) const {
+        const int mine = i + lane < p.count ? i + lane : p.count - 1;
+        const uint32_t b = (uint32_t)p.tiles.at(p.first + mine * p.step);
+        uint32_t pi = a.plan.page_magic ? __umulhi(b, a.plan.page_magic) : b;  // b / page_blocks, or one more
+        if ((int32_t)(b - pi * a.page_blocks) < 0) --pi;
+        const int id = p.table[pi];
+        // a page outside the cache holds nothing that a row sees
+        uint32_t block = ((uint32_t)id * (uint32_t)a.kv_heads + p.h) * a.page_blocks + (b - pi * a.page_blocks);
+        asm("" : "+v"(block));  // (a choice of two values, not of two paths)
+        p.blocks = (uint32_t)id < a.n_pages ? block : kNoBlock;
+    }
+    // Tile i, the last looked up or the first of the next 64.
     __device__ __forceinline__ uint32_t block_of(Pages& p, int i) const {
-        if ((i & 63) == 0) {
-            const int mine = i + lane < p.count ? i + lane : p.count - 1;
-            const uint32_t b = (uint32_t)p.tiles.at(p.first + mine * p.step);
-            const uint32_t pi = b / a.page_blocks;
-            const int id = p.table[pi];
-            // a page outside the cache holds nothing that a row sees
-            uint32_t block = ((uint32_t)id * (uint32_t)a.kv_heads + p.h) * a.page_blocks + (b - pi * a.page_blocks);
-            asm("" : "+v"(block));  // (a choice of two values, not of two paths)
-            p.blocks = (uint32_t)id < a.n_pages ? block : kNoBlock;
-        }
+        if (i && (i & 63) == 0) look_up(p, i);
         return (uint32_t)__builtin_amdgcn_readlane((int)p.blocks, i & 63);
     }
     static __device__ __forceinline__ int64_t bytes_at(uint32_t block) {
         return (int64_t)(block == kNoBlock ? 0u : block) * kTile;
     }
 
-    // Steps [s0, s1) of an entry for kv head h; the result to `slot`, or where
-    // this is all there is of the rows (slot < 0) to the output.  R: 32-row
-    // tiles of a wave; kShared: the waves share their tiles.
+    // A job.  R: row tiles of a wave; kShared: the waves share their tiles;
+    // by_wave: each wave has a job of its own (and meets no other in it).
     template <int R, bool kShared>
-    __device__ __forceinline__ void run(int h, bool prefix, int seq, int tile, Tiles tiles, int s0, int s1, int64_t slot) {
-        const RowSplit& split = prefix ? a.plan.prefix : a.plan.own;
-        const int rg = kShared ? wave : wave & ((1 << split.log2_rg) - 1), tg = kShared ? 0 : wave >> split.log2_rg;
-        const int step = kShared ? 1 : kWaves >> split.log2_rg;
-        Seq sq = {0, a.n_tokens, a.prefix_len};
-        if (!prefix) {
-            sq = seq_at(a, seq);
-            sq = {uniform(sq.q0), uniform(sq.n), uniform(sq.length)};
-        }
-        const int base = prefix ? 0 : a.prefix_len;
+    __device__ __forceinline__ void run(const Job& job, const RowSplit& split, bool prefix, bool by_wave, bool plain) {
+        const int rg = kShared ? wave : by_wave ? 0 : wave & ((1 << split.log2_rg) - 1);
+        const int tg = kShared || by_wave ? 0 : wave >> split.log2_rg;
+        const int step = split.step();
+        const Seq& sq = job.sq;
+        const Tiles& tiles = job.tiles;
+        const int h = job.h;
         const int row_end = sq.n * a.group;
-        const int row0 = tile * split.rows + rg * 32 * R;  // this wave's first row
+        const int row0 = (job.tile << split.log2_rows) + rg * kRows * R;  // this wave's first row
 
         // this wave's tiles: step * s0 + tg, and every step-th after it
         Pages pages;
-        pages.table = prefix ? a.prefix_pages : a.pages + (int64_t)seq * a.pages_per_seq;
+        pages.table = prefix ? a.prefix_pages : a.pages + (int64_t)job.seq * a.pages_per_seq;
         pages.tiles = tiles;
-        pages.first = s0 * step + tg;
+        pages.first = job.s0 * step + tg;
         pages.step = step;
         pages.h = h;
-        const int end = s1 * step < tiles.count() ? s1 * step : tiles.count();
-        pages.count = (kShared || row0 < row_end) && pages.first < end ? (end - pages.first + step - 1) / step : 0;
+        const int end = job.s1 * step < tiles.count() ? job.s1 * step : tiles.count();
+        pages.count =
+            (kShared || row0 < row_end) && pages.first < end ? (end - pages.first + step - 1) >> split.log2_tiles : 0;
         const uint8_t* const kbase = static_cast<const uint8_t*>(a.ck);
         const uint8_t* const vbase = static_cast<const uint8_t*>(a.cv);
 
-        __syncthreads();  // the ring is free
+        if (!by_wave) __syncthreads();  // the ring is free
+        else wait_lds();
         constexpr int kFit = kShared ? kRing / (2 * kTile) : kRing / kWaves / (2 * kTile);
-        constexpr int kMarks = R * 32 * D / 4;  // bytes of a wave's marks; shared tiles leave room for them in the ring
-        constexpr int kPairs = kFit < 4 ? kFit : 2 * kTile * 4 + kWaves * kMarks <= kRing ? 4 : 3;
+        constexpr int kMarks = R * kRows * D / 4;  // bytes of a wave's marks; shared tiles leave room in the ring
+        static_assert(kShared || kMarks <= sizeof(sh.marks[0]) || kRows == 16, "room for the marks");
+        constexpr int kPairs = kFit < 4 ? kFit : !kShared || 2 * kTile * 4 + kWaves * kMarks <= kRing ? 4 : 3;
         static_assert(!kShared || 2 * kTile * kPairs + kWaves * kMarks <= kRing, "tiles and marks fit the ring");
         uint32_t* const marks = kShared ? reinterpret_cast<uint32_t*>(sh.ring + 2 * kTile * kPairs + wave * kMarks)
                                         : sh.marks[wave];
@@ -724,15 +1078,13 @@ struct Unit {
             note(block);
             const int64_t at = bytes_at(block);
             uint8_t* const to = ring + (i % kPairs) * 2 * kTile;
-            if constexpr (kKb >= 2) {
-                const uint8_t* const from = wave < 2 ? kbase : vbase;
-                const int part = (wave & 1) * (kTile / 2);
-                copy_kb<kKb / 2>(from + at + part, to + (wave < 2 ? 0 : kTile) + part, lane);
-            }
+            const uint8_t* const from = wave < 2 ? kbase : vbase;
+            const int part = (wave & 1) * (kTile / 2);
+            copy_kb<kKb / 2>(from + at + part, to + (wave < 2 ? 0 : kTile) + part, lane);
         };
 
         Rows<R> w;
-        if (pages.count) block_of(pages, 0);
+        if (pages.count) look_up(pages, 0);
         load_queries<R>(w, sq, h, row0, row_end);
         int loaded = 0;
         if constexpr (kShared) {
@@ -746,7 +1098,7 @@ struct Unit {
                 copy_kb<kKb>(vbase + bytes_at(block), to + kTile, lane);
             }
         }
-        start_rows<R, kShared>(w, sq, prefix, base, row0, row_end);
+        start_rows<R, kShared>(w, sq, prefix, plain, row0, row_end);
         use_queries<R>(w);  // (here the queries are waited for, not in the tile loop)
 
         if constexpr (kShared) {
@@ -762,8 +1114,8 @@ struct Unit {
                 const int t0 = tiles.at(pages.first + i) * 32;
                 const bool masked = partly<R>(w, t0, there);
                 if (masked) split_off_infinities<R, true>(at + kTile, w, t0, there, marks);
-                acc_t s[R];
-                vec8 p[R][2];
+                acc s[R][kB];
+                vec8 p[R][kK];
                 scores<R>(at, w, s);
                 softmax<R>(w, s, t0, masked, there, p);
                 add_values<R>(at + kTile, w, p);
@@ -777,8 +1129,8 @@ struct Unit {
                 const bool more = loaded < pages.count;
                 const int t0 = tiles.at(pages.first + i * step) * 32;
                 const bool masked = partly<R>(w, t0, there);
-                acc_t s[R];
-                vec8 p[R][2];
+                acc s[R][kB];
+                vec8 p[R][kK];
                 if (more) wait_vm<kLater>();
                 else wait_vm<0>();
                 scores<R>(at, w, s);
@@ -802,84 +1154,107 @@ struct Unit {
         }
         if (__builtin_expect(w.marked, 0)) add_infinities<R>(w, marks);
 #pragma unroll
-        for (int r = 0; r < R; ++r) w.l[r] = row_sum(w.l[r]);
+        for (int r = 0; r < R; ++r) w.l[r] = row_sum<kRows>(w.l[r]);
 
         const float v_scale = F8 && a.v_scale ? a.v_scale[h] : 1.0f;
-        float* const part = a.part + (slot < 0 ? 0 : slot) * slot_floats(a.plan.slot_rows, D);
-        const int part_row0 = rg * 32 * R;
-        float4_t* const mine = reinterpret_cast<float4_t*>(sh.ring + wave * (kRing / kWaves)) + lane;
-        static_assert(32 * D * 4 <= kRing / kWaves, "a wave's sums of 32 rows fit its part of the ring");
-        auto leave = [&](int r) {  // 32 rows' sums, in lane order
-#pragma unroll
-            for (int t = 0; t < kT; ++t)
-#pragma unroll
-                for (int c = 0; c < 4; ++c) mine[(t * 4 + c) * 64] = quad(w.o[r][t], c);
-        };
-        if constexpr (kShared) {
-            if (slot >= 0) {
-#pragma unroll
-                for (int r = 0; r < R; ++r) {
-                    if (row0 + r * 32 + n < row_end) {
-                        float* const to = part + (int64_t)(part_row0 + r * 32 + n) * D + g * 4;
-#pragma unroll
-                        for (int t = 0; t < kT; ++t)
-#pragma unroll
-                            for (int c = 0; c < 4; ++c)
-                                *reinterpret_cast<float4_t*>(to + t * 32 + c * 8) = quad(w.o[r][t], c);
-                        if (g == 0) put_stats(part, part_row0 + r * 32 + n, w.mx[r], w.l[r]);
-                    }
-                }
-            } else {
-                __syncthreads();  // (the tiles are read)
-#pragma unroll
-                for (int r = 0; r < R; ++r) {
-                    leave(r);
-                    const int row = row0 + r * 32 + n;
-                    if (row < row_end) {
-#pragma unroll 1
-                        for (int i = 0; i < kT * 4; ++i)
-                            put(part, slot, sq.q0, row, 0, h, (i >> 2) * 32 + (i & 3) * 8 + g * 4, mine[i * 64], w.l[r],
-                                v_scale);
-                    }
-                    wait_lds();
-                }
-            }
-        } else {
-            // The waves of a row group join: each leaves its sums in LDS in
-            // lane order, then adds up every step-th of all of theirs.
-            static_assert(R == 1, "a wave of its own tiles has 32 rows");
+        static_assert(kRows * D * 4 <= kRing / kWaves, "a wave's sums of a row tile fit its part of the ring");
+        if (!kShared && !by_wave) {
+            // The waves of a row group join: each leaves its sums in LDS, then
+            // adds up every step-th group of all of theirs.
+            static_assert(kShared || R == 1, "a wave of its own tiles has one of rows");
             if (g == 0) {
                 sh.m[wave][n] = w.mx[0];
                 sh.l[wave][n] = w.l[0];
             }
-            leave(0);
+            leave<R>(w, 0);
             __syncthreads();
-            const int row = row0 + n;
-            float top = -__builtin_inff();
-            for (int v = 0; v < step; ++v) top = fmaxf(top, sh.m[rg + (v << split.log2_rg)][n]);
-            float weight[kWaves], sum = 0.0f;
+            if (split.log2_rg == 0) join_waves<4>(job, rg, tg, row0, row_end, v_scale);
+            else join_waves<2>(job, rg, tg, row0, row_end, v_scale);
+            return;
+        }
+        if (kShared && !job.part) __syncthreads();  // (the tiles are read)
 #pragma unroll
-            for (int v = 0; v < kWaves; ++v) {
-                weight[v] = 0.0f;
-                if (v < step) {
-                    weight[v] = part_weight(sh.m[rg + (v << split.log2_rg)][n], top);
-                    sum += weight[v] * sh.l[rg + (v << split.log2_rg)][n];
+        for (int r = 0; r < R; ++r) {
+            const int row = row0 + r * kRows + n, part_row = (rg * R + r) * kRows + n;
+            if (job.part) {
+                if (row < row_end) {
+                    float* const to = job.part + part_row * D + g * 4;
+#pragma unroll
+                    for (int i = 0; i < kQuads; ++i)
+                        *reinterpret_cast<float4_t*>(to + i * kQuadCols) = quad<R>(w, r, i);
+                    if (g == 0) put_stats(job.part, split, part_row, w.mx[r], w.l[r]);
                 }
-            }
-            if (row < row_end) {
+            } else {
+                leave<R>(w, r);
+                const int tok = token_of(a, row), head = h * a.group + row - tok * a.group;
+                const float inv = w.l[r] == 0.0f ? 0.0f : v_scale / w.l[r];
+                if (row < row_end) {
 #pragma unroll 1
-                for (int i = tg; i < kT * 4; i += step) {
-                    float4_t acc = {0, 0, 0, 0};
+                    for (int i = 0; i < kQuads; i += 4) {
+                        float x[4][4];
 #pragma unroll
-                    for (int v = 0; v < kWaves; ++v)
-                        if (v < step && weight[v] != 0.0f)
-                            acc += weight[v] * reinterpret_cast<const float4_t*>(
-                                                   sh.ring + (rg + (v << split.log2_rg)) * (kRing / kWaves))[i * 64 + lane];
-                    put(part, slot, sq.q0, row, part_row0 + n, h, (i >> 2) * 32 + (i & 3) * 8 + g * 4, acc, sum, v_scale);
+                        for (int c = 0; c < 4; ++c) {
+                            const float4_t y = left(wave)[(i + c) * 64 + lane];
+#pragma unroll
+                            for (int j = 0; j < 4; ++j) x[c][j] = y[j] * inv;
+                        }
+                        finish(a, sq.q0 + tok, head, i * kQuadCols + g * 4, kQuadCols, x);
+                    }
                 }
-                if (slot >= 0 && tg == 0 && g == 0) put_stats(part, part_row0 + n, top, sum);
+                wait_lds();
             }
         }
+    }
+
+    // A row tile's sums in LDS, in lane order.
+    __device__ __forceinline__ float4_t* left(int by) const {
+        return reinterpret_cast<float4_t*>(sh.ring + by * (kRing / kWaves));
+    }
+    template <int R>
+    __device__ __forceinline__ void leave(const Rows<R>& w, int r) const {
+#pragma unroll
+        for (int i = 0; i < kQuads; ++i) left(wave)[i * 64 + lane] = quad<R>(w, r, i);
+    }
+    template <int R>
+    static __device__ __forceinline__ float4_t quad(const Rows<R>& w, int r, int i) {
+        const acc& v = w.o[r][i * 4 / kAcc];
+        const int c = i * 4 % kAcc;
+        return float4_t{v[c], v[c + 1], v[c + 2], v[c + 3]};
+    }
+
+    template <int kStep>
+    __device__ __forceinline__ void join_waves(const Job& job, int rg, int tg, int row0, int row_end,
+                                               float v_scale) const {
+        constexpr int kRg = kWaves / kStep, K = kQuads / kStep;
+        float weight[kStep], top = -__builtin_inff(), sum = 0.0f;
+#pragma unroll
+        for (int v = 0; v < kStep; ++v) {
+            weight[v] = sh.m[rg + v * kRg][n];
+            top = fmaxf(top, weight[v]);
+        }
+#pragma unroll
+        for (int v = 0; v < kStep; ++v) {
+            weight[v] = part_weight(weight[v], top);
+            sum += weight[v] * sh.l[rg + v * kRg][n];
+        }
+        const int row = row0 + n;
+        if (row >= row_end) return;
+        float x[K][4];
+#pragma unroll
+        for (int k = 0; k < K; ++k) {
+            float4_t acc4 = {0, 0, 0, 0};
+#pragma unroll
+            for (int v = 0; v < kStep; ++v) acc4 += weight[v] * left(rg + v * kRg)[(tg + k * kStep) * 64 + lane];
+#pragma unroll
+            for (int j = 0; j < 4; ++j) x[k][j] = acc4[j];
+        }
+        // (a workgroup joins its waves for the prefix only: its rows have other parts too)
+        const int part_row = rg * kRows + n;
+        float* const to = job.part + part_row * D + kQuadCols * tg + 4 * g;
+#pragma unroll
+        for (int k = 0; k < K; ++k)
+            *reinterpret_cast<float4_t*>(to + k * kQuadCols * kStep) = float4_t{x[k][0], x[k][1], x[k][2], x[k][3]};
+        if (tg == 0 && g == 0) put_stats(job.part, a.plan.prefix, part_row, top, sum);
     }
 
     // This lane's queries (asked for; use_queries waits).
@@ -887,21 +1262,22 @@ struct Unit {
     __device__ __forceinline__ void load_queries(Rows<R>& w, const Seq& sq, int h, int row0, int row_end) const {
 #pragma unroll
         for (int r = 0; r < R; ++r) {
-            const int row = row0 + r * 32 + n;
+            const int row = row0 + r * kRows + n;
             const bool on = row < row_end;
-            const int t = sq.q0 + (on ? row / a.group : 0), head = h * a.group + (on ? row % a.group : 0);
+            const int tok = on ? token_of(a, row) : 0;
+            const int t = sq.q0 + tok, head = h * a.group + (on ? row - tok * a.group : 0);
             const typename E::elem* p = static_cast<const typename E::elem*>(a.q.data) + t * a.q.token_stride +
                                         head * a.q.head_stride + g * 8;
 #pragma unroll
             for (int m = 0; m < kM; ++m) w.q[r][m] = vec8{};
             if (on && a.q.vec) {
 #pragma unroll
-                for (int m = 0; m < kM; ++m) w.q[r][m] = *reinterpret_cast<const vec8*>(p + m * 16);
+                for (int m = 0; m < kM; ++m) w.q[r][m] = *reinterpret_cast<const vec8*>(p + m * 8 * kGroups);
             } else if (on) {
 #pragma unroll
                 for (int m = 0; m < kM; ++m) {
 #pragma unroll
-                    for (int j = 0; j < 8; ++j) w.q[r][m][j] = p[m * 16 + j];
+                    for (int j = 0; j < 8; ++j) w.q[r][m][j] = p[m * 8 * kGroups + j];
                     asm volatile("" ::: "memory");  // (eight loads at a time)
                 }
             }
@@ -927,38 +1303,39 @@ struct Unit {
 
     // What this lane's rows see.
     template <int R, bool kShared>
-    __device__ __forceinline__ void start_rows(Rows<R>& w, const Seq& sq, bool prefix, int base, int row0,
+    __device__ __forceinline__ void start_rows(Rows<R>& w, const Seq& sq, bool prefix, bool plain, int row0,
                                                int row_end) const {
         w.marked = false;
         w.all_lo = 0;
         w.all_hi = w.all_sink = 0x7fffffff;
 #pragma unroll
         for (int r = 0; r < R; ++r) {
-            const int row = row0 + r * 32 + n;
+            const int row = row0 + r * kRows + n;
             const bool on = row < row_end;
-            const int t = sq.q0 + (on ? row / a.group : 0);
+            const int tok = on ? token_of(a, row) : 0, t = sq.q0 + tok;
             w.lim[r] = Limits{0, 0, 0};
             if (on) {
                 if (!prefix) {
-                    w.lim[r] = limits_of(a, (int64_t)base + sq.length - sq.n + row / a.group, base, sq.length);
+                    w.lim[r] = own_limits(a, sq, upto_of(sq, tok));
+                } else if (plain) {
+                    w.lim[r].hi = a.prefix_len;
                 } else {
-                    int s, stop = 0, ahead = 0;
+                    int s, stop = 0, upto = 0;
                     if (a.n_seqs <= kSeqs) {
                         s = a.starts ? last_at(sh.start, a.n_seqs, t) : t;
                         if (s >= 0) {
                             stop = sh.end[s];
-                            ahead = sh.ahead[s];
+                            upto = sh.upto[s];
                         }
                     } else {
                         s = seq_of(a, t);
                         if (s >= 0) {
                             const Seq mine = seq_at(a, s);
                             stop = mine.q0 + mine.n;
-                            ahead = mine.length - mine.n - mine.q0;
+                            upto = upto_of(mine, -mine.q0);
                         }
                     }
-                    if (s >= 0 && t < stop)
-                        w.lim[r] = limits_of(a, (int64_t)a.prefix_len + ahead + t, 0, a.prefix_len);
+                    if (s >= 0 && t < stop) w.lim[r] = prefix_limits(a, upto + t);
                 }
                 w.all_lo = w.lim[r].lo > w.all_lo ? w.lim[r].lo : w.all_lo;
                 w.all_hi = w.lim[r].hi < w.all_hi ? w.lim[r].hi : w.all_hi;
@@ -967,18 +1344,11 @@ struct Unit {
             w.mx[r] = -__builtin_inff();
             w.l[r] = 0.0f;
 #pragma unroll
-            for (int t2 = 0; t2 < kT; ++t2) w.o[r][t2] = acc_t{};
+            for (int t2 = 0; t2 < kT; ++t2) w.o[r][t2] = acc{};
         }
-#pragma unroll
-        for (int o = 1; o < 32; o *= 2) {
-            const int lo = __shfl_xor(w.all_lo, o), hi = __shfl_xor(w.all_hi, o), sk = __shfl_xor(w.all_sink, o);
-            w.all_lo = lo > w.all_lo ? lo : w.all_lo;
-            w.all_hi = hi < w.all_hi ? hi : w.all_hi;
-            w.all_sink = sk < w.all_sink ? sk : w.all_sink;
-        }
-        w.all_lo = uniform(w.all_lo);
-        w.all_hi = uniform(w.all_hi);
-        w.all_sink = uniform(w.all_sink);
+        w.all_lo = lane_max(w.all_lo, 0);
+        w.all_hi = lane_min(w.all_hi, 0x7fffffff);
+        w.all_sink = lane_min(w.all_sink, 0x7fffffff);
         if constexpr (kShared) {
             // what every row of the workgroup sees: its waves take a tile apart together or not at all
             if (lane == 0) sh.all[wave] = Limits{w.all_lo, w.all_hi, w.all_sink};
@@ -997,158 +1367,46 @@ struct Unit {
         return there & (token < l.hi) & ((token >= l.lo) | (token < l.sink));
     }
 
-    static __device__ __forceinline__ float4_t quad(const acc_t& v, int c) {
-        return float4_t{v[4 * c], v[4 * c + 1], v[4 * c + 2], v[4 * c + 3]};
-    }
-
-    // Four columns of a row: sums into the partial slot, or the finished output.
-    __device__ __forceinline__ void put(float* part, int64_t slot, int q0, int row, int part_row, int h, int col,
-                                        float4_t v, float sum, float v_scale) const {
-        if (slot >= 0) {
-            *reinterpret_cast<float4_t*>(part + (int64_t)part_row * D + col) = v;
-            return;
-        }
-        const float inv = sum == 0.0f ? 0.0f : v_scale / sum;
-        float x[4] = {v[0] * inv, v[1] * inv, v[2] * inv, v[3] * inv};
-        finish<4>(a, q0 + row / a.group, h * a.group + row % a.group, col, x);
-    }
-
-    __device__ __forceinline__ void put_stats(float* part, int part_row, float m, float l) const {
-        part[(int64_t)a.plan.slot_rows * D + part_row] = m;
-        part[(int64_t)a.plan.slot_rows * (D + 1) + part_row] = l;
-    }
-
-    // Whether a granule of the tile of values holds an infinity or a NaN.
-    __device__ __forceinline__ bool not_finite(const uint8_t* tile) const {
-        typedef short bits_t __attribute__((ext_vector_type(8)));
-        bits_t top = {};
-#pragma unroll 4
-        for (int t = 0; t < 2 * kT; ++t)
-            top = __builtin_elementwise_max(
-                top, __builtin_bit_cast(bits_t, value(tile, t >> 1, t & 1)) & (short)0x7fff);
-        bool bad = false;
-#pragma unroll
-        for (int j = 0; j < 8; ++j) bad |= top[j] >= E::kInf;
-        return bad;
-    }
-
-    // For a tile with infinities or NaN among its values of which some rows
-    // see only a part: what a row does not see must not reach it even as
-    // 0 x NaN, which the matrix instruction would add.  The product takes the
-    // finite values; which infinities (a NaN is both) a row saw in which column
-    // is kept, a bit each, and added when the unit's tiles are done.
-    //   marks: [r][t][sign][32 rows], bits of the tile's 32 columns; lane (n, g)
-    // keeps sign g of row n.  (No branch here or in the tile loop depends on the
-    // lane: the paths would keep copies of the accumulators where they meet.)
-    template <int R>
-    __device__ __forceinline__ void mark_infinities(const uint8_t* tile, Rows<R>& w, int t0, bool there,
-                                                    uint32_t* marks) const {
-        if (!w.marked) {
-            w.marked = true;
-#pragma unroll 1
-            for (int i = 0; i < R * kT; ++i) marks[i * 64 + lane] = 0;
-        }
-#pragma unroll 1
-        for (int i = 0; i < 2 * kT; ++i) {
-            typedef short bits_t __attribute__((ext_vector_type(8)));
-            bits_t v = __builtin_bit_cast(bits_t, value(tile, i >> 1, i & 1));
-#pragma unroll 1
-            for (int j = 0; j < 8; ++j) {
-                const short mine = v[0], size = mine & 0x7fff;
-                v = __builtin_shufflevector(v, v, 1, 2, 3, 4, 5, 6, 7, 0);
-                const uint64_t up = __ballot(size > E::kInf || mine == E::kInf);
-                const uint64_t down = __ballot(size > E::kInf || (size == E::kInf && mine < 0));
-                if ((up | down) == 0) continue;
-                const uint64_t sign = g ? down : up;  // columns 32 (i / 2) ..: of token j, and of token 8 + j
-                const int at = t0 + (i & 1) * 16 + j;
-#pragma unroll
-                for (int r = 0; r < R; ++r)
-                    marks[(r * kT + (i >> 1)) * 64 + lane] |=
-                        (sees(w.lim[r], at, there) ? (uint32_t)sign : 0u) |
-                        (sees(w.lim[r], at + 8, there) ? (uint32_t)(sign >> 32) : 0u);
-            }
-        }
-    }
-
-    template <int R>
-    __device__ __forceinline__ void add_infinities(Rows<R>& w, const uint32_t* marks) const {
-        wait_lds();
-#pragma unroll
-        for (int r = 0; r < R; ++r)
-#pragma unroll
-            for (int t = 0; t < kT; ++t) {
-                const uint32_t up = marks[(r * kT + t) * 64 + n], down = marks[(r * kT + t) * 64 + 32 + n];
-#pragma unroll
-                for (int c = 0; c < 16; ++c) {
-                    const int col = (c >> 2) * 8 + g * 4 + (c & 3);
-                    const float inf = __builtin_inff();
-                    w.o[r][t][c] += (up >> col & 1 ? inf : 0.0f) - (down >> col & 1 ? inf : 0.0f);
-                }
-                __builtin_amdgcn_sched_barrier(0);
-            }
+    __device__ __forceinline__ void put_stats(float* part, const RowSplit& split, int part_row, float m, float l) const {
+        part[(D << split.log2_rows) + part_row] = m;
+        part[((D + 1) << split.log2_rows) + part_row] = l;
     }
 };
 
-// kR: 32-row tiles of a wave where waves share their tiles; 0: no unit of the launch does.
+// kR: row tiles of a wave where waves share their tiles; 0: no unit of the launch does.
 template <int D, class E, bool F8, int kR>
 __global__ __launch_bounds__(kThreads, D == 256 || kR == 2 ? 1 : 2) void prefix_attention_kernel(AttnArgs a) {
     extern __shared__ __align__(16) uint8_t lds[];
     Shared<D>& sh = *reinterpret_cast<Shared<D>*>(lds);
     uint64_t* const cost = reinterpret_cast<uint64_t*>(lds + sizeof(Shared<D>));
-    uint32_t* const info = reinterpret_cast<uint32_t*>(cost + a.plan.max_entries + 1);
-    const Line line = build_line(a, cost, info, sh);
-    // Pieces follow each other by XCD (workgroup b runs on XCD b % 8), so that
-    // the row tiles of one kv head, which read the same keys, share an L2.
-    const int grid = a.plan.workgroups;
-    const int w = grid % 8 ? blockIdx.x : (blockIdx.x % 8) * (grid / 8) + blockIdx.x / 8;
-    const uint64_t all = line.head_cost * (uint64_t)a.kv_heads;
-    const uint64_t x0 = line.per * (uint64_t)w, x1 = x0 + line.per < all ? x0 + line.per : all;
-    uint64_t x = x0;
-    Unit<D, E, F8> unit(a, sh);
-    while (x < x1) {
-        const int h = (int)quotient(x, line.head_cost);
-        const uint64_t at = x - h * line.head_cost;  // within the head
-        int lo = 0, hi = line.entries;               // the entry: cost[lo] <= at < cost[lo + 1]
-        while (hi - lo > 1) {
-            const int mid = (lo + hi) / 2;
-            if (cost[mid] <= at) lo = mid;
-            else hi = mid;
-        }
-        const int e = uniform(lo);
-        const bool prefix = e < a.plan.prefix_entries;
-        const RowSplit& split = prefix ? a.plan.prefix : a.plan.own;
-        const uint32_t c = (uint32_t)split.cost;
-        const uint64_t e0 = uniform(cost[e]), e1 = uniform(cost[e + 1]);
-        const uint64_t head0 = h * line.head_cost;
-        const uint64_t stop = x1 - head0 < e1 ? x1 - head0 : e1;
-        // steps whose first point lies in the piece (an entry has less than 2^32)
-        const int s0 = (int)(((uint32_t)(at - e0) + c - 1) / c), s1 = (int)(((uint32_t)(stop - e0) + c - 1) / c);
-        const uint32_t who = prefix ? e : uniform((int)info[e]);
-        const int seq = prefix ? 0 : (int)(who >> 16), tile = prefix ? e : (int)(who & 0xffff);
-        Tiles tiles;
-        if (prefix) tiles = prefix_tiles(a, line.min_pos);
-        else tiles = own_tiles(a, seq_at(a, seq), tile);
-        tiles = {uniform(tiles.sink), uniform(tiles.lo), uniform(tiles.hi)};
-        // all of the entry's steps begin in this piece
-        const bool alone = !a.plan.prefix_entries && x - at + e0 >= x0 && head0 + e1 - c < x0 + line.per;
-        if (s0 < s1) {
-            const int64_t slot = alone ? -1 : (int64_t)w + (int64_t)h * line.entries + e;
-            if (kR == 0 || !split.shared) unit.template run<1, false>(h, prefix, seq, tile, tiles, s0, s1, slot);
-            else unit.template run<kR ? kR : 1, true>(h, prefix, seq, tile, tiles, s0, s1, slot);
-        }
-        x = head0 + stop;
+    uint32_t* const info = reinterpret_cast<uint32_t*>(cost + a.plan.own_entries + 1);
+    Line line = build_line(a, cost, info, sh);
+    const RowSplit &pre = a.plan.prefix, &own = a.plan.own;
+    Job job;
+    while (next_prefix(a, line, job, D)) {
+        if (job.s0 >= job.s1) continue;
+        if (kR && pre.shared) Unit<D, E, F8, 32>(a, sh).template run<kR ? kR : 1, true>(job, pre, true, false, line.plain);
+        else if (pre.narrow) Unit<D, E, F8, 16>(a, sh).template run<1, false>(job, pre, true, false, line.plain);
+        else Unit<D, E, F8, 32>(a, sh).template run<1, false>(job, pre, true, false, line.plain);
+    }
+    if (a.plan.prefix_entries) __syncthreads();  // (the ring: from here on a wave may meet no other)
+    while (next_own(a, line, cost, info, sh, job, D)) {
+        if (job.s0 >= job.s1) continue;
+        if (kR && own.shared) Unit<D, E, F8, 32>(a, sh).template run<kR ? kR : 1, true>(job, own, false, false, false);
+        else if (own.narrow) Unit<D, E, F8, 16>(a, sh).template run<1, false>(job, own, false, true, false);
+        else Unit<D, E, F8, 32>(a, sh).template run<1, false>(job, own, false, true, false);
     }
 }
 
 // Dynamic LDS of a launch: the tiles and the line of entries.
 template <int D>
-size_t lds_bytes(int max_entries) {
-    return sizeof(Shared<D>) + 8 * ((size_t)max_entries + 1) + 4 * (size_t)max_entries;
+size_t lds_bytes(int own_entries) {
+    return sizeof(Shared<D>) + 8 * ((size_t)own_entries + 1) + 4 * (size_t)own_entries;
 }
 
 template <int D, class E, bool F8, int kR>
 hipError_t launch_as(const AttnArgs& a, hipStream_t stream) {
-    prefix_attention_kernel<D, E, F8, kR><<<dim3((unsigned)a.plan.workgroups), kThreads, lds_bytes<D>(a.plan.max_entries), stream>>>(a);
+    prefix_attention_kernel<D, E, F8, kR><<<dim3(1u << a.plan.log2_workgroups), kThreads, lds_bytes<D>(a.plan.own_entries), stream>>>(a);
     return hipGetLastError();
 }
 

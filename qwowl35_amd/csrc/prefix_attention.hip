@@ -4,95 +4,91 @@
 
 namespace qw35 {
 
-using attn::MetaHead;
-
 namespace {
 
-RowSplit split_rows(int64_t rows, int shared_r) {
-    if (rows <= 32) return {0, 32, 3, 0};
-    if (rows <= 64) return {1, 64, 2, 0};
-    return {2, 128 * shared_r, shared_r, 1};
+constexpr int kBatch = 16;  // parts whose loads are in flight together
+
+__device__ __forceinline__ float lane_max_f(float v) {
+#pragma unroll
+    for (int o = 1; o < 16; o *= 2) v = fmaxf(v, __shfl_xor(v, o));
+    return attn::row_max<16>(v);
 }
 
-// A unit's pieces: workgroups w0.., slots slot0...
-struct Pieces {
-    int64_t slot0;
-    int n;
-    int row;  // row of the slots
-};
+// lead and cost of a step in units of a quarter of a tile of a wave
+RowSplit split_prefix(int64_t rows, int shared_r) {
+    if (rows <= 16) return {2, 0, 4, 1, 0, 4, 2};
+    if (rows <= 32) return {2, 0, 5, 0, 0, 4, 2};
+    if (rows <= 64) return {1, 1, 6, 0, 0, 4, 2};
+    return {0, 2, shared_r == 2 ? 8 : 7, 0, 1, 8, 2};
+}
 
-__device__ __forceinline__ Pieces pieces_of(const MetaHead& m, const uint64_t* cost, int h, int e, int row,
-                                            const RowSplit& split) {
-    Pieces p = {0, 0, row % split.rows};
-    if (e >= m.entries) return p;
-    const uint64_t e0 = cost[e], e1 = cost[e + 1];
-    if (e0 == e1) return p;
-    const uint64_t head0 = h * m.head_cost;
-    const uint64_t w0 = (head0 + e0) / m.per, w1 = (head0 + e1 - split.cost) / m.per;
-    p.slot0 = (int64_t)(w0 + (uint64_t)h * m.entries + e);
-    p.n = (int)(w1 - w0) + 1;
-    return p;
+RowSplit split_own(int64_t rows, int shared_r) {
+    if (rows <= 16) return {0, 0, 4, 1, 0, 4, 2};
+    if (rows <= 64) return {0, 0, 5, 0, 0, 4, 2};
+    return {0, 2, shared_r == 2 ? 8 : 7, 0, 1, 8, 2};
 }
 
 // One row (token, head) for each `waves` waves of a workgroup of four: with
 // few rows the four waves take every fourth part of one row and join in LDS.
-// Bound by latency there (two dependent reads and the parts), by the parts'
-// bytes otherwise.
+// Bound by latency: the row's sequence, its list of parts, their maxima and
+// sums, and then the parts are four reads that wait for each other; a lane
+// looks up one part of 64, and a part is a load and N products a lane.
 template <int D>
 __global__ __launch_bounds__(256) void prefix_attention_join(AttnArgs a, int waves) {
     constexpr int N = D / 64;  // columns of a lane
     typedef float vec_t __attribute__((ext_vector_type(N == 1 ? 2 : N)));
     __shared__ float sh_o[4][D];
     __shared__ float sh_m[4], sh_l[4];
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    const int lane = threadIdx.x & 63, wave = attn::uniform((int)(threadIdx.x >> 6));
     const int heads = a.kv_heads * a.group;
-    const int64_t item = waves == 1 ? (int64_t)blockIdx.x * 4 + wave : blockIdx.x;
-    if (waves == 1 && item >= (int64_t)a.n_tokens * heads) return;
-    const int t = (int)(item / heads), head = (int)(item % heads);
-    const int h = head / a.group;
-    const MetaHead m = *reinterpret_cast<const MetaHead*>(a.meta);
+    const int item = waves == 1 ? (int)blockIdx.x * 4 + wave : (int)blockIdx.x;  // below 2^30
+    const int t = (int)((uint32_t)item / (uint32_t)heads), head = item - t * heads;
+    if (t >= a.n_tokens) return;
+    const int h = attn::token_of(a, head), in_group = head - h * a.group;
+    const attn::MetaHead meta = *reinterpret_cast<const attn::MetaHead*>(a.meta);
     const int* const first = reinterpret_cast<const int*>(a.meta + attn::meta_first_at());
-    const uint64_t* const cost = reinterpret_cast<const uint64_t*>(a.meta + attn::meta_cost_at(a.n_seqs));
-    const int s = attn::seq_of_wave(a, t, lane);
-    Pieces own = {0, 0, 0}, pre = {0, 0, 0};
-    bool on = false;
+    const int s = attn::uniform(attn::seq_of_wave(a, t, lane));
+    attn::Pieces own = {0, 0}, pre = {0, 0};
+    int own_row = 0, pre_row = 0;
     if (s >= 0) {
-        const attn::Seq q = attn::seq_at(a, s);
-        on = t >= q.q0 && t < q.q0 + q.n;
-        if (on) {
-            const int row = (t - q.q0) * a.group + head % a.group;
-            own = pieces_of(m, cost, h, first[s] + row / a.plan.own.rows, row, a.plan.own);
+        const int q0 = a.starts ? attn::clampi(a.starts[s], 0, a.n_tokens) : t;
+        const int q1 = a.starts ? attn::clampi(a.starts[s + 1], q0, a.n_tokens) : t + 1;
+        if (t >= q0 && t < q1) {
+            const attn::Pieces* const pieces =
+                reinterpret_cast<const attn::Pieces*>(a.meta + attn::meta_pieces_at(a.n_seqs)) +
+                (int64_t)h * (a.plan.prefix_entries + meta.own_entries);
+            own_row = (t - q0) * a.group + in_group;
+            const int e = (meta.lanes ? s : first[s]) + (own_row >> a.plan.own.log2_rows);
+            own_row &= (1 << a.plan.own.log2_rows) - 1;
+            if (e < meta.own_entries) own = pieces[a.plan.prefix_entries + e];
+            if (a.plan.prefix_entries) {
+                pre_row = t * a.group + in_group;
+                pre = pieces[pre_row >> a.plan.prefix.log2_rows];
+                pre_row &= (1 << a.plan.prefix.log2_rows) - 1;
+            }
         }
     }
-    if (a.plan.prefix_entries) {
-        const int row = t * a.group + head % a.group;
-        if (on) pre = pieces_of(m, cost, h, row / a.plan.prefix.rows, row, a.plan.prefix);
-    } else if (own.n == 1) {
-        return;  // the main kernel finished this row (all waves of it return)
-    }
-    const uint64_t slot_floats = attn::slot_floats(a.plan.slot_rows, D);
-    const int n = own.n + pre.n;
+    if (!a.plan.prefix_entries && own.n == 1) return;  // the main kernel finished this row (all waves of it return)
+    const int n = attn::uniform((int)(own.n + pre.n)), own_n = (int)own.n;
     const int k0 = waves == 1 ? 0 : wave;
-    const float* const part = a.part;
-    auto slot_of = [&](int k) {
-        return part + (uint64_t)(k < own.n ? own.slot0 + k : pre.slot0 + (k - own.n)) * slot_floats;
-    };
     float top = -__builtin_inff(), sum = 0.0f;
     float acc[N] = {};
     // 64 parts at a time: lane i reads the maximum and sum of part i, then every lane its columns of all of them
     for (int k = k0; k < n; k += 64 * waves) {
         const int mine = k + lane * waves;
+        const float* at = a.part;
         float pm = -__builtin_inff(), pl = 0.0f;
         if (mine < n) {
-            const float* const p = slot_of(mine);
-            const int row = mine < own.n ? own.row : pre.row;
-            pm = p[(int64_t)a.plan.slot_rows * D + row];
-            pl = p[(int64_t)a.plan.slot_rows * (D + 1) + row];
+            const bool is_own = mine < own_n;
+            const int log2_rows = is_own ? a.plan.own.log2_rows : a.plan.prefix.log2_rows;
+            const int row = is_own ? own_row : pre_row;
+            const uint64_t slot = is_own ? own.slot0 + mine : pre.slot0 + (mine - own_n);
+            const float* const p = (is_own ? a.own_part : a.part) + slot * attn::slot_floats(1 << log2_rows, D);
+            at = p + row * D;
+            pm = p[(D << log2_rows) + row];
+            pl = p[((D + 1) << log2_rows) + row];
         }
-        float chunk = pm;
-#pragma unroll
-        for (int o = 1; o < 64; o *= 2) chunk = fmaxf(chunk, __shfl_xor(chunk, o));
-        const float now = fmaxf(top, chunk);
+        const float now = fmaxf(top, lane_max_f(pm));
         const float shrink = attn::part_weight(top, now);
         top = now;
         sum *= shrink;
@@ -100,19 +96,39 @@ __global__ __launch_bounds__(256) void prefix_attention_join(AttnArgs a, int wav
         for (int j = 0; j < N; ++j) acc[j] *= shrink;
         const float weight = attn::part_weight(pm, now);
         sum += weight * pl;
-        const int count = (n - k + waves - 1) / waves < 64 ? (n - k + waves - 1) / waves : 64;
-#pragma unroll 8
-        for (int i = 0; i < count; ++i) {
+        const int rest = (n - k + waves - 1) / waves, count = rest < 64 ? rest : 64;
+        const int64_t addr = reinterpret_cast<int64_t>(at);
+        auto part = [&](int i) {
+            const uint32_t lo = (uint32_t)__builtin_amdgcn_readlane((int)addr, i);
+            const uint32_t hi = (uint32_t)__builtin_amdgcn_readlane((int)(addr >> 32), i);
+            return reinterpret_cast<const float*>((uint64_t)hi << 32 | lo) + lane * N;
+        };
+        auto add = [&](int i, const vec_t& v) {
             const float w = __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, weight), i));
-            const int j = k + i * waves;
-            const float* const p = slot_of(j) + (int64_t)(j < own.n ? own.row : pre.row) * D + lane * N;
-            if constexpr (N == 1) {
-                acc[0] += w == 0.0f ? 0.0f : w * p[0];
-            } else {
-                const vec_t v = *reinterpret_cast<const vec_t*>(p);
 #pragma unroll
-                for (int c = 0; c < N; ++c) acc[c] += w == 0.0f ? 0.0f : w * v[c];
-            }
+            for (int c = 0; c < N; ++c) acc[c] += w == 0.0f ? 0.0f : w * v[c];
+        };
+        auto load = [&](int i) {
+            vec_t v;
+            if constexpr (N == 1) v[0] = *part(i);
+            else v = *reinterpret_cast<const vec_t*>(part(i));
+            return v;
+        };
+        int i = 0;
+        for (; i + kBatch <= count; i += kBatch) {
+            vec_t v[kBatch];
+#pragma unroll
+            for (int j = 0; j < kBatch; ++j) v[j] = load(i + j);
+#pragma unroll
+            for (int j = 0; j < kBatch; ++j) add(i + j, v[j]);
+        }
+        if (i < count) {  // the last few: one load twice rather than one after the other
+            vec_t v[kBatch];
+#pragma unroll
+            for (int j = 0; j < kBatch; ++j) v[j] = load(i + j < count ? i + j : count - 1);
+#pragma unroll
+            for (int j = 0; j < kBatch; ++j)
+                if (i + j < count) add(i + j, v[j]);
         }
     }
     // sum: each lane holds its parts' share, rescaled alike
@@ -140,9 +156,10 @@ __global__ __launch_bounds__(256) void prefix_attention_join(AttnArgs a, int wav
         }
     }
     const float inv = sum == 0.0f ? 0.0f : (a.v_scale ? a.v_scale[h] : 1.0f) / sum;
+    float out[1][N];
 #pragma unroll
-    for (int c = 0; c < N; ++c) acc[c] *= inv;
-    attn::finish<N>(a, t, head, lane * N, acc);
+    for (int c = 0; c < N; ++c) out[0][c] = acc[c] * inv;
+    attn::finish(a, t, head, lane * N, 0, out);
 }
 
 template <int D>
@@ -156,24 +173,34 @@ hipError_t launch_join(const AttnArgs& a, hipStream_t stream) {
 
 }  // namespace
 
-AttnPlan plan_attention(int dim, int kv_heads, int group, int n_seqs, int n_tokens, int max_new, bool prefix) {
+AttnPlan plan_attention(const AttnShape& s) {
     AttnPlan p = {};
-    const int64_t rows_prefix = prefix ? (int64_t)n_tokens * group : 0, rows_own = (int64_t)max_new * group;
+    const int64_t rows_prefix = s.prefix_len ? (int64_t)s.n_tokens * s.group : 0, rows_own = (int64_t)s.max_new * s.group;
     const int64_t most = rows_prefix > rows_own ? rows_prefix : rows_own;
-    p.shared_r = most <= 64 ? 0 : most <= 128 || dim == 256 ? 1 : 2;
-    p.prefix = split_rows(rows_prefix, p.shared_r);
-    p.own = split_rows(rows_own, p.shared_r);
-    p.workgroups = dim == 256 || p.shared_r == 2 ? 256 : 512;
-    p.prefix_entries = (int)((rows_prefix + p.prefix.rows - 1) / p.prefix.rows);
+    p.shared_r = most <= 64 ? 0 : most <= 128 || s.dim == 256 ? 1 : 2;
+    p.prefix = split_prefix(rows_prefix, p.shared_r);
+    p.own = split_own(rows_own, p.shared_r);
+    p.log2_workgroups = s.dim == 256 || p.shared_r == 2 ? 8 : 9;
+    p.group_magic = s.group > 1 ? (uint32_t)((1ull << 32) / s.group + 1) : 0;
+    p.page_magic = s.page_blocks > 1 ? (uint32_t)((1ull << 32) / s.page_blocks + 1) : 0;
+    p.prefix_entries = (int)((rows_prefix + (1 << p.prefix.log2_rows) - 1) >> p.prefix.log2_rows);
     // every sequence's last row tile may be a part of one
-    p.max_entries = p.prefix_entries + n_seqs + (int)((int64_t)n_tokens * group / p.own.rows);
-    p.slot_rows = p.prefix.rows > p.own.rows && prefix ? p.prefix.rows : p.own.rows;
-    p.slots = (uint64_t)p.workgroups + (uint64_t)kv_heads * p.max_entries;
-    p.meta_bytes = (attn::meta_cost_at(n_seqs) + 8 * ((uint64_t)p.max_entries + 1) + 255) / 256 * 256;
-    p.lds_bytes = dim == 64    ? attn::lds_bytes<64>(p.max_entries)
-                  : dim == 128 ? attn::lds_bytes<128>(p.max_entries)
-                               : attn::lds_bytes<256>(p.max_entries);
-    p.workspace_bytes = p.meta_bytes + 4 * p.slots * attn::slot_floats(p.slot_rows, dim);
+    p.own_entries = s.n_seqs + (int)((int64_t)s.n_tokens * s.group >> p.own.log2_rows);
+    auto cost = [](const RowSplit& r, int64_t tokens) {
+        return r.lead + (((tokens + 31) / 32 + r.step()) / r.step() << r.log2_cost);
+    };
+    p.lanes = s.n_seqs <= 64 && s.kv_heads * p.prefix_entries * cost(p.prefix, s.prefix_len) < 1 << 30 &&
+              s.kv_heads * s.n_seqs * cost(p.own, s.own_tokens) < 1 << 30;
+    const uint64_t prefix_slots = p.prefix_entries ? (1ull << p.log2_workgroups) + (uint64_t)s.kv_heads * p.prefix_entries : 0;
+    const uint64_t own_slots = (p.own.shared ? 1ull : 4ull) << p.log2_workgroups;
+    p.own_part = prefix_slots * attn::slot_floats(1 << p.prefix.log2_rows, s.dim);
+    p.meta_bytes = (attn::meta_pieces_at(s.n_seqs) + 8 * (uint64_t)s.kv_heads * (p.prefix_entries + p.own_entries) + 255) /
+                   256 * 256;
+    p.lds_bytes = s.dim == 64    ? attn::lds_bytes<64>(p.own_entries)
+                  : s.dim == 128 ? attn::lds_bytes<128>(p.own_entries)
+                                 : attn::lds_bytes<256>(p.own_entries);
+    p.workspace_bytes = p.meta_bytes + 4 * (p.own_part + (own_slots + (uint64_t)s.kv_heads * p.own_entries) *
+                                                             attn::slot_floats(1 << p.own.log2_rows, s.dim));
     return p;
 }
 
