@@ -451,8 +451,8 @@ __device__ __forceinline__ void line_in_lds(const AttnArgs& a, uint64_t* cost, u
         __syncthreads();
 #pragma unroll
         for (int w = 0; w < kWaves; ++w) least = top[w] < least ? top[w] : least;
-        least = uniform(least);
     }
+    least = uniform(least);
     set_prefix(a, line, least);
     __syncthreads();
     uint64_t sum = 0;
@@ -677,14 +677,21 @@ __device__ __forceinline__ float row_sum(float v) {
     return p.a + p.b;
 }
 
-// v *= f in v's own registers (the compiler's products would go to others,
-// with a copy of every accumulator where the paths meet).
-template <class Acc>
+// v *= f in v's own registers, accumulation ones in the kernels that have them
+// (the compiler's products would go to others, and the accumulators with them
+// from one kind to the other in every tile).  The matrix instructions that
+// wrote v are a tile's scores away, past any wait that reading them needs.
+template <bool kAgpr, class Acc>
 __device__ __forceinline__ void scale_in_place(Acc& v, float f) {
 #pragma unroll
     for (int i = 0; i < (int)(sizeof(Acc) / 4); ++i) {
         float x = v[i];
-        asm("v_mul_f32 %0, %1, %0" : "+v"(x) : "v"(f));
+        if constexpr (kAgpr) {
+            float y;
+            asm("v_accvgpr_read_b32 %1, %0\n\tv_mul_f32 %1, %2, %1\n\tv_accvgpr_write_b32 %0, %1" : "+a"(x), "=&v"(y) : "v"(f));
+        } else {
+            asm("v_mul_f32 %0, %1, %0" : "+v"(x) : "v"(f));
+        }
         v[i] = x;
     }
 }
@@ -726,9 +733,10 @@ __device__ __forceinline__ void copy_kb(const uint8_t* from, uint8_t* to, int la
     }
 }
 
-template <int D>
+// kR as the kernel's.
+template <int D, int kR>
 struct Shared {
-    static constexpr int kRing = D == 256 ? 128 * 1024 : 64 * 1024;
+    static constexpr int kRing = D == 256 || kR == 2 ? 128 * 1024 : 64 * 1024;
     uint8_t ring[kRing];  // tiles on their way; at a unit's end the waves' sums
     float m[kWaves][32];
     float l[kWaves][32];
@@ -752,7 +760,7 @@ __device__ __forceinline__ typename E::vec8 operand(raw8<F8> w) {
 }
 
 // kRows: rows of a wave's tile, 16 or 32.
-template <int D, class E, bool F8, int kRows>
+template <int D, class E, bool F8, int kRows, int kR>
 struct Unit {
     typedef typename E::vec8 vec8;
     typedef raw8<F8> raw;
@@ -769,17 +777,18 @@ struct Unit {
     static constexpr int kElem = F8 ? 1 : 2;
     static constexpr int kTile = 32 * D * kElem;  // bytes of a tile's keys, and of its values
     static constexpr int kKb = kTile / 1024;
-    static constexpr int kRing = Shared<D>::kRing;
+    static constexpr int kRing = Shared<D, kR>::kRing;
     // The exponents' reference follows the maximum only when that has risen by
     // 2^8: sums then hold up to 2^8 times a row's largest term, which costs
     // neither type precision, and most tiles rescale nothing.
     static constexpr float kRise = 8.0f;
+    static constexpr bool kAgpr = D == 256 || kR == 2;  // one wave a SIMD, accumulation registers beside the others
 
     const AttnArgs& a;
-    Shared<D>& sh;
+    Shared<D, kR>& sh;
     const int lane, wave, n, g;  // this lane's row of a tile, and which of the row's lanes it is
 
-    __device__ Unit(const AttnArgs& a_, Shared<D>& sh_)
+    __device__ Unit(const AttnArgs& a_, Shared<D, kR>& sh_)
         : a(a_), sh(sh_), lane(threadIdx.x & 63), wave(__builtin_amdgcn_readfirstlane(threadIdx.x >> 6)),
           n(threadIdx.x & (kRows - 1)), g((threadIdx.x & 63) / kRows) {}
 
@@ -863,7 +872,7 @@ struct Unit {
                 const float shrink = m_new == w.mx[r] ? 1.0f : __builtin_amdgcn_exp2f(w.mx[r] - m_new);
                 w.l[r] *= shrink;
 #pragma unroll
-                for (int t = 0; t < kT; ++t) scale_in_place(w.o[r][t], shrink);
+                for (int t = 0; t < kT; ++t) scale_in_place<kAgpr>(w.o[r][t], shrink);
                 w.mx[r] = m_new;
             }
             const float ref = w.mx[r] == -__builtin_inff() ? 0.0f : w.mx[r];
@@ -1065,7 +1074,9 @@ struct Unit {
         constexpr int kFit = kShared ? kRing / (2 * kTile) : kRing / kWaves / (2 * kTile);
         constexpr int kMarks = R * kRows * D / 4;  // bytes of a wave's marks; shared tiles leave room in the ring
         static_assert(kShared || kMarks <= sizeof(sh.marks[0]) || kRows == 16, "room for the marks");
-        constexpr int kPairs = kFit < 4 ? kFit : !kShared || 2 * kTile * 4 + kWaves * kMarks <= kRing ? 4 : 3;
+        constexpr int kRoom = kShared ? (kRing - kWaves * kMarks) / (2 * kTile) : kFit;
+        constexpr int kMost = kShared ? 6 : 4;
+        constexpr int kPairs = kRoom < kMost ? kRoom : kMost;
         static_assert(!kShared || 2 * kTile * kPairs + kWaves * kMarks <= kRing, "tiles and marks fit the ring");
         uint32_t* const marks = kShared ? reinterpret_cast<uint32_t*>(sh.ring + 2 * kTile * kPairs + wave * kMarks)
                                         : sh.marks[wave];
@@ -1377,36 +1388,36 @@ struct Unit {
 template <int D, class E, bool F8, int kR>
 __global__ __launch_bounds__(kThreads, D == 256 || kR == 2 ? 1 : 2) void prefix_attention_kernel(AttnArgs a) {
     extern __shared__ __align__(16) uint8_t lds[];
-    Shared<D>& sh = *reinterpret_cast<Shared<D>*>(lds);
-    uint64_t* const cost = reinterpret_cast<uint64_t*>(lds + sizeof(Shared<D>));
+    Shared<D, kR>& sh = *reinterpret_cast<Shared<D, kR>*>(lds);
+    uint64_t* const cost = reinterpret_cast<uint64_t*>(lds + sizeof(Shared<D, kR>));
     uint32_t* const info = reinterpret_cast<uint32_t*>(cost + a.plan.own_entries + 1);
     Line line = build_line(a, cost, info, sh);
     const RowSplit &pre = a.plan.prefix, &own = a.plan.own;
     Job job;
     while (next_prefix(a, line, job, D)) {
         if (job.s0 >= job.s1) continue;
-        if (kR && pre.shared) Unit<D, E, F8, 32>(a, sh).template run<kR ? kR : 1, true>(job, pre, true, false, line.plain);
-        else if (pre.narrow) Unit<D, E, F8, 16>(a, sh).template run<1, false>(job, pre, true, false, line.plain);
-        else Unit<D, E, F8, 32>(a, sh).template run<1, false>(job, pre, true, false, line.plain);
+        if (kR && pre.shared) Unit<D, E, F8, 32, kR>(a, sh).template run<kR ? kR : 1, true>(job, pre, true, false, line.plain);
+        else if (pre.narrow) Unit<D, E, F8, 16, kR>(a, sh).template run<1, false>(job, pre, true, false, line.plain);
+        else Unit<D, E, F8, 32, kR>(a, sh).template run<1, false>(job, pre, true, false, line.plain);
     }
     if (a.plan.prefix_entries) __syncthreads();  // (the ring: from here on a wave may meet no other)
     while (next_own(a, line, cost, info, sh, job, D)) {
         if (job.s0 >= job.s1) continue;
-        if (kR && own.shared) Unit<D, E, F8, 32>(a, sh).template run<kR ? kR : 1, true>(job, own, false, false, false);
-        else if (own.narrow) Unit<D, E, F8, 16>(a, sh).template run<1, false>(job, own, false, true, false);
-        else Unit<D, E, F8, 32>(a, sh).template run<1, false>(job, own, false, true, false);
+        if (kR && own.shared) Unit<D, E, F8, 32, kR>(a, sh).template run<kR ? kR : 1, true>(job, own, false, false, false);
+        else if (own.narrow) Unit<D, E, F8, 16, kR>(a, sh).template run<1, false>(job, own, false, true, false);
+        else Unit<D, E, F8, 32, kR>(a, sh).template run<1, false>(job, own, false, true, false);
     }
 }
 
 // Dynamic LDS of a launch: the tiles and the line of entries.
 template <int D>
-size_t lds_bytes(int own_entries) {
-    return sizeof(Shared<D>) + 8 * ((size_t)own_entries + 1) + 4 * (size_t)own_entries;
+size_t lds_bytes(int shared_r, int own_entries) {
+    return (shared_r == 2 ? sizeof(Shared<D, 2>) : sizeof(Shared<D, 0>)) + 8 * ((size_t)own_entries + 1) + 4 * (size_t)own_entries;
 }
 
 template <int D, class E, bool F8, int kR>
 hipError_t launch_as(const AttnArgs& a, hipStream_t stream) {
-    prefix_attention_kernel<D, E, F8, kR><<<dim3(1u << a.plan.log2_workgroups), kThreads, lds_bytes<D>(a.plan.own_entries), stream>>>(a);
+    prefix_attention_kernel<D, E, F8, kR><<<dim3(1u << a.plan.log2_workgroups), kThreads, lds_bytes<D>(kR, a.plan.own_entries), stream>>>(a);
     return hipGetLastError();
 }
 

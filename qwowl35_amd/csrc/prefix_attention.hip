@@ -196,9 +196,9 @@ AttnPlan plan_attention(const AttnShape& s) {
     p.own_part = prefix_slots * attn::slot_floats(1 << p.prefix.log2_rows, s.dim);
     p.meta_bytes = (attn::meta_pieces_at(s.n_seqs) + 8 * (uint64_t)s.kv_heads * (p.prefix_entries + p.own_entries) + 255) /
                    256 * 256;
-    p.lds_bytes = s.dim == 64    ? attn::lds_bytes<64>(p.own_entries)
-                  : s.dim == 128 ? attn::lds_bytes<128>(p.own_entries)
-                                 : attn::lds_bytes<256>(p.own_entries);
+    p.lds_bytes = s.dim == 64    ? attn::lds_bytes<64>(p.shared_r, p.own_entries)
+                  : s.dim == 128 ? attn::lds_bytes<128>(p.shared_r, p.own_entries)
+                                 : attn::lds_bytes<256>(p.shared_r, p.own_entries);
     p.workspace_bytes = p.meta_bytes + 4 * (p.own_part + (own_slots + (uint64_t)s.kv_heads * p.own_entries) *
                                                              attn::slot_floats(1 << p.own.log2_rows, s.dim));
     return p;
