@@ -40,7 +40,7 @@ hipError_t launch_kv_append(const qw35_hip_kv_cache& cache, const HeadsView& k, 
 // tokens by itself.
 //   Prefix units of up to 64 rows: a workgroup, 16 or 32 rows a wave, the waves
 // of a row group on different 32-token tiles (a step is 4 or 2 tiles).
-//   More rows: a workgroup, 32 or 64 rows a wave, all four on the same tile.
+//   More rows: a workgroup, 32 rows a wave, all four on the same tile.
 struct RowSplit {
     int log2_tiles;  // tiles of a step
     int log2_rg;     // row groups of the workgroup's waves
@@ -53,8 +53,8 @@ struct RowSplit {
 };
 
 struct AttnPlan {
-    int shared_r;  // 32-row tiles of a wave where waves share tiles (0: no unit does)
     RowSplit prefix, own;
+    int shared;  // of either
     int log2_workgroups;
     int lanes;           // up to 64 sequences whose costs fit 32 bits
     uint32_t group_magic, page_magic;  // 2^32 / group and page_blocks, rounded up (0: they are 1)

@@ -246,7 +246,7 @@ uint64_t qw35_hip_prefix_attention_workspace_size(const qw35_hip_kv_cache* cache
     if (!check_batch(cache, n_heads, n_seqs, n_tokens, nullptr, 0)) return 0;
     const uint32_t group = n_heads / cache->kv_heads;
     // every division of the rows that a call of this batch may take: the most rows of a sequence that each has
-    const uint32_t most[] = {1, 16 / group, 32 / group, 64 / group, 128 / group, 128 / group + 1, n_tokens};
+    const uint32_t most[] = {1, 16 / group, 32 / group, 64 / group, 64 / group + 1, n_tokens};
     uint64_t need = 256;
     for (uint32_t prefix = 0; prefix < 2; ++prefix)
         for (uint32_t max_new : most) {

@@ -335,15 +335,14 @@ __device__ __forceinline__ uint64_t line_quotient(const Line& l, uint64_t x, uin
     return l.lanes ? quotient((uint32_t)x, (uint32_t)d) : quotient(x, d);
 }
 
-// A piece of a line of `all`, for one of 2^log2_places.
-__device__ __forceinline__ Piece piece_of(uint64_t all, int log2_places, int place, const RowSplit& s, uint64_t least) {
-    Piece p;
-    p.place = place;
-    p.per = (all + (1ull << log2_places) - 1) >> log2_places;
-    if (least < 1u << s.log2_cost) least = 1u << s.log2_cost;  // a step
-    if (p.per < least) p.per = least;
+// The piece of a line of `all` at a place of several (past them: none).
+__device__ __forceinline__ Piece piece_of(uint64_t all, int places, int place, const RowSplit& s) {
+    Piece p = {1, 0, 0, 0, place};
+    if (!places) return p;
+    p.per = quotient(all + (uint64_t)(places - 1), (uint64_t)places);
+    if (p.per < 1u << s.log2_cost) p.per = 1u << s.log2_cost;  // a step
     p.x = p.x0 = p.per * (uint64_t)place;
-    p.x1 = p.x0 + p.per < all ? p.x0 + p.per : all;
+    p.x1 = (uint32_t)place >= (uint32_t)places ? 0 : p.x0 + p.per < all ? p.x0 + p.per : all;
     return p;
 }
 
@@ -476,23 +475,28 @@ template <class S>
 __device__ __forceinline__ Line build_line(const AttnArgs& a, uint64_t* cost, uint32_t* info, S& sh) {
     const AttnPlan& p = a.plan;
     const int grid = 1 << p.log2_workgroups;
-    // Pieces follow each other by XCD (workgroup b runs on XCD b % 8), so that
-    // the row tiles of one kv head, which read the same keys, share an L2.
-    const int w = (int)((blockIdx.x & 7) << (p.log2_workgroups - 3) | blockIdx.x >> 3);
-    const bool writes = w == grid / 2;  // (in a small launch without a piece of its own)
+    const bool writes = (int)blockIdx.x == grid - 1;
     Line line;
     line.prefix_cost = 0;
     line.prefix_tiles = {0, 0, 0};
     line.lanes = p.lanes && line_in_lanes(a, sh, line);
     if (!line.lanes) line_in_lds(a, cost, info, sh, line, writes);
-    // the own line from the other end, so that in a small launch a workgroup has a piece of one line only
-    line.prefix = piece_of((uint64_t)line.prefix_cost * (uint64_t)(p.prefix_entries * a.kv_heads), p.log2_workgroups, w,
-                           p.prefix, 0);
-    // (next to a long piece of the prefix, a piece of up to four steps rather than more parts to join)
-    const uint64_t beside = line.prefix.per >> 2, most = 4u << p.own.log2_cost;
-    line.own = piece_of(line.head_cost * (uint64_t)a.kv_heads, p.log2_workgroups + (p.own.shared ? 0 : 2),
-                        p.own.shared ? grid - 1 - w : (grid - 1 - w) * kWaves + uniform((int)(threadIdx.x >> 6)), p.own,
-                        !p.prefix_entries ? 0 : beside < most ? beside : most);
+    // The workgroups are divided between the lines by what they cost (a launch
+    // of both phases in every workgroup pays for beginning and ending twice).
+    // Those of an XCD (workgroup b runs on XCD b % 8) have pieces that follow
+    // each other, so that the row tiles of a kv head, which read the same keys,
+    // share an L2, and every XCD has its part of either line.
+    const uint64_t prefix = (uint64_t)line.prefix_cost * (uint64_t)(p.prefix_entries * a.kv_heads);
+    const uint64_t own = line.head_cost * (uint64_t)a.kv_heads;
+    const uint64_t own_by_group = p.own.shared ? own : own >> 2;
+    int eighth = grid / 8;  // workgroups of an XCD for the prefix
+    if (!prefix) eighth = 0;
+    else if (own) eighth = clampi((int)((double)prefix / (double)(prefix + own_by_group) * (double)eighth), 1, eighth - 1);
+    const int xcd = (int)(blockIdx.x & 7), at = (int)(blockIdx.x >> 3), rest = grid / 8 - eighth;
+    line.prefix = piece_of(prefix, eighth * 8, at < eighth ? xcd * eighth + at : -1, p.prefix);
+    const int group = at < eighth ? -1 : xcd * rest + at - eighth;
+    if (p.own.shared) line.own = piece_of(own, rest * 8, group, p.own);
+    else line.own = piece_of(own, rest * 8 * kWaves, group < 0 ? -1 : group * kWaves + uniform((int)(threadIdx.x >> 6)), p.own);
     if (writes) {  // for the join
         Pieces* const pieces = reinterpret_cast<Pieces*>(a.meta + meta_pieces_at(a.n_seqs));
         if (threadIdx.x == 0) *reinterpret_cast<MetaHead*>(a.meta) = MetaHead{line.own_entries, line.lanes};
@@ -733,10 +737,9 @@ __device__ __forceinline__ void copy_kb(const uint8_t* from, uint8_t* to, int la
     }
 }
 
-// kR as the kernel's.
-template <int D, int kR>
+template <int D>
 struct Shared {
-    static constexpr int kRing = D == 256 || kR == 2 ? 128 * 1024 : 64 * 1024;
+    static constexpr int kRing = D == 256 ? 128 * 1024 : 64 * 1024;
     uint8_t ring[kRing];  // tiles on their way; at a unit's end the waves' sums
     float m[kWaves][32];
     float l[kWaves][32];
@@ -760,7 +763,7 @@ __device__ __forceinline__ typename E::vec8 operand(raw8<F8> w) {
 }
 
 // kRows: rows of a wave's tile, 16 or 32.
-template <int D, class E, bool F8, int kRows, int kR>
+template <int D, class E, bool F8, int kRows>
 struct Unit {
     typedef typename E::vec8 vec8;
     typedef raw8<F8> raw;
@@ -777,28 +780,27 @@ struct Unit {
     static constexpr int kElem = F8 ? 1 : 2;
     static constexpr int kTile = 32 * D * kElem;  // bytes of a tile's keys, and of its values
     static constexpr int kKb = kTile / 1024;
-    static constexpr int kRing = Shared<D, kR>::kRing;
+    static constexpr int kRing = Shared<D>::kRing;
     // The exponents' reference follows the maximum only when that has risen by
     // 2^8: sums then hold up to 2^8 times a row's largest term, which costs
     // neither type precision, and most tiles rescale nothing.
     static constexpr float kRise = 8.0f;
-    static constexpr bool kAgpr = D == 256 || kR == 2;  // one wave a SIMD, accumulation registers beside the others
+    static constexpr bool kAgpr = D == 256;  // one wave a SIMD, accumulation registers beside the others
 
     const AttnArgs& a;
-    Shared<D, kR>& sh;
+    Shared<D>& sh;
     const int lane, wave, n, g;  // this lane's row of a tile, and which of the row's lanes it is
 
-    __device__ Unit(const AttnArgs& a_, Shared<D, kR>& sh_)
+    __device__ Unit(const AttnArgs& a_, Shared<D>& sh_)
         : a(a_), sh(sh_), lane(threadIdx.x & 63), wave(__builtin_amdgcn_readfirstlane(threadIdx.x >> 6)),
           n(threadIdx.x & (kRows - 1)), g((threadIdx.x & 63) / kRows) {}
 
     // What a wave carries through its tiles.
-    template <int R>
     struct Rows {
-        vec8 q[R][kM];
-        acc o[R][kT];
-        float mx[R], l[R];
-        Limits lim[R];
+        vec8 q[kM];
+        acc o[kT];
+        float mx, l;
+        Limits lim;
         int all_lo, all_hi, all_sink;  // what every row of the wave sees
         float scale;
         bool marked;  // infinities to add at the end
@@ -817,77 +819,98 @@ struct Unit {
     // Token of a lane's score j.
     __device__ __forceinline__ int token(int j) const { return kRows == 32 ? (j & 8) * 2 + g * 8 + (j & 7) : g * 8 + j; }
 
-    template <int R>
-    __device__ __forceinline__ void scores(const uint8_t* keys, const Rows<R>& w, acc (&s)[R][kB]) const {
-        constexpr int kSteps = kM * kB, kAhead = kSteps < 4 ? kSteps : 4;
+    struct Nothing {
+        __device__ __forceinline__ void operator()(int) const {}
+    };
+
+    // `beside`(step): other work, a part after the matrix instructions of each step.
+    static constexpr int kScoreSteps = kM * kB, kValueSteps = kK * kT;
+    template <class F = Nothing>
+    __device__ __forceinline__ void scores(const uint8_t* keys, const Rows& w, acc (&s)[kB], F beside = {}) const {
+        constexpr int kSteps = kScoreSteps, kAhead = kSteps < 4 ? kSteps : 4;
         vec8 k[kAhead];
 #pragma unroll
         for (int i = 0; i < kAhead; ++i) k[i] = key(keys, i / kB, i % kB);
 #pragma unroll
-        for (int r = 0; r < R; ++r)
-#pragma unroll
-            for (int b = 0; b < kB; ++b) s[r][b] = acc{};
+            for (int b = 0; b < kB; ++b) s[b] = acc{};
 #pragma unroll
         for (int i = 0; i < kSteps; ++i) {
             const vec8 kk = k[i % kAhead];
             if (i + kAhead < kSteps) k[i % kAhead] = key(keys, (i + kAhead) / kB, (i + kAhead) % kB);
-#pragma unroll
-            for (int r = 0; r < R; ++r) s[r][i % kB] = E::mfma(kk, w.q[r][i / kB], s[r][i % kB]);
+            s[i % kB] = E::mfma(kk, w.q[i / kB], s[i % kB]);
+            beside(i);
+            if (!std::is_same_v<F, Nothing>) __builtin_amdgcn_sched_barrier(0);
         }
-        interleave<kSteps, R, kAhead>();
+        if (std::is_same_v<F, Nothing>) interleave<kSteps, kAhead>();
     }
 
     // LDS reads kAhead ahead of the matrix instructions that take them.
-    template <int kSteps, int R, int kAhead>
+    template <int kSteps, int kAhead>
     static __device__ __forceinline__ void interleave() {
         __builtin_amdgcn_sched_group_barrier(0x100, kAhead, 0);
 #pragma unroll
         for (int m = 0; m < kSteps; ++m) {
             if (F8) __builtin_amdgcn_sched_group_barrier(0x002, 4, 0);
-            __builtin_amdgcn_sched_group_barrier(0x008, R, 0);
+            __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
             if (m + kAhead < kSteps) __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);
         }
     }
 
-    // Softmax of a tile's scores: its terms to p, the running reference, sum and output kept.
-    template <int R>
-    __device__ __forceinline__ void softmax(Rows<R>& w, acc (&s)[R][kB], int t0, bool masked, bool there,
-                                            vec8 (&p)[R][kK]) const {
+    // Scores that a row does not see leave the softmax.
+    __device__ __forceinline__ void mask(const Rows& w, acc (&s)[kB], int t0, bool there) const {
 #pragma unroll
-        for (int r = 0; r < R; ++r) {
-            float x[kScores];
+            for (int j = 0; j < kScores; ++j)
+                s[j / kAcc][j % kAcc] =
+                    sees(w.lim, t0 + token(j), there) ? s[j / kAcc][j % kAcc] : -__builtin_inff();
+    }
+
+    // The largest of this lane's scores of row tile r.
+    static __device__ __forceinline__ float largest(const acc (&s)[kB]) {
+        float top = s[0][0];
 #pragma unroll
-            for (int j = 0; j < kScores; ++j) x[j] = s[r][j / kAcc][j % kAcc];
-            if (masked) {
+        for (int j = 1; j < kScores; ++j) top = fmaxf(top, s[j / kAcc][j % kAcc]);
+        return top;
+    }
+
+    // The reference follows the rows' largest scores.
+    __device__ __forceinline__ void follow(Rows& w, float largest_) const {
+        const float top = row_max<kRows>(largest_) * w.scale;
+        if (__builtin_expect(__any(top > w.mx + kRise), 0)) {
+            const float m_new = fmaxf(w.mx, top);
+            const float shrink = m_new == w.mx ? 1.0f : __builtin_amdgcn_exp2f(w.mx - m_new);
+            w.l *= shrink;
 #pragma unroll
-                for (int j = 0; j < kScores; ++j)
-                    x[j] = sees(w.lim[r], t0 + token(j), there) ? x[j] : -__builtin_inff();
-            }
-            float top = x[0];
-#pragma unroll
-            for (int j = 1; j < kScores; ++j) top = fmaxf(top, x[j]);
-            top = row_max<kRows>(top) * w.scale;
-            if (__builtin_expect(__any(top > w.mx[r] + kRise), 0)) {
-                const float m_new = fmaxf(w.mx[r], top);
-                const float shrink = m_new == w.mx[r] ? 1.0f : __builtin_amdgcn_exp2f(w.mx[r] - m_new);
-                w.l[r] *= shrink;
-#pragma unroll
-                for (int t = 0; t < kT; ++t) scale_in_place<kAgpr>(w.o[r][t], shrink);
-                w.mx[r] = m_new;
-            }
-            const float ref = w.mx[r] == -__builtin_inff() ? 0.0f : w.mx[r];
-#pragma unroll
-            for (int j = 0; j < kScores; ++j) {
-                const float e = __builtin_amdgcn_exp2f(fmaf(x[j], w.scale, -ref));
-                w.l[r] += e;
-                p[r][j / 8][j % 8] = (typename E::elem)e;
-            }
+            for (int t = 0; t < kT; ++t) scale_in_place<kAgpr>(w.o[t], shrink);
+            w.mx = m_new;
         }
     }
 
-    template <int R>
-    __device__ __forceinline__ void add_values(const uint8_t* values, Rows<R>& w, const vec8 (&p)[R][kK]) const {
-        constexpr int kSteps = kK * kT, kAhead = kSteps < 4 ? kSteps : 4;
+    // The softmax' terms of a tile, and their sums: of the scores j0 .. j1 - 1 of all row tiles' together.
+    __device__ __forceinline__ void terms(Rows& w, const acc (&s)[kB], vec8 (&p)[kK], int j0 = 0,
+                                          int j1 = kScores) const {
+#pragma unroll
+        for (int i = j0; i < j1; ++i) {
+            const int j = i;
+            const float ref = w.mx == -__builtin_inff() ? 0.0f : w.mx;
+            const float e = __builtin_amdgcn_exp2f(fmaf(s[j / kAcc][j % kAcc], w.scale, -ref));
+            w.l += e;
+            p[j / 8][j % 8] = (typename E::elem)e;
+        }
+    }
+
+    __device__ __forceinline__ void softmax(Rows& w, acc (&s)[kB], int t0, bool masked, bool there,
+                                            vec8 (&p)[kK]) const {
+        if (masked) mask(w, s, t0, there);
+        float top;
+        top = largest(s);
+        follow(w, top);
+        terms(w, s, p);
+    }
+
+    template <class F = Nothing>
+    __device__ __forceinline__ void add_values(const uint8_t* values, Rows& w, const vec8 (&p)[kK],
+                                               F beside = {}) const {
+        constexpr int kSteps = kValueSteps, kAhead = kSteps < 4 ? kSteps : 4;
         vec8 v[kAhead];
 #pragma unroll
         for (int i = 0; i < kAhead; ++i) v[i] = value(values, i / kK, i % kK);
@@ -895,19 +918,20 @@ struct Unit {
         for (int i = 0; i < kSteps; ++i) {
             const vec8 vv = v[i % kAhead];
             if (i + kAhead < kSteps) v[i % kAhead] = value(values, (i + kAhead) / kK, (i + kAhead) % kK);
-#pragma unroll
-            for (int r = 0; r < R; ++r) w.o[r][i / kK] = E::mfma(vv, p[r][i % kK], w.o[r][i / kK]);
+            w.o[i / kK] = E::mfma(vv, p[i % kK], w.o[i / kK]);
+            beside(i);
+            if (!std::is_same_v<F, Nothing>) __builtin_amdgcn_sched_barrier(0);
         }
-        interleave<kSteps, R, kAhead>();
+        if (std::is_same_v<F, Nothing>) interleave<kSteps, kAhead>();
     }
 
     // Keeps infinities and NaN of a tile's values, of which some rows see only
     // a part, from the product (all waves of a shared tile come here together).
-    template <int R, bool kShared>
-    __device__ __forceinline__ void split_off_infinities(uint8_t* tile, Rows<R>& w, int t0, bool there,
+    template <bool kShared>
+    __device__ __forceinline__ void split_off_infinities(uint8_t* tile, Rows& w, int t0, bool there,
                                                          uint32_t* marks) const {
         if (__builtin_expect(!__any(not_finite(tile)), 1)) return;
-        mark_infinities<R>(tile, w, t0, there, marks);
+        mark_infinities(tile, w, t0, there, marks);
         if (kShared) __syncthreads();
         make_finite(tile, kShared ? wave : 0, kShared ? kWaves : 1);
         if (kShared) __syncthreads();
@@ -952,17 +976,16 @@ struct Unit {
     // 0 x NaN, which the matrix instruction would add.  The product takes the
     // finite values; which infinities (a NaN is both) a row saw in which column
     // is kept, a bit each, and added when the unit's tiles are done.
-    //   marks: [r][t][sign][kRows], bits of the tile's kRows columns; a lane
+    //   marks: [t][sign][kRows], bits of the tile's kRows columns; a lane
     // keeps sign g % 2 of row n.  (No branch here or in the tile loop depends on
     // the lane: the paths would keep copies of the accumulators where they meet.)
-    template <int R>
-    __device__ __forceinline__ void mark_infinities(const uint8_t* tile, Rows<R>& w, int t0, bool there,
+    __device__ __forceinline__ void mark_infinities(const uint8_t* tile, Rows& w, int t0, bool there,
                                                     uint32_t* marks) const {
         const int mine = (g & 1) * kRows + n;
         if (!w.marked) {
             w.marked = true;
 #pragma unroll 1
-            for (int i = 0; i < R * kT; ++i) marks[i * 2 * kRows + mine] = 0;
+            for (int i = 0; i < kT; ++i) marks[i * 2 * kRows + mine] = 0;
         }
 #pragma unroll 1
         for (int i = 0; i < kK * kT; ++i) {
@@ -978,38 +1001,31 @@ struct Unit {
                 if ((up | down) == 0) continue;
                 uint64_t sign = g & 1 ? down : up;  // kRows columns: of token j, 8 + j ...
                 const int at = t0 + kk * 16 + j;
+                uint32_t see = 0;
 #pragma unroll
-                for (int r = 0; r < R; ++r) {
-                    uint32_t see = 0;
-#pragma unroll
-                    for (int k = 0; k < kGroups; ++k)
-                        see |= sees(w.lim[r], at + 8 * k, there) ? (uint32_t)(sign >> kRows * k) : 0u;
-                    marks[(r * kT + t) * 2 * kRows + mine] |= see;
-                }
+                for (int k = 0; k < kGroups; ++k)
+                    see |= sees(w.lim, at + 8 * k, there) ? (uint32_t)(sign >> kRows * k) : 0u;
+                marks[t * 2 * kRows + mine] |= see;
             }
         }
     }
 
-    template <int R>
-    __device__ __forceinline__ void add_infinities(Rows<R>& w, const uint32_t* marks) const {
+    __device__ __forceinline__ void add_infinities(Rows& w, const uint32_t* marks) const {
         wait_lds();
 #pragma unroll
-        for (int r = 0; r < R; ++r)
-#pragma unroll
             for (int t = 0; t < kT; ++t) {
-                const uint32_t up = marks[(r * kT + t) * 2 * kRows + n], down = marks[(r * kT + t) * 2 * kRows + kRows + n];
+                const uint32_t up = marks[t * 2 * kRows + n], down = marks[t * 2 * kRows + kRows + n];
 #pragma unroll
                 for (int c = 0; c < kAcc; ++c) {
                     const int col = (c >> 2) * 8 + g * 4 + (c & 3);
                     const float inf = __builtin_inff();
-                    w.o[r][t][c] += (up >> col & 1 ? inf : 0.0f) - (down >> col & 1 ? inf : 0.0f);
+                    w.o[t][c] += (up >> col & 1 ? inf : 0.0f) - (down >> col & 1 ? inf : 0.0f);
                 }
                 __builtin_amdgcn_sched_barrier(0);
             }
     }
 
-    template <int R>
-    __device__ __forceinline__ bool partly(const Rows<R>& w, int t0, bool there) const {
+    __device__ __forceinline__ bool partly(const Rows& w, int t0, bool there) const {
         return !there || !((t0 >= w.all_lo && t0 + 32 <= w.all_hi) || t0 + 32 <= w.all_sink);
     }
 
@@ -1043,9 +1059,9 @@ struct Unit {
         return (int64_t)(block == kNoBlock ? 0u : block) * kTile;
     }
 
-    // A job.  R: row tiles of a wave; kShared: the waves share their tiles;
-    // by_wave: each wave has a job of its own (and meets no other in it).
-    template <int R, bool kShared>
+    // A job.  kShared: the waves share their tiles; by_wave: each wave has a
+    // job of its own (and meets no other in it).
+    template <bool kShared>
     __device__ __forceinline__ void run(const Job& job, const RowSplit& split, bool prefix, bool by_wave, bool plain) {
         const int rg = kShared ? wave : by_wave ? 0 : wave & ((1 << split.log2_rg) - 1);
         const int tg = kShared || by_wave ? 0 : wave >> split.log2_rg;
@@ -1054,7 +1070,7 @@ struct Unit {
         const Tiles& tiles = job.tiles;
         const int h = job.h;
         const int row_end = sq.n * a.group;
-        const int row0 = (job.tile << split.log2_rows) + rg * kRows * R;  // this wave's first row
+        const int row0 = (job.tile << split.log2_rows) + rg * kRows;  // this wave's first row
 
         // this wave's tiles: step * s0 + tg, and every step-th after it
         Pages pages;
@@ -1072,14 +1088,10 @@ struct Unit {
         if (!by_wave) __syncthreads();  // the ring is free
         else wait_lds();
         constexpr int kFit = kShared ? kRing / (2 * kTile) : kRing / kWaves / (2 * kTile);
-        constexpr int kMarks = R * kRows * D / 4;  // bytes of a wave's marks; shared tiles leave room in the ring
-        static_assert(kShared || kMarks <= sizeof(sh.marks[0]) || kRows == 16, "room for the marks");
-        constexpr int kRoom = kShared ? (kRing - kWaves * kMarks) / (2 * kTile) : kFit;
+        static_assert(kRows * D / 4 <= sizeof(sh.marks[0]), "room for the marks");
         constexpr int kMost = kShared ? 6 : 4;
-        constexpr int kPairs = kRoom < kMost ? kRoom : kMost;
-        static_assert(!kShared || 2 * kTile * kPairs + kWaves * kMarks <= kRing, "tiles and marks fit the ring");
-        uint32_t* const marks = kShared ? reinterpret_cast<uint32_t*>(sh.ring + 2 * kTile * kPairs + wave * kMarks)
-                                        : sh.marks[wave];
+        constexpr int kPairs = kFit < kMost ? kFit : kMost;
+        uint32_t* const marks = sh.marks[wave];
         uint8_t* const ring = sh.ring + (kShared ? 0 : wave * (kRing / kWaves));
         uint32_t there_bits = 0;  // of the tiles loaded last, the newest in bit 0
         auto note = [&](uint32_t block) { there_bits = there_bits << 1 | (block != kNoBlock ? 1u : 0u); };
@@ -1094,9 +1106,9 @@ struct Unit {
             copy_kb<kKb / 2>(from + at + part, to + (wave < 2 ? 0 : kTile) + part, lane);
         };
 
-        Rows<R> w;
+        Rows w;
         if (pages.count) look_up(pages, 0);
-        load_queries<R>(w, sq, h, row0, row_end);
+        load_queries(w, sq, h, row0, row_end);
         int loaded = 0;
         if constexpr (kShared) {
             for (; loaded < kPairs - 1 && loaded < pages.count; ++loaded) load_quarter(loaded);
@@ -1109,29 +1121,62 @@ struct Unit {
                 copy_kb<kKb>(vbase + bytes_at(block), to + kTile, lane);
             }
         }
-        start_rows<R, kShared>(w, sq, prefix, plain, row0, row_end);
-        use_queries<R>(w);  // (here the queries are waited for, not in the tile loop)
+        start_rows<kShared>(w, sq, prefix, plain, row0, row_end);
+        use_queries(w);  // (here the queries are waited for, not in the tile loop)
 
         if constexpr (kShared) {
+            // In one step the matrix unit makes the next tile's scores while
+            // the vector unit turns this one's into the softmax' terms, then
+            // the values' product while it looks for the largest of the next.
             constexpr int kEach = kKb / 2;  // a wave's copies of a pair
-            for (int i = 0; i < pages.count; ++i) {
-                if (i + kPairs - 2 < pages.count) wait_vm<(kPairs - 2) * kEach>();
-                else wait_vm<0>();
-                __builtin_amdgcn_s_barrier();  // tile i is there, and tile i - 1 read by all
-                asm volatile("" ::: "memory");
-                if (loaded < pages.count) load_quarter(loaded++);
-                uint8_t* const at = ring + (i % kPairs) * 2 * kTile;
+            acc s[kB];
+            float top;
+            if (kPairs - 2 < pages.count) wait_vm<(kPairs - 2) * kEach>();  // (a job has a step, and a step a tile)
+            else wait_vm<0>();
+            __builtin_amdgcn_s_barrier();
+            asm volatile("" ::: "memory");
+            scores(ring, w, s);
+            top = largest(s);
+            auto see_and_follow = [&](int i) {
                 const bool there = there_bits >> (loaded - 1 - i) & 1;
                 const int t0 = tiles.at(pages.first + i) * 32;
-                const bool masked = partly<R>(w, t0, there);
-                if (masked) split_off_infinities<R, true>(at + kTile, w, t0, there, marks);
-                acc s[R][kB];
-                vec8 p[R][kK];
-                scores<R>(at, w, s);
-                softmax<R>(w, s, t0, masked, there, p);
-                add_values<R>(at + kTile, w, p);
+                if (partly(w, t0, there)) {
+                    split_off_infinities<true>(ring + (i % kPairs) * 2 * kTile + kTile, w, t0, there, marks);
+                    mask(w, s, t0, there);
+                    top = largest(s);
+                }
+                follow(w, top);
+            };
+            vec8 p[kK];
+            int i = 0;
+            for (; i + 1 < pages.count; ++i) {
+                see_and_follow(i);
+                if (i + kPairs - 2 < pages.count) wait_vm<(kPairs - 3) * kEach>();
+                else wait_vm<0>();
+                __builtin_amdgcn_s_barrier();  // tile i + 1 is there, and tile i - 1 read by all
+                asm volatile("" ::: "memory");
+                if (loaded < pages.count) load_quarter(loaded++);
+                __builtin_amdgcn_sched_barrier(0);
+                acc next[kB];
+                constexpr int kAll = kScores;
+                scores(ring + ((i + 1) % kPairs) * 2 * kTile, w, next, [&](int m) {
+                    terms(w, s, p, kAll * m / kScoreSteps, kAll * (m + 1) / kScoreSteps);
+                });
+                top = -__builtin_inff();
+                add_values(ring + (i % kPairs) * 2 * kTile + kTile, w, p, [&](int m) {
+#pragma unroll
+                    for (int x = kAll * m / kValueSteps; x < kAll * (m + 1) / kValueSteps; ++x) {
+                        const int j = x;
+                        top = fmaxf(top, next[j / kAcc][j % kAcc]);
+                        s[j / kAcc][j % kAcc] = next[j / kAcc][j % kAcc];
+                    }
+                });
                 wait_lds();
             }
+            see_and_follow(i);
+            terms(w, s, p);
+            add_values(ring + (i % kPairs) * 2 * kTile + kTile, w, p);
+            wait_lds();
         } else {
             constexpr int kLater = (2 * kPairs - 1) * kKb;  // copies issued after the keys of a tile, or after its values
             for (int i = 0; i < pages.count; ++i) {
@@ -1139,12 +1184,12 @@ struct Unit {
                 const bool there = there_bits >> (loaded - 1 - i) & 1;
                 const bool more = loaded < pages.count;
                 const int t0 = tiles.at(pages.first + i * step) * 32;
-                const bool masked = partly<R>(w, t0, there);
-                acc s[R][kB];
-                vec8 p[R][kK];
+                const bool masked = partly(w, t0, there);
+                acc s[kB];
+                vec8 p[kK];
                 if (more) wait_vm<kLater>();
                 else wait_vm<0>();
-                scores<R>(at, w, s);
+                scores(at, w, s);
                 uint32_t block = 0;
                 if (more) {
                     wait_lds();
@@ -1153,67 +1198,62 @@ struct Unit {
                     ++loaded;
                     copy_kb<kKb>(kbase + bytes_at(block), at, lane);
                 }
-                softmax<R>(w, s, t0, masked, there, p);
+                softmax(w, s, t0, masked, there, p);
                 if (more) wait_vm<kLater>();
-                if (masked) split_off_infinities<R, false>(at + kTile, w, t0, there, marks);
-                add_values<R>(at + kTile, w, p);
+                if (masked) split_off_infinities<false>(at + kTile, w, t0, there, marks);
+                add_values(at + kTile, w, p);
                 if (more) {
                     wait_lds();
                     copy_kb<kKb>(vbase + bytes_at(block), at + kTile, lane);
                 }
             }
         }
-        if (__builtin_expect(w.marked, 0)) add_infinities<R>(w, marks);
-#pragma unroll
-        for (int r = 0; r < R; ++r) w.l[r] = row_sum<kRows>(w.l[r]);
+        if (__builtin_expect(w.marked, 0)) add_infinities(w, marks);
+        w.l = row_sum<kRows>(w.l);
 
         const float v_scale = F8 && a.v_scale ? a.v_scale[h] : 1.0f;
         static_assert(kRows * D * 4 <= kRing / kWaves, "a wave's sums of a row tile fit its part of the ring");
         if (!kShared && !by_wave) {
             // The waves of a row group join: each leaves its sums in LDS, then
             // adds up every step-th group of all of theirs.
-            static_assert(kShared || R == 1, "a wave of its own tiles has one of rows");
             if (g == 0) {
-                sh.m[wave][n] = w.mx[0];
-                sh.l[wave][n] = w.l[0];
+                sh.m[wave][n] = w.mx;
+                sh.l[wave][n] = w.l;
             }
-            leave<R>(w, 0);
+            leave(w);
             __syncthreads();
             if (split.log2_rg == 0) join_waves<4>(job, rg, tg, row0, row_end, v_scale);
             else join_waves<2>(job, rg, tg, row0, row_end, v_scale);
             return;
         }
         if (kShared && !job.part) __syncthreads();  // (the tiles are read)
+        const int row = row0 + n, part_row = rg * kRows + n;
+        if (job.part) {
+            if (row < row_end) {
+                float* const to = job.part + part_row * D + g * 4;
 #pragma unroll
-        for (int r = 0; r < R; ++r) {
-            const int row = row0 + r * kRows + n, part_row = (rg * R + r) * kRows + n;
-            if (job.part) {
-                if (row < row_end) {
-                    float* const to = job.part + part_row * D + g * 4;
-#pragma unroll
-                    for (int i = 0; i < kQuads; ++i)
-                        *reinterpret_cast<float4_t*>(to + i * kQuadCols) = quad<R>(w, r, i);
-                    if (g == 0) put_stats(job.part, split, part_row, w.mx[r], w.l[r]);
-                }
-            } else {
-                leave<R>(w, r);
-                const int tok = token_of(a, row), head = h * a.group + row - tok * a.group;
-                const float inv = w.l[r] == 0.0f ? 0.0f : v_scale / w.l[r];
-                if (row < row_end) {
-#pragma unroll 1
-                    for (int i = 0; i < kQuads; i += 4) {
-                        float x[4][4];
-#pragma unroll
-                        for (int c = 0; c < 4; ++c) {
-                            const float4_t y = left(wave)[(i + c) * 64 + lane];
-#pragma unroll
-                            for (int j = 0; j < 4; ++j) x[c][j] = y[j] * inv;
-                        }
-                        finish(a, sq.q0 + tok, head, i * kQuadCols + g * 4, kQuadCols, x);
-                    }
-                }
-                wait_lds();
+                for (int i = 0; i < kQuads; ++i)
+                    *reinterpret_cast<float4_t*>(to + i * kQuadCols) = quad(w, i);
+                if (g == 0) put_stats(job.part, split, part_row, w.mx, w.l);
             }
+        } else {
+            leave(w);
+            const int tok = token_of(a, row), head = h * a.group + row - tok * a.group;
+            const float inv = w.l == 0.0f ? 0.0f : v_scale / w.l;
+            if (row < row_end) {
+#pragma unroll 1
+                for (int i = 0; i < kQuads; i += 4) {
+                    float x[4][4];
+#pragma unroll
+                    for (int c = 0; c < 4; ++c) {
+                        const float4_t y = left(wave)[(i + c) * 64 + lane];
+#pragma unroll
+                        for (int j = 0; j < 4; ++j) x[c][j] = y[j] * inv;
+                    }
+                    finish(a, sq.q0 + tok, head, i * kQuadCols + g * 4, kQuadCols, x);
+                }
+            }
+            wait_lds();
         }
     }
 
@@ -1221,14 +1261,12 @@ struct Unit {
     __device__ __forceinline__ float4_t* left(int by) const {
         return reinterpret_cast<float4_t*>(sh.ring + by * (kRing / kWaves));
     }
-    template <int R>
-    __device__ __forceinline__ void leave(const Rows<R>& w, int r) const {
+    __device__ __forceinline__ void leave(const Rows& w) const {
 #pragma unroll
-        for (int i = 0; i < kQuads; ++i) left(wave)[i * 64 + lane] = quad<R>(w, r, i);
+        for (int i = 0; i < kQuads; ++i) left(wave)[i * 64 + lane] = quad(w, i);
     }
-    template <int R>
-    static __device__ __forceinline__ float4_t quad(const Rows<R>& w, int r, int i) {
-        const acc& v = w.o[r][i * 4 / kAcc];
+    static __device__ __forceinline__ float4_t quad(const Rows& w, int i) {
+        const acc& v = w.o[i * 4 / kAcc];
         const int c = i * 4 % kAcc;
         return float4_t{v[c], v[c + 1], v[c + 2], v[c + 3]};
     }
@@ -1269,94 +1307,84 @@ struct Unit {
     }
 
     // This lane's queries (asked for; use_queries waits).
-    template <int R>
-    __device__ __forceinline__ void load_queries(Rows<R>& w, const Seq& sq, int h, int row0, int row_end) const {
+    __device__ __forceinline__ void load_queries(Rows& w, const Seq& sq, int h, int row0, int row_end) const {
+        const int row = row0 + n;
+        const bool on = row < row_end;
+        const int tok = on ? token_of(a, row) : 0;
+        const int t = sq.q0 + tok, head = h * a.group + (on ? row - tok * a.group : 0);
+        const typename E::elem* p = static_cast<const typename E::elem*>(a.q.data) + t * a.q.token_stride +
+                                    head * a.q.head_stride + g * 8;
 #pragma unroll
-        for (int r = 0; r < R; ++r) {
-            const int row = row0 + r * kRows + n;
-            const bool on = row < row_end;
-            const int tok = on ? token_of(a, row) : 0;
-            const int t = sq.q0 + tok, head = h * a.group + (on ? row - tok * a.group : 0);
-            const typename E::elem* p = static_cast<const typename E::elem*>(a.q.data) + t * a.q.token_stride +
-                                        head * a.q.head_stride + g * 8;
+        for (int m = 0; m < kM; ++m) w.q[m] = vec8{};
+        if (on && a.q.vec) {
 #pragma unroll
-            for (int m = 0; m < kM; ++m) w.q[r][m] = vec8{};
-            if (on && a.q.vec) {
+            for (int m = 0; m < kM; ++m) w.q[m] = *reinterpret_cast<const vec8*>(p + m * 8 * kGroups);
+        } else if (on) {
 #pragma unroll
-                for (int m = 0; m < kM; ++m) w.q[r][m] = *reinterpret_cast<const vec8*>(p + m * 8 * kGroups);
-            } else if (on) {
+            for (int m = 0; m < kM; ++m) {
 #pragma unroll
-                for (int m = 0; m < kM; ++m) {
-#pragma unroll
-                    for (int j = 0; j < 8; ++j) w.q[r][m][j] = p[m * 8 * kGroups + j];
-                    asm volatile("" ::: "memory");  // (eight loads at a time)
-                }
+                for (int j = 0; j < 8; ++j) w.q[m][j] = p[m * 8 * kGroups + j];
+                asm volatile("" ::: "memory");  // (eight loads at a time)
             }
         }
         w.scale = a.scale_log2 * (F8 && a.k_scale ? a.k_scale[h] : 1.0f);
     }
 
-    template <int R>
-    __device__ __forceinline__ void use_queries(Rows<R>& w) const {
+    __device__ __forceinline__ void use_queries(Rows& w) const {
         // a negative scale turns the queries' signs, so that the largest score has the largest product
         const uint32_t flip = w.scale < 0.0f ? 0x80008000u : 0u;
         w.scale = fabsf(w.scale);
         if (w.scale < 2e-38f) w.scale = 2e-38f;  // (zero: every finite score alike, and a masked one still none)
 #pragma unroll
-        for (int r = 0; r < R; ++r)
-#pragma unroll
             for (int m = 0; m < kM; ++m) {
-                uint4_t x = __builtin_bit_cast(uint4_t, w.q[r][m]) ^ flip;
+                uint4_t x = __builtin_bit_cast(uint4_t, w.q[m]) ^ flip;
                 asm volatile("" : "+v"(x));
-                w.q[r][m] = __builtin_bit_cast(vec8, x);
+                w.q[m] = __builtin_bit_cast(vec8, x);
             }
     }
 
     // What this lane's rows see.
-    template <int R, bool kShared>
-    __device__ __forceinline__ void start_rows(Rows<R>& w, const Seq& sq, bool prefix, bool plain, int row0,
+    template <bool kShared>
+    __device__ __forceinline__ void start_rows(Rows& w, const Seq& sq, bool prefix, bool plain, int row0,
                                                int row_end) const {
         w.marked = false;
         w.all_lo = 0;
         w.all_hi = w.all_sink = 0x7fffffff;
-#pragma unroll
-        for (int r = 0; r < R; ++r) {
-            const int row = row0 + r * kRows + n;
-            const bool on = row < row_end;
-            const int tok = on ? token_of(a, row) : 0, t = sq.q0 + tok;
-            w.lim[r] = Limits{0, 0, 0};
-            if (on) {
-                if (!prefix) {
-                    w.lim[r] = own_limits(a, sq, upto_of(sq, tok));
-                } else if (plain) {
-                    w.lim[r].hi = a.prefix_len;
-                } else {
-                    int s, stop = 0, upto = 0;
-                    if (a.n_seqs <= kSeqs) {
-                        s = a.starts ? last_at(sh.start, a.n_seqs, t) : t;
-                        if (s >= 0) {
-                            stop = sh.end[s];
-                            upto = sh.upto[s];
-                        }
-                    } else {
-                        s = seq_of(a, t);
-                        if (s >= 0) {
-                            const Seq mine = seq_at(a, s);
-                            stop = mine.q0 + mine.n;
-                            upto = upto_of(mine, -mine.q0);
-                        }
+        const int row = row0 + n;
+        const bool on = row < row_end;
+        const int tok = on ? token_of(a, row) : 0, t = sq.q0 + tok;
+        w.lim = Limits{0, 0, 0};
+        if (on) {
+            if (!prefix) {
+                w.lim = own_limits(a, sq, upto_of(sq, tok));
+            } else if (plain) {
+                w.lim.hi = a.prefix_len;
+            } else {
+                int s, stop = 0, upto = 0;
+                if (a.n_seqs <= kSeqs) {
+                    s = a.starts ? last_at(sh.start, a.n_seqs, t) : t;
+                    if (s >= 0) {
+                        stop = sh.end[s];
+                        upto = sh.upto[s];
                     }
-                    if (s >= 0 && t < stop) w.lim[r] = prefix_limits(a, upto + t);
+                } else {
+                    s = seq_of(a, t);
+                    if (s >= 0) {
+                        const Seq mine = seq_at(a, s);
+                        stop = mine.q0 + mine.n;
+                        upto = upto_of(mine, -mine.q0);
+                    }
                 }
-                w.all_lo = w.lim[r].lo > w.all_lo ? w.lim[r].lo : w.all_lo;
-                w.all_hi = w.lim[r].hi < w.all_hi ? w.lim[r].hi : w.all_hi;
-                w.all_sink = w.lim[r].sink < w.all_sink ? w.lim[r].sink : w.all_sink;
+                if (s >= 0 && t < stop) w.lim = prefix_limits(a, upto + t);
             }
-            w.mx[r] = -__builtin_inff();
-            w.l[r] = 0.0f;
-#pragma unroll
-            for (int t2 = 0; t2 < kT; ++t2) w.o[r][t2] = acc{};
+            w.all_lo = w.lim.lo > w.all_lo ? w.lim.lo : w.all_lo;
+            w.all_hi = w.lim.hi < w.all_hi ? w.lim.hi : w.all_hi;
+            w.all_sink = w.lim.sink < w.all_sink ? w.lim.sink : w.all_sink;
         }
+        w.mx = -__builtin_inff();
+        w.l = 0.0f;
+#pragma unroll
+        for (int t2 = 0; t2 < kT; ++t2) w.o[t2] = acc{};
         w.all_lo = lane_max(w.all_lo, 0);
         w.all_hi = lane_min(w.all_hi, 0x7fffffff);
         w.all_sink = lane_min(w.all_sink, 0x7fffffff);
@@ -1384,50 +1412,46 @@ struct Unit {
     }
 };
 
-// kR: row tiles of a wave where waves share their tiles; 0: no unit of the launch does.
-template <int D, class E, bool F8, int kR>
-__global__ __launch_bounds__(kThreads, D == 256 || kR == 2 ? 1 : 2) void prefix_attention_kernel(AttnArgs a) {
+// kWide: waves share their tiles in some unit of the launch.
+template <int D, class E, bool F8, bool kWide>
+__global__ __launch_bounds__(kThreads, D == 256 ? 1 : 2) void prefix_attention_kernel(AttnArgs a) {
     extern __shared__ __align__(16) uint8_t lds[];
-    Shared<D, kR>& sh = *reinterpret_cast<Shared<D, kR>*>(lds);
-    uint64_t* const cost = reinterpret_cast<uint64_t*>(lds + sizeof(Shared<D, kR>));
+    Shared<D>& sh = *reinterpret_cast<Shared<D>*>(lds);
+    uint64_t* const cost = reinterpret_cast<uint64_t*>(lds + sizeof(Shared<D>));
     uint32_t* const info = reinterpret_cast<uint32_t*>(cost + a.plan.own_entries + 1);
     Line line = build_line(a, cost, info, sh);
     const RowSplit &pre = a.plan.prefix, &own = a.plan.own;
     Job job;
     while (next_prefix(a, line, job, D)) {
         if (job.s0 >= job.s1) continue;
-        if (kR && pre.shared) Unit<D, E, F8, 32, kR>(a, sh).template run<kR ? kR : 1, true>(job, pre, true, false, line.plain);
-        else if (pre.narrow) Unit<D, E, F8, 16, kR>(a, sh).template run<1, false>(job, pre, true, false, line.plain);
-        else Unit<D, E, F8, 32, kR>(a, sh).template run<1, false>(job, pre, true, false, line.plain);
+        if (kWide && pre.shared) Unit<D, E, F8, 32>(a, sh).template run<true>(job, pre, true, false, line.plain);
+        else if (pre.narrow) Unit<D, E, F8, 16>(a, sh).template run<false>(job, pre, true, false, line.plain);
+        else Unit<D, E, F8, 32>(a, sh).template run<false>(job, pre, true, false, line.plain);
     }
-    if (a.plan.prefix_entries) __syncthreads();  // (the ring: from here on a wave may meet no other)
     while (next_own(a, line, cost, info, sh, job, D)) {
         if (job.s0 >= job.s1) continue;
-        if (kR && own.shared) Unit<D, E, F8, 32, kR>(a, sh).template run<kR ? kR : 1, true>(job, own, false, false, false);
-        else if (own.narrow) Unit<D, E, F8, 16, kR>(a, sh).template run<1, false>(job, own, false, true, false);
-        else Unit<D, E, F8, 32, kR>(a, sh).template run<1, false>(job, own, false, true, false);
+        if (kWide && own.shared) Unit<D, E, F8, 32>(a, sh).template run<true>(job, own, false, false, false);
+        else if (own.narrow) Unit<D, E, F8, 16>(a, sh).template run<false>(job, own, false, true, false);
+        else Unit<D, E, F8, 32>(a, sh).template run<false>(job, own, false, true, false);
     }
 }
 
 // Dynamic LDS of a launch: the tiles and the line of entries.
 template <int D>
-size_t lds_bytes(int shared_r, int own_entries) {
-    return (shared_r == 2 ? sizeof(Shared<D, 2>) : sizeof(Shared<D, 0>)) + 8 * ((size_t)own_entries + 1) + 4 * (size_t)own_entries;
+size_t lds_bytes(int own_entries) {
+    return sizeof(Shared<D>) + 8 * ((size_t)own_entries + 1) + 4 * (size_t)own_entries;
 }
 
-template <int D, class E, bool F8, int kR>
+template <int D, class E, bool F8, bool kWide>
 hipError_t launch_as(const AttnArgs& a, hipStream_t stream) {
-    prefix_attention_kernel<D, E, F8, kR><<<dim3(1u << a.plan.log2_workgroups), kThreads, lds_bytes<D>(kR, a.plan.own_entries), stream>>>(a);
+    prefix_attention_kernel<D, E, F8, kWide><<<dim3(1u << a.plan.log2_workgroups), kThreads, lds_bytes<D>(a.plan.own_entries), stream>>>(a);
     return hipGetLastError();
 }
 
 template <int D, class E, bool F8>
 hipError_t launch_rows(const AttnArgs& a, hipStream_t stream) {
-    if (a.plan.shared_r == 0) return launch_as<D, E, F8, 0>(a, stream);
-    if constexpr (D < 256) {
-        if (a.plan.shared_r == 2) return launch_as<D, E, F8, 2>(a, stream);
-    }
-    return launch_as<D, E, F8, 1>(a, stream);
+    if (!a.plan.shared) return launch_as<D, E, F8, false>(a, stream);
+    return launch_as<D, E, F8, true>(a, stream);
 }
 
 template <int D>

@@ -14,18 +14,23 @@ __device__ __forceinline__ float lane_max_f(float v) {
     return attn::row_max<16>(v);
 }
 
-// lead and cost of a step in units of a quarter of a tile of a wave
-RowSplit split_prefix(int64_t rows, int shared_r) {
-    if (rows <= 16) return {2, 0, 4, 1, 0, 4, 2};
-    if (rows <= 32) return {2, 0, 5, 0, 0, 4, 2};
-    if (rows <= 64) return {1, 1, 6, 0, 0, 4, 2};
-    return {0, 2, shared_r == 2 ? 8 : 7, 0, 1, 8, 2};
+// Leads and costs in quarters of a microsecond, measured with all compute
+// units at it: a step of a wave's own tiles waits for HBM (7 us for 128 KB of a
+// compute unit's waves; 2.5 where few are at it, so 4 is taken), one of shared
+// tiles for the matrix unit.
+RowSplit split_prefix(int64_t rows, int dim) {
+    const int wait = dim == 64 ? 3 : 4;
+    if (rows <= 16) return {2, 0, 4, 1, 0, 24, wait};
+    if (rows <= 32) return {2, 0, 5, 0, 0, 24, wait};
+    if (rows <= 64) return {1, 1, 6, 0, 0, 24, wait};
+    return {0, 2, 7, 0, 1, 32, dim == 64 ? 2 : 3};
 }
 
-RowSplit split_own(int64_t rows, int shared_r) {
-    if (rows <= 16) return {0, 0, 4, 1, 0, 4, 2};
-    if (rows <= 64) return {0, 0, 5, 0, 0, 4, 2};
-    return {0, 2, shared_r == 2 ? 8 : 7, 0, 1, 8, 2};
+RowSplit split_own(int64_t rows, int dim) {
+    const int wait = dim == 64 ? 3 : 4;
+    if (rows <= 16) return {0, 0, 4, 1, 0, 16, wait};
+    if (rows <= 64) return {0, 0, 5, 0, 0, 16, wait};
+    return {0, 2, 7, 0, 1, 32, dim == 64 ? 2 : 3};
 }
 
 // One row (token, head) for each `waves` waves of a workgroup of four: with
@@ -176,11 +181,10 @@ hipError_t launch_join(const AttnArgs& a, hipStream_t stream) {
 AttnPlan plan_attention(const AttnShape& s) {
     AttnPlan p = {};
     const int64_t rows_prefix = s.prefix_len ? (int64_t)s.n_tokens * s.group : 0, rows_own = (int64_t)s.max_new * s.group;
-    const int64_t most = rows_prefix > rows_own ? rows_prefix : rows_own;
-    p.shared_r = most <= 64 ? 0 : most <= 128 || s.dim == 256 ? 1 : 2;
-    p.prefix = split_prefix(rows_prefix, p.shared_r);
-    p.own = split_own(rows_own, p.shared_r);
-    p.log2_workgroups = s.dim == 256 || p.shared_r == 2 ? 8 : 9;
+    p.prefix = split_prefix(rows_prefix, s.dim);
+    p.own = split_own(rows_own, s.dim);
+    p.shared = p.prefix.shared || p.own.shared;
+    p.log2_workgroups = s.dim == 256 ? 8 : 9;
     p.group_magic = s.group > 1 ? (uint32_t)((1ull << 32) / s.group + 1) : 0;
     p.page_magic = s.page_blocks > 1 ? (uint32_t)((1ull << 32) / s.page_blocks + 1) : 0;
     p.prefix_entries = (int)((rows_prefix + (1 << p.prefix.log2_rows) - 1) >> p.prefix.log2_rows);
@@ -196,9 +200,9 @@ AttnPlan plan_attention(const AttnShape& s) {
     p.own_part = prefix_slots * attn::slot_floats(1 << p.prefix.log2_rows, s.dim);
     p.meta_bytes = (attn::meta_pieces_at(s.n_seqs) + 8 * (uint64_t)s.kv_heads * (p.prefix_entries + p.own_entries) + 255) /
                    256 * 256;
-    p.lds_bytes = s.dim == 64    ? attn::lds_bytes<64>(p.shared_r, p.own_entries)
-                  : s.dim == 128 ? attn::lds_bytes<128>(p.shared_r, p.own_entries)
-                                 : attn::lds_bytes<256>(p.shared_r, p.own_entries);
+    p.lds_bytes = s.dim == 64    ? attn::lds_bytes<64>(p.own_entries)
+                  : s.dim == 128 ? attn::lds_bytes<128>(p.own_entries)
+                                 : attn::lds_bytes<256>(p.own_entries);
     p.workspace_bytes = p.meta_bytes + 4 * (p.own_part + (own_slots + (uint64_t)s.kv_heads * p.own_entries) *
                                                              attn::slot_floats(1 << p.own.log2_rows, s.dim));
     return p;
