@@ -20,6 +20,7 @@ from __future__ import annotations
 
 import ctypes as C
 import math
+import struct
 
 import torch
 
@@ -27,29 +28,67 @@ from . import _ffi
 from . import runtime as rt
 from ._ffi import Qw35Error
 
-_DTYPE = {torch.float32: _ffi.DTYPE_F32, torch.bfloat16: _ffi.DTYPE_BF16, torch.float16: _ffi.DTYPE_F16,
-          torch.float8_e4m3fn: _ffi.DTYPE_E4M3}
-_ptr, _stream = rt._ptr, rt._stream
+_FLOAT = {torch.float32: _ffi.DTYPE_F32, torch.bfloat16: _ffi.DTYPE_BF16, torch.float16: _ffi.DTYPE_F16}
+_CACHE = {torch.bfloat16: _ffi.DTYPE_BF16, torch.float16: _ffi.DTYPE_F16, torch.float8_e4m3fn: _ffi.DTYPE_E4M3}
+
+# A small call's time is this module's: structs are packed rather than built
+# field by field, and their functions take addresses as plain numbers.
+_HEADS = struct.Struct("=QqqII")
+_ATTENTION = struct.Struct("=" + 3 * "QqqII" + "4I4Q5IfQQ")
+_NO_HEADS = (0, 0, 0, 0, 0)
+assert _HEADS.size == C.sizeof(_ffi.Heads) and _ATTENTION.size == C.sizeof(_ffi.Attention)
+_at, _u32, _err = C.c_void_p, C.c_uint32, [C.c_char_p, C.c_size_t]
+_ARGS = {
+    "qw35_hip_rotate": [_at, _at, _u32, _u32, _u32, _at, _at, _u32, _at, C.c_float, _at],
+    "qw35_hip_kv_append": [_at, _at, _at, _u32, _at, _at, _at, _u32, _at, C.c_float, _at],
+    "qw35_hip_prefix_attention": [_at, _at, _at],
+}
+_functions: dict = {}
 
 
-def _heads(x: torch.Tensor, name: str) -> _ffi.Heads:
-    """``qw35_hip_heads`` of a [n_tokens, heads, dim] tensor with unit column stride."""
-    if x.dim() != 3 or not x.is_cuda or x.dtype not in _DTYPE:
+def _call(name: str, *args) -> None:
+    fn = _functions.get(name)
+    if fn is None:
+        fn = _functions[name] = C.CFUNCTYPE(C.c_int, *_ARGS[name], *_err)((name, _ffi.load()))
+    err = _ffi._ErrBuffer()
+    if not fn(*args, err, 512):
+        raise Qw35Error(f"{name}: {err.value.decode(errors='replace')}")
+
+
+def _stream(stream) -> int:
+    return rt._raw_stream(torch.cuda.current_device()) if stream is None else stream.cuda_stream
+
+
+def _heads(x: torch.Tensor, name: str) -> tuple:
+    """The fields of the ``qw35_hip_heads`` of a [n_tokens, heads, dim] tensor with unit column stride."""
+    code = _FLOAT.get(x.dtype)
+    if code is None or not x.is_cuda or x.dim() != 3:
         raise Qw35Error(f"{name} must be an fp32, bf16 or fp16 [n_tokens, heads, dim] device tensor")
-    if x.stride(2) != 1 and x.shape[2] > 1:
+    token, head, column = x.stride()
+    if column != 1 and x.shape[2] > 1:
         raise Qw35Error(f"{name} must have unit column stride, got strides {x.stride()}")
-    return _ffi.Heads(x.data_ptr(), x.stride(0), x.stride(1), _DTYPE[x.dtype], 0)
+    return x.data_ptr(), token, head, code, 0
 
 
-def _index(x: torch.Tensor, dtype: torch.dtype, shape: tuple, like: torch.Tensor, name: str) -> None:
-    if x.dtype != dtype or tuple(x.shape) != shape or not x.is_contiguous() or x.device != like.device:
-        raise Qw35Error(f"{name} must be a contiguous {dtype} {list(shape)} tensor on {like.device}, got "
+def _index(x: torch.Tensor, dtype: torch.dtype, shape: tuple, device: int, name: str) -> int:
+    """The address of a contiguous tensor of that type and shape on cuda:``device``."""
+    if x.dtype is not dtype or x.shape != shape or x.get_device() != device or not x.is_contiguous():
+        raise Qw35Error(f"{name} must be a contiguous {dtype} {list(shape)} tensor on cuda:{device}, got "
                         f"{x.dtype} {list(x.shape)} on {x.device}")
+    return x.data_ptr()
 
 
-def _vector(x: torch.Tensor | None, n: int, like: torch.Tensor, name: str) -> None:
-    if x is not None:
-        _index(x, torch.float32, (n,), like, name)
+def _vector(x: torch.Tensor | None, n: int, device: int, name: str) -> int | None:
+    return None if x is None else _index(x, torch.float32, (n,), device, name)
+
+
+def _output(out: torch.Tensor | None, dtype: torch.dtype | None, like: torch.Tensor) -> torch.Tensor:
+    """``out``, or a new tensor of like's shape."""
+    if out is None:
+        return like.new_empty(like.shape, dtype=dtype or like.dtype)
+    if out.shape != like.shape or out.device != like.device or (dtype or out.dtype) != out.dtype:
+        raise Qw35Error(f"out must be a {list(like.shape)} tensor of out_dtype on {like.device}")
+    return out
 
 
 class Rotary:
@@ -72,21 +111,23 @@ class Rotary:
         self.axes = max([i + 1 for i, s in enumerate(sections) if s], default=1)
         self.view = _ffi.Rope(self.freq.data_ptr(), rot_dim, int(interleaved),
                               (C.c_uint32 * 4)(*(sections + [0] * (4 - len(sections)))))
+        self._at = C.addressof(self.view)
 
 
-def _turn(rope: Rotary | None, positions, n: int, like: torch.Tensor) -> tuple:
+def _turn(rope: Rotary | None, positions, n: int, device: int) -> tuple:
     """The rope, positions and n_axes arguments of a call."""
     if rope is None:
         return None, None, 0
     if positions is None:
         raise Qw35Error("positions are needed with a rope")
-    if rope.freq.device != like.device:
-        raise Qw35Error(f"the rope lives on {rope.freq.device}, the input on {like.device}")
-    axes = 1 if positions.dim() == 1 else int(positions.shape[0])
-    _index(positions, torch.int32, (n,) if positions.dim() == 1 else (axes, n), like, "positions")
-    if axes not in (1, rope.axes):
+    if rope.freq.get_device() != device:
+        raise Qw35Error(f"the rope lives on {rope.freq.device}, the input on cuda:{device}")
+    if positions.dim() == 1:
+        return rope._at, _index(positions, torch.int32, (n,), device, "positions"), 1
+    axes = int(positions.shape[0])
+    if axes != 1 and axes != rope.axes:
         raise Qw35Error(f"positions have {axes} axes, the sections 1 or {rope.axes}")
-    return C.byref(rope.view), _ptr(positions), axes
+    return rope._at, _index(positions, torch.int32, (axes, n), device, "positions"), axes
 
 
 def rotate(x: torch.Tensor, rope: Rotary | None, positions: torch.Tensor | None = None, norm: torch.Tensor | None = None,
@@ -100,16 +141,13 @@ def rotate(x: torch.Tensor, rope: Rotary | None, positions: torch.Tensor | None 
     type).  ``out`` may be x."""
     hx = _heads(x, "x")
     n, heads, dim = x.shape
-    if out is None:
-        out = torch.empty((n, heads, dim), dtype=out_dtype or x.dtype, device=x.device)
-    elif out.shape != x.shape or out.device != x.device or (out_dtype or out.dtype) != out.dtype:
-        raise Qw35Error(f"out must be a {list(x.shape)} tensor of out_dtype on {x.device}")
+    device = x.get_device()
+    out = _output(out, out_dtype, x)
     hy = _heads(out, "out")
-    _vector(norm, dim, x, "norm")
-    turn, pos, axes = _turn(rope, positions, n, x)
-    if n == 0:
-        return out
-    _ffi.call("qw35_hip_rotate", C.byref(hx), C.byref(hy), n, heads, dim, turn, pos, axes, _ptr(norm), eps,
+    weight = _vector(norm, dim, device, "norm")
+    turn, pos, axes = _turn(rope, positions, n, device)
+    if n:
+        _call("qw35_hip_rotate", _HEADS.pack(*hx), _HEADS.pack(*hy), n, heads, dim, turn, pos, axes, weight, eps,
               _stream(stream))
     return out
 
@@ -131,17 +169,17 @@ class PagedCache:
         want = (pages, heads, blocks * 4, octets * 8, 8)
         if tuple(v.shape) != want or v.dtype != k.dtype or v.device != k.device or not v.is_contiguous():
             raise Qw35Error(f"cache values must be a contiguous {k.dtype} {list(want)} tensor on {k.device}")
-        if k.dtype not in _DTYPE or k.dtype == torch.float32:
+        if k.dtype not in _CACHE:
             raise Qw35Error(f"a cache is float16, bfloat16 or float8_e4m3fn, got {k.dtype}")
         if k.dtype != torch.float8_e4m3fn and (k_scale is not None or v_scale is not None):
             raise Qw35Error("only a float8_e4m3fn cache has scales")
-        _vector(k_scale, heads, k, "k_scale")
-        _vector(v_scale, heads, k, "v_scale")
+        device = k.get_device()
+        at_k, at_v = _vector(k_scale, heads, device, "k_scale"), _vector(v_scale, heads, device, "v_scale")
         self.k, self.v, self.k_scale, self.v_scale = k, v, k_scale, v_scale
         self.n_pages, self.kv_heads, self.page_size, self.head_dim = pages, heads, blocks * 32, octets * 8
-        at = lambda t: t.data_ptr() if t is not None else None  # noqa: E731
-        self.view = _ffi.KvCache(at(k), at(v), at(k_scale), at(v_scale), pages, self.page_size, heads, self.head_dim,
-                                 _DTYPE[k.dtype], 0)
+        self.view = _ffi.KvCache(k.data_ptr(), v.data_ptr(), at_k, at_v, pages, self.page_size, heads, self.head_dim,
+                                 _CACHE[k.dtype], 0)
+        self._at, self._device = C.addressof(self.view), device
 
     @classmethod
     def empty(cls, n_pages: int, kv_heads: int, page_size: int, head_dim: int, dtype: torch.dtype = torch.float16,
@@ -167,19 +205,18 @@ def kv_append(cache: PagedCache, k: torch.Tensor, v: torch.Tensor, slots: torch.
     Into an e4m3 cache go the values over the head's scale, rounded to nearest
     even, past +-448 to +-448."""
     hk, hv = _heads(k, "k"), _heads(v, "v")
-    n = int(k.shape[0])
-    if tuple(k.shape) != (n, cache.kv_heads, cache.head_dim) or v.shape != k.shape or k.dtype != v.dtype:
+    n, device = int(k.shape[0]), cache._device
+    if k.shape != (n, cache.kv_heads, cache.head_dim) or v.shape != k.shape or k.dtype != v.dtype:
         raise Qw35Error(f"k and v must be [n_tokens, {cache.kv_heads}, {cache.head_dim}] of one type, got "
                         f"{list(k.shape)} {k.dtype} and {list(v.shape)} {v.dtype}")
-    if k.device != cache.k.device or v.device != cache.k.device:
+    if k.get_device() != device or v.get_device() != device:
         raise Qw35Error(f"k and v must be on the cache's {cache.k.device}")
-    _index(slots, torch.int64, (n,), k, "slots")
-    _vector(norm, cache.head_dim, k, "norm")
-    turn, pos, axes = _turn(rope, positions, n, k)
-    if n == 0:
-        return
-    _ffi.call("qw35_hip_kv_append", C.byref(cache.view), C.byref(hk), C.byref(hv), n, _ptr(slots), turn, pos, axes,
-              _ptr(norm), eps, _stream(stream))
+    where = _index(slots, torch.int64, (n,), device, "slots")
+    weight = _vector(norm, cache.head_dim, device, "norm")
+    turn, pos, axes = _turn(rope, positions, n, device)
+    if n:
+        _call("qw35_hip_kv_append", cache._at, _HEADS.pack(*hk), _HEADS.pack(*hv), n, where, turn, pos, axes, weight,
+              eps, _stream(stream))
 
 
 def prefix_attention_workspace(cache: PagedCache, n_heads: int, n_seqs: int, n_tokens: int, device="cuda") -> torch.Tensor:
@@ -213,44 +250,40 @@ def prefix_attention(q: torch.Tensor, cache: PagedCache, pages: torch.Tensor, le
     a recorded call serves every later step."""
     hq = _heads(q, "q")
     n, heads, dim = q.shape
-    if dim != cache.head_dim or q.device != cache.k.device:
+    device = cache._device
+    if dim != cache.head_dim or q.get_device() != device:
         raise Qw35Error(f"q must be [n_tokens, n_heads, {cache.head_dim}] on {cache.k.device}, got {list(q.shape)}")
-    seqs = int(lengths.shape[0])
-    _index(lengths, torch.int32, (seqs,), q, "lengths")
-    if pages.dim() != 2:
-        raise Qw35Error("pages must be int32 [n_seqs, pages_per_seq]")
-    _index(pages, torch.int32, (seqs, int(pages.shape[1])), q, "pages")
-    if starts is not None:
-        _index(starts, torch.int32, (seqs + 1,), q, "starts")
+    if lengths.dim() != 1 or pages.dim() != 2:
+        raise Qw35Error("lengths must be int32 [n_seqs], pages int32 [n_seqs, pages_per_seq]")
+    seqs, per_seq = pages.shape
+    at_lengths = _index(lengths, torch.int32, (seqs,), device, "lengths")
+    at_pages = _index(pages, torch.int32, (seqs, per_seq), device, "pages")
+    at_starts = 0 if starts is None else _index(starts, torch.int32, (seqs + 1,), device, "starts")
     if prefix_len and prefix_pages is None:
         raise Qw35Error("prefix_len needs prefix_pages")
+    at_prefix = shared = 0
     if prefix_pages is not None:
-        _index(prefix_pages, torch.int32, (int(prefix_pages.numel()),), q, "prefix_pages")
-    if min(max_new, prefix_len, window, sink) < 0:
+        shared = prefix_pages.numel()
+        at_prefix = _index(prefix_pages, torch.int32, (shared,), device, "prefix_pages")
+    if max_new < 0 or prefix_len < 0 or window < 0 or sink < 0:
         raise Qw35Error("max_new, prefix_len, window and sink cannot be negative")
-    if out is None:
-        out = torch.empty((n, heads, dim), dtype=out_dtype or q.dtype, device=q.device)
-    elif out.shape != q.shape or out.device != q.device or (out_dtype or out.dtype) != out.dtype:
-        raise Qw35Error(f"out must be a {list(q.shape)} tensor of out_dtype on {q.device}")
-    op = _ffi.Attention()
-    op.q, op.out = hq, _heads(out, "out")
+    out = _output(out, out_dtype, q)
+    ho = _heads(out, "out")
+    hg = _NO_HEADS
     if gate is not None:
-        if gate.shape != q.shape or gate.device != q.device:
+        if gate.shape != q.shape or gate.get_device() != device:
             raise Qw35Error(f"gate must be a {list(q.shape)} tensor on {q.device}")
-        op.gate = _heads(gate, "gate")
+        hg = _heads(gate, "gate")
     if n == 0:
         return out
     if workspace is None:  # this call's own
         workspace = prefix_attention_workspace(cache, heads, seqs, n, device=q.device)
-    if workspace.device != q.device or not workspace.is_contiguous():
+    if workspace.get_device() != device or not workspace.is_contiguous():
         raise Qw35Error(f"workspace must be a contiguous tensor on {q.device}")
-    op.n_tokens, op.n_heads, op.n_seqs, op.max_new = n, heads, seqs, max_new
-    op.starts = starts.data_ptr() if starts is not None else None
-    op.lengths, op.pages, op.pages_per_seq = lengths.data_ptr(), pages.data_ptr(), int(pages.shape[1])
-    if prefix_len:
-        op.prefix_pages, op.n_prefix_pages = prefix_pages.data_ptr(), prefix_pages.numel()
-    op.prefix_len, op.window, op.sink = prefix_len, window, sink
-    op.scale = 1.0 / math.sqrt(dim) if scale is None else scale
-    op.workspace, op.workspace_bytes = workspace.data_ptr(), workspace.numel() * workspace.element_size()
-    _ffi.call("qw35_hip_prefix_attention", C.byref(op), C.byref(cache.view), _stream(stream))
+    if not prefix_len:
+        at_prefix = shared = 0
+    op = _ATTENTION.pack(*hq, *ho, *hg, n, heads, seqs, max_new, at_starts, at_lengths, at_pages, at_prefix, per_seq,
+                         shared, prefix_len, window, sink, 1.0 / math.sqrt(dim) if scale is None else scale,
+                         workspace.data_ptr(), workspace.nbytes)
+    _call("qw35_hip_prefix_attention", op, cache._at, _stream(stream))
     return out

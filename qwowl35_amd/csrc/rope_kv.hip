@@ -15,10 +15,14 @@
 // 2^64: the wrapping product with the position is the angle's fraction of a
 // turn, exact to position * 2^-65, for one 64-bit integer multiply.
 //
-// What bounds it: bytes (10 flop an element).  A lane holds eight columns, a
-// row lies in dim / 8 lanes, so a wave works on several rows at once, every
-// load and store is 16 bytes a lane, and a pair's other half is one lane
-// exchange away (rot_dim is a multiple of 16).
+// What bounds it: bytes (10 flop an element), once the angles, 8 sines and
+// cosines a lane, serve several heads: a lane holds eight columns of up to
+// eight heads of a token, so every load and store is 16 bytes a lane, a wave
+// works on several rows at once, and a pair's other half is one lane exchange
+// away (rot_dim is a multiple of 16).  With fewer heads a lane where a call
+// would fill the card with less than 1024 waves: there latency counts
+// (8192 tokens x 32 heads x 128 bf16: 57 us with one head a lane, 33 with
+// eight; one token x 16 heads x 256: 4.6 us with one, 9 with eight).
 #include "attention.h"
 #include "qw35_device.h"
 
@@ -160,27 +164,29 @@ __device__ __forceinline__ void norm_and_turn(const RopeArgs& r, int dim, int la
     }
 }
 
-// Workgroups of four waves; `lanes` lanes a row.  An item is a token with
-// `per_item` heads, which share the angles.
-template <class TI, class TO>
+// Workgroups of four waves; 2^log2_lanes lanes a row.  An item is a token with up
+// to H heads, which share the angles.
+template <class TI, class TO, int H>
 __global__ __launch_bounds__(256) void rotate_kernel(HeadsView x, HeadsView y, int n_tokens, int heads, int dim,
-                                                     int lanes, int per_item, RopeArgs rope) {
-    const int lane = threadIdx.x & 63;
-    const int li = lane & (lanes - 1);
-    const int groups = (heads + per_item - 1) / per_item;
-    const int64_t item = ((int64_t)blockIdx.x * 256 + threadIdx.x) / lanes;
-    const int64_t t64 = item / groups;
-    const bool live = t64 < n_tokens && li * 8 < dim;
-    const int t = live ? (int)t64 : 0;
-    const int h0 = (int)(item - t64 * groups) * per_item;
+                                                     int log2_lanes, RopeArgs rope) {
+    const int lanes = 1 << log2_lanes, li = threadIdx.x & (lanes - 1);
+    const int groups = (heads + H - 1) / H;
+    const int item = (int)(blockIdx.x << (8 - log2_lanes) | threadIdx.x >> log2_lanes);  // below 2^31
+    const int t0 = item / groups, h0 = (item - t0 * groups) * H;
+    const bool live = t0 < n_tokens && li * 8 < dim;
+    const int t = live ? t0 : 0;
+    float v[H][8] = {};
+#pragma unroll
+    for (int h = 0; h < H; ++h)
+        if (live && h0 + h < heads)
+            load8<TI>(x.data, t * x.token_stride + (h0 + h) * x.head_stride + li * 8, x.vec, v[h]);
     Turn turn = {};
     if (rope.freq && live && li * 8 < rope.rot_dim) turn = turn_of(rope, n_tokens, t, li * 8);
-    for (int h = h0; h < h0 + per_item; ++h) {
-        const bool on = live && h < heads;
-        float v[8] = {};
-        if (on) load8<TI>(x.data, t * x.token_stride + h * x.head_stride + li * 8, x.vec, v);
-        norm_and_turn(rope, dim, lanes, li, turn, v);
-        if (on) store8<TO>(y.data, t * y.token_stride + h * y.head_stride + li * 8, y.vec, v);
+#pragma unroll
+    for (int h = 0; h < H; ++h) {
+        norm_and_turn(rope, dim, lanes, li, turn, v[h]);
+        if (live && h0 + h < heads)
+            store8<TO>(y.data, t * y.token_stride + (h0 + h) * y.head_stride + li * 8, y.vec, v[h]);
     }
 }
 
@@ -196,97 +202,136 @@ __device__ __forceinline__ Slot slot_of(int64_t slot, int page_size, bool small)
     return s;
 }
 
-// blockIdx.y 0: keys, 1: values.  An item is one head's row of a token; the
-// rows of a wave are consecutive tokens of a head, whose 16-byte granules of a
-// key page are neighbours.
-//
-// A value page holds eight tokens of a column together, so a single token's
-// row is dim elements at a stride of eight.  Where all eight tokens of such a
-// granule are in this call, in order (a prompt), the token of the first slot
-// reads the eight rows and writes whole granules, and the other seven write
-// nothing; which is the case each row sees from the eight slots around its own.
-template <class TI, class C>
-__global__ __launch_bounds__(256) void kv_append_kernel(qw35_hip_kv_cache cache, HeadsView k, HeadsView v,
-                                                        int n_tokens, const int64_t* slots, int lanes, RopeArgs rope) {
-    const int lane = threadIdx.x & 63;
-    const int li = lane & (lanes - 1);
+// Keys.  An item is a token with up to H heads, as in rotate_kernel; the rows
+// of a wave are consecutive tokens, whose 16-byte granules of a key page are
+// neighbours.
+template <class TI, class C, int H>
+__device__ __forceinline__ void append_keys(const qw35_hip_kv_cache& cache, const HeadsView& k, int n_tokens,
+                                            const int64_t* slots, int log2_lanes, const RopeArgs& rope) {
+    const int lanes = 1 << log2_lanes, li = threadIdx.x & (lanes - 1);
     const int dim = (int)cache.head_dim, heads = (int)cache.kv_heads, page = (int)cache.page_size;
     const int64_t n_slots = (int64_t)cache.n_pages * page;
-    const bool small = n_slots <= 0xffffffffll;
-    const int64_t item = ((int64_t)blockIdx.x * 256 + threadIdx.x) / lanes;
-    const int64_t h64 = item / n_tokens;
-    const int t = (int)(item - h64 * n_tokens);
-    const int64_t slot = h64 < heads ? slots[t] : -1;
+    const int groups = (heads + H - 1) / H;
+    const int item = (int)(blockIdx.x << (8 - log2_lanes) | threadIdx.x >> log2_lanes);  // below 2^31
+    const int group = item / n_tokens, t = item - group * n_tokens, h0 = group * H;
+    const int64_t slot = group < groups ? slots[t] : -1;
     const bool live = slot >= 0 && slot < n_slots;
-    const int h = live ? (int)h64 : 0;
-    const Slot s = live ? slot_of(slot, page, small) : Slot{0, 0};
-    const int64_t base = (s.page * heads + h) * ((int64_t)page * dim);
-    float x[8] = {};
-    if (blockIdx.y == 0) {
-        Turn turn = {};
-        if (live) {
-            load8<TI>(k.data, t * k.token_stride + h * k.head_stride + li * 8, k.vec, x);
-            if (rope.freq && li * 8 < rope.rot_dim) turn = turn_of(rope, n_tokens, t, li * 8);
-        }
-        norm_and_turn(rope, dim, lanes, li, turn, x);
-        if (!live) return;
-        if constexpr (std::is_same_v<C, Fp8>) {
-            const float scale = cache.k_scale ? cache.k_scale[h] : 1.0f;
+    float x[H][8] = {};
 #pragma unroll
-            for (int j = 0; j < 8; ++j) x[j] /= scale;
+    for (int h = 0; h < H; ++h)
+        if (live && h0 + h < heads)
+            load8<TI>(k.data, t * k.token_stride + (h0 + h) * k.head_stride + li * 8, k.vec, x[h]);
+    Turn turn = {};
+    if (rope.freq && live && li * 8 < rope.rot_dim) turn = turn_of(rope, n_tokens, t, li * 8);
+    const Slot s = live ? slot_of(slot, page, n_slots <= 0xffffffffll) : Slot{0, 0};
+    const int64_t at = s.page * heads * ((int64_t)page * dim) + (s.at / 32) * 32 * dim + li * 256 + (s.at & 31) * 8;
+#pragma unroll
+    for (int h = 0; h < H; ++h) {
+        norm_and_turn(rope, dim, lanes, li, turn, x[h]);
+        if (live && h0 + h < heads) {
+            if constexpr (std::is_same_v<C, Fp8>) {
+                const float scale = cache.k_scale ? cache.k_scale[h0 + h] : 1.0f;
+#pragma unroll
+                for (int j = 0; j < 8; ++j) x[h][j] /= scale;
+            }
+            store_granule<C>(cache.k, at + (int64_t)(h0 + h) * page * dim, x[h]);
         }
-        store_granule<C>(cache.k, base + (int64_t)(s.at / 32) * 32 * dim + li * 256 + (s.at & 31) * 8, x);
-        return;
     }
+}
+
+// Values.  A value page holds eight tokens of a column together, so a token's
+// row by itself is dim elements at a stride of eight.  A wave takes eight
+// tokens of a head, eight lanes a token; where they are the eight of a granule
+// (a prompt, whose first token's slot says where granules begin), they change
+// places in LDS and the wave writes 64 whole granules, 1 KB, at a time.
+// Otherwise every lane writes its elements.
+template <class TI, class C>
+__device__ __forceinline__ void append_values(const qw35_hip_kv_cache& cache, const HeadsView& v, int n_tokens,
+                                              const int64_t* slots) {
+    // 8 columns x 8 tokens a lane group, 8 floats apart from the next: a wave's writes and reads meet no bank twice
+    __shared__ __align__(16) float block[4][8 * 72];
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, j = lane >> 3, part = lane & 7;
+    const int dim = (int)cache.head_dim, heads = (int)cache.kv_heads, page = (int)cache.page_size;
+    const int64_t n_slots = (int64_t)cache.n_pages * page;
+    const int item = (int)blockIdx.x * 4 + wave, octet = item / heads, h = item - octet * heads;
+    const int shift = (int)(slots[0] & 7);
+    if (octet * 8 - shift >= n_tokens) return;
+    const int t = octet * 8 - shift + j;
+    const bool in = t >= 0 && t < n_tokens;
+    const int64_t slot = in ? slots[t] : -1;
+    const bool live = slot >= 0 && slot < n_slots;
+    const int64_t first = (int64_t)((uint64_t)(uint32_t)__builtin_amdgcn_readfirstlane((int)(slot >> 32)) << 32 |
+                                    (uint32_t)__builtin_amdgcn_readfirstlane((int)slot));
+    const bool whole = __all(live && slot == first + j && (first & 7) == 0);
     float scale = 1.0f;
     if constexpr (std::is_same_v<C, Fp8>) {
         if (cache.v_scale) scale = cache.v_scale[h];
     }
-    // the slots of this row's granule: lane j of the row looks at its j-th token
-    const int first = t - (s.at & 7);
-    bool mine = false;
-    if (live && li < 8) {
-        const int i = first + li;
-        mine = i >= 0 && i < n_tokens && slots[i] == slot - (s.at & 7) + li;
-    }
-    const uint64_t votes = __ballot(mine) >> (lane & ~(lanes - 1));
-    if (!live) return;
-    const int64_t at = base + (int64_t)(s.at / 8) * 8 * dim + li * 64;
-    if ((votes & 0xff) == 0xff) {
-        if (s.at & 7) return;
-        float w[8][8];  // [column][token]
+    const Slot s = live ? slot_of(slot, page, n_slots <= 0xffffffffll) : Slot{0, 0};
+    const int64_t at = (s.page * heads + h) * ((int64_t)page * dim) + (int64_t)(s.at / 8) * 8 * dim;
+    for (int c0 = 0; c0 < dim; c0 += 64) {
+        const int col = c0 + part * 8;
+        float x[8] = {};
+        if (live) load8<TI>(v.data, t * v.token_stride + h * v.head_stride + col, v.vec, x);
+        if constexpr (std::is_same_v<C, Fp8>) {
 #pragma unroll
-        for (int i = 0; i < 8; ++i) {
-            load8<TI>(v.data, (t + i) * v.token_stride + h * v.head_stride + li * 8, v.vec, x);
-#pragma unroll
-            for (int j = 0; j < 8; ++j) w[j][i] = std::is_same_v<C, Fp8> ? x[j] / scale : x[j];
+            for (int i = 0; i < 8; ++i) x[i] /= scale;
         }
+        if (whole) {
+            float* const b = block[wave];
 #pragma unroll
-        for (int j = 0; j < 8; ++j) store_granule<C>(cache.v, at + j * 8, w[j]);
-        return;
+            for (int i = 0; i < 8; ++i) b[part * 72 + i * 8 + j] = x[i];
+            __builtin_amdgcn_wave_barrier();
+            const float4_t* const g = reinterpret_cast<const float4_t*>(b + lane * 8 + (lane >> 3) * 8);
+            const float4_t lo = g[0], hi = g[1];
+            __builtin_amdgcn_wave_barrier();
+            const float w[8] = {lo[0], lo[1], lo[2], lo[3], hi[0], hi[1], hi[2], hi[3]};
+            store_granule<C>(cache.v, at + (c0 + lane) * 8, w);
+        } else if (live) {
+#pragma unroll
+            for (int i = 0; i < 8; ++i) store_one<C>(cache.v, at + (col + i) * 8 + (s.at & 7), x[i]);
+        }
     }
-    load8<TI>(v.data, t * v.token_stride + h * v.head_stride + li * 8, v.vec, x);
-#pragma unroll
-    for (int j = 0; j < 8; ++j)
-        store_one<C>(cache.v, at + j * 8 + (s.at & 7), std::is_same_v<C, Fp8> ? x[j] / scale : x[j]);
+}
+
+// blockIdx.y 0: keys, 1: values.
+template <class TI, class C, int H>
+__global__ __launch_bounds__(256) void kv_append_kernel(qw35_hip_kv_cache cache, HeadsView k, HeadsView v,
+                                                        int n_tokens, const int64_t* slots, int log2_lanes, RopeArgs rope) {
+    if (blockIdx.y == 0) append_keys<TI, C, H>(cache, k, n_tokens, slots, log2_lanes, rope);
+    else append_values<TI, C>(cache, v, n_tokens, slots);
 }
 
 // Lanes of a row: the power of two that holds dim / 8.
-int row_lanes(int dim) {
-    int lanes = 1;
-    while (lanes * 8 < dim) lanes *= 2;
-    return lanes;
+int row_lanes_log2(int dim) {
+    int n = 0;
+    while (8 << n < dim) ++n;
+    return n;
+}
+
+// Heads of a lane: as many as leave 1024 waves.
+int lane_heads(int n_tokens, int heads, int log2_lanes) {
+    const int64_t waves = ((int64_t)n_tokens * heads << log2_lanes) / 64;
+    return heads >= 8 && waves >= 8 * 1024 ? 8 : heads >= 4 && waves >= 4 * 1024 ? 4 : 1;
+}
+
+template <class TI, class TO, int H>
+hipError_t rotate_heads(const HeadsView& x, const HeadsView& y, int n_tokens, int heads, int dim, int log2_lanes,
+                        const RopeArgs& rope, hipStream_t stream) {
+    const int64_t items = (int64_t)n_tokens * ((heads + H - 1) / H);
+    rotate_kernel<TI, TO, H>
+        <<<dim3((unsigned)(((items << log2_lanes) + 255) / 256)), 256, 0, stream>>>(x, y, n_tokens, heads, dim, log2_lanes,
+                                                                            rope);
+    return hipGetLastError();
 }
 
 template <class TI, class TO>
 hipError_t rotate_as(const HeadsView& x, const HeadsView& y, int n_tokens, int heads, int dim, const RopeArgs& rope,
                      hipStream_t stream) {
-    const int lanes = row_lanes(dim);
-    const int per_item = 1;
-    const int64_t items = (int64_t)n_tokens * ((heads + per_item - 1) / per_item);
-    const int64_t grid = (items * lanes + 255) / 256;
-    rotate_kernel<TI, TO><<<dim3((unsigned)grid), 256, 0, stream>>>(x, y, n_tokens, heads, dim, lanes, per_item, rope);
-    return hipGetLastError();
+    const int lanes = row_lanes_log2(dim), h = lane_heads(n_tokens, heads, lanes);
+    return h == 8   ? rotate_heads<TI, TO, 8>(x, y, n_tokens, heads, dim, lanes, rope, stream)
+           : h == 4 ? rotate_heads<TI, TO, 4>(x, y, n_tokens, heads, dim, lanes, rope, stream)
+                    : rotate_heads<TI, TO, 1>(x, y, n_tokens, heads, dim, lanes, rope, stream);
 }
 
 template <class TI>
@@ -299,13 +344,23 @@ hipError_t rotate_from(const HeadsView& x, const HeadsView& y, int n, int heads,
     }
 }
 
+template <class TI, class C, int H>
+hipError_t append_heads(const qw35_hip_kv_cache& cache, const HeadsView& k, const HeadsView& v, int n, int log2_lanes,
+                        const int64_t* slots, const RopeArgs& rope, hipStream_t stream) {
+    const int heads = (int)cache.kv_heads;
+    const int64_t keys = (((int64_t)n * ((heads + H - 1) / H) << log2_lanes) + 255) / 256;
+    const int64_t values = ((int64_t)(n + 14) / 8 * heads + 3) / 4;  // (the first octet may begin before the tokens)
+    kv_append_kernel<TI, C, H><<<dim3((unsigned)(keys > values ? keys : values), 2), 256, 0, stream>>>(cache, k, v, n, slots,
+                                                                                                   log2_lanes, rope);
+    return hipGetLastError();
+}
+
 template <class TI, class C>
 hipError_t append_as(const qw35_hip_kv_cache& cache, const HeadsView& k, const HeadsView& v, int n,
                      const int64_t* slots, const RopeArgs& rope, hipStream_t stream) {
-    const int lanes = row_lanes((int)cache.head_dim);
-    const int64_t grid = ((int64_t)n * cache.kv_heads * lanes + 255) / 256;
-    kv_append_kernel<TI, C><<<dim3((unsigned)grid, 2), 256, 0, stream>>>(cache, k, v, n, slots, lanes, rope);
-    return hipGetLastError();
+    const int lanes = row_lanes_log2((int)cache.head_dim), h = lane_heads(n, (int)cache.kv_heads, lanes);
+    return h >= 4 ? append_heads<TI, C, 4>(cache, k, v, n, lanes, slots, rope, stream)
+                  : append_heads<TI, C, 1>(cache, k, v, n, lanes, slots, rope, stream);
 }
 
 template <class TI>
