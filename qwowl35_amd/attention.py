@@ -287,3 +287,79 @@ def prefix_attention(q: torch.Tensor, cache: PagedCache, pages: torch.Tensor, le
                          workspace.data_ptr(), workspace.nbytes)
     _call("qw35_hip_prefix_attention", op, cache._at, _stream(stream))
     return out
+
+
+class GatedAttention:
+    """One attention layer between its input norm and the residual stream, as the
+    reference records it (Qw35MetalRuntime+Attention.m:13-117): the q / k / v
+    projections, ``rotate`` of the queries, ``kv_append``, ``prefix_attention``
+    with the output gate and the output projection added to the residual.
+
+    ``weights``: ``attn_q`` (heads x [queries, then gates] if the rows are twice
+    heads x dim, else queries only), ``attn_k``, ``attn_v`` and ``attn_output`` as
+    ``HipWeight``.  Up to 8 tokens run the decode GEMVs, more the prefill matmul
+    (fp32 activations).  Nothing of a call is kept but the cache: a call can be
+    recorded into a graph, with lengths, slots, positions and pages on the device."""
+
+    def __init__(self, weights: dict, cache: PagedCache, heads: int, rope: Rotary | None,
+                 q_norm: torch.Tensor | None = None, k_norm: torch.Tensor | None = None, eps: float = 1e-6,
+                 max_seqs: int = 8, max_tokens: int = 8, window: int = 0, sink: int = 0):
+        dim, q_rows = cache.head_dim, weights["attn_q"].rows
+        self.gated = q_rows == 2 * heads * dim
+        kv = cache.kv_heads * dim
+        if q_rows not in (heads * dim, 2 * heads * dim) or weights["attn_k"].rows != kv or weights["attn_v"].rows != kv:
+            raise Qw35Error(f"attn_q, attn_k and attn_v have {q_rows}, {weights['attn_k'].rows} and "
+                            f"{weights['attn_v'].rows} rows for {heads} heads and {cache.kv_heads} kv heads of {dim}")
+        if weights["attn_output"].k != heads * dim:
+            raise Qw35Error(f"attn_output has {weights['attn_output'].k} columns for {heads} heads of {dim}")
+        device = cache.k.device
+        self.weights, self.cache, self.heads, self.rope, self.eps = weights, cache, heads, rope, eps
+        self.q_norm, self.k_norm, self.window, self.sink = q_norm, k_norm, window, sink
+        # an 8-bit cache takes either 16-bit type: fp16 keeps more of a normed query
+        self.q_dtype = torch.float16 if cache.k.dtype == torch.float8_e4m3fn else cache.k.dtype
+        self.max_seqs, self.max_tokens = max_seqs, max_tokens
+        self.workspace = prefix_attention_workspace(cache, heads, max_seqs, max_tokens, device=device)
+        self.prefill_workspace = None
+        if max_tokens > _ffi.MAX_BATCH:
+            size = max(int(_ffi.load().qw35_hip_matmul_prefill_workspace_size(C.byref(w.prefill.view), max_tokens))
+                       for w in weights.values())
+            self.prefill_workspace = torch.empty(size, dtype=torch.uint8, device=device)
+
+    def _project(self, name: str, x: torch.Tensor, stream) -> torch.Tensor:
+        w = self.weights[name]
+        if x.shape[0] <= _ffi.MAX_BATCH:
+            return rt.decode_matvec(w, x, stream=stream)
+        return rt.matmul_prefill(w.prefill, x, out_dtype=torch.float32, workspace=self.prefill_workspace, stream=stream)
+
+    def __call__(self, x: torch.Tensor, residual: torch.Tensor, positions: torch.Tensor, slots: torch.Tensor,
+                 pages: torch.Tensor, lengths: torch.Tensor, starts: torch.Tensor | None = None, max_new: int = 0,
+                 prefix_pages: torch.Tensor | None = None, prefix_len: int = 0, stream=None) -> torch.Tensor:
+        """Adds the layer's output for the normed inputs x (fp32 [n_tokens, embedding])
+        to ``residual`` (fp32, same shape) and returns it.  ``slots`` are the new
+        tokens' places in the cache, the other arguments ``rotate``'s and
+        ``prefix_attention``'s (``lengths`` count the new tokens)."""
+        n, dim, cache = int(x.shape[0]), self.cache.head_dim, self.cache
+        if n > self.max_tokens or lengths.shape[0] > self.max_seqs:
+            raise Qw35Error(f"{n} tokens of {lengths.shape[0]} sequences are over the layer's {self.max_tokens} and "
+                            f"{self.max_seqs}")
+        if residual.shape != x.shape or residual.dtype != torch.float32 or not residual.is_contiguous():
+            raise Qw35Error(f"residual must be a contiguous fp32 {list(x.shape)} tensor")
+        if n == 0:
+            return residual
+        q = self._project("attn_q", x, stream).view(n, self.heads, -1)
+        k = self._project("attn_k", x, stream).view(n, cache.kv_heads, dim)
+        v = self._project("attn_v", x, stream).view(n, cache.kv_heads, dim)
+        turned = rotate(q[..., :dim], self.rope, positions, norm=self.q_norm, eps=self.eps, out_dtype=self.q_dtype,
+                        stream=stream)
+        kv_append(cache, k, v, slots, rope=self.rope, positions=positions, norm=self.k_norm, eps=self.eps, stream=stream)
+        core = prefix_attention(turned, cache, pages, lengths, starts, max_new=max_new, prefix_pages=prefix_pages,
+                                prefix_len=prefix_len, window=self.window, sink=self.sink,
+                                gate=q[..., dim:] if self.gated else None, out_dtype=torch.float32,
+                                workspace=self.workspace, stream=stream).view(n, -1)
+        out = self.weights["attn_output"]
+        if n <= _ffi.MAX_BATCH:
+            rt.decode_matvec(out, core, dst=residual, residual=True, stream=stream)
+        else:
+            rt.matmul_prefill(out.prefill, core, out_dtype=torch.float32, dst=residual, workspace=self.prefill_workspace,
+                              epilogue=_ffi.EPILOGUE_ADD, stream=stream)
+        return residual
