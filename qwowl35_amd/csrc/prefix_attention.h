@@ -198,17 +198,28 @@ __device__ __forceinline__ int seq_of(const AttnArgs& a, int t) {
     return a.starts ? last_at(a.starts, a.n_seqs, t) : t;
 }
 
-// The same of a token that the wave's lanes have alike: 64 starts a load.
-__device__ __forceinline__ int seq_of_wave(const AttnArgs& a, int t, int lane) {
-    if (!a.starts) return t;
-    int s = -1;
+// The same of a token that the wave's lanes have alike, with the new tokens of
+// that sequence (none of a token in no sequence): 64 starts a load.
+struct Place {
+    int s, q0, q1;
+};
+__device__ __forceinline__ Place place_of(const AttnArgs& a, int t, int lane) {
+    if (!a.starts) return {t, t, t + 1};
+    Place p = {-1, 0, 0};
     for (int s0 = 0; s0 < a.n_seqs; s0 += 64) {
-        const bool at = s0 + lane < a.n_seqs && a.starts[s0 + lane] <= t;
-        const uint64_t votes = __ballot(at);
-        if (votes) s = s0 + 63 - __builtin_clzll(votes);
+        const int at = s0 + lane < a.n_seqs ? s0 + lane : a.n_seqs - 1;
+        const int start = a.starts[at], end = a.starts[at + 1];
+        const uint64_t votes = __ballot(s0 + lane < a.n_seqs && start <= t);
+        if (votes) {
+            const int l = 63 - __builtin_clzll(votes);
+            p.s = s0 + l;
+            p.q0 = clampi(__builtin_amdgcn_readlane(start, l), 0, a.n_tokens);
+            p.q1 = clampi(__builtin_amdgcn_readlane(end, l), p.q0, a.n_tokens);
+        }
         if (votes != ~0ull) break;
     }
-    return s;
+    if (t < p.q0 || t >= p.q1) p.s = -1;
+    return p;
 }
 
 // Tokens [lo, hi) and [0, sink) of a unit's n are seen.
@@ -585,34 +596,39 @@ __device__ __forceinline__ bool next_own(const AttnArgs& a, Line& line, const ui
 // ---- a row's result ------------------------------------------------------------------------------------------------
 
 // K groups of N (4, 2 or 1) consecutive columns, from `col` on and `stride`
-// apart, gated, in the output's type.
+// apart: the gates of a row, and the row gated, in the output's type.
 template <int K, int N>
-__device__ __forceinline__ void finish(const AttnArgs& a, int t, int head, int col, int stride, float (&v)[K][N]) {
+__device__ __forceinline__ void load_gates(const AttnArgs& a, int t, int head, int col, int stride, float (&g)[K][N]) {
+    if (!a.gate.data) return;
+    const int64_t at = t * a.gate.token_stride + head * a.gate.head_stride + col;
+    auto get = [&](auto zero) {
+        typedef decltype(zero) T;
+        typedef T vec_t __attribute__((ext_vector_type(N > 1 ? N : 2)));
+        const T* const from = static_cast<const T*>(a.gate.data) + at;
+        if (N > 1 && a.gate.vec) {
+            vec_t w[K];
+#pragma unroll
+            for (int k = 0; k < K; ++k) w[k] = *reinterpret_cast<const vec_t*>(from + k * stride);
+#pragma unroll
+            for (int k = 0; k < K; ++k)
+#pragma unroll
+                for (int j = 0; j < N; ++j) g[k][j] = (float)w[k][j];
+        } else {
+#pragma unroll
+            for (int k = 0; k < K; ++k)
+#pragma unroll
+                for (int j = 0; j < N; ++j) g[k][j] = (float)from[k * stride + j];
+        }
+    };
+    if (a.gate.dtype == QW35_HIP_DTYPE_F32) get(0.0f);
+    else if (a.gate.dtype == QW35_HIP_DTYPE_F16) get((_Float16)0.0f);
+    else get((__bf16)0.0f);
+}
+
+template <int K, int N>
+__device__ __forceinline__ void finish(const AttnArgs& a, int t, int head, int col, int stride, const float (&g)[K][N],
+                                       float (&v)[K][N]) {
     if (a.gate.data) {
-        const int64_t at = t * a.gate.token_stride + head * a.gate.head_stride + col;
-        float g[K][N];
-        auto get = [&](auto zero) {
-            typedef decltype(zero) T;
-            typedef T vec_t __attribute__((ext_vector_type(N > 1 ? N : 2)));
-            const T* const from = static_cast<const T*>(a.gate.data) + at;
-            if (N > 1 && a.gate.vec) {
-                vec_t w[K];
-#pragma unroll
-                for (int k = 0; k < K; ++k) w[k] = *reinterpret_cast<const vec_t*>(from + k * stride);
-#pragma unroll
-                for (int k = 0; k < K; ++k)
-#pragma unroll
-                    for (int j = 0; j < N; ++j) g[k][j] = (float)w[k][j];
-            } else {
-#pragma unroll
-                for (int k = 0; k < K; ++k)
-#pragma unroll
-                    for (int j = 0; j < N; ++j) g[k][j] = (float)from[k * stride + j];
-            }
-        };
-        if (a.gate.dtype == QW35_HIP_DTYPE_F32) get(0.0f);
-        else if (a.gate.dtype == QW35_HIP_DTYPE_F16) get((_Float16)0.0f);
-        else get((__bf16)0.0f);
 #pragma unroll
         for (int k = 0; k < K; ++k)
 #pragma unroll
@@ -735,6 +751,11 @@ __device__ __forceinline__ void copy_kb(const uint8_t* from, uint8_t* to, int la
         if (i + 2 < kCount) __builtin_amdgcn_global_load_lds((global_t*)g, (lds_t*)l, 16, 2048, 0);
         if (i + 3 < kCount) __builtin_amdgcn_global_load_lds((global_t*)g, (lds_t*)l, 16, 3072, 0);
     }
+}
+
+// KB i of such a copy.
+__device__ __forceinline__ void copy_1kb(const uint8_t* from, uint8_t* to, int i, int lane) {
+    copy_kb<1>(from + i * 1024, to + i * 1024, lane);
 }
 
 template <int D>
@@ -872,11 +893,10 @@ struct Unit {
         return top;
     }
 
-    // The reference follows the rows' largest scores.
-    __device__ __forceinline__ void follow(Rows& w, float largest_) const {
-        const float top = row_max<kRows>(largest_) * w.scale;
-        if (__builtin_expect(__any(top > w.mx + kRise), 0)) {
-            const float m_new = fmaxf(w.mx, top);
+    // The reference follows the rows' largest scores (`largest`: of this lane's).
+    __device__ __forceinline__ void follow(Rows& w, float largest) const {
+        if (__builtin_expect(__any(largest * w.scale > w.mx + kRise), 0)) {
+            const float m_new = fmaxf(w.mx, row_max<kRows>(largest) * w.scale);
             const float shrink = m_new == w.mx ? 1.0f : __builtin_amdgcn_exp2f(w.mx - m_new);
             w.l *= shrink;
 #pragma unroll
@@ -1094,16 +1114,18 @@ struct Unit {
         uint32_t* const marks = sh.marks[wave];
         uint8_t* const ring = sh.ring + (kShared ? 0 : wave * (kRing / kWaves));
         uint32_t there_bits = 0;  // of the tiles loaded last, the newest in bit 0
-        auto note = [&](uint32_t block) { there_bits = there_bits << 1 | (block != kNoBlock ? 1u : 0u); };
+        bool missing = false;     // one of them is not there
+        auto note = [&](uint32_t block) {
+            there_bits = there_bits << 1 | (block != kNoBlock ? 1u : 0u);
+            missing |= block == kNoBlock;
+        };
         // shared: this wave's quarter of a pair of tiles
-        auto load_quarter = [&](int i) {
+        auto quarter_of = [&](int i, const uint8_t*& from, uint8_t*& to) {
             const uint32_t block = block_of(pages, i);
             note(block);
-            const int64_t at = bytes_at(block);
-            uint8_t* const to = ring + (i % kPairs) * 2 * kTile;
-            const uint8_t* const from = wave < 2 ? kbase : vbase;
             const int part = (wave & 1) * (kTile / 2);
-            copy_kb<kKb / 2>(from + at + part, to + (wave < 2 ? 0 : kTile) + part, lane);
+            from = (wave < 2 ? kbase : vbase) + bytes_at(block) + part;
+            to = ring + (i % kPairs) * 2 * kTile + (wave < 2 ? 0 : kTile) + part;
         };
 
         Rows w;
@@ -1111,7 +1133,12 @@ struct Unit {
         load_queries(w, sq, h, row0, row_end);
         int loaded = 0;
         if constexpr (kShared) {
-            for (; loaded < kPairs - 1 && loaded < pages.count; ++loaded) load_quarter(loaded);
+            for (; loaded < kPairs - 1 && loaded < pages.count; ++loaded) {
+                const uint8_t* from;
+                uint8_t* to;
+                quarter_of(loaded, from, to);
+                copy_kb<kKb / 2>(from, to, lane);
+            }
         } else {
             for (; loaded < kPairs && loaded < pages.count; ++loaded) {
                 const uint32_t block = block_of(pages, loaded);
@@ -1137,10 +1164,13 @@ struct Unit {
             asm volatile("" ::: "memory");
             scores(ring, w, s);
             top = largest(s);
+            // steps between which every row sees all of a tile (none of the sink's)
+            const int clear0 = tiles.sink + ((w.all_lo + 31) / 32 > tiles.lo ? (w.all_lo + 31) / 32 - tiles.lo : 0) - pages.first;
+            const int clear1 = tiles.sink + w.all_hi / 32 - tiles.lo - pages.first;
             auto see_and_follow = [&](int i) {
-                const bool there = there_bits >> (loaded - 1 - i) & 1;
-                const int t0 = tiles.at(pages.first + i) * 32;
-                if (partly(w, t0, there)) {
+                if (i < clear0 || i >= clear1 || missing) {
+                    const bool there = there_bits >> (loaded - 1 - i) & 1;
+                    const int t0 = tiles.at(pages.first + i) * 32;
                     split_off_infinities<true>(ring + (i % kPairs) * 2 * kTile + kTile, w, t0, there, marks);
                     mask(w, s, t0, there);
                     top = largest(s);
@@ -1148,31 +1178,37 @@ struct Unit {
                 follow(w, top);
             };
             vec8 p[kK];
-            int i = 0;
-            for (; i + 1 < pages.count; ++i) {
+            // A tile's copies go out one by one among the matrix instructions:
+            // together they would wait for each other (32 KB at 64 bytes a cycle).
+            auto step = [&](int i, auto copies) {
                 see_and_follow(i);
-                if (i + kPairs - 2 < pages.count) wait_vm<(kPairs - 3) * kEach>();
+                if (copies) wait_vm<(kPairs - 3) * kEach>();
                 else wait_vm<0>();
                 __builtin_amdgcn_s_barrier();  // tile i + 1 is there, and tile i - 1 read by all
                 asm volatile("" ::: "memory");
-                if (loaded < pages.count) load_quarter(loaded++);
+                const uint8_t* from = nullptr;
+                uint8_t* to = nullptr;
+                if (copies) quarter_of(loaded++, from, to);
                 __builtin_amdgcn_sched_barrier(0);
                 acc next[kB];
-                constexpr int kAll = kScores;
+                static_assert(kEach <= kScoreSteps, "a copy a step");
                 scores(ring + ((i + 1) % kPairs) * 2 * kTile, w, next, [&](int m) {
-                    terms(w, s, p, kAll * m / kScoreSteps, kAll * (m + 1) / kScoreSteps);
+                    if (copies && m < kEach) copy_1kb(from, to, m, lane);
+                    terms(w, s, p, kScores * m / kScoreSteps, kScores * (m + 1) / kScoreSteps);
                 });
                 top = -__builtin_inff();
                 add_values(ring + (i % kPairs) * 2 * kTile + kTile, w, p, [&](int m) {
 #pragma unroll
-                    for (int x = kAll * m / kValueSteps; x < kAll * (m + 1) / kValueSteps; ++x) {
-                        const int j = x;
+                    for (int j = kScores * m / kValueSteps; j < kScores * (m + 1) / kValueSteps; ++j) {
                         top = fmaxf(top, next[j / kAcc][j % kAcc]);
                         s[j / kAcc][j % kAcc] = next[j / kAcc][j % kAcc];
                     }
                 });
                 wait_lds();
-            }
+            };
+            int i = 0;
+            for (; i + kPairs - 1 < pages.count; ++i) step(i, std::true_type{});
+            for (; i + 1 < pages.count; ++i) step(i, std::false_type{});
             see_and_follow(i);
             terms(w, s, p);
             add_values(ring + (i % kPairs) * 2 * kTile + kTile, w, p);
@@ -1243,14 +1279,15 @@ struct Unit {
             if (row < row_end) {
 #pragma unroll 1
                 for (int i = 0; i < kQuads; i += 4) {
-                    float x[4][4];
+                    float x[4][4], gates[4][4];
+                    load_gates(a, sq.q0 + tok, head, i * kQuadCols + g * 4, kQuadCols, gates);
 #pragma unroll
                     for (int c = 0; c < 4; ++c) {
                         const float4_t y = left(wave)[(i + c) * 64 + lane];
 #pragma unroll
                         for (int j = 0; j < 4; ++j) x[c][j] = y[j] * inv;
                     }
-                    finish(a, sq.q0 + tok, head, i * kQuadCols + g * 4, kQuadCols, x);
+                    finish(a, sq.q0 + tok, head, i * kQuadCols + g * 4, kQuadCols, gates, x);
                 }
             }
             wait_lds();

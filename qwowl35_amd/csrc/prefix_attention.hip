@@ -46,31 +46,30 @@ __global__ __launch_bounds__(256) void prefix_attention_join(AttnArgs a, int wav
     __shared__ float sh_m[4], sh_l[4];
     const int lane = threadIdx.x & 63, wave = attn::uniform((int)(threadIdx.x >> 6));
     const int heads = a.kv_heads * a.group;
+    const bool waves_join = waves > 1;
     const int item = waves == 1 ? (int)blockIdx.x * 4 + wave : (int)blockIdx.x;  // below 2^30
     const int t = (int)((uint32_t)item / (uint32_t)heads), head = item - t * heads;
     if (t >= a.n_tokens) return;
     const int h = attn::token_of(a, head), in_group = head - h * a.group;
     const attn::MetaHead meta = *reinterpret_cast<const attn::MetaHead*>(a.meta);
     const int* const first = reinterpret_cast<const int*>(a.meta + attn::meta_first_at());
-    const int s = attn::uniform(attn::seq_of_wave(a, t, lane));
+    float gates[1][N];
+    if (!waves_join || wave == 0) attn::load_gates(a, t, head, lane * N, 0, gates);  // (on their way meanwhile)
+    const attn::Place at = attn::place_of(a, t, lane);
     attn::Pieces own = {0, 0}, pre = {0, 0};
     int own_row = 0, pre_row = 0;
-    if (s >= 0) {
-        const int q0 = a.starts ? attn::clampi(a.starts[s], 0, a.n_tokens) : t;
-        const int q1 = a.starts ? attn::clampi(a.starts[s + 1], q0, a.n_tokens) : t + 1;
-        if (t >= q0 && t < q1) {
-            const attn::Pieces* const pieces =
-                reinterpret_cast<const attn::Pieces*>(a.meta + attn::meta_pieces_at(a.n_seqs)) +
-                (int64_t)h * (a.plan.prefix_entries + meta.own_entries);
-            own_row = (t - q0) * a.group + in_group;
-            const int e = (meta.lanes ? s : first[s]) + (own_row >> a.plan.own.log2_rows);
-            own_row &= (1 << a.plan.own.log2_rows) - 1;
-            if (e < meta.own_entries) own = pieces[a.plan.prefix_entries + e];
-            if (a.plan.prefix_entries) {
-                pre_row = t * a.group + in_group;
-                pre = pieces[pre_row >> a.plan.prefix.log2_rows];
-                pre_row &= (1 << a.plan.prefix.log2_rows) - 1;
-            }
+    if (at.s >= 0) {
+        const attn::Pieces* const pieces =
+            reinterpret_cast<const attn::Pieces*>(a.meta + attn::meta_pieces_at(a.n_seqs)) +
+            (int64_t)h * (a.plan.prefix_entries + meta.own_entries);
+        own_row = (t - at.q0) * a.group + in_group;
+        const int e = (meta.lanes ? at.s : first[at.s]) + (own_row >> a.plan.own.log2_rows);
+        own_row &= (1 << a.plan.own.log2_rows) - 1;
+        if (e < meta.own_entries) own = pieces[a.plan.prefix_entries + e];
+        if (a.plan.prefix_entries) {
+            pre_row = t * a.group + in_group;
+            pre = pieces[pre_row >> a.plan.prefix.log2_rows];
+            pre_row &= (1 << a.plan.prefix.log2_rows) - 1;
         }
     }
     if (!a.plan.prefix_entries && own.n == 1) return;  // the main kernel finished this row (all waves of it return)
@@ -81,7 +80,7 @@ __global__ __launch_bounds__(256) void prefix_attention_join(AttnArgs a, int wav
     // 64 parts at a time: lane i reads the maximum and sum of part i, then every lane its columns of all of them
     for (int k = k0; k < n; k += 64 * waves) {
         const int mine = k + lane * waves;
-        const float* at = a.part;
+        const float* row_at = a.part;
         float pm = -__builtin_inff(), pl = 0.0f;
         if (mine < n) {
             const bool is_own = mine < own_n;
@@ -89,7 +88,7 @@ __global__ __launch_bounds__(256) void prefix_attention_join(AttnArgs a, int wav
             const int row = is_own ? own_row : pre_row;
             const uint64_t slot = is_own ? own.slot0 + mine : pre.slot0 + (mine - own_n);
             const float* const p = (is_own ? a.own_part : a.part) + slot * attn::slot_floats(1 << log2_rows, D);
-            at = p + row * D;
+            row_at = p + row * D;
             pm = p[(D << log2_rows) + row];
             pl = p[((D + 1) << log2_rows) + row];
         }
@@ -102,7 +101,7 @@ __global__ __launch_bounds__(256) void prefix_attention_join(AttnArgs a, int wav
         const float weight = attn::part_weight(pm, now);
         sum += weight * pl;
         const int rest = (n - k + waves - 1) / waves, count = rest < 64 ? rest : 64;
-        const int64_t addr = reinterpret_cast<int64_t>(at);
+        const int64_t addr = reinterpret_cast<int64_t>(row_at);
         auto part = [&](int i) {
             const uint32_t lo = (uint32_t)__builtin_amdgcn_readlane((int)addr, i);
             const uint32_t hi = (uint32_t)__builtin_amdgcn_readlane((int)(addr >> 32), i);
@@ -139,7 +138,7 @@ __global__ __launch_bounds__(256) void prefix_attention_join(AttnArgs a, int wav
     // sum: each lane holds its parts' share, rescaled alike
 #pragma unroll
     for (int o = 1; o < 64; o *= 2) sum += __shfl_xor(sum, o);
-    if (waves > 1) {
+    if (waves_join) {
 #pragma unroll
         for (int c = 0; c < N; ++c) sh_o[wave][lane * N + c] = acc[c];
         if (lane == 0) {
@@ -164,7 +163,7 @@ __global__ __launch_bounds__(256) void prefix_attention_join(AttnArgs a, int wav
     float out[1][N];
 #pragma unroll
     for (int c = 0; c < N; ++c) out[0][c] = acc[c] * inv;
-    attn::finish(a, t, head, lane * N, 0, out);
+    attn::finish(a, t, head, lane * N, 0, gates, out);
 }
 
 template <int D>
