@@ -17,19 +17,22 @@ __device__ __forceinline__ float lane_max_f(float v) {
 // Leads and costs in quarters of a microsecond, measured with all compute
 // units at it: a step of a wave's own tiles waits for HBM (7 us for 128 KB of a
 // compute unit's waves; 2.5 where few are at it, so 4 is taken), one of shared
-// tiles for the matrix unit.
+// tiles for the matrix unit.  (Over 16 batches, steps at half and twice these
+// costs, leads of 8 and 32 for own units of 16 rows and of 64 for shared tiles
+// were no faster; 16 instead of 32 for own units of 32 rows cost four windowed
+// sequences 13%, 32 instead of 16 for those of 16 rows 64 short ones 11%.)
 RowSplit split_prefix(int64_t rows, int dim) {
     const int wait = dim == 64 ? 3 : 4;
-    if (rows <= 16) return {2, 0, 4, 1, 0, 24, wait};
-    if (rows <= 32) return {2, 0, 5, 0, 0, 24, wait};
-    if (rows <= 64) return {1, 1, 6, 0, 0, 24, wait};
+    if (rows <= 16) return {2, 0, 4, 1, 0, 48, wait};
+    if (rows <= 32) return {2, 0, 5, 0, 0, 48, wait};
+    if (rows <= 64) return {1, 1, 6, 0, 0, 48, wait};
     return {0, 2, 7, 0, 1, 32, dim == 64 ? 2 : 3};
 }
 
 RowSplit split_own(int64_t rows, int dim) {
     const int wait = dim == 64 ? 3 : 4;
     if (rows <= 16) return {0, 0, 4, 1, 0, 16, wait};
-    if (rows <= 64) return {0, 0, 5, 0, 0, 16, wait};
+    if (rows <= 64) return {0, 0, 5, 0, 0, 32, wait};
     return {0, 2, 7, 0, 1, 32, dim == 64 ? 2 : 3};
 }
 
