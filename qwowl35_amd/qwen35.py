@@ -24,9 +24,10 @@ The layout follows the reference runtime:
   * state, attn_gate rows = ssm_inner, ssm_beta / ssm_alpha rows =
   time_step_rank, ssm_out k = ssm_inner.
 
-Only the projections are run here; the attention, DeltaNet recurrence, norms
-and residual adds between them are not part of this library, so the plan reads
-its inputs from buffers the caller owns and refreshes.
+Only the projections are run here: the plan reads its inputs from buffers the
+caller owns and refreshes.  An attention layer's operators between them are in
+``attention`` (``GatedAttention`` runs a layer); the DeltaNet recurrence, the
+norms and the residual adds are not part of this library.
 """
 from __future__ import annotations
 
