@@ -89,7 +89,7 @@ __global__ __launch_bounds__(256) void prefix_attention_join(AttnArgs a, int wav
             const bool is_own = mine < own_n;
             const int log2_rows = is_own ? a.plan.own.log2_rows : a.plan.prefix.log2_rows;
             const int row = is_own ? own_row : pre_row;
-            const uint64_t slot = is_own ? own.slot0 + mine : pre.slot0 + (mine - own_n);
+            const uint64_t slot = is_own ? own.slot0 + mine : pre.slot0 + (mine - own_n) * meta.prefix_stride;
             const float* const p = (is_own ? a.own_part : a.part) + slot * attn::slot_floats(1 << log2_rows, D);
             row_at = p + row * D;
             pm = p[(D << log2_rows) + row];
