@@ -350,10 +350,12 @@ __device__ __forceinline__ uint64_t line_quotient(const Line& l, uint64_t x, uin
 }
 
 // The piece of a line of `all` at a place of several (past them: none).
-__device__ __forceinline__ Piece piece_of(uint64_t all, int places, int place, const RowSplit& s) {
+__device__ __forceinline__ Piece piece_of(const Line& l, uint64_t all, int places, int place, const RowSplit& s) {
     Piece p = {1, 0, 0, 0, place};
     if (!places) return p;
-    p.per = quotient(all + (uint64_t)(places - 1), (uint64_t)places);
+    // (with 32-bit costs a little more than the quotient will do: every place has the same)
+    if (l.lanes) p.per = (uint32_t)((float)(uint32_t)all * __builtin_amdgcn_rcpf((float)places) * (1.0f + 0x1p-20f)) + 1;
+    else p.per = quotient(all + (uint64_t)(places - 1), (uint64_t)places);
     if (p.per < 1u << s.log2_cost) p.per = 1u << s.log2_cost;  // a step
     p.x = p.x0 = p.per * (uint64_t)place;
     p.x1 = (uint32_t)place >= (uint32_t)places ? 0 : p.x0 + p.per < all ? p.x0 + p.per : all;
@@ -505,7 +507,9 @@ __device__ __forceinline__ Line build_line(const AttnArgs& a, uint64_t* cost, ui
     const uint64_t own_by_group = p.own.shared ? own : own >> 2;
     int eighth = grid / 8;  // workgroups of an XCD for the prefix
     if (!prefix) eighth = 0;
-    else if (own) eighth = clampi((int)((double)prefix / (double)(prefix + own_by_group) * (double)eighth), 1, eighth - 1);
+    else if (own)
+        eighth = clampi((int)((float)prefix * __builtin_amdgcn_rcpf((float)(prefix + own_by_group)) * (float)eighth), 1,
+                        eighth - 1);
     const int xcd = (int)(blockIdx.x & 7), at = (int)(blockIdx.x >> 3), rest = grid / 8 - eighth;
     // Several row tiles go abreast, each with its own workgroup, over the same
     // steps of a head's prefix, which they then read from the L2 (behind each
@@ -514,11 +518,11 @@ __device__ __forceinline__ Line build_line(const AttnArgs& a, uint64_t* cost, ui
     const int tiles = p.prefix_entries, abreast = tiles > 1 && tiles <= eighth ? tiles : 1;
     const int place = xcd * eighth + at, group_of = place / abreast;
     line.prefix_tile = abreast > 1 ? place - group_of * abreast : -1;
-    line.prefix = piece_of(abreast > 1 ? (uint64_t)line.prefix_cost * (uint64_t)a.kv_heads : prefix, eighth * 8 / abreast,
+    line.prefix = piece_of(line, abreast > 1 ? (uint64_t)line.prefix_cost * (uint64_t)a.kv_heads : prefix, eighth * 8 / abreast,
                            at < eighth ? group_of : -1, p.prefix);
     const int group = at < eighth ? -1 : xcd * rest + at - eighth;
-    if (p.own.shared) line.own = piece_of(own, rest * 8, group, p.own);
-    else line.own = piece_of(own, rest * 8 * kWaves, group < 0 ? -1 : group * kWaves + uniform((int)(threadIdx.x >> 6)), p.own);
+    if (p.own.shared) line.own = piece_of(line, own, rest * 8, group, p.own);
+    else line.own = piece_of(line, own, rest * 8 * kWaves, group < 0 ? -1 : group * kWaves + uniform((int)(threadIdx.x >> 6)), p.own);
     if (writes) {  // for the join
         Pieces* const pieces = reinterpret_cast<Pieces*>(a.meta + meta_pieces_at(a.n_seqs));
         if (threadIdx.x == 0) *reinterpret_cast<MetaHead*>(a.meta) = MetaHead{line.own_entries, line.lanes, abreast, 0};
