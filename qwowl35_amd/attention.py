@@ -85,7 +85,7 @@ def _vector(x: torch.Tensor | None, n: int, device: int, name: str) -> int | Non
 def _output(out: torch.Tensor | None, dtype: torch.dtype | None, like: torch.Tensor) -> torch.Tensor:
     """``out``, or a new tensor of like's shape."""
     if out is None:
-        return like.new_empty(like.shape, dtype=dtype or like.dtype)
+        return torch.empty_like(like, dtype=dtype, memory_format=torch.contiguous_format)
     if out.shape != like.shape or out.device != like.device or (dtype or out.dtype) != out.dtype:
         raise Qw35Error(f"out must be a {list(like.shape)} tensor of out_dtype on {like.device}")
     return out

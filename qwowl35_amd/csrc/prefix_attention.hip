@@ -8,10 +8,21 @@ namespace {
 
 constexpr int kBatch = 16;  // parts whose loads are in flight together
 
-__device__ __forceinline__ float lane_max_f(float v) {
-#pragma unroll
-    for (int o = 1; o < 16; o *= 2) v = fmaxf(v, __shfl_xor(v, o));
-    return attn::row_max<16>(v);
+// Over a wave's 64 lanes, in each of them.
+template <class Op>
+__device__ __forceinline__ float over_lanes(float v, Op op) {
+    auto turn = [&](auto by) {  // of 16 lanes
+        const int u = __builtin_bit_cast(int, v);
+        v = op(v, __builtin_bit_cast(float, __builtin_amdgcn_update_dpp(u, u, 0x120 + decltype(by)::value, 0xf, 0xf, false)));
+    };
+    turn(std::integral_constant<int, 8>{});
+    turn(std::integral_constant<int, 4>{});
+    turn(std::integral_constant<int, 2>{});
+    turn(std::integral_constant<int, 1>{});
+    const attn::Pair p = attn::pair_xor16(v);
+    v = op(p.a, p.b);
+    const attn::Pair q = attn::pair_xor32(v);
+    return op(q.a, q.b);
 }
 
 // Leads and costs in quarters of a microsecond, measured with all compute
@@ -39,8 +50,9 @@ RowSplit split_own(int64_t rows, int dim) {
 // One row (token, head) for each `waves` waves of a workgroup of four: with
 // few rows the four waves take every fourth part of one row and join in LDS.
 // Bound by latency: the row's sequence, its list of parts, their maxima and
-// sums, and then the parts are four reads that wait for each other; a lane
-// looks up one part of 64, and a part is a load and N products a lane.
+// sums are three reads that wait for each other (the first sixteen parts come
+// with the third); a lane looks up one part of 64, and a part is a load and N
+// products a lane.
 template <int D>
 __global__ __launch_bounds__(256) void prefix_attention_join(AttnArgs a, int waves) {
     constexpr int N = D / 64;  // columns of a lane
@@ -95,7 +107,23 @@ __global__ __launch_bounds__(256) void prefix_attention_join(AttnArgs a, int wav
             pm = p[(D << log2_rows) + row];
             pl = p[((D + 1) << log2_rows) + row];
         }
-        const float now = fmaxf(top, lane_max_f(pm));
+        const int rest = (n - k + waves - 1) / waves, count = rest < 64 ? rest : 64;
+        const int64_t addr = reinterpret_cast<int64_t>(row_at);
+        // (a part past the last: the last once more, of weight zero)
+        auto load = [&](int i, vec_t (&v)[kBatch]) {
+#pragma unroll
+            for (int j = 0; j < kBatch; ++j) {
+                const int part = i + j < count ? i + j : count - 1;
+                const uint32_t lo = (uint32_t)__builtin_amdgcn_readlane((int)addr, part);
+                const uint32_t hi = (uint32_t)__builtin_amdgcn_readlane((int)(addr >> 32), part);
+                const float* const from = reinterpret_cast<const float*>((uint64_t)hi << 32 | lo) + lane * N;
+                if constexpr (N == 1) v[j][0] = *from;
+                else v[j] = *reinterpret_cast<const vec_t*>(from);
+            }
+        };
+        vec_t v[kBatch];
+        load(0, v);  // (on their way while the weights are made)
+        const float now = fmaxf(top, over_lanes(pm, [](float x, float y) { return fmaxf(x, y); }));
         const float shrink = attn::part_weight(top, now);
         top = now;
         sum *= shrink;
@@ -103,44 +131,18 @@ __global__ __launch_bounds__(256) void prefix_attention_join(AttnArgs a, int wav
         for (int j = 0; j < N; ++j) acc[j] *= shrink;
         const float weight = attn::part_weight(pm, now);
         sum += weight * pl;
-        const int rest = (n - k + waves - 1) / waves, count = rest < 64 ? rest : 64;
-        const int64_t addr = reinterpret_cast<int64_t>(row_at);
-        auto part = [&](int i) {
-            const uint32_t lo = (uint32_t)__builtin_amdgcn_readlane((int)addr, i);
-            const uint32_t hi = (uint32_t)__builtin_amdgcn_readlane((int)(addr >> 32), i);
-            return reinterpret_cast<const float*>((uint64_t)hi << 32 | lo) + lane * N;
-        };
-        auto add = [&](int i, const vec_t& v) {
-            const float w = __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, weight), i));
+        for (int i = 0; i < count; i += kBatch) {
+            if (i) load(i, v);
 #pragma unroll
-            for (int c = 0; c < N; ++c) acc[c] += w == 0.0f ? 0.0f : w * v[c];
-        };
-        auto load = [&](int i) {
-            vec_t v;
-            if constexpr (N == 1) v[0] = *part(i);
-            else v = *reinterpret_cast<const vec_t*>(part(i));
-            return v;
-        };
-        int i = 0;
-        for (; i + kBatch <= count; i += kBatch) {
-            vec_t v[kBatch];
+            for (int j = 0; j < kBatch; ++j) {
+                const float w = __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, weight), i + j));
 #pragma unroll
-            for (int j = 0; j < kBatch; ++j) v[j] = load(i + j);
-#pragma unroll
-            for (int j = 0; j < kBatch; ++j) add(i + j, v[j]);
-        }
-        if (i < count) {  // the last few: one load twice rather than one after the other
-            vec_t v[kBatch];
-#pragma unroll
-            for (int j = 0; j < kBatch; ++j) v[j] = load(i + j < count ? i + j : count - 1);
-#pragma unroll
-            for (int j = 0; j < kBatch; ++j)
-                if (i + j < count) add(i + j, v[j]);
+                for (int c = 0; c < N; ++c) acc[c] += w == 0.0f ? 0.0f : w * v[j][c];
+            }
         }
     }
-    // sum: each lane holds its parts' share, rescaled alike
-#pragma unroll
-    for (int o = 1; o < 64; o *= 2) sum += __shfl_xor(sum, o);
+    // each lane holds its parts' share, rescaled alike
+    sum = over_lanes(sum, [](float x, float y) { return x + y; });
     if (waves_join) {
 #pragma unroll
         for (int c = 0; c < N; ++c) sh_o[wave][lane * N + c] = acc[c];
