@@ -20,9 +20,10 @@
 // eight heads of a token, so every load and store is 16 bytes a lane, a wave
 // works on several rows at once, and a pair's other half is one lane exchange
 // away (rot_dim is a multiple of 16).  With fewer heads a lane where a call
-// would fill the card with less than 1024 waves: there latency counts
-// (8192 tokens x 32 heads x 128 bf16: 57 us with one head a lane, 33 with
-// eight; one token x 16 heads x 256: 4.6 us with one, 9 with eight).
+// would fill the card with less than 2048 waves: there latency counts
+// (32 heads x 128 bf16, one, four, eight heads a lane: 8192 tokens 54, 34, 29
+// us, 4096 30, 20, 16, 1024 9.5, 7.5, 8.4; one token x 16 heads x 256 fp32:
+// 4.3, 6.8, 10).
 #include "attention.h"
 #include "qw35_device.h"
 
@@ -309,10 +310,10 @@ int row_lanes_log2(int dim) {
     return n;
 }
 
-// Heads of a lane: as many as leave 1024 waves.
+// Heads of a lane: eight if they leave 2048 waves, four if they leave 1024.
 int lane_heads(int n_tokens, int heads, int log2_lanes) {
     const int64_t waves = ((int64_t)n_tokens * heads << log2_lanes) / 64;
-    return heads >= 8 && waves >= 8 * 1024 ? 8 : heads >= 4 && waves >= 4 * 1024 ? 4 : 1;
+    return heads >= 8 && waves >= 8 * 2048 ? 8 : heads >= 4 && waves >= 4 * 1024 ? 4 : 1;
 }
 
 template <class TI, class TO, int H>
