@@ -247,13 +247,16 @@ uint64_t qw35_hip_prefix_attention_workspace_size(const qw35_hip_kv_cache* cache
     const uint32_t group = n_heads / cache->kv_heads;
     // every division of the rows that a call of this batch may take: the most rows of a sequence that each has
     const uint32_t most[] = {1, 16 / group, 32 / group, 64 / group, 64 / group + 1, n_tokens};
+    // and the most sequences that are few, whose units have more rows
+    const uint32_t few = qw35::kFewOwnUnits / cache->kv_heads;
     uint64_t need = 256;
     for (uint32_t prefix = 0; prefix < 2; ++prefix)
-        for (uint32_t max_new : most) {
-            if (max_new == 0 || max_new > n_tokens) continue;
-            const qw35::AttnPlan p = plan_of(cache, n_heads, n_seqs, n_tokens, max_new, prefix, 1u << 15);
-            if (p.workspace_bytes > need) need = p.workspace_bytes;
-        }
+        for (uint32_t max_new : most)
+            for (uint32_t seqs : {n_seqs, few}) {
+                if (max_new == 0 || max_new > n_tokens || seqs > n_seqs) continue;
+                const qw35::AttnPlan p = plan_of(cache, n_heads, seqs, n_tokens, max_new, prefix, 1u << 15);
+                if (p.workspace_bytes > need) need = p.workspace_bytes;
+            }
     return need;
 }
 

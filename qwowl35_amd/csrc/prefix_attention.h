@@ -13,10 +13,12 @@
 // a kv head and a tile of rows out of the whole batch: the prefix is read once
 // for all of them.  An own unit is a kv head, a sequence and a tile of its
 // rows.  The steps of all prefix units lie behind each other on one line, those
-// of all own units on another, and each workgroup (on the own line each wave,
-// unless units have over 64 rows) takes an equal piece of either, crossing
-// units where it has to: lengths live on the device, and whatever they are the
-// load is even and the grid constant.  A piece's part of a unit goes to the
+// of all own units on another.  The workgroups are divided between the two by
+// cost, and each (on the own line each wave, unless its units share their
+// tiles) takes an equal piece, crossing units where it has to: lengths live on
+// the device, and whatever they are the load is even and the grid constant.
+// Row tiles of a prefix head stand abreast, on the same steps at a time, so
+// that all but one read them from the L2.  A piece's part of a unit goes to the
 // partial slot (place of the piece + unit), which no other has; one workgroup
 // lists every unit's slots for the join.
 //
@@ -36,13 +38,20 @@
 // Data.  Tiles go from HBM to LDS by copies that take no registers, as far
 // ahead as the ring has room (128 KB for 256 columns), and from there to the
 // matrix instructions: 16 bytes a lane, a wave's reads consecutive.  With up to
-// 64 rows in a unit each wave (or pair) has its own tiles, since then a compute
-// unit only waits for HBM; more rows share a tile among the four waves, which
-// reads it once for 128 or 256 rows.
+// 64 rows in a prefix unit each wave (or pair) has its own tiles, since then a
+// compute unit only waits for HBM; more rows share a tile among the four waves,
+// which read it once for 128 rows.
+//
+// What bounds it.  Up to 64 rows HBM, where the context is long (five sequences
+// of 16 heads over 100003 tokens, 256 columns e4m3: 4.7 TB/s in the tile loop,
+// where a copy reaches 4.9; 58 us), else latency (one sequence of 517 tokens: 11
+// us and 5 of the join).  Over that the matrix unit and the LDS reads that feed
+// it (256 tokens x 16 heads over 16001 tokens: 690 TFLOP/s, a large product
+// reaches 1100; 98304 tokens of 128 columns: 724).
 //
 // Rounding.  Scores, maxima, sums and O are fp32.  P is rounded once to the
-// cache's 16-bit type for the second product (relative 2^-12 fp16, 2^-9 bf16
-// each, signs mixed); e4m3 is exact in either 16-bit type.
+// cache's 16-bit type for the second product (relative 2^-11 fp16, 2^-8 bf16 at
+// most, signs mixed); e4m3 is exact in either 16-bit type.
 #pragma once
 
 #include "attention.h"

@@ -239,3 +239,15 @@ def test_python_checks_come_before_any_device_work():
         at.PagedCache.empty(1, 1, 40, 64, device="cpu")
     with pytest.raises(Qw35Error, match="contiguous"):
         at.PagedCache(torch.zeros(1, 1, 1, 8, 32, 8), torch.zeros(1, 1, 4, 64, 8))
+
+
+@pytest.mark.parametrize("n_heads,seqs,tokens", [(2, 200, 400), (4, 33, 2000), (16, 1000, 1000)])
+def test_the_workspace_serves_fewer_sequences(n_heads, seqs, tokens):
+    """Few sequences have their rows in larger units than many."""
+    lib, c = _ffi.load(), cache(n_pages=1 << 16)
+    size = lib.qw35_hip_prefix_attention_workspace_size(C.byref(c), n_heads, seqs, tokens)
+    for s in (1, 15, 16, 31, 32, 33, 64, 65, seqs):
+        for new in (1, 9, 20, 33, 64, 65, tokens):
+            with pytest.raises(Qw35Error, match="needs a 256-byte aligned workspace of") as e:
+                attend(c=c, n_heads=n_heads, n_seqs=min(s, seqs), n_tokens=tokens, max_new=new, starts=AT, workspace=None)
+            assert int(re.search(r"of (\d+) bytes", str(e.value)).group(1)) <= size, (s, new)

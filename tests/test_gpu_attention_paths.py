@@ -54,7 +54,7 @@ def test_a_wrong_max_new_only_divides_otherwise(cuda, max_new):
     ref.close(b.run(max_new=max_new), want, bound, f"max_new {max_new}")
 
 
-@pytest.mark.parametrize("new", [3, 12, 30, 40])  # 6, 24, 60 and 80 rows: 16-row, 32-row and shared tiles
+@pytest.mark.parametrize("new", [3, 12, 30, 40])  # 6, 24, 60 and 80 rows: 16-row and shared tiles
 @pytest.mark.parametrize("bad", [math.inf, -math.inf, math.nan])
 @pytest.mark.parametrize("dtype", [F16, BF16])
 def test_infinities_that_some_rows_see(cuda, new, bad, dtype):
@@ -124,3 +124,48 @@ def test_queries_that_are_not_aligned(cuda, dim):
         odd = torch.empty(n * 2 * (dim + 3) + 1, dtype=BF16, device=cuda)[1:].view(n, 2, dim + 3)[..., :dim]
         b.q = odd.copy_(b.q)
         ref.close(b.run(), want, bound, f"{new}")
+
+
+@pytest.mark.parametrize("new", [17, 32, 33, 64])
+@pytest.mark.parametrize("dim,dtype,cache", [(64, F16, F16), (128, BF16, E4M3), (256, F16, F16)])
+def test_rows_of_many_sequences(cuda, new, dim, dtype, cache):
+    """17 to 64 rows where there are many units: each wave has 32 of them and its own tiles."""
+    b = Batch(cuda, [1] * 70 + [new], [1 + s % 40 for s in range(70)] + [new + 90], 70, 1, 1, dim, 32, dtype, cache,
+              seed=new)
+    want, bound = b.want()
+    ref.close(b.run(), want, bound, f"{new} rows")
+    want, bound = b.want(window=30, sink=3)
+    ref.close(b.run(window=30, sink=3), want, bound, f"{new} rows in a window")
+
+
+@pytest.mark.parametrize("new", [24, 60])
+@pytest.mark.parametrize("bad", [math.inf, -math.inf, math.nan])
+@pytest.mark.parametrize("dtype", [F16, BF16])
+def test_infinities_of_many_sequences(cuda, new, bad, dtype):
+    b = Batch(cuda, [new] + [1] * 70, [70] + [5] * 70, 0, 1, 1, 64, 32, dtype, dtype, seed=16)
+    mid = new // 2
+    slot = b.cache.slots(b.pages[0], torch.tensor([70 - new + mid], device=cuda))
+    k, v = ref.unpack(b.cache, slot)
+    clean, bound = b.want()
+    v[0, :, 3] = bad
+    ref.pack(b.cache, slot, k, v)
+    got = b.run()
+    ref.close(got[:mid], clean[:mid], bound[:mid], "rows before")
+    ref.close(got[new:], clean[new:], bound[new:], "other sequences")
+    hit = got[mid:new, :, 3].double().cpu()
+    assert torch.isnan(hit).all() if math.isnan(bad) else (hit == bad).all()
+    keep = [c for c in range(64) if c != 3]
+    ref.close(got[mid:new][..., keep], clean[mid:new][..., keep], bound[mid:new][..., keep], "other columns")
+
+
+@pytest.mark.parametrize("seqs", [1, 8, 9, 32, 33])
+@pytest.mark.parametrize("new", [17, 40])
+def test_few_and_many_units_of_some_rows(cuda, seqs, new):
+    """Two kv heads: up to 32 sequences share tiles, more do not; the workspace of a larger batch serves both."""
+    from qwowl35_amd import attention as at
+
+    b = Batch(cuda, [new] + [3] * (seqs - 1), [new + 300] + [3 + 7 * s for s in range(seqs - 1)], 40, 2, 2, 64, 32,
+              F16, F16, seed=seqs)
+    want, bound = b.want()
+    ws = at.prefix_attention_workspace(b.cache, 2, 40, 200)
+    ref.close(b.run(workspace=ws), want, bound, f"{seqs} sequences")
