@@ -223,6 +223,15 @@ def _stream(stream) -> C.c_void_p:
     return C.c_void_p(stream.cuda_stream)
 
 
+def _new(shape, dtype: torch.dtype, device, stream, make=torch.empty) -> torch.Tensor:
+    """A call's own tensor, made (and filled, by ``torch.zeros``) on the stream that the call runs on: one of another
+    stream's memory could still be written there, or be given to that stream's next tensor before the call is done."""
+    if stream is None:
+        return make(shape, dtype=dtype, device=device)
+    with torch.cuda.stream(stream):
+        return make(shape, dtype=dtype, device=device)
+
+
 def _check_act(x: torch.Tensor, k: int, name: str) -> int:
     if x.dtype != torch.float32 or not x.is_cuda or not x.is_contiguous():
         raise Qw35Error(f"{name} must be a contiguous fp32 device tensor")
@@ -264,7 +273,7 @@ def decode_matvec(w: HipWeight, x: torch.Tensor, dst: torch.Tensor | None = None
     nb = _check_act(x, w.k, "x")
     _check_awq(awq, w.k, x)
     if dst is None:
-        dst = torch.zeros((nb, w.rows) if x.dim() == 2 else (w.rows,), dtype=torch.float32, device=x.device)
+        dst = _new((nb, w.rows) if x.dim() == 2 else (w.rows,), torch.float32, x.device, stream, torch.zeros)
     _check_out(dst, nb, w.rows, x, "dst")
     if workspace is None:
         _ffi.call("qw35_hip_decode_matvec", C.byref(w.view), _ptr(x), _ptr(awq), _ptr(dst), nb,
@@ -283,7 +292,7 @@ def ffn_gate_up_swiglu(gate: HipWeight, up: HipWeight, x: torch.Tensor, dst: tor
     nb = _check_act(x, gate.k, "x")
     _check_awq(awq, gate.k, x)
     if dst is None:
-        dst = torch.empty((nb, gate.rows) if x.dim() == 2 else (gate.rows,), dtype=torch.float32, device=x.device)
+        dst = _new((nb, gate.rows) if x.dim() == 2 else (gate.rows,), torch.float32, x.device, stream)
     _check_out(dst, nb, gate.rows, x, "dst")
     _ffi.call("qw35_hip_ffn_gate_up_swiglu", C.byref(gate.view), C.byref(up.view), _ptr(x), _ptr(awq), _ptr(dst),
               nb, _stream(stream))
@@ -337,25 +346,25 @@ def output_argmax(w: HipWeight, x: torch.Tensor, awq: torch.Tensor | None = None
         _refuse_unchunked(w, "output_argmax")
         raise Qw35Error("output_argmax: invalid weight or batch")
     if workspace is None:  # this call's own
-        workspace = torch.empty(need + 256, dtype=torch.uint8, device=x.device)
+        workspace = _new(need + 256, torch.uint8, x.device, stream)
     base = workspace.data_ptr()
     pad = (-base) % 256
     if workspace.numel() - pad < need:
         raise Qw35Error(f"output_argmax: workspace needs {need} bytes after 256-byte alignment")
-    token = torch.empty(nb, dtype=torch.int32, device=x.device)
-    logit = torch.empty(nb, dtype=torch.float32, device=x.device)
+    token = _new(nb, torch.int32, x.device, stream)
+    logit = _new(nb, torch.float32, x.device, stream)
     _ffi.call("qw35_hip_output_argmax", C.byref(w.view), _ptr(x), _ptr(awq), nb, _ptr(token), _ptr(logit),
               C.c_void_p(base + pad), C.c_uint64(workspace.numel() - pad), _stream(stream))
     return token, logit
 
 
-def prefill_workspace(w: HipWeight, n_tokens: int, device="cuda") -> torch.Tensor:
+def prefill_workspace(w: HipWeight, n_tokens: int, device="cuda", stream=None) -> torch.Tensor:
     """Device workspace for ``matmul_prefill`` of ``n_tokens`` tokens on ``w`` (256-byte aligned uint8)."""
     n = int(_ffi.load().qw35_hip_matmul_prefill_workspace_size(C.byref(w.view), n_tokens))
     if n == 0:
         _refuse_unchunked(w, "matmul_prefill")
         raise Qw35Error(f"prefill workspace: unsupported weight or n_tokens={n_tokens}")
-    return torch.empty(n, dtype=torch.uint8, device=device)  # the caching allocator aligns to 512 B
+    return _new(n, torch.uint8, device, stream)  # the caching allocator aligns to 512 B
 
 
 def matmul_prefill(w: HipWeight, a: torch.Tensor, awq: torch.Tensor | None = None,
@@ -385,13 +394,13 @@ def matmul_prefill(w: HipWeight, a: torch.Tensor, awq: torch.Tensor | None = Non
         raise Qw35Error("matmul_prefill: out_dtype must be bfloat16 or float32")
     n = int(a.shape[0])
     if dst is None:
-        dst = torch.empty((n, w.rows), dtype=out_dtype, device=a.device)
+        dst = _new((n, w.rows), out_dtype, a.device, stream)
     elif dst.dtype != out_dtype or tuple(dst.shape) != (n, w.rows) or not dst.is_contiguous():
         raise Qw35Error("matmul_prefill: dst must be a contiguous [n_tokens, rows] tensor of out_dtype")
     a_dt = _ffi.DTYPE_BF16 if a.dtype == torch.bfloat16 else _ffi.DTYPE_F32
     c_dt = _ffi.DTYPE_BF16 if out_dtype == torch.bfloat16 else _ffi.DTYPE_F32
     if workspace is True:
-        workspace = prefill_workspace(w, n, device=a.device)
+        workspace = prefill_workspace(w, n, device=a.device, stream=stream)
     elif workspace is False:
         workspace = None
     ws_bytes = workspace.numel() * workspace.element_size() if workspace is not None else 0
@@ -433,19 +442,22 @@ def matvec_batch(w: HipWeight, x: torch.Tensor, dst: torch.Tensor | None = None,
         # q8_0 rows of k % 256 != 0: the prefill matmul works in 256-column chunks,
         # so such a chunk runs the row-wise decode GEMV MAX_BATCH tokens at a time
         if dst is None:
-            dst = torch.empty((x.shape[0], w.rows), dtype=torch.float32, device=x.device)
+            dst = _new((x.shape[0], w.rows), torch.float32, x.device, stream)
         _check_out(dst, x.shape[0], w.rows, x, "dst")
         for t0 in range(0, x.shape[0], _ffi.MAX_BATCH):
             t1 = min(t0 + _ffi.MAX_BATCH, x.shape[0])
             decode_matvec(w, x[t0:t1], dst[t0:t1], residual=False, stream=stream)
         return dst
-    return matmul_prefill(w.prefill, x, out_dtype=torch.float32, dst=dst, stream=stream)
+    if stream is None:
+        return matmul_prefill(w.prefill, x, out_dtype=torch.float32, dst=dst)
+    with torch.cuda.stream(stream):  # (an image of the weight's first use too)
+        return matmul_prefill(w.prefill, x, out_dtype=torch.float32, dst=dst)
 
 
 def prefill_image(w: HipWeight, stream=None) -> HipWeight:
     """fp16_rne of the dequantised weight as a new F16 ``HipWeight``
     (``qw35_hip_dequantize_f16``), the operand of ``matmul_prefill``."""
-    dst = torch.empty(w.rows * w.k * 2, dtype=torch.uint8, device=_device_of(w))
+    dst = _new(w.rows * w.k * 2, torch.uint8, _device_of(w), stream)
     _ffi.call("qw35_hip_dequantize_f16", C.byref(w.view), _ptr(dst), _stream(stream))
     return HipWeight.from_device(dst, TYPE_F16, w.rows, w.k)
 
@@ -458,7 +470,7 @@ def dequantize(w: HipWeight, row_ids: torch.Tensor | None = None, stream=None) -
         n = int(row_ids.numel())
     else:
         n = w.rows
-    dst = torch.empty((n, w.k), dtype=torch.float32, device=_device_of(w))
+    dst = _new((n, w.k), torch.float32, _device_of(w), stream)
     _ffi.call("qw35_hip_dequantize", C.byref(w.view), _ptr(row_ids), n, _ptr(dst), _stream(stream))
     return dst
 
@@ -476,7 +488,7 @@ def quantize(src: torch.Tensor, type_id: int, col_scale: torch.Tensor | None = N
                                   or col_scale.numel() != src.shape[1] or not col_scale.is_contiguous()):
         raise Qw35Error("quantize: col_scale must be a contiguous fp32 device tensor of length k")
     rows, k = int(src.shape[0]), int(src.shape[1])
-    out = torch.empty(rows * row_bytes(type_id, k), dtype=torch.uint8, device=src.device)
+    out = _new(rows * row_bytes(type_id, k), torch.uint8, src.device, stream)
     _ffi.call("qw35_hip_quantize", type_id, _ptr(src), rows, k, _ptr(col_scale), _ptr(out), _stream(stream))
     return out
 
@@ -749,7 +761,7 @@ def stream_read(buf: torch.Tensor, sink: torch.Tensor | None = None, stream=None
     nbytes = buf.numel() * buf.element_size()
     n = int(_ffi.load().qw35_hip_stream_read_sink_len(nbytes))
     if sink is None:
-        sink = torch.empty(n, dtype=torch.int32, device=buf.device)
+        sink = _new(n, torch.int32, buf.device, stream)
     _ffi.call("qw35_hip_stream_read", _ptr(buf), nbytes, _ptr(sink), _stream(stream))
     return sink
 
@@ -762,7 +774,7 @@ def mfma_probe(n_workgroups: int, iters: int, sink: torch.Tensor | None = None, 
     """MFMA throughput probe (fp16 32x32x16, no memory traffic): the work is
     ``n_workgroups * iters * MFMA_PROBE_FLOPS_PER_WG_ITER`` flops; returns the sink."""
     if sink is None:
-        sink = torch.empty(n_workgroups * 256, dtype=torch.float32, device=device)
+        sink = _new(n_workgroups * 256, torch.float32, device, stream)
     _ffi.call("qw35_hip_mfma_probe", n_workgroups, iters, _ptr(sink), _stream(stream))
     return sink
 
