@@ -13,11 +13,14 @@ that norms, rotates and caches, flash attention and the output projection
 ``GatedAttention`` runs a whole layer of them with the projections.
 
 Device memory and streams come from torch; every computation is a call into
-``libqw35_hip.so``, asynchronous on ``stream`` (default: the current one).
-Tensors made on another stream than that must be synchronised with it first.
+``libqw35_hip.so``, asynchronous on the current stream.  With another ``stream``
+a call runs there, behind what the current one holds by then, and what it makes
+is that stream's memory; to leave the current stream's work aside, call under
+``torch.cuda.stream(stream)`` instead, with the inputs synchronised.
 """
 from __future__ import annotations
 
+import contextlib
 import ctypes as C
 import math
 import struct
@@ -55,8 +58,18 @@ def _call(name: str, *args) -> None:
         raise Qw35Error(f"{name}: {err.value.decode(errors='replace')}")
 
 
-def _stream(stream) -> int:
-    return rt._raw_stream(torch.cuda.current_device()) if stream is None else stream.cuda_stream
+def _stream() -> int:
+    return rt._raw_stream(torch.cuda.current_device())
+
+
+@contextlib.contextmanager
+def _behind(stream, x: torch.Tensor):
+    """``stream`` as the current one, behind what the one before holds."""
+    if stream.device != x.device:
+        raise Qw35Error(f"the stream is on {stream.device}, the input on {x.device}")
+    stream.wait_stream(torch.cuda.current_stream(x.device))
+    with torch.cuda.stream(stream):
+        yield
 
 
 def _heads(x: torch.Tensor, name: str) -> tuple:
@@ -139,6 +152,9 @@ def rotate(x: torch.Tensor, rope: Rotary | None, positions: torch.Tensor | None 
     [n_tokens], or [axes, n_tokens] for the rope's sections.  Statistics and
     rotation in fp32, rounded once to ``out_dtype`` (default: ``out``'s or x's
     type).  ``out`` may be x."""
+    if stream is not None:
+        with _behind(stream, x):
+            return rotate(x, rope, positions, norm, eps, out, out_dtype)
     hx = _heads(x, "x")
     n, heads, dim = x.shape
     device = x.get_device()
@@ -148,7 +164,7 @@ def rotate(x: torch.Tensor, rope: Rotary | None, positions: torch.Tensor | None 
     turn, pos, axes = _turn(rope, positions, n, device)
     if n:
         _call("qw35_hip_rotate", _HEADS.pack(*hx), _HEADS.pack(*hy), n, heads, dim, turn, pos, axes, weight, eps,
-              _stream(stream))
+              _stream())
     return out
 
 
@@ -204,6 +220,9 @@ def kv_append(cache: PagedCache, k: torch.Tensor, v: torch.Tensor, slots: torch.
 
     Into an e4m3 cache go the values over the head's scale, rounded to nearest
     even, past +-448 to +-448."""
+    if stream is not None:
+        with _behind(stream, k):
+            return kv_append(cache, k, v, slots, rope, positions, norm, eps)
     hk, hv = _heads(k, "k"), _heads(v, "v")
     n, device = int(k.shape[0]), cache._device
     if k.shape != (n, cache.kv_heads, cache.head_dim) or v.shape != k.shape or k.dtype != v.dtype:
@@ -216,7 +235,7 @@ def kv_append(cache: PagedCache, k: torch.Tensor, v: torch.Tensor, slots: torch.
     turn, pos, axes = _turn(rope, positions, n, device)
     if n:
         _call("qw35_hip_kv_append", cache._at, _HEADS.pack(*hk), _HEADS.pack(*hv), n, where, turn, pos, axes, weight,
-              eps, _stream(stream))
+              eps, _stream())
 
 
 def prefix_attention_workspace(cache: PagedCache, n_heads: int, n_seqs: int, n_tokens: int, device="cuda") -> torch.Tensor:
@@ -248,6 +267,10 @@ def prefix_attention(q: torch.Tensor, cache: PagedCache, pages: torch.Tensor, le
     ``max_new``: the most new tokens of a sequence, where it is known: it chooses
     how rows are divided, not what is computed.  All lengths live on the device, so
     a recorded call serves every later step."""
+    if stream is not None:
+        with _behind(stream, q):
+            return prefix_attention(q, cache, pages, lengths, starts, max_new, prefix_pages, prefix_len, scale, window,
+                                    sink, gate, out, out_dtype, workspace)
     hq = _heads(q, "q")
     n, heads, dim = q.shape
     device = cache._device
@@ -285,7 +308,7 @@ def prefix_attention(q: torch.Tensor, cache: PagedCache, pages: torch.Tensor, le
     op = _ATTENTION.pack(*hq, *ho, *hg, n, heads, seqs, max_new, at_starts, at_lengths, at_pages, at_prefix, per_seq,
                          shared, prefix_len, window, sink, 1.0 / math.sqrt(dim) if scale is None else scale,
                          workspace.data_ptr(), workspace.nbytes)
-    _call("qw35_hip_prefix_attention", op, cache._at, _stream(stream))
+    _call("qw35_hip_prefix_attention", op, cache._at, _stream())
     return out
 
 
@@ -325,11 +348,11 @@ class GatedAttention:
                        for w in weights.values())
             self.prefill_workspace = torch.empty(size, dtype=torch.uint8, device=device)
 
-    def _project(self, name: str, x: torch.Tensor, stream) -> torch.Tensor:
+    def _project(self, name: str, x: torch.Tensor) -> torch.Tensor:
         w = self.weights[name]
         if x.shape[0] <= _ffi.MAX_BATCH:
-            return rt.decode_matvec(w, x, stream=stream)
-        return rt.matmul_prefill(w.prefill, x, out_dtype=torch.float32, workspace=self.prefill_workspace, stream=stream)
+            return rt.decode_matvec(w, x)
+        return rt.matmul_prefill(w.prefill, x, out_dtype=torch.float32, workspace=self.prefill_workspace)
 
     def __call__(self, x: torch.Tensor, residual: torch.Tensor, positions: torch.Tensor, slots: torch.Tensor,
                  pages: torch.Tensor, lengths: torch.Tensor, starts: torch.Tensor | None = None, max_new: int = 0,
@@ -338,6 +361,9 @@ class GatedAttention:
         to ``residual`` (fp32, same shape) and returns it.  ``slots`` are the new
         tokens' places in the cache, the other arguments ``rotate``'s and
         ``prefix_attention``'s (``lengths`` count the new tokens)."""
+        if stream is not None:
+            with _behind(stream, x):
+                return self(x, residual, positions, slots, pages, lengths, starts, max_new, prefix_pages, prefix_len)
         n, dim, cache = int(x.shape[0]), self.cache.head_dim, self.cache
         if n > self.max_tokens or lengths.shape[0] > self.max_seqs:
             raise Qw35Error(f"{n} tokens of {lengths.shape[0]} sequences are over the layer's {self.max_tokens} and "
@@ -346,20 +372,19 @@ class GatedAttention:
             raise Qw35Error(f"residual must be a contiguous fp32 {list(x.shape)} tensor")
         if n == 0:
             return residual
-        q = self._project("attn_q", x, stream).view(n, self.heads, -1)
-        k = self._project("attn_k", x, stream).view(n, cache.kv_heads, dim)
-        v = self._project("attn_v", x, stream).view(n, cache.kv_heads, dim)
-        turned = rotate(q[..., :dim], self.rope, positions, norm=self.q_norm, eps=self.eps, out_dtype=self.q_dtype,
-                        stream=stream)
-        kv_append(cache, k, v, slots, rope=self.rope, positions=positions, norm=self.k_norm, eps=self.eps, stream=stream)
+        q = self._project("attn_q", x).view(n, self.heads, -1)
+        k = self._project("attn_k", x).view(n, cache.kv_heads, dim)
+        v = self._project("attn_v", x).view(n, cache.kv_heads, dim)
+        turned = rotate(q[..., :dim], self.rope, positions, norm=self.q_norm, eps=self.eps, out_dtype=self.q_dtype)
+        kv_append(cache, k, v, slots, rope=self.rope, positions=positions, norm=self.k_norm, eps=self.eps)
         core = prefix_attention(turned, cache, pages, lengths, starts, max_new=max_new, prefix_pages=prefix_pages,
                                 prefix_len=prefix_len, window=self.window, sink=self.sink,
                                 gate=q[..., dim:] if self.gated else None, out_dtype=torch.float32,
-                                workspace=self.workspace, stream=stream).view(n, -1)
+                                workspace=self.workspace).view(n, -1)
         out = self.weights["attn_output"]
         if n <= _ffi.MAX_BATCH:
-            rt.decode_matvec(out, core, dst=residual, residual=True, stream=stream)
+            rt.decode_matvec(out, core, dst=residual, residual=True)
         else:
             rt.matmul_prefill(out.prefill, core, out_dtype=torch.float32, dst=residual, workspace=self.prefill_workspace,
-                              epilogue=_ffi.EPILOGUE_ADD, stream=stream)
+                              epilogue=_ffi.EPILOGUE_ADD)
         return residual
