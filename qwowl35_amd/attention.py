@@ -238,13 +238,17 @@ def kv_append(cache: PagedCache, k: torch.Tensor, v: torch.Tensor, slots: torch.
               eps, _stream())
 
 
-def prefix_attention_workspace(cache: PagedCache, n_heads: int, n_seqs: int, n_tokens: int, device="cuda") -> torch.Tensor:
-    """A workspace for ``prefix_attention`` of up to this batch (its contents do not
-    matter; calls that overlap need one each)."""
+def _workspace_bytes(cache: PagedCache, n_heads: int, n_seqs: int, n_tokens: int) -> int:
     size = int(_ffi.load().qw35_hip_prefix_attention_workspace_size(C.byref(cache.view), n_heads, n_seqs, n_tokens))
     if size == 0:
         raise Qw35Error(f"prefix_attention: no workspace for n_heads={n_heads}, n_seqs={n_seqs}, n_tokens={n_tokens}")
-    return torch.empty(size, dtype=torch.uint8, device=device)
+    return size
+
+
+def prefix_attention_workspace(cache: PagedCache, n_heads: int, n_seqs: int, n_tokens: int, device="cuda") -> torch.Tensor:
+    """A workspace for ``prefix_attention`` of up to this batch (its contents do not
+    matter; calls that overlap need one each)."""
+    return torch.empty(_workspace_bytes(cache, n_heads, n_seqs, n_tokens), dtype=torch.uint8, device=device)
 
 
 def prefix_attention(q: torch.Tensor, cache: PagedCache, pages: torch.Tensor, lengths: torch.Tensor,
@@ -321,8 +325,10 @@ class GatedAttention:
     ``weights``: ``attn_q`` (heads x [queries, then gates] if the rows are twice
     heads x dim, else queries only), ``attn_k``, ``attn_v`` and ``attn_output`` as
     ``HipWeight``.  Up to 8 tokens run the decode GEMVs, more the prefill matmul
-    (fp32 activations).  Nothing of a call is kept but the cache: a call can be
-    recorded into a graph, with lengths, slots, positions and pages on the device."""
+    (fp32 activations).  Nothing of a call is kept but the cache, workspaces
+    included (torch's allocator serves them): calls of one layer may overlap on
+    several streams as far as their slots differ, and a call can be recorded into a
+    graph, with lengths, slots, positions and pages on the device."""
 
     def __init__(self, weights: dict, cache: PagedCache, heads: int, rope: Rotary | None,
                  q_norm: torch.Tensor | None = None, k_norm: torch.Tensor | None = None, eps: float = 1e-6,
@@ -335,24 +341,21 @@ class GatedAttention:
                             f"{weights['attn_v'].rows} rows for {heads} heads and {cache.kv_heads} kv heads of {dim}")
         if weights["attn_output"].k != heads * dim:
             raise Qw35Error(f"attn_output has {weights['attn_output'].k} columns for {heads} heads of {dim}")
-        device = cache.k.device
         self.weights, self.cache, self.heads, self.rope, self.eps = weights, cache, heads, rope, eps
         self.q_norm, self.k_norm, self.window, self.sink = q_norm, k_norm, window, sink
         # an 8-bit cache takes either 16-bit type: fp16 keeps more of a normed query
         self.q_dtype = torch.float16 if cache.k.dtype == torch.float8_e4m3fn else cache.k.dtype
         self.max_seqs, self.max_tokens = max_seqs, max_tokens
-        self.workspace = prefix_attention_workspace(cache, heads, max_seqs, max_tokens, device=device)
-        self.prefill_workspace = None
+        self.workspace_bytes = _workspace_bytes(cache, heads, max_seqs, max_tokens)
         if max_tokens > _ffi.MAX_BATCH:
-            size = max(int(_ffi.load().qw35_hip_matmul_prefill_workspace_size(C.byref(w.prefill.view), max_tokens))
-                       for w in weights.values())
-            self.prefill_workspace = torch.empty(size, dtype=torch.uint8, device=device)
+            for w in weights.values():
+                w.prefill  # (a k-quant's fp16 image, here and not in a call)
 
     def _project(self, name: str, x: torch.Tensor) -> torch.Tensor:
         w = self.weights[name]
         if x.shape[0] <= _ffi.MAX_BATCH:
             return rt.decode_matvec(w, x)
-        return rt.matmul_prefill(w.prefill, x, out_dtype=torch.float32, workspace=self.prefill_workspace)
+        return rt.matmul_prefill(w.prefill, x, out_dtype=torch.float32)
 
     def __call__(self, x: torch.Tensor, residual: torch.Tensor, positions: torch.Tensor, slots: torch.Tensor,
                  pages: torch.Tensor, lengths: torch.Tensor, starts: torch.Tensor | None = None, max_new: int = 0,
@@ -380,11 +383,10 @@ class GatedAttention:
         core = prefix_attention(turned, cache, pages, lengths, starts, max_new=max_new, prefix_pages=prefix_pages,
                                 prefix_len=prefix_len, window=self.window, sink=self.sink,
                                 gate=q[..., dim:] if self.gated else None, out_dtype=torch.float32,
-                                workspace=self.workspace).view(n, -1)
+                                workspace=torch.empty(self.workspace_bytes, dtype=torch.uint8, device=x.device)).view(n, -1)
         out = self.weights["attn_output"]
         if n <= _ffi.MAX_BATCH:
             rt.decode_matvec(out, core, dst=residual, residual=True)
         else:
-            rt.matmul_prefill(out.prefill, core, out_dtype=torch.float32, dst=residual, workspace=self.prefill_workspace,
-                              epilogue=_ffi.EPILOGUE_ADD)
+            rt.matmul_prefill(out.prefill, core, out_dtype=torch.float32, dst=residual, epilogue=_ffi.EPILOGUE_ADD)
         return residual

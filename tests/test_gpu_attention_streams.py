@@ -97,3 +97,59 @@ def test_the_current_stream_by_argument(cuda):
     b = Batch(cuda, [1, 2], [33, 64], 20, 4, 2, 64, 32, F16, F16, seed=12)
     want = b.run()
     assert torch.equal(b.run(stream=torch.cuda.current_stream()), want)
+
+
+@pytest.mark.parametrize("tokens", [3, 20])
+def test_overlapping_calls_of_one_layer(cuda, tokens, monkeypatch):
+    """Calls of a layer on several streams at a time, over pages of their own: no two have a workspace in common."""
+    from qwowl35_amd import attention as at
+    from qwowl35_amd import runtime as rt
+
+    layer, rand = _layer(cuda, True, F16)
+    other, _ = _layer(cuda, True, F16)
+    n = torch.arange(tokens, device=cuda, dtype=torch.int32)
+    lengths, starts = (torch.tensor(v, dtype=torch.int32, device=cuda) for v in ([tokens], [0, tokens]))
+    pages = [torch.tensor([[p]], dtype=torch.int32, device=cuda) for p in (1, 4, 6)]
+    slots = [layer.cache.slots(p[0], n) for p in pages]
+    x, res = [rand(tokens, E) for _ in pages], [torch.zeros(tokens, E, device=cuda) for _ in pages]
+    want = [other(x[i], torch.zeros_like(x[i]), n, slots[i], p, lengths, starts) for i, p in enumerate(pages)]
+    used, attend, make = [], at.prefix_attention, rt.prefill_workspace
+    monkeypatch.setattr(at, "prefix_attention", lambda *a, **k: (used.append(k["workspace"]), attend(*a, **k))[1])
+    monkeypatch.setattr(rt, "prefill_workspace", lambda *a, **k: (used.append(make(*a, **k)), used[-1])[1])
+    streams = [torch.cuda.Stream() for _ in pages]
+    torch.cuda.synchronize()
+    for i, s in enumerate(streams):
+        with torch.cuda.stream(s):
+            _busy()
+            layer(x[i], res[i], n, slots[i], pages[i], lengths, starts)
+    torch.cuda.synchronize()
+    for got, w in zip(res, want):
+        assert torch.equal(got, w)
+    assert len({t.data_ptr() for t in used}) == len(used) == (3 if tokens <= 8 else 15)
+
+
+def test_a_chunk_has_the_workspace_of_its_own_size(cuda, monkeypatch):
+    """A chunk of 90 tokens splits an 8192 x 4096 product further than one of 96: it has the room that it asks for."""
+    import ctypes as C
+
+    from qwowl35_amd import _ffi
+    from qwowl35_amd import attention as at
+    from qwowl35_amd import runtime as rt
+
+    heads, kv, dim, wide = 16, 4, 256, 4096
+    g = torch.Generator(device=cuda)
+    g.manual_seed(4)
+    weights = {n: rt.quantize_weight(torch.randn(rows, wide, generator=g, device=cuda) * 0.02, rt.TYPE_Q8_0)
+               for n, rows in (("attn_q", 2 * heads * dim), ("attn_k", kv * dim), ("attn_v", kv * dim), ("attn_output", wide))}
+    layer = at.GatedAttention(weights, at.PagedCache.empty(2, kv, 96, dim, device=cuda), heads, None, max_tokens=96)
+    made, run = [], rt.matmul_prefill
+    monkeypatch.setattr(rt, "matmul_prefill", lambda w, a, **k: (made.append((w, k.get("workspace", True))),
+                                                                 run(w, a, **k))[1])
+    n = torch.arange(90, device=cuda, dtype=torch.int32)
+    pages, x = torch.tensor([[1]], dtype=torch.int32, device=cuda), torch.randn(90, wide, device=cuda)
+    lengths, starts = (torch.tensor(v, dtype=torch.int32, device=cuda) for v in ([90], [0, 90]))
+    layer(x, torch.zeros_like(x), n, layer.cache.slots(pages[0], n), pages, lengths, starts)
+    assert len(made) == 4
+    for w, ws in made:  # (True: of this call's size)
+        need = int(_ffi.load().qw35_hip_matmul_prefill_workspace_size(C.byref(w.view), 90))
+        assert ws is True or ws.numel() >= need
