@@ -58,8 +58,9 @@ def _call(name: str, *args) -> None:
         raise Qw35Error(f"{name}: {err.value.decode(errors='replace')}")
 
 
-def _stream() -> int:
-    return rt._raw_stream(torch.cuda.current_device())
+def _elsewhere(device: int) -> bool:
+    """Whether a call over tensors on cuda:``device`` has to make that device the current one first."""
+    return device >= 0 and device != torch.cuda.current_device()
 
 
 @contextlib.contextmanager
@@ -155,16 +156,19 @@ def rotate(x: torch.Tensor, rope: Rotary | None, positions: torch.Tensor | None 
     if stream is not None:
         with _behind(stream, x):
             return rotate(x, rope, positions, norm, eps, out, out_dtype)
+    device = x.get_device()
+    if _elsewhere(device):
+        with torch.cuda.device(device):
+            return rotate(x, rope, positions, norm, eps, out, out_dtype)
     hx = _heads(x, "x")
     n, heads, dim = x.shape
-    device = x.get_device()
     out = _output(out, out_dtype, x)
     hy = _heads(out, "out")
     weight = _vector(norm, dim, device, "norm")
     turn, pos, axes = _turn(rope, positions, n, device)
     if n:
         _call("qw35_hip_rotate", _HEADS.pack(*hx), _HEADS.pack(*hy), n, heads, dim, turn, pos, axes, weight, eps,
-              _stream())
+              rt._raw_stream(device))
     return out
 
 
@@ -223,8 +227,12 @@ def kv_append(cache: PagedCache, k: torch.Tensor, v: torch.Tensor, slots: torch.
     if stream is not None:
         with _behind(stream, k):
             return kv_append(cache, k, v, slots, rope, positions, norm, eps)
+    device = cache._device
+    if _elsewhere(device):
+        with torch.cuda.device(device):
+            return kv_append(cache, k, v, slots, rope, positions, norm, eps)
     hk, hv = _heads(k, "k"), _heads(v, "v")
-    n, device = int(k.shape[0]), cache._device
+    n = int(k.shape[0])
     if k.shape != (n, cache.kv_heads, cache.head_dim) or v.shape != k.shape or k.dtype != v.dtype:
         raise Qw35Error(f"k and v must be [n_tokens, {cache.kv_heads}, {cache.head_dim}] of one type, got "
                         f"{list(k.shape)} {k.dtype} and {list(v.shape)} {v.dtype}")
@@ -235,7 +243,7 @@ def kv_append(cache: PagedCache, k: torch.Tensor, v: torch.Tensor, slots: torch.
     turn, pos, axes = _turn(rope, positions, n, device)
     if n:
         _call("qw35_hip_kv_append", cache._at, _HEADS.pack(*hk), _HEADS.pack(*hv), n, where, turn, pos, axes, weight,
-              eps, _stream())
+              eps, rt._raw_stream(device))
 
 
 def _workspace_bytes(cache: PagedCache, n_heads: int, n_seqs: int, n_tokens: int) -> int:
@@ -275,9 +283,13 @@ def prefix_attention(q: torch.Tensor, cache: PagedCache, pages: torch.Tensor, le
         with _behind(stream, q):
             return prefix_attention(q, cache, pages, lengths, starts, max_new, prefix_pages, prefix_len, scale, window,
                                     sink, gate, out, out_dtype, workspace)
+    device = cache._device
+    if _elsewhere(device):
+        with torch.cuda.device(device):
+            return prefix_attention(q, cache, pages, lengths, starts, max_new, prefix_pages, prefix_len, scale, window,
+                                    sink, gate, out, out_dtype, workspace)
     hq = _heads(q, "q")
     n, heads, dim = q.shape
-    device = cache._device
     if dim != cache.head_dim or q.get_device() != device:
         raise Qw35Error(f"q must be [n_tokens, n_heads, {cache.head_dim}] on {cache.k.device}, got {list(q.shape)}")
     if lengths.dim() != 1 or pages.dim() != 2:
@@ -312,7 +324,7 @@ def prefix_attention(q: torch.Tensor, cache: PagedCache, pages: torch.Tensor, le
     op = _ATTENTION.pack(*hq, *ho, *hg, n, heads, seqs, max_new, at_starts, at_lengths, at_pages, at_prefix, per_seq,
                          shared, prefix_len, window, sink, 1.0 / math.sqrt(dim) if scale is None else scale,
                          workspace.data_ptr(), workspace.nbytes)
-    _call("qw35_hip_prefix_attention", op, cache._at, _stream())
+    _call("qw35_hip_prefix_attention", op, cache._at, rt._raw_stream(device))
     return out
 
 
@@ -367,12 +379,18 @@ class GatedAttention:
         if stream is not None:
             with _behind(stream, x):
                 return self(x, residual, positions, slots, pages, lengths, starts, max_new, prefix_pages, prefix_len)
+        if _elsewhere(self.cache._device):
+            with torch.cuda.device(self.cache._device):
+                return self(x, residual, positions, slots, pages, lengths, starts, max_new, prefix_pages, prefix_len)
         n, dim, cache = int(x.shape[0]), self.cache.head_dim, self.cache
         if n > self.max_tokens or lengths.shape[0] > self.max_seqs:
             raise Qw35Error(f"{n} tokens of {lengths.shape[0]} sequences are over the layer's {self.max_tokens} and "
                             f"{self.max_seqs}")
-        if residual.shape != x.shape or residual.dtype != torch.float32 or not residual.is_contiguous():
-            raise Qw35Error(f"residual must be a contiguous fp32 {list(x.shape)} tensor")
+        if x.get_device() != cache._device:
+            raise Qw35Error(f"x must be on the cache's {cache.k.device}, got {x.device}")
+        if (residual.shape != x.shape or residual.dtype != torch.float32 or not residual.is_contiguous()
+                or residual.device != x.device):
+            raise Qw35Error(f"residual must be a contiguous fp32 {list(x.shape)} tensor on {x.device}")
         if n == 0:
             return residual
         q = self._project("attn_q", x).view(n, self.heads, -1)
