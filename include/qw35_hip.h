@@ -637,10 +637,11 @@ int qw35_hip_kv_append(const qw35_hip_kv_cache *cache, const qw35_hip_heads *k, 
  *   q: F16 or BF16, the cache's type (either for an E4M3 cache); out and gate:
  * F32, BF16 or F16.  n_heads a multiple of the cache's kv_heads: query head h
  * reads kv head h / (n_heads / kv_heads).
- *   max_new: the most new tokens of a sequence (0: n_tokens); it only chooses
- * how rows are divided.  workspace: device, 256-byte aligned, of
- * qw35_hip_prefix_attention_workspace_size bytes for this or a larger batch;
- * its contents do not matter, and calls that overlap need one each.
+ *   max_new: the most new tokens of a sequence (0: n_tokens; without starts
+ * always 1); it only chooses how rows are divided.  workspace: device, 256-byte
+ * aligned, of qw35_hip_prefix_attention_workspace_size bytes for this or a
+ * larger batch; its contents do not matter, and calls that overlap need one
+ * each.
  *   Bad device data is kept in bounds, not reported: lengths past the page
  * table count as its capacity, tokens of a page number outside the cache as
  * not there, and rows of q outside every sequence give zero. */

@@ -308,7 +308,10 @@ int qw35_hip_prefix_attention(const qw35_hip_attention* op, const qw35_hip_kv_ca
         set_err(err, err_len, "%s: window=%u and sink=%u are at most 2^30", what, op->window, op->sink);
         return 0;
     }
-    const uint32_t max_new = op->max_new == 0 || op->max_new > op->n_tokens ? op->n_tokens : op->max_new;
+    // (without starts every sequence has one new token, whatever max_new says)
+    const uint32_t max_new = !op->starts                                          ? 1
+                             : op->max_new == 0 || op->max_new > op->n_tokens ? op->n_tokens
+                                                                              : op->max_new;
     a.plan = plan_of(cache, op->n_heads, op->n_seqs, op->n_tokens, max_new, op->prefix_len, op->pages_per_seq);
     if (a.plan.lds_bytes > kMaxLds) {
         set_err(err, err_len, "%s: %d row tiles in a call are %llu over the list's room; give it fewer tokens or sequences",

@@ -251,3 +251,16 @@ def test_the_workspace_serves_fewer_sequences(n_heads, seqs, tokens):
             with pytest.raises(Qw35Error, match="needs a 256-byte aligned workspace of") as e:
                 attend(c=c, n_heads=n_heads, n_seqs=min(s, seqs), n_tokens=tokens, max_new=new, starts=AT, workspace=None)
             assert int(re.search(r"of (\d+) bytes", str(e.value)).group(1)) <= size, (s, new)
+
+
+@pytest.mark.parametrize("seqs", [1, 8, 64, 300])
+@pytest.mark.parametrize("max_new", [0, 1, 7])
+def test_a_token_each_is_divided_as_such(seqs, max_new):
+    """Without starts max_new does not matter: rows are divided as for one new token of a sequence."""
+    need = []
+    c = cache(n_pages=1 << 16, kv_heads=4, head_dim=256)
+    for kw in ({"max_new": max_new}, {"max_new": 1}):
+        with pytest.raises(Qw35Error, match="needs a 256-byte aligned workspace of") as e:
+            attend(c=c, n_heads=16, n_seqs=seqs, n_tokens=seqs, workspace=None, **kw)
+        need.append(int(re.search(r"of (\d+) bytes", str(e.value)).group(1)))
+    assert need[0] == need[1]
