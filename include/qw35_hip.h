@@ -667,8 +667,10 @@ typedef struct qw35_hip_attention {
     uint64_t workspace_bytes;
 } qw35_hip_attention;
 
-/* Bytes for a batch of n_seqs sequences and n_tokens new tokens, whatever its
- * max_new and prefix (0: a cache or batch that the call refuses). */
+/* Bytes for a batch of up to n_seqs sequences and n_tokens new tokens, whatever
+ * its max_new and prefix.  0: a cache or batch that the call refuses, too many
+ * sequences and tokens for a call's list of row tiles among them (of 256
+ * columns about 1590 sequences that have a token each). */
 uint64_t qw35_hip_prefix_attention_workspace_size(const qw35_hip_kv_cache *cache, uint32_t n_heads, uint32_t n_seqs,
                                                   uint32_t n_tokens);
 int qw35_hip_prefix_attention(const qw35_hip_attention *op, const qw35_hip_kv_cache *cache, void *stream, char *err,

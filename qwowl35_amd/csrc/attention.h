@@ -65,7 +65,6 @@ struct AttnPlan {
     uint64_t own_part;   // floats of the prefix' partial slots
     uint64_t meta_bytes;
     uint64_t workspace_bytes;
-    uint64_t lds_bytes;
 };
 
 struct AttnArgs {
@@ -95,11 +94,15 @@ struct AttnArgs {
     AttnPlan plan;
 };
 
-// A batch as the plan sees it; `own_tokens`: the most own tokens that a sequence's page table holds.
+// A batch as the plan sees it; `own_tokens`: the most own tokens that a
+// sequence's page table holds; `single`: every sequence has one new token.
 struct AttnShape {
     int dim, kv_heads, group, n_seqs, n_tokens, max_new, page_blocks, prefix_len;
     int64_t own_tokens;
+    bool single;
+    int most_entries;  // the plan counts no more own entries than these
 };
+int most_own_entries(int dim);  // that a compute unit's LDS lists
 AttnPlan plan_attention(const AttnShape& s);
 hipError_t launch_prefix_attention(const AttnArgs& a, int dim, uint32_t q_dtype, uint32_t cache_dtype,
                                    hipStream_t stream);

@@ -1,4 +1,5 @@
 // extern "C" entry points of the attention operators: argument checks and launch.
+#include <limits.h>
 #include <math.h>
 
 #include "abi_error.h"
@@ -15,7 +16,6 @@ using qw35::set_err;
 constexpr uint32_t kMaxTokens = 1u << 22;   // rows of a call and their heads stay within 32 bits
 constexpr uint32_t kMaxHeads = 256;
 constexpr uint64_t kMaxLength = 1u << 30;   // positions
-constexpr uint64_t kMaxLds = 160 * 1024;    // of a compute unit: a call's row tiles are listed there
 
 size_t dtype_size(uint32_t t) { return t == QW35_HIP_DTYPE_F32 ? 4 : t == QW35_HIP_DTYPE_E4M3 ? 1 : 2; }
 
@@ -235,10 +235,11 @@ static bool check_batch(const qw35_hip_kv_cache* cache, uint32_t n_heads, uint32
 }
 
 static qw35::AttnPlan plan_of(const qw35_hip_kv_cache* c, uint32_t n_heads, uint32_t n_seqs, uint32_t n_tokens,
-                              uint32_t max_new, uint32_t prefix_len, uint32_t pages_per_seq) {
+                              uint32_t max_new, uint32_t prefix_len, uint32_t pages_per_seq, bool single,
+                              int most_entries) {
     return qw35::plan_attention({(int)c->head_dim, (int)c->kv_heads, (int)(n_heads / c->kv_heads), (int)n_seqs,
                                  (int)n_tokens, (int)max_new, (int)(c->page_size / 32), (int)prefix_len,
-                                 (int64_t)pages_per_seq * c->page_size});
+                                 (int64_t)pages_per_seq * c->page_size, single, most_entries});
 }
 
 uint64_t qw35_hip_prefix_attention_workspace_size(const qw35_hip_kv_cache* cache, uint32_t n_heads, uint32_t n_seqs,
@@ -249,15 +250,24 @@ uint64_t qw35_hip_prefix_attention_workspace_size(const qw35_hip_kv_cache* cache
     const uint32_t most[] = {1, 16 / group, 32 / group, 64 / group, 64 / group + 1, n_tokens};
     // and the most sequences that are few, whose units have more rows
     const uint32_t few = qw35::kFewOwnUnits / cache->kv_heads;
+    // A division whose row tiles the list does not hold is refused for this
+    // batch, but smaller ones may take it: its size then is that of a full list.
+    const int room = qw35::most_own_entries((int)cache->head_dim);
     uint64_t need = 256;
+    bool served = n_tokens == 0;
+    if (n_seqs == n_tokens)
+        served |= plan_of(cache, n_heads, n_seqs, n_tokens, 1, 0, 1u << 15, true, INT_MAX).own_entries <= room;
     for (uint32_t prefix = 0; prefix < 2; ++prefix)
         for (uint32_t max_new : most)
             for (uint32_t seqs : {n_seqs, few}) {
                 if (max_new == 0 || max_new > n_tokens || seqs > n_seqs) continue;
-                const qw35::AttnPlan p = plan_of(cache, n_heads, seqs, n_tokens, max_new, prefix, 1u << 15);
+                const qw35::AttnPlan p = plan_of(cache, n_heads, seqs, n_tokens, max_new, prefix, 1u << 15, false, room);
                 if (p.workspace_bytes > need) need = p.workspace_bytes;
+                if (seqs == n_seqs)
+                    served |= plan_of(cache, n_heads, seqs, n_tokens, max_new, prefix, 1u << 15, false, INT_MAX)
+                                  .own_entries <= room;
             }
-    return need;
+    return served ? need : 0;
 }
 
 int qw35_hip_prefix_attention(const qw35_hip_attention* op, const qw35_hip_kv_cache* cache, void* stream, char* err,
@@ -312,10 +322,12 @@ int qw35_hip_prefix_attention(const qw35_hip_attention* op, const qw35_hip_kv_ca
     const uint32_t max_new = !op->starts                                          ? 1
                              : op->max_new == 0 || op->max_new > op->n_tokens ? op->n_tokens
                                                                               : op->max_new;
-    a.plan = plan_of(cache, op->n_heads, op->n_seqs, op->n_tokens, max_new, op->prefix_len, op->pages_per_seq);
-    if (a.plan.lds_bytes > kMaxLds) {
-        set_err(err, err_len, "%s: %d row tiles in a call are %llu over the list's room; give it fewer tokens or sequences",
-                what, a.plan.own_entries, (unsigned long long)((a.plan.lds_bytes - kMaxLds + 11) / 12));
+    a.plan = plan_of(cache, op->n_heads, op->n_seqs, op->n_tokens, max_new, op->prefix_len, op->pages_per_seq,
+                     !op->starts, INT_MAX);
+    const int room = qw35::most_own_entries((int)cache->head_dim);
+    if (a.plan.own_entries > room) {
+        set_err(err, err_len, "%s: %d row tiles in a call are %d over the list's room; give it fewer tokens or sequences",
+                what, a.plan.own_entries, a.plan.own_entries - room);
         return 0;
     }
     if (!op->workspace || ((uintptr_t)op->workspace & 255u) || op->workspace_bytes < a.plan.workspace_bytes) {

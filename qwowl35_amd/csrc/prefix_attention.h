@@ -1507,7 +1507,7 @@ __global__ __launch_bounds__(kThreads, D == 256 ? 1 : 2) void prefix_attention_k
 
 // Dynamic LDS of a launch: the tiles and the line of entries.
 template <int D>
-size_t lds_bytes(int own_entries) {
+constexpr size_t lds_bytes(int own_entries) {
     return sizeof(Shared<D>) + 8 * ((size_t)own_entries + 1) + 4 * (size_t)own_entries;
 }
 

@@ -187,6 +187,15 @@ hipError_t launch_join(const AttnArgs& a, hipStream_t stream) {
 
 }  // namespace
 
+int most_own_entries(int dim) {
+    constexpr size_t kLds = 160 * 1024, kEntry = 12;
+    static_assert(attn::lds_bytes<64>(1) - attn::lds_bytes<64>(0) == kEntry);
+    const size_t rest = kLds - (dim == 64    ? attn::lds_bytes<64>(0)
+                                : dim == 128 ? attn::lds_bytes<128>(0)
+                                             : attn::lds_bytes<256>(0));
+    return (int)(rest / kEntry);
+}
+
 AttnPlan plan_attention(const AttnShape& s) {
     AttnPlan p = {};
     const int64_t rows_prefix = s.prefix_len ? (int64_t)s.n_tokens * s.group : 0, rows_own = (int64_t)s.max_new * s.group;
@@ -197,8 +206,10 @@ AttnPlan plan_attention(const AttnShape& s) {
     p.group_magic = s.group > 1 ? (uint32_t)((1ull << 32) / s.group + 1) : 0;
     p.page_magic = s.page_blocks > 1 ? (uint32_t)((1ull << 32) / s.page_blocks + 1) : 0;
     p.prefix_entries = (int)((rows_prefix + (1 << p.prefix.log2_rows) - 1) >> p.prefix.log2_rows);
+    if (s.single) p.own_entries = s.n_seqs * ((s.group + (1 << p.own.log2_rows) - 1) >> p.own.log2_rows);
     // every sequence's last row tile may be a part of one
-    p.own_entries = s.n_seqs + (int)((int64_t)s.n_tokens * s.group >> p.own.log2_rows);
+    else p.own_entries = s.n_seqs + (int)((int64_t)s.n_tokens * s.group >> p.own.log2_rows);
+    if (p.own_entries > s.most_entries) p.own_entries = s.most_entries;
     auto cost = [](const RowSplit& r, int64_t tokens) {
         return r.lead + (((tokens + 31) / 32 + r.step()) / r.step() << r.log2_cost);
     };
@@ -209,9 +220,6 @@ AttnPlan plan_attention(const AttnShape& s) {
     p.own_part = prefix_slots * attn::slot_floats(1 << p.prefix.log2_rows, s.dim);
     p.meta_bytes = (attn::meta_pieces_at(s.n_seqs) + 8 * (uint64_t)s.kv_heads * (p.prefix_entries + p.own_entries) + 255) /
                    256 * 256;
-    p.lds_bytes = s.dim == 64    ? attn::lds_bytes<64>(p.own_entries)
-                  : s.dim == 128 ? attn::lds_bytes<128>(p.own_entries)
-                                 : attn::lds_bytes<256>(p.own_entries);
     p.workspace_bytes = p.meta_bytes + 4 * (p.own_part + (own_slots + (uint64_t)s.kv_heads * p.own_entries) *
                                                              attn::slot_floats(1 << p.own.log2_rows, s.dim));
     return p;

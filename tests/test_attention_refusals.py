@@ -264,3 +264,48 @@ def test_a_token_each_is_divided_as_such(seqs, max_new):
             attend(c=c, n_heads=16, n_seqs=seqs, n_tokens=seqs, workspace=None, **kw)
         need.append(int(re.search(r"of (\d+) bytes", str(e.value)).group(1)))
     assert need[0] == need[1]
+
+
+def _needs(c, heads, seqs, tokens, starts, max_new=0):
+    """The workspace that a call asks for; 0: it has more row tiles than the list holds."""
+    with pytest.raises(Qw35Error) as e:
+        attend(c=c, n_heads=heads, n_seqs=seqs, n_tokens=tokens, starts=starts, max_new=max_new, workspace=None)
+    m = re.search(r"workspace of (\d+) bytes", str(e.value))
+    assert m or "row tiles in a call" in str(e.value), str(e.value)
+    return int(m.group(1)) if m else 0
+
+
+@pytest.mark.parametrize("dim,kv,heads", [(256, 4, 16), (256, 1, 16), (128, 2, 40), (64, 3, 3)])
+def test_the_size_and_the_call_agree_on_what_is_too_much(dim, kv, heads):
+    """On either side of the largest batch of single tokens, and of the largest chunk."""
+    lib, c = _ffi.load(), cache(n_pages=1 << 16, kv_heads=kv, head_dim=dim)
+    size = lambda s, t: lib.qw35_hip_prefix_attention_workspace_size(C.byref(c), heads, s, t)  # noqa: E731
+
+    def largest(serves):
+        lo, hi = 1, 1 << 22
+        while lo < hi:
+            mid = (lo + hi + 1) // 2
+            lo, hi = (mid, hi) if serves(mid) else (lo, mid - 1)
+        return lo
+
+    most = largest(lambda n: n < 65536 and _needs(c, heads, n, n, None))
+    room = {256: 1500, 128: 6000, 64: 6000}[dim]
+    assert most >= room // (1 if heads // kv <= 16 else 2)
+    for n in (most - 1, most):
+        assert size(n, n) >= _needs(c, heads, n, n, None) > 0
+    assert size(65535, 65535) == 0 and _needs(c, heads, 65535, 65535, None) == 0
+    chunk = largest(lambda n: _needs(c, heads, 1, n, AT))
+    assert size(1, chunk) >= _needs(c, heads, 1, chunk, AT) > 0
+    assert size(1, chunk + 1) == 0
+    # what a size serves, smaller batches have room in, however their rows are divided
+    group = heads // kv
+    for seqs, tokens in ((most, most), (most // 2, most), (1, chunk), (7, chunk // 3)):
+        have = size(seqs, tokens)
+        for s in {1, seqs // 3 + 1, seqs}:
+            for t in {s, tokens // 2, tokens}:
+                if not s <= t:
+                    continue
+                for new in {1, 16 // group or 1, 64 // group or 1, 64 // group + 1, t}:
+                    assert _needs(c, heads, s, t, AT, min(new, t)) <= have
+                if s == t:
+                    assert _needs(c, heads, s, t, None) <= have
