@@ -50,8 +50,11 @@
 // reaches 1100; 98304 tokens of 128 columns: 724).
 //
 // Rounding.  Scores, maxima, sums and O are fp32.  P is rounded once to the
-// cache's 16-bit type for the second product (relative 2^-11 fp16, 2^-8 bf16 at
-// most, signs mixed); e4m3 is exact in either 16-bit type.
+// queries' 16-bit type for the second product, whatever the output's type (the
+// matrix unit takes both operands of a kind: relative 2^-11 fp16, 2^-8 bf16 at
+// most, signs mixed); e4m3 is exact in either 16-bit type.  The sum of P takes it
+// before the rounding: a result is then off by at most that of its weights, by
+// the rounded ones' sum at most twice that.
 #pragma once
 
 #include "attention.h"
@@ -843,8 +846,12 @@ struct Unit {
     static constexpr int kRing = Shared<D>::kRing;
     // The exponents' reference follows the maximum only when that has risen by
     // 2^8: sums then hold up to 2^8 times a row's largest term, which costs
-    // neither type precision, and most tiles rescale nothing.
-    static constexpr float kRise = 8.0f;
+    // neither type precision, and most tiles rescale nothing.  It follows to 2^7
+    // below the maximum of fp16: terms of up to 2^15 fit, and one is lost below
+    // 2^-32 of a row's largest instead of 2^-25 (31 terms of 2^-27 beside one
+    // whose value is zero were).
+    static constexpr float kLift = std::is_same_v<E, Half> ? 7.0f : 0.0f;
+    static constexpr float kRise = 8.0f + kLift;
     static constexpr bool kAgpr = D == 256;  // one wave a SIMD, accumulation registers beside the others
 
     const AttnArgs& a;
@@ -935,7 +942,7 @@ struct Unit {
     // The reference follows the rows' largest scores (`largest`: of this lane's).
     __device__ __forceinline__ void follow(Rows& w, float largest) const {
         if (__builtin_expect(__any(largest * w.scale > w.mx + kRise), 0)) {
-            const float m_new = fmaxf(w.mx, row_max<kRows>(largest) * w.scale);
+            const float m_new = fmaxf(w.mx, row_max<kRows>(largest) * w.scale - kLift);
             const float shrink = m_new == w.mx ? 1.0f : __builtin_amdgcn_exp2f(w.mx - m_new);
             const float by = after_matrix(shrink);
             w.l *= by;
