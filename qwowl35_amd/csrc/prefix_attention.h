@@ -735,14 +735,10 @@ __device__ __forceinline__ float row_sum(float v) {
 // v *= f in v's own registers, accumulation ones in the kernels that have them
 // (the compiler's products would go to others, and the accumulators with them
 // from one kind to the other in every tile).  The compiler does not count the
-// wait states from the matrix instructions that wrote v to inline assembly: f
-// comes from after_matrix.
-__device__ __forceinline__ float after_matrix(float f) {
-    // 20 wait states, the most that a matrix instruction's result needs (with own tiles a tile's scores lie between
-    // too; with shared ones the values' product is the last thing before)
-    asm volatile("s_nop 15\n\ts_nop 3" : "+v"(f));
-    return f;
-}
+// wait states from the matrix instructions that wrote v to inline assembly (12
+// of 32 rows, 8 of 16).  With own tiles a tile's scores lie between, with shared
+// ones the choice whether to come here, a lane exchange and an exponential; the
+// tests count them in the built library.  (s_nop here: 0.5 us of a call of 53.)
 template <bool kAgpr, class Acc>
 __device__ __forceinline__ void scale_in_place(Acc& v, float f) {
 #pragma unroll
@@ -944,10 +940,9 @@ struct Unit {
         if (__builtin_expect(__any(largest * w.scale > w.mx + kRise), 0)) {
             const float m_new = fmaxf(w.mx, row_max<kRows>(largest) * w.scale - kLift);
             const float shrink = m_new == w.mx ? 1.0f : __builtin_amdgcn_exp2f(w.mx - m_new);
-            const float by = after_matrix(shrink);
-            w.l *= by;
+            w.l *= shrink;
 #pragma unroll
-            for (int t = 0; t < kT; ++t) scale_in_place<kAgpr>(w.o[t], by);
+            for (int t = 0; t < kT; ++t) scale_in_place<kAgpr>(w.o[t], shrink);
             w.mx = m_new;
         }
     }
