@@ -73,6 +73,7 @@ struct AttnArgs {
     const void* cv;
     const float* k_scale;
     const float* v_scale;
+    int half_values;  // the cache is fp16
     uint32_t n_pages;
     uint32_t page_blocks;  // 32-token blocks of a page
     int kv_heads;

@@ -340,6 +340,7 @@ int qw35_hip_prefix_attention(const qw35_hip_attention* op, const qw35_hip_kv_ca
     a.cv = cache->v;
     a.k_scale = cache->k_scale;
     a.v_scale = cache->v_scale;
+    a.half_values = cache->dtype == QW35_HIP_DTYPE_F16;
     a.n_pages = cache->n_pages;
     a.page_blocks = cache->page_size / 32;
     a.kv_heads = (int)cache->kv_heads;

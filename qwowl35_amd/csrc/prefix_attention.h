@@ -296,6 +296,69 @@ __device__ __forceinline__ Tiles prefix_tiles(const AttnArgs& a, int least_upto)
     return tiles_of(l);
 }
 
+__device__ __forceinline__ bool sees(const Limits& l, int token, bool there) {
+    return there & (token < l.hi) & ((token >= l.lo) | (token < l.sink));
+}
+
+// An infinity of an fp16 cache whose weight is rounded to zero gives NaN in the
+// product, where the formula has an infinity.  (Tiles that a row sees a part of
+// keep infinities apart anyway; bf16 weights get to zero only 2^-126 below.)  For
+// rows whose result is NaN though its sum of weights is not, the values that the
+// row sees are looked through: bit k of `up` is set by a +inf in column(k),
+// k < K, of `down` by a -inf, of both by a NaN.
+struct Infinities {
+    uint32_t up, down;
+    __device__ __forceinline__ float of(int k, float otherwise) const {
+        const bool u = up >> k & 1, d = down >> k & 1;
+        return u == d ? otherwise : u ? __builtin_inff() : -__builtin_inff();
+    }
+};
+// The kernel's arguments (its first parameter) for such a path: read where it is
+// taken, not kept for it (kept, they cost 0.7 us of each call).
+__device__ __forceinline__ const AttnArgs& args_again() {
+    const AttnArgs* p = (const AttnArgs*)__builtin_amdgcn_kernarg_segment_ptr();
+    asm volatile("" : "+s"(p));
+    return *p;
+}
+template <int D, int K, class Column>
+__device__ __forceinline__ void find_infinities(const AttnArgs& a, const int32_t* table, int h, const Limits& l,
+                                                Column column, Infinities& found) {
+    typedef short bits_t __attribute__((ext_vector_type(8)));
+    constexpr uint32_t kAll = K == 32 ? ~0u : (1u << K) - 1;
+#pragma unroll 1
+    for (int t0 = 0; t0 < l.hi && (found.up & found.down) != kAll; t0 += 8) {  // eight tokens of a column lie together
+        if (t0 >= l.sink && t0 + 8 <= l.lo) t0 = l.lo / 8 * 8;
+        if (t0 >= l.hi) break;
+        const uint32_t block = (uint32_t)t0 / 32, page = block / a.page_blocks;
+        const uint32_t id = (uint32_t)table[page];
+        if (id >= a.n_pages) continue;
+        const int64_t at = ((int64_t)id * a.kv_heads + h) * a.page_blocks + (block - page * a.page_blocks);
+        const short* const from = static_cast<const short*>(a.cv) + (at * 4 + (t0 % 32) / 8) * (8 * D);
+#pragma unroll 1
+        for (int k = 0; k < K; ++k) {
+            const bits_t v = *reinterpret_cast<const bits_t*>(from + column(k) * 8);
+#pragma unroll
+            for (int j = 0; j < 8; ++j) {
+                const int size = v[j] & 0x7fff;
+                if (size < 0x7c00 || !sees(l, t0 + j, true)) continue;
+                if (size > 0x7c00 || v[j] > 0) found.up |= 1u << k;
+                if (size > 0x7c00 || v[j] < 0) found.down |= 1u << k;
+            }
+        }
+    }
+}
+
+// A value of a row that the main kernel finishes, if it is NaN.  (Inlined, it cost
+// 64 sequences of 30 tokens x 8 kv heads 0.6 of 11.1 us.)
+template <int D>
+__attribute__((noinline)) __device__ float lost_value(const AttnArgs& a, int seq, int h, int lo, int hi, int sink, int col,
+                                                      float x) {
+    if (x == x) return x;
+    Infinities found = {0, 0};
+    find_infinities<D, 1>(a, a.pages + (int64_t)seq * a.pages_per_seq, h, Limits{lo, hi, sink}, [&](int) { return col; }, found);
+    return found.of(0, x);
+}
+
 // ---- entries and the line they form --------------------------------------------------------------------------------
 
 template <class T>
@@ -848,6 +911,7 @@ struct Unit {
     // whose value is zero were).
     static constexpr float kLift = std::is_same_v<E, Half> ? 7.0f : 0.0f;
     static constexpr float kRise = 8.0f + kLift;
+    static constexpr bool kLoses = std::is_same_v<E, Half> && !F8;  // weights of zero may meet infinities
     static constexpr bool kAgpr = D == 256;  // one wave a SIMD, accumulation registers beside the others
 
     const AttnArgs& a;
@@ -1329,6 +1393,17 @@ struct Unit {
 #pragma unroll
                         for (int j = 0; j < 4; ++j) x[c][j] = y[j] * inv;
                     }
+                    if constexpr (kLoses) {
+                        float all = 0.0f;
+#pragma unroll
+                        for (int c = 0; c < 16; ++c) all += x[c / 4][c % 4];
+                        if (__builtin_expect(all != all && w.l == w.l, 0)) {
+#pragma unroll
+                            for (int c = 0; c < 16; ++c)
+                                x[c / 4][c % 4] = lost_value<D>(args_again(), job.seq, h, w.lim.lo, w.lim.hi, w.lim.sink,
+                                                                (i + c / 4) * kQuadCols + g * 4 + c % 4, x[c / 4][c % 4]);
+                        }
+                    }
                     finish(a, sq.q0 + tok, head, i * kQuadCols + g * 4, kQuadCols, gates, x);
                 }
             }
@@ -1479,10 +1554,6 @@ struct Unit {
                 w.all_sink = uniform(l.sink < w.all_sink ? l.sink : w.all_sink);
             }
         }
-    }
-
-    static __device__ __forceinline__ bool sees(const Limits& l, int token, bool there) {
-        return there & (token < l.hi) & ((token >= l.lo) | (token < l.sink));
     }
 
     __device__ __forceinline__ void put_stats(float* part, const RowSplit& split, int part_row, float m, float l) const {

@@ -173,6 +173,25 @@ __global__ __launch_bounds__(256) void prefix_attention_join(AttnArgs a, int wav
     float out[1][N];
 #pragma unroll
     for (int c = 0; c < N; ++c) out[0][c] = acc[c] * inv;
+    bool lost = false;
+#pragma unroll
+    for (int c = 0; c < N; ++c) lost |= out[0][c] != out[0][c];
+    if (__builtin_expect(lost && sum == sum, 0)) {
+        const AttnArgs& b = attn::args_again();
+        if (b.half_values) {
+            const attn::Seq q = attn::seq_at(b, at.s);
+            const int upto = attn::upto_of(q, t - q.q0);
+            attn::Infinities found = {0, 0};
+            const auto column = [&](int k) { return lane * N + k; };
+            if (b.plan.prefix_entries)
+                attn::find_infinities<D, N>(b, b.prefix_pages, h, attn::prefix_limits(b, upto), column, found);
+            attn::find_infinities<D, N>(b, b.pages + (int64_t)at.s * b.pages_per_seq, h, attn::own_limits(b, q, upto),
+                                        column, found);
+#pragma unroll
+            for (int c = 0; c < N; ++c)
+                if (out[0][c] != out[0][c]) out[0][c] = found.of(c, out[0][c]);
+        }
+    }
     attn::finish(a, t, head, lane * N, 0, gates, out);
 }
 

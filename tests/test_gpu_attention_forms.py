@@ -1,6 +1,8 @@
 """Forms of the attention kernels that only long or large calls take."""
 from __future__ import annotations
 
+import math
+
 import pytest
 import torch
 
@@ -55,3 +57,63 @@ def test_small_weights_beside_a_large_one(cuda, rows, dim, dtype, cache):
     off = 8.0 * top * (dim + 4) * 2.0 ** -24
     bound = (ref.EPS[dtype] + 2.0 ** -18 + 2 * off) * want + (2.0 ** -32 * 32 if dtype == F16 else 0.0)
     ref.close(b.run(out_dtype=F32), want, bound, rows)
+
+
+FAR = {  # new tokens, shared tokens, heads
+    "one_tile": ([1], 0, 1), "parts_16": ([1, 2], 0, 2), "shared_20": ([20], 0, 1), "shared_100": ([100], 0, 1),
+    "alone_16": ([1] * 300, 0, 8), "alone_32": ([20] * 300, 0, 8), "alone_shared": ([70] * 70, 0, 8),
+    "prefix_16": ([1], 64, 1), "prefix_64": ([50], 64, 1), "prefix_shared": ([100], 64, 2),
+}
+
+
+@pytest.mark.parametrize("rows,dim", [(r, d) for r in FAR for d in (64, 128, 256) if d == 64 or FAR[r][2] < 8])
+def test_an_infinity_of_small_weight_stays_one(cuda, rows, dim):
+    """Weights of 2^-40, which fp16 rounds to zero: a value that is infinite is so in the result, NaN of both signs."""
+    new, prefix, heads = FAR[rows]
+    more = 0 if prefix else 31 if rows == "one_tile" else 40
+    b = Batch(cuda, new, [n + more for n in new], prefix, heads, heads, dim, 32, F16, F16, seed=3)
+    b.q.fill_(8.0 / dim ** 0.5)
+    where = [(b.prefix_pages, prefix)] if prefix else list(zip(b.pages, b.lens))
+    for pages, n in where:
+        slots = b.cache.slots(pages, torch.arange(n, device=cuda))
+        k, v = ref.unpack(b.cache, slots)
+        k[:2], k[2:] = -27.7 / 8, k[2:].clamp(-0.02, 0.02)
+        ref.pack(b.cache, slots, k, v)
+    if prefix:  # (and the new tokens' own ones)
+        for s, n in enumerate(b.lens):
+            slots = b.cache.slots(b.pages[s], torch.arange(n, device=cuda))
+            k, v = ref.unpack(b.cache, slots)
+            ref.pack(b.cache, slots, k.clamp(-0.02, 0.02), v)
+    clean, bound = b.want()
+    for pages, _ in where:
+        slots = b.cache.slots(pages, torch.arange(2, device=cuda))
+        k, v = ref.unpack(b.cache, slots)
+        v[0, :, 3], v[0, :, 5], v[1, :, 9] = math.inf, -math.inf, math.nan
+        v[0, :, 7], v[1, :, 7] = math.inf, -math.inf
+        v[0, :, dim - 1], v[1, :, dim - 1] = 1.0, -math.inf
+        ref.pack(b.cache, slots, k, v)
+    for out in (F16, F32):
+        got = b.run(out_dtype=out)
+        assert (got[..., 3] == math.inf).all() and (got[..., 5] == -math.inf).all()
+        assert got[..., 7].isnan().all() and got[..., 9].isnan().all() and (got[..., dim - 1] == -math.inf).all()
+        keep = [c for c in range(dim - 1) if c not in (3, 5, 7, 9)]
+        ref.close(got[..., keep], clean[..., keep], bound[..., keep], rows)
+
+
+@pytest.mark.parametrize("window,sink", [(100, 0), (100, 8), (40, 3)])
+def test_an_infinity_outside_the_window_is_not_looked_at(cuda, window, sink):
+    """A row whose result is lost to an infinity that it sees gets that one and none that it does not see."""
+    b = Batch(cuda, [2], [300], 0, 1, 1, 64, 32, F16, F16, seed=4)
+    b.q.fill_(1.0)
+    slots = b.cache.slots(b.pages[0], torch.arange(300, device=cuda))
+    k, v = ref.unpack(b.cache, slots)
+    k[:], v[:] = 0.0, 1.0
+    k[270] = -3.46
+    v[270, :, 3] = math.inf                       # seen, of weight 2^-40
+    v[150, :, 3], v[150, :, 4] = -math.inf, -math.inf  # before either window, behind the sinks
+    if sink:
+        k[1], v[1, :, 5] = -3.46, -math.inf
+    ref.pack(b.cache, slots, k, v)
+    got = b.run(window=window, sink=sink)
+    assert (got[..., 3] == math.inf).all() and (got[..., 4] == 1.0).all()
+    assert (got[..., 5] == (-math.inf if sink else 1.0)).all()
