@@ -321,9 +321,12 @@ def prefix_attention(q: torch.Tensor, cache: PagedCache, pages: torch.Tensor, le
         raise Qw35Error(f"workspace must be a contiguous tensor on {q.device}")
     if not prefix_len:
         at_prefix = shared = 0
-    op = _ATTENTION.pack(*hq, *ho, *hg, n, heads, seqs, max_new, at_starts, at_lengths, at_pages, at_prefix, per_seq,
-                         shared, prefix_len, window, sink, 1.0 / math.sqrt(dim) if scale is None else scale,
-                         workspace.data_ptr(), workspace.nbytes)
+    try:
+        op = _ATTENTION.pack(*hq, *ho, *hg, n, heads, seqs, max_new, at_starts, at_lengths, at_pages, at_prefix, per_seq,
+                             shared, prefix_len, window, sink, 1.0 / math.sqrt(dim) if scale is None else scale,
+                             workspace.data_ptr(), workspace.nbytes)
+    except (struct.error, OverflowError) as e:
+        raise Qw35Error(f"prefix_attention: max_new, prefix_len, window, sink or scale out of range: {e}") from None
     _call("qw35_hip_prefix_attention", op, cache._at, rt._raw_stream(device))
     return out
 
