@@ -37,11 +37,11 @@ hipError_t launch_kv_append(const qw35_hip_kv_cache& cache, const HeadsView& k, 
 
 // How a launch divides the rows (new token x head of a group) of a kind of unit.
 //   Own units of up to 16 rows, and of up to 64 where there are more than
-// kFewOwnUnits: a wave has 16 or 32 rows and goes through the tokens by itself.
+// few_own_units: a wave has 16 or 32 rows and goes through the tokens by itself.
 //   Prefix units of up to 64 rows: a workgroup, 16 or 32 rows a wave, the waves
 // of a row group on different 32-token tiles (a step is 4 or 2 tiles).
 //   All others: a workgroup, 32 rows a wave, all four on the same tile.
-constexpr int kFewOwnUnits = 64;  // sequences x kv heads
+int few_own_units(int64_t rows, int dim);  // sequences x kv heads
 
 struct RowSplit {
     int log2_tiles;  // tiles of a step

@@ -242,14 +242,16 @@ static qw35::AttnPlan plan_of(const qw35_hip_kv_cache* c, uint32_t n_heads, uint
                                  (int64_t)pages_per_seq * c->page_size, single, most_entries});
 }
 
+static uint32_t few_own_seqs(const qw35_hip_kv_cache* c, uint64_t rows) {
+    return (uint32_t)qw35::few_own_units((int64_t)rows, (int)c->head_dim) / c->kv_heads;
+}
+
 uint64_t qw35_hip_prefix_attention_workspace_size(const qw35_hip_kv_cache* cache, uint32_t n_heads, uint32_t n_seqs,
                                                   uint32_t n_tokens) {
     if (!check_batch(cache, n_heads, n_seqs, n_tokens, nullptr, 0)) return 0;
     const uint32_t group = n_heads / cache->kv_heads;
     // every division of the rows that a call of this batch may take: the most rows of a sequence that each has
     const uint32_t most[] = {1, 16 / group, 32 / group, 64 / group, 64 / group + 1, n_tokens};
-    // and the most sequences that are few, whose units have more rows
-    const uint32_t few = qw35::kFewOwnUnits / cache->kv_heads;
     // A division whose row tiles the list does not hold is refused for this
     // batch, but smaller ones may take it: its size then is that of a full list.
     const int room = qw35::most_own_entries((int)cache->head_dim);
@@ -259,7 +261,8 @@ uint64_t qw35_hip_prefix_attention_workspace_size(const qw35_hip_kv_cache* cache
         served |= plan_of(cache, n_heads, n_seqs, n_tokens, 1, 0, 1u << 15, true, INT_MAX).own_entries <= room;
     for (uint32_t prefix = 0; prefix < 2; ++prefix)
         for (uint32_t max_new : most)
-            for (uint32_t seqs : {n_seqs, few}) {
+            // and the most sequences that are few, whose units have more rows
+            for (uint32_t seqs : {n_seqs, few_own_seqs(cache, (uint64_t)max_new * group)}) {
                 if (max_new == 0 || max_new > n_tokens || seqs > n_seqs) continue;
                 const qw35::AttnPlan p = plan_of(cache, n_heads, seqs, n_tokens, max_new, prefix, 1u << 15, false, room);
                 if (p.workspace_bytes > need) need = p.workspace_bytes;

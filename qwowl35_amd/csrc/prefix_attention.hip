@@ -40,15 +40,28 @@ RowSplit split_prefix(int64_t rows, int dim) {
     return {0, 2, 7, 0, 1, 32, dim == 64 ? 2 : 3};
 }
 
+}  // namespace
+
 // Own units of 17 to 64 rows: where there are few of them, a wave alone with its
 // tile waits for itself, and four waves on one tile are faster though some have
-// no row (256 columns, sequences of 40 rows and 3000 tokens x 4 kv heads: one
-// 29.4 us by a wave each, 21.7 shared; four 32.4, 29.6; eight 37.8, 36.6; 64
-// sequences of 20 tokens 21.3, 29.2).
+// no row.  Of 128 units and fewer that holds at every length from 20 to 12000
+// tokens, alike, ragged or with one long chunk among single tokens (256 columns x 4
+// kv heads, 40 rows, 3000 tokens, us by a wave each and shared: 4 units 30, 20;
+// 16 30, 27; 48 63, 41; 96 106, 69; 128 97, 94; 20 rows of 20 tokens 16, 16 at 128
+// units), of 192 about evenly, of 256 only over long sequences (20 tokens 16, 25;
+// 64 22, 31; 12000 571, 546; 128 columns, 512 units of 20 tokens 14, 20).  With 64
+// columns a tile is too little for four waves of which two have rows: 17 to 32
+// rows are shared up to 16 units (20 rows, 3000 tokens: 8 units 15, 13; 16 16, 15;
+// 48 20, 21; 128 27, 31; 12000 tokens: 16 21, 21; 32 27, 30; 96 57, 69).  Lost by
+// this: one of four sequences under a window of 4096, 5 to 36 rows: 30.5, 32.
+int few_own_units(int64_t rows, int dim) { return dim == 64 && rows <= 32 ? 16 : 128; }
+
+namespace {
+
 RowSplit split_own(int64_t rows, int64_t units, int dim) {
     const int wait = dim == 64 ? 3 : 4;
     if (rows <= 16) return {0, 0, 4, 1, 0, 16, wait};
-    if (rows <= 64 && units > kFewOwnUnits) return {0, 0, 5, 0, 0, 32, wait};
+    if (rows <= 64 && units > few_own_units(rows, dim)) return {0, 0, 5, 0, 0, 32, wait};
     return {0, 2, 7, 0, 1, 32, dim == 64 ? 2 : 3};
 }
 

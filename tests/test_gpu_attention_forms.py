@@ -25,7 +25,7 @@ def test_as_many_sequences_as_the_list_holds(cuda):
 
 
 ROWS = {  # new tokens of the sequences (one head: a new token is a row), shared tokens
-    "own_16": ([1], 0), "own_shared_20": ([20], 0), "own_shared_100": ([100], 0), "own_32": ([20] + [1] * 70, 0),
+    "own_16": ([1], 0), "own_shared_20": ([20], 0), "own_shared_100": ([100], 0), "own_32": ([20] + [1] * 140, 0),
     "prefix_16": ([1], 32), "prefix_32": ([20], 32), "prefix_64": ([50], 32), "prefix_shared": ([100], 32),
 }
 
@@ -329,3 +329,46 @@ def test_more_tiles_of_a_wave_than_are_looked_up_at_once(cuda, form):
             slots = torch.cat([c.slots(shared, torch.arange(prefix, device=cuda)), slots])
         want, bound = _one(q[s * new:(s + 1) * new, h], c, slots, h, upto=True)
         ref.close(got[s * new:(s + 1) * new, h], want, bound, f"sequence {s}, head {h}")
+
+
+@pytest.mark.parametrize("new", [17, 32, 33, 64])
+@pytest.mark.parametrize("dim,dtype,cache", [(64, F16, F16), (128, BF16, E4M3), (256, F16, F16)])
+def test_some_rows_of_many_sequences(cuda, new, dim, dtype, cache):
+    """17 to 64 rows where there are many units: each wave has 32 of them and its own tiles."""
+    b = Batch(cuda, [1] * 140 + [new], [1 + s % 40 for s in range(140)] + [new + 90], 70, 1, 1, dim, 32, dtype, cache,
+              seed=new)
+    want, bound = b.want()
+    ref.close(b.run(), want, bound, f"{new} rows")
+    want, bound = b.want(window=30, sink=3)
+    ref.close(b.run(window=30, sink=3), want, bound, f"{new} rows in a window")
+
+
+@pytest.mark.parametrize("bad", [math.inf, -math.inf, math.nan])
+@pytest.mark.parametrize("dtype", [F16, BF16])
+def test_infinities_that_some_rows_of_many_sequences_see(cuda, bad, dtype):
+    b = Batch(cuda, [60] + [1] * 140, [70] + [5] * 140, 0, 1, 1, 64, 32, dtype, dtype, seed=16)
+    slot = b.cache.slots(b.pages[0], torch.tensor([40], device=cuda))  # new token 30
+    k, v = ref.unpack(b.cache, slot)
+    clean, bound = b.want()
+    v[0, :, 3] = bad
+    ref.pack(b.cache, slot, k, v)
+    got = b.run()
+    ref.close(got[:30], clean[:30], bound[:30], "rows before")
+    ref.close(got[60:], clean[60:], bound[60:], "other sequences")
+    hit = got[30:60, :, 3].double().cpu()
+    assert torch.isnan(hit).all() if math.isnan(bad) else (hit == bad).all()
+    keep = [c for c in range(64) if c != 3]
+    ref.close(got[30:60][..., keep], clean[30:60][..., keep], bound[30:60][..., keep], "other columns")
+
+
+@pytest.mark.parametrize("seqs", [8, 9, 64, 65])
+@pytest.mark.parametrize("new", [17, 33])
+def test_either_side_of_few_units(cuda, seqs, new):
+    """Two kv heads of 64 columns: 17 rows share their tiles up to 8 sequences, 33 up to 64."""
+    from qwowl35_amd import attention as at
+
+    b = Batch(cuda, [new] + [3] * (seqs - 1), [new + 300] + [3 + 7 * (s % 40) for s in range(seqs - 1)], 40, 2, 2, 64, 32,
+              F16, F16, seed=seqs)
+    want, bound = b.want()
+    ws = at.prefix_attention_workspace(b.cache, 2, 80, 300)
+    ref.close(b.run(workspace=ws), want, bound, f"{seqs} sequences")
