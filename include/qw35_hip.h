@@ -633,7 +633,9 @@ int qw35_hip_kv_append(const qw35_hip_kv_cache *cache, const qw35_hip_heads *k, 
  * those > p - window and those < sink.  out = softmax(scale * q . k) v over
  * what it sees, zero where it sees nothing, times 1 / (1 + exp(-gate)) with a
  * gate (data NULL: none).  What a token does not see does not reach its row,
- * infinities and NaN included.
+ * infinities and NaN included; an infinity that it sees does, however small its
+ * weight.  Scores, sums and results are fp32; the weights exp(..) are rounded once
+ * to q's type on their way to the product with v, whatever out's type is.
  *   q: F16 or BF16, the cache's type (either for an E4M3 cache); out and gate:
  * F32, BF16 or F16.  n_heads a multiple of the cache's kv_heads: query head h
  * reads kv head h / (n_heads / kv_heads).

@@ -274,7 +274,8 @@ def prefix_attention(q: torch.Tensor, cache: PagedCache, pages: torch.Tensor, le
     positions up to its own, with ``window`` only the last ``window`` of them and
     the first ``sink``.  Result: softmax(scale q k) v (scale default
     1 / sqrt(head_dim)), zeros where nothing is seen, times sigmoid(``gate``), in
-    ``out_dtype`` (default q's type).
+    ``out_dtype`` (default q's type); the softmax' weights have q's precision in the
+    product with v whatever ``out_dtype`` is, everything else is fp32.
 
     ``max_new``: the most new tokens of a sequence, where it is known: it chooses
     how rows are divided, not what is computed.  All lengths live on the device, so

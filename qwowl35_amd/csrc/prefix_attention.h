@@ -45,9 +45,11 @@
 // What bounds it.  Up to 64 rows HBM, where the context is long (five sequences
 // of 16 heads over 100003 tokens, 256 columns e4m3: 4.7 TB/s in the tile loop,
 // where a copy reaches 4.9; 58 us), else latency (one sequence of 517 tokens: 11
-// us and 5 of the join).  Over that the matrix unit and the LDS reads that feed
-// it (256 tokens x 16 heads over 16001 tokens: 690 TFLOP/s, a large product
-// reaches 1100; 98304 tokens of 128 columns: 724).
+// us and 5 of the join).  Over that no unit by itself but the chain within a wave
+// (256 columns, one wave a SIMD, 1024 rows over 32768 tokens: the matrix unit is
+// busy 39% of the time, the vector unit 28%, LDS reads 20%, and the wave waits for
+// a third; 690 TFLOP/s, a large product reaches 1100.  128 columns, two waves a
+// SIMD, 256 rows over 98304 tokens: matrix unit 48%, 700).
 //
 // Rounding.  Scores, maxima, sums and O are fp32.  P is rounded once to the
 // queries' 16-bit type for the second product, whatever the output's type (the
@@ -588,7 +590,7 @@ __device__ __forceinline__ Line build_line(const AttnArgs& a, uint64_t* cost, ui
     const int xcd = (int)(blockIdx.x & 7), at = (int)(blockIdx.x >> 3), rest = grid / 8 - eighth;
     // Several row tiles go abreast, each with its own workgroup, over the same
     // steps of a head's prefix, which they then read from the L2 (behind each
-    // other 256 rows took 175 us for 98304 tokens, 154 abreast), while there
+    // other 256 rows took 175 us for 98304 tokens, 150 abreast), while there
     // are at least eight workgroups for each.
     const int tiles = p.prefix_entries, abreast = tiles > 1 && tiles <= eighth ? tiles : 1;
     const int place = xcd * eighth + at, group_of = place / abreast;
