@@ -467,6 +467,8 @@ const void *qw35_hip_runtime_store(void *runtime);
 #define QW35_HIP_DTYPE_BF16 1u
 #define QW35_HIP_DTYPE_F16 2u
 #define QW35_HIP_DTYPE_E4M3 3u /* 8-bit float (OCP e4m3), key/value caches only */
+#define QW35_HIP_DTYPE_E4M3_BLOCKS 4u /* e4m3 with a scale for each 32 tokens of a head, key/value caches only */
+#define QW35_HIP_DTYPE_I8_BLOCKS 5u   /* signed 8-bit integers (up to +-127) with such scales, key/value caches only */
 /* workspace: NULL, or device memory of
  * qw35_hip_matmul_prefill_workspace_size(w, n_tokens) bytes (256-byte
  * aligned, owned by the caller, not shared by concurrent calls).
@@ -599,6 +601,11 @@ int qw35_hip_rotate(const qw35_hip_heads *x, const qw35_hip_heads *y, uint32_t n
  * dtype QW35_HIP_DTYPE_F16, BF16 or E4M3; for E4M3 a stored element stands for
  * itself times the head's scale (k_scale, v_scale: device fp32 [kv_heads],
  * nullable = 1), and appended elements past 448 scales become 448.
+ *   Block-scaled caches, dtype E4M3_BLOCKS or I8_BLOCKS: k_scale and v_scale are
+ * device fp32 [n_pages][kv_heads][page_size / 32], and a stored element stands for
+ * itself times the scale of its block, the 32 tokens of a head with one slot / 32.
+ * Scales are zero (a block of zeros) or 2^-60 to 2^122; qw35_hip_kv_append writes
+ * them, so one cache needs no calibration.
  * head_dim 64, 128 or 256. */
 typedef struct qw35_hip_kv_cache {
     void *k;
@@ -616,10 +623,26 @@ typedef struct qw35_hip_kv_cache {
 /* Appends n_tokens tokens: keys k (normed and rotated as qw35_hip_rotate does)
  * and values v, [n_tokens][kv_heads][head_dim] of one type, to the slots
  * slots[n_tokens] (device int64).  A token whose slot is negative or past the
- * cache is left out (padding).  Slots of a call should differ. */
+ * cache is left out (padding).  Slots of a call should differ.
+ *   Into a block-scaled cache: with m the largest finite magnitude of the call's
+ * tokens in a block and Q the largest code (448, 127), the block's scale s doubles
+ * until m <= Q s, the tokens that it held are rounded to the new scale, and the
+ * call's are stored as their multiples of s, rounded to nearest even.  A block
+ * begins anew when a call writes its first token, or when its scale is zero: its
+ * scale is then the least power of two with m <= Q s (2^-60 at least; zero if m is),
+ * and its other tokens are zero.  Infinities become the largest code, NaN zero in
+ * I8_BLOCKS and NaN in E4M3_BLOCKS.  Of tokens with one slot the last counts; more
+ * than 16384 tokens are written as calls of 16384 would. */
 int qw35_hip_kv_append(const qw35_hip_kv_cache *cache, const qw35_hip_heads *k, const qw35_hip_heads *v,
                        uint32_t n_tokens, const int64_t *slots, const qw35_hip_rope *rope, const int32_t *positions,
                        uint32_t n_axes, const float *norm, float eps, void *stream, char *err, uintptr_t err_len);
+
+/* Reads tokens back: k and v, [n_tokens][kv_heads][head_dim] of one type (F32, BF16
+ * or F16), become the elements in slots[n_tokens] (device int64) times their
+ * scales, in fp32 and rounded once; zero for a negative slot or one past the
+ * cache.  Any kind of cache; slots may repeat. */
+int qw35_hip_kv_read(const qw35_hip_kv_cache *cache, const qw35_hip_heads *k, const qw35_hip_heads *v,
+                     uint32_t n_tokens, const int64_t *slots, void *stream, char *err, uintptr_t err_len);
 
 /* Attention of a ragged batch whose sequences share a prefix of prefix_len
  * tokens, which is read once for all of them.
@@ -636,7 +659,8 @@ int qw35_hip_kv_append(const qw35_hip_kv_cache *cache, const qw35_hip_heads *k, 
  * infinities and NaN included; an infinity that it sees does, however small its
  * weight.  Scores, sums and results are fp32; the weights exp(..) are rounded once
  * to q's type on their way to the product with v, whatever out's type is.
- *   q: F16 or BF16, the cache's type (either for an E4M3 cache); out and gate:
+ *   q: F16 or BF16, the cache's type (either for an E4M3 or E4M3_BLOCKS cache, F16
+ * for an I8_BLOCKS one, whose codes it takes exactly); out and gate:
  * F32, BF16 or F16.  n_heads a multiple of the cache's kv_heads: query head h
  * reads kv head h / (n_heads / kv_heads).
  *   max_new: the most new tokens of a sequence (0: n_tokens; without starts

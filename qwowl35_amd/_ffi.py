@@ -24,6 +24,8 @@ DTYPE_F32 = 0
 DTYPE_BF16 = 1
 DTYPE_F16 = 2
 DTYPE_E4M3 = 3
+DTYPE_E4M3_BLOCKS = 4
+DTYPE_I8_BLOCKS = 5
 
 
 class TensorDesc(C.Structure):
@@ -296,6 +298,11 @@ PROTOTYPES: dict[str, tuple] = {
         C.c_int,
         [C.POINTER(KvCache), C.POINTER(Heads), C.POINTER(Heads), C.c_uint32, C.c_void_p, C.POINTER(Rope), C.c_void_p,
          C.c_uint32, C.c_void_p, C.c_float, C.c_void_p, C.c_char_p, C.c_size_t],
+    ),
+    "qw35_hip_kv_read": (
+        C.c_int,
+        [C.POINTER(KvCache), C.POINTER(Heads), C.POINTER(Heads), C.c_uint32, C.c_void_p, C.c_void_p, C.c_char_p,
+         C.c_size_t],
     ),
     "qw35_hip_prefix_attention_workspace_size": (
         C.c_uint64, [C.POINTER(KvCache), C.c_uint32, C.c_uint32, C.c_uint32]),

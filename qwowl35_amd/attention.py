@@ -6,7 +6,9 @@ that norms, rotates and caches, flash attention and the output projection
 (qw35-server/src/metal/bridge/Qw35MetalRuntime+Attention.m:35-113).  Here:
 
 * ``rotate``            RMS norm and multi-axis rotary of the queries
-* ``kv_append``         the same of the keys, and keys and values into the cache
+* ``kv_append``         the same of the keys, and keys and values into the cache,
+  which may hold them in 8 bits with a scale for each 32 tokens of a head
+* ``kv_read``           tokens of a cache back as numbers
 * ``prefix_attention``  softmax attention of one or more new tokens of each
   sequence over the shared prefix (read once for the batch) and their own pages
 
@@ -33,6 +35,7 @@ from ._ffi import Qw35Error
 
 _FLOAT = {torch.float32: _ffi.DTYPE_F32, torch.bfloat16: _ffi.DTYPE_BF16, torch.float16: _ffi.DTYPE_F16}
 _CACHE = {torch.bfloat16: _ffi.DTYPE_BF16, torch.float16: _ffi.DTYPE_F16, torch.float8_e4m3fn: _ffi.DTYPE_E4M3}
+_BLOCKS = {torch.float8_e4m3fn: _ffi.DTYPE_E4M3_BLOCKS, torch.int8: _ffi.DTYPE_I8_BLOCKS}
 
 # A small call's time is this module's: structs are packed rather than built
 # field by field, and their functions take addresses as plain numbers.
@@ -44,6 +47,7 @@ _at, _u32, _err = C.c_void_p, C.c_uint32, [C.c_char_p, C.c_size_t]
 _ARGS = {
     "qw35_hip_rotate": [_at, _at, _u32, _u32, _u32, _at, _at, _u32, _at, C.c_float, _at],
     "qw35_hip_kv_append": [_at, _at, _at, _u32, _at, _at, _at, _u32, _at, C.c_float, _at],
+    "qw35_hip_kv_read": [_at, _at, _at, _u32, _at, _at],
     "qw35_hip_prefix_attention": [_at, _at, _at],
 }
 _functions: dict = {}
@@ -178,7 +182,12 @@ class PagedCache:
     k [n_pages, kv_heads, page_size / 32, dim / 8, 32, 8] and
     v [n_pages, kv_heads, page_size / 8, dim, 8], fp16, bf16 or float8_e4m3fn
     (then with an fp32 scale per kv head, default 1).  Slot ``s`` is token
-    ``s % page_size`` of page ``s // page_size``."""
+    ``s % page_size`` of page ``s // page_size``.
+
+    With scales fp32 [n_pages, kv_heads, page_size / 32] the cache is block-scaled,
+    float8_e4m3fn or int8: the 32 tokens of a head with one ``s // 32`` have a scale
+    of their own, for keys and for values, which ``kv_append`` writes (0 for a block
+    of zeros, as a new cache's)."""
 
     def __init__(self, k: torch.Tensor, v: torch.Tensor, k_scale: torch.Tensor | None = None,
                  v_scale: torch.Tensor | None = None):
@@ -189,25 +198,44 @@ class PagedCache:
         want = (pages, heads, blocks * 4, octets * 8, 8)
         if tuple(v.shape) != want or v.dtype != k.dtype or v.device != k.device or not v.is_contiguous():
             raise Qw35Error(f"cache values must be a contiguous {k.dtype} {list(want)} tensor on {k.device}")
-        if k.dtype not in _CACHE:
-            raise Qw35Error(f"a cache is float16, bfloat16 or float8_e4m3fn, got {k.dtype}")
-        if k.dtype != torch.float8_e4m3fn and (k_scale is not None or v_scale is not None):
+        self.block_scales = k.dtype == torch.int8 or any(s is not None and s.dim() == 3 for s in (k_scale, v_scale))
+        codes = _BLOCKS if self.block_scales else _CACHE
+        if k.dtype not in codes:
+            raise Qw35Error(f"a cache is float16, bfloat16 or float8_e4m3fn, with block scales float8_e4m3fn or int8, "
+                            f"got {k.dtype}")
+        if k.dtype != torch.float8_e4m3fn and not self.block_scales and (k_scale is not None or v_scale is not None):
             raise Qw35Error("only a float8_e4m3fn cache has scales")
         device = k.get_device()
-        at_k, at_v = _vector(k_scale, heads, device, "k_scale"), _vector(v_scale, heads, device, "v_scale")
+        if self.block_scales:
+            if k_scale is None or v_scale is None:
+                raise Qw35Error(f"a block-scaled cache needs k_scale and v_scale [{pages}, {heads}, {blocks}]")
+            at_k = _index(k_scale, torch.float32, (pages, heads, blocks), device, "k_scale")
+            at_v = _index(v_scale, torch.float32, (pages, heads, blocks), device, "v_scale")
+        else:
+            at_k, at_v = _vector(k_scale, heads, device, "k_scale"), _vector(v_scale, heads, device, "v_scale")
         self.k, self.v, self.k_scale, self.v_scale = k, v, k_scale, v_scale
         self.n_pages, self.kv_heads, self.page_size, self.head_dim = pages, heads, blocks * 32, octets * 8
         self.view = _ffi.KvCache(k.data_ptr(), v.data_ptr(), at_k, at_v, pages, self.page_size, heads, self.head_dim,
-                                 _CACHE[k.dtype], 0)
+                                 codes[k.dtype], 0)
         self._at, self._device = C.addressof(self.view), device
 
     @classmethod
     def empty(cls, n_pages: int, kv_heads: int, page_size: int, head_dim: int, dtype: torch.dtype = torch.float16,
-              k_scale: torch.Tensor | None = None, v_scale: torch.Tensor | None = None, device="cuda") -> "PagedCache":
+              k_scale: torch.Tensor | None = None, v_scale: torch.Tensor | None = None, device="cuda",
+              block_scales: bool = False) -> "PagedCache":
+        """A new cache; block-scaled (int8, or float8_e4m3fn with ``block_scales``) of zeros."""
         if page_size <= 0 or page_size % 32 or head_dim not in (64, 128, 256):
             raise Qw35Error(f"page_size={page_size} must be a multiple of 32 and head_dim={head_dim} 64, 128 or 256")
-        k = torch.empty((n_pages, kv_heads, page_size // 32, head_dim // 8, 32, 8), dtype=dtype, device=device)
-        v = torch.empty((n_pages, kv_heads, page_size // 8, head_dim, 8), dtype=dtype, device=device)
+        shapes = ((n_pages, kv_heads, page_size // 32, head_dim // 8, 32, 8), (n_pages, kv_heads, page_size // 8, head_dim, 8))
+        if block_scales or dtype == torch.int8:
+            if k_scale is not None or v_scale is not None:
+                raise Qw35Error("a new block-scaled cache makes its own scales")
+            if dtype not in _BLOCKS:
+                raise Qw35Error(f"a cache is float8_e4m3fn or int8 with block scales, got {dtype}")
+            k, v = (torch.zeros(s, dtype=torch.uint8, device=device).view(dtype) for s in shapes)
+            k_scale, v_scale = (torch.zeros((n_pages, kv_heads, page_size // 32), device=device) for _ in range(2))
+        else:
+            k, v = (torch.empty(s, dtype=dtype, device=device) for s in shapes)
         return cls(k, v, k_scale, v_scale)
 
     def slots(self, pages: torch.Tensor, at: torch.Tensor) -> torch.Tensor:
@@ -223,7 +251,10 @@ def kv_append(cache: PagedCache, k: torch.Tensor, v: torch.Tensor, slots: torch.
     head_dim] into ``slots`` (int64 [n_tokens]; a negative one leaves its token out).
 
     Into an e4m3 cache go the values over the head's scale, rounded to nearest
-    even, past +-448 to +-448."""
+    even, past +-448 to +-448.  In a block-scaled cache a block's scale doubles until
+    the tokens fit its largest code (448, 127), and what the block held is rounded to
+    it; writing a block's first token begins the block anew, at the least power of
+    two, with its other tokens zero (``qw35_hip_kv_append`` has the details)."""
     if stream is not None:
         with _behind(stream, k):
             return kv_append(cache, k, v, slots, rope, positions, norm, eps)
@@ -244,6 +275,39 @@ def kv_append(cache: PagedCache, k: torch.Tensor, v: torch.Tensor, slots: torch.
     if n:
         _call("qw35_hip_kv_append", cache._at, _HEADS.pack(*hk), _HEADS.pack(*hv), n, where, turn, pos, axes, weight,
               eps, rt._raw_stream(device))
+
+
+def kv_read(cache: PagedCache, slots: torch.Tensor, dtype: torch.dtype | None = None, k: torch.Tensor | None = None,
+            v: torch.Tensor | None = None, stream=None) -> tuple[torch.Tensor, torch.Tensor]:
+    """The keys and values [n_tokens, kv_heads, head_dim] in ``slots`` (int64
+    [n_tokens], repeats allowed; zeros for a negative one or one past the cache): the
+    cache's elements times their scales, rounded once to ``dtype`` (fp32, bf16 or
+    fp16; default ``k``'s type, else the cache's, fp16 of an 8-bit one).  Into ``k``
+    and ``v`` where they are given, any token and head stride."""
+    if stream is not None:
+        with _behind(stream, slots):
+            return kv_read(cache, slots, dtype, k, v)
+    device = cache._device
+    if _elsewhere(device):
+        with torch.cuda.device(device):
+            return kv_read(cache, slots, dtype, k, v)
+    if slots.dim() != 1:
+        raise Qw35Error("slots must be int64 [n_tokens]")
+    n = int(slots.shape[0])
+    where = _index(slots, torch.int64, (n,), device, "slots")
+    if dtype is None:
+        dtype = next((x.dtype for x in (k, v) if x is not None), cache.k.dtype)
+        dtype = torch.float16 if dtype.itemsize == 1 else dtype
+    shape = (n, cache.kv_heads, cache.head_dim)
+    k, v = (torch.empty(shape, dtype=dtype, device=cache.k.device) if x is None else x for x in (k, v))
+    for name, x in (("k", k), ("v", v)):
+        if x.shape != shape or x.dtype != dtype or x.get_device() != device:
+            raise Qw35Error(f"{name} must be a {dtype} {list(shape)} tensor on {cache.k.device}, got {x.dtype} "
+                            f"{list(x.shape)} on {x.device}")
+    hk, hv = _heads(k, "k"), _heads(v, "v")
+    if n:
+        _call("qw35_hip_kv_read", cache._at, _HEADS.pack(*hk), _HEADS.pack(*hv), n, where, rt._raw_stream(device))
+    return k, v
 
 
 def _workspace_bytes(cache: PagedCache, n_heads: int, n_seqs: int, n_tokens: int) -> int:
@@ -359,8 +423,8 @@ class GatedAttention:
             raise Qw35Error(f"attn_output has {weights['attn_output'].k} columns for {heads} heads of {dim}")
         self.weights, self.cache, self.heads, self.rope, self.eps = weights, cache, heads, rope, eps
         self.q_norm, self.k_norm, self.window, self.sink = q_norm, k_norm, window, sink
-        # an 8-bit cache takes either 16-bit type: fp16 keeps more of a normed query
-        self.q_dtype = torch.float16 if cache.k.dtype == torch.float8_e4m3fn else cache.k.dtype
+        # an e4m3 cache takes either 16-bit type: fp16 keeps more of a normed query
+        self.q_dtype = torch.float16 if cache.k.dtype.itemsize == 1 else cache.k.dtype
         self.max_seqs, self.max_tokens = max_seqs, max_tokens
         self.workspace_bytes = _workspace_bytes(cache, heads, max_seqs, max_tokens)
         if max_tokens > _ffi.MAX_BATCH:

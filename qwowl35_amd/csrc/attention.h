@@ -1,5 +1,5 @@
 // Host-side launch interface of the attention operators (rope_kv.hip,
-// prefix_attention.hip): internal to the library, the public C ABI is
+// block_cache.hip, prefix_attention.hip): internal to the library, the public C ABI is
 // include/qw35_hip.h.
 #pragma once
 
@@ -34,6 +34,15 @@ hipError_t launch_rotate(const HeadsView& x, const HeadsView& y, int n_tokens, i
                          hipStream_t stream);
 hipError_t launch_kv_append(const qw35_hip_kv_cache& cache, const HeadsView& k, const HeadsView& v, int n_tokens,
                             const int64_t* slots, const RopeArgs& rope, hipStream_t stream);
+
+// Caches with a scale for each block of 32 tokens and head.
+inline bool block_scaled(uint32_t dtype) { return dtype == QW35_HIP_DTYPE_E4M3_BLOCKS || dtype == QW35_HIP_DTYPE_I8_BLOCKS; }
+// Tokens of a launch of their append: a block's first token looks through all of them.
+constexpr int kAppendSlice = 16384;
+hipError_t launch_kv_append_blocks(const qw35_hip_kv_cache& cache, const HeadsView& k, const HeadsView& v, int n_tokens,
+                                   const int64_t* slots, const RopeArgs& rope, hipStream_t stream);
+hipError_t launch_kv_read(const qw35_hip_kv_cache& cache, const HeadsView& k, const HeadsView& v, int n_tokens,
+                          const int64_t* slots, hipStream_t stream);
 
 // How a launch divides the rows (new token x head of a group) of a kind of unit.
 //   Own units of up to 16 rows, and of up to 64 where there are more than
@@ -93,6 +102,8 @@ struct AttnArgs {
     float* part;      // partial slots: of the prefix
     float* own_part;  // and of own units
     AttnPlan plan;
+    const float* k_blocks;  // scales of a block-scaled cache, [page][kv head][block]
+    const float* v_blocks;
 };
 
 // A batch as the plan sees it; `own_tokens`: the most own tokens that a
@@ -103,7 +114,7 @@ struct AttnShape {
     bool single;
     int most_entries;  // the plan counts no more own entries than these
 };
-int most_own_entries(int dim);  // that a compute unit's LDS lists
+int most_own_entries(int dim, bool blocks);  // that a compute unit's LDS lists
 AttnPlan plan_attention(const AttnShape& s);
 hipError_t launch_prefix_attention(const AttnArgs& a, int dim, uint32_t q_dtype, uint32_t cache_dtype,
                                    hipStream_t stream);
@@ -112,5 +123,9 @@ hipError_t launch_prefix_attention(const AttnArgs& a, int dim, uint32_t q_dtype,
 hipError_t launch_attn_d64(const AttnArgs& a, bool bf16, bool f8, hipStream_t stream);
 hipError_t launch_attn_d128(const AttnArgs& a, bool bf16, bool f8, hipStream_t stream);
 hipError_t launch_attn_d256(const AttnArgs& a, bool bf16, bool f8, hipStream_t stream);
+// And of block-scaled caches (attn_blocks_d<dim>.hip).
+hipError_t launch_attn_blocks_d64(const AttnArgs& a, bool bf16, bool i8, hipStream_t stream);
+hipError_t launch_attn_blocks_d128(const AttnArgs& a, bool bf16, bool i8, hipStream_t stream);
+hipError_t launch_attn_blocks_d256(const AttnArgs& a, bool bf16, bool i8, hipStream_t stream);
 
 }  // namespace qw35

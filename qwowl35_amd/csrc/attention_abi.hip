@@ -116,11 +116,17 @@ bool check_cache(const qw35_hip_kv_cache* c, const char* what, char* err, uintpt
         set_err(err, err_len, "%s: cache pages must be 16-byte aligned, their scales 4-byte", what);
         return false;
     }
-    if (c->dtype != QW35_HIP_DTYPE_F16 && c->dtype != QW35_HIP_DTYPE_BF16 && c->dtype != QW35_HIP_DTYPE_E4M3) {
-        set_err(err, err_len, "%s: a cache is f16, bf16 or e4m3, got dtype %u", what, c->dtype);
+    const bool blocks = qw35::block_scaled(c->dtype);
+    if (c->dtype != QW35_HIP_DTYPE_F16 && c->dtype != QW35_HIP_DTYPE_BF16 && c->dtype != QW35_HIP_DTYPE_E4M3 && !blocks) {
+        set_err(err, err_len, "%s: a cache is f16, bf16 or e4m3, or e4m3 or i8 with block scales, got dtype %u", what,
+                c->dtype);
         return false;
     }
-    if (c->dtype != QW35_HIP_DTYPE_E4M3 && (c->k_scale || c->v_scale)) {
+    if (blocks && (!c->k_scale || !c->v_scale)) {
+        set_err(err, err_len, "%s: null scales of a block-scaled cache", what);
+        return false;
+    }
+    if (c->dtype != QW35_HIP_DTYPE_E4M3 && !blocks && (c->k_scale || c->v_scale)) {
         set_err(err, err_len, "%s: only an e4m3 cache has scales", what);
         return false;
     }
@@ -213,9 +219,31 @@ int qw35_hip_kv_append(const qw35_hip_kv_cache* cache, const qw35_hip_heads* k, 
         set_err(err, err_len, "kv_append: slots must be an 8-byte aligned device array");
         return 0;
     }
-    return check_hip(qw35::launch_kv_append(*cache, vk, vv, (int)n_tokens, slots, r,
-                                            static_cast<hipStream_t>(stream)),
-                     "kv_append", err, err_len);
+    const auto launch = qw35::block_scaled(cache->dtype) ? qw35::launch_kv_append_blocks : qw35::launch_kv_append;
+    return check_hip(launch(*cache, vk, vv, (int)n_tokens, slots, r, static_cast<hipStream_t>(stream)), "kv_append", err,
+                     err_len);
+}
+
+int qw35_hip_kv_read(const qw35_hip_kv_cache* cache, const qw35_hip_heads* k, const qw35_hip_heads* v, uint32_t n_tokens,
+                     const int64_t* slots, void* stream, char* err, uintptr_t err_len) {
+    HeadsView vk, vv;
+    if (!check_cache(cache, "kv_read", err, err_len)) return 0;
+    if (n_tokens > kMaxTokens) {
+        set_err(err, err_len, "kv_read: n_tokens=%u is over %u", n_tokens, kMaxTokens);
+        return 0;
+    }
+    if (n_tokens == 0) return 1;
+    if (!check_heads(k, "kv_read", "k", &vk, err, err_len) || !check_heads(v, "kv_read", "v", &vv, err, err_len)) return 0;
+    if (vk.dtype != vv.dtype) {
+        set_err(err, err_len, "kv_read: k and v must have one type, got dtypes %u and %u", vk.dtype, vv.dtype);
+        return 0;
+    }
+    if (!slots || ((uintptr_t)slots & 7u)) {
+        set_err(err, err_len, "kv_read: slots must be an 8-byte aligned device array");
+        return 0;
+    }
+    return check_hip(qw35::launch_kv_read(*cache, vk, vv, (int)n_tokens, slots, static_cast<hipStream_t>(stream)),
+                     "kv_read", err, err_len);
 }
 
 static bool check_batch(const qw35_hip_kv_cache* cache, uint32_t n_heads, uint32_t n_seqs, uint32_t n_tokens,
@@ -254,7 +282,7 @@ uint64_t qw35_hip_prefix_attention_workspace_size(const qw35_hip_kv_cache* cache
     const uint32_t most[] = {1, 16 / group, 32 / group, 64 / group, 64 / group + 1, n_tokens};
     // A division whose row tiles the list does not hold is refused for this
     // batch, but smaller ones may take it: its size then is that of a full list.
-    const int room = qw35::most_own_entries((int)cache->head_dim);
+    const int room = qw35::most_own_entries((int)cache->head_dim, qw35::block_scaled(cache->dtype));
     uint64_t need = 256;
     bool served = n_tokens == 0;
     if (n_seqs == n_tokens)
@@ -286,9 +314,11 @@ int qw35_hip_prefix_attention(const qw35_hip_attention* op, const qw35_hip_kv_ca
     if (!check_heads(&op->q, what, "q", &a.q, err, err_len) || !check_heads(&op->out, what, "out", &a.out, err, err_len))
         return 0;
     if (op->gate.data && !check_heads(&op->gate, what, "gate", &a.gate, err, err_len)) return 0;
-    if (a.q.dtype == QW35_HIP_DTYPE_F32 || (cache->dtype != QW35_HIP_DTYPE_E4M3 && a.q.dtype != cache->dtype)) {
-        set_err(err, err_len, "%s: q must have the cache's type (f16 or bf16 for an e4m3 cache), got dtype %u", what,
-                a.q.dtype);
+    const bool either = cache->dtype == QW35_HIP_DTYPE_E4M3 || cache->dtype == QW35_HIP_DTYPE_E4M3_BLOCKS;
+    const uint32_t q_dtype = cache->dtype == QW35_HIP_DTYPE_I8_BLOCKS ? QW35_HIP_DTYPE_F16 : cache->dtype;
+    if (a.q.dtype == QW35_HIP_DTYPE_F32 || (!either && a.q.dtype != q_dtype)) {
+        set_err(err, err_len, "%s: q must have the cache's type (f16 or bf16 for an e4m3 cache, f16 for an i8 one), got dtype %u",
+                what, a.q.dtype);
         return 0;
     }
     if (!op->starts && op->n_seqs != op->n_tokens) {
@@ -327,7 +357,8 @@ int qw35_hip_prefix_attention(const qw35_hip_attention* op, const qw35_hip_kv_ca
                                                                               : op->max_new;
     a.plan = plan_of(cache, op->n_heads, op->n_seqs, op->n_tokens, max_new, op->prefix_len, op->pages_per_seq,
                      !op->starts, INT_MAX);
-    const int room = qw35::most_own_entries((int)cache->head_dim);
+    const bool blocks = qw35::block_scaled(cache->dtype);
+    const int room = qw35::most_own_entries((int)cache->head_dim, blocks);
     if (a.plan.own_entries > room) {
         set_err(err, err_len, "%s: %d row tiles in a call are %d over the list's room; give it fewer tokens or sequences",
                 what, a.plan.own_entries, a.plan.own_entries - room);
@@ -341,8 +372,8 @@ int qw35_hip_prefix_attention(const qw35_hip_attention* op, const qw35_hip_kv_ca
     }
     a.ck = cache->k;
     a.cv = cache->v;
-    a.k_scale = cache->k_scale;
-    a.v_scale = cache->v_scale;
+    (blocks ? a.k_blocks : a.k_scale) = cache->k_scale;
+    (blocks ? a.v_blocks : a.v_scale) = cache->v_scale;
     a.half_values = cache->dtype == QW35_HIP_DTYPE_F16;
     a.n_pages = cache->n_pages;
     a.page_blocks = cache->page_size / 32;

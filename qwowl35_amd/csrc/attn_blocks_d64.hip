@@ -1,0 +1,10 @@
+// Shared-prefix attention over a block-scaled cache, head dimension 64: see prefix_attention.h.
+#include "prefix_attention.h"
+
+namespace qw35 {
+
+hipError_t launch_attn_blocks_d64(const AttnArgs& a, bool bf16, bool i8, hipStream_t stream) {
+    return attn::launch_blocks<64>(a, bf16, i8, stream);
+}
+
+}  // namespace qw35

@@ -91,6 +91,17 @@ struct Half {
         r[3] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(w.y, 1.0f, true));
         return __builtin_bit_cast(vec8, r);
     }
+    // A code c, moved up by 128, under the exponent of 1024 (whose steps are 1) is 1152 + c: exact.
+    static __device__ __forceinline__ vec8 from_i8(uint2 w) {
+        const half2_t down = {(_Float16)-1152.0f, (_Float16)-1152.0f};
+        const uint32_t x = w.x ^ 0x80808080u, y = w.y ^ 0x80808080u;
+        uint4_t r;
+        r[0] = as_u32(as_half2(__builtin_amdgcn_perm(0x64646464u, x, 0x04010400u)) + down);
+        r[1] = as_u32(as_half2(__builtin_amdgcn_perm(0x64646464u, x, 0x04030402u)) + down);
+        r[2] = as_u32(as_half2(__builtin_amdgcn_perm(0x64646464u, y, 0x04010400u)) + down);
+        r[3] = as_u32(as_half2(__builtin_amdgcn_perm(0x64646464u, y, 0x04030402u)) + down);
+        return __builtin_bit_cast(vec8, r);
+    }
 };
 
 struct Bf16 {
@@ -876,21 +887,37 @@ struct Shared {
     int lane_line[5][64];  // of a line in lanes: cost before, cost, and q0, n, length
 };
 
-// Raw granules of a tile: 16 bytes of a 16-bit cache, 8 of an e4m3 one.
-template <bool F8>
-using raw8 = std::conditional_t<F8, uint2, uint4_t>;
+// The block scales of a wave's tiles, keys' and values': of the 64 looked up last and of the 64 before.
+template <int D>
+struct SharedBlocks : Shared<D> {
+    float scales[kWaves][2][2][64];
+};
 
-template <class E, bool F8>
-__device__ __forceinline__ typename E::vec8 operand(raw8<F8> w) {
-    if constexpr (F8) return E::from_e4m3(w);
+// What a cache holds: 16-bit numbers of the queries' type, e4m3 with a scale of the
+// head, or e4m3 or int8 with a scale for each 32 tokens of a head.
+enum class Kind { wide, e4m3, e4m3_blocks, i8_blocks };
+template <int D, Kind C>
+using shared_of = std::conditional_t<(C >= Kind::e4m3_blocks), SharedBlocks<D>, Shared<D>>;
+
+// Raw granules of a tile: 16 bytes of a 16-bit cache, 8 of an 8-bit one.
+template <Kind C>
+using raw8 = std::conditional_t<C != Kind::wide, uint2, uint4_t>;
+
+template <class E, Kind C>
+__device__ __forceinline__ typename E::vec8 operand(raw8<C> w) {
+    if constexpr (C == Kind::i8_blocks) return E::from_i8(w);
+    else if constexpr (C != Kind::wide) return E::from_e4m3(w);
     else return __builtin_bit_cast(typename E::vec8, w);
 }
 
 // kRows: rows of a wave's tile, 16 or 32.
-template <int D, class E, bool F8, int kRows>
+template <int D, class E, Kind C, int kRows>
 struct Unit {
+    static constexpr bool F8 = C != Kind::wide;             // 8-bit elements
+    static constexpr bool kBlocks = C >= Kind::e4m3_blocks;  // with a scale of the tile
+    static constexpr bool kFinite = C == Kind::i8_blocks;    // that are numbers all
     typedef typename E::vec8 vec8;
-    typedef raw8<F8> raw;
+    typedef raw8<C> raw;
     typedef std::conditional_t<kRows == 32, acc_t, float4_t> acc;  // of a matrix instruction
     static constexpr int kAcc = sizeof(acc) / 4;
     static constexpr int kGroups = 64 / kRows;      // lanes of a row
@@ -917,13 +944,26 @@ struct Unit {
     static constexpr bool kAgpr = D == 256;  // one wave a SIMD, accumulation registers beside the others
 
     const AttnArgs& a;
-    Shared<D>& sh;
+    shared_of<D, C>& sh;
     const int lane, wave, n, g;  // this lane's row of a tile, and which of the row's lanes it is
 
-    __device__ Unit(const AttnArgs& a_, Shared<D>& sh_)
+    __device__ Unit(const AttnArgs& a_, shared_of<D, C>& sh_)
         : a(a_), sh(sh_), lane(threadIdx.x & 63), wave(__builtin_amdgcn_readfirstlane(threadIdx.x >> 6)),
           n(threadIdx.x & (kRows - 1)), g((threadIdx.x & 63) / kRows) {}
 
+    struct Nothing {
+        __device__ __forceinline__ void operator()(int) const {}
+    };
+
+    // A block-scaled tile: with keys s^k c and values s^v c a term is 2^(scale s^k q.c - m) s^v c.  The values'
+    // scale goes into the exponent, u = scale s^k q.c + log2 s^v, and the reference m follows the largest u: the
+    // product's weights 2^(u - m) take what a row's values weigh, whatever the scales, and the sum of the
+    // softmax' terms gets the tile's back at once, by 2^-log2 s^v.  Four instructions a tile and none an element.
+    struct Blocks {
+        float key, lift, unlift;  // scale s^k, log2 s^v, 2^-log2 s^v
+        float sum;                // of the tile's weights
+        uint32_t keep;            // all ones; zero where the values are, by a scale of zero
+    };
     // What a wave carries through its tiles.
     struct Rows {
         vec8 q[kM];
@@ -933,24 +973,53 @@ struct Unit {
         int all_lo, all_hi, all_sink;  // what every row of the wave sees
         float scale;
         bool marked;  // infinities to add at the end
+        std::conditional_t<kBlocks, Blocks, Nothing> tile;
     };
+
+    // Tile i's, whose scales came with its copies.
+    __device__ __forceinline__ void scale_tile(Rows& w, int i) const {
+        if constexpr (kBlocks) {
+            const float(&from)[2][64] = sh.scales[wave][i >> 6 & 1];
+            const float v = from[1][i & 63];
+            // (zero: every finite score alike; a missing tile's may be anything, and its scores are masked)
+            w.tile.key = fminf(fmaxf(w.scale * from[0][i & 63], 2e-38f), 3e38f);
+            const bool some = v > 0.0f;
+            const float lift = __builtin_amdgcn_logf(v);
+            w.tile.lift = some ? lift : w.tile.lift;
+            w.tile.unlift = __builtin_amdgcn_exp2f(-w.tile.lift);
+            w.tile.keep = some ? ~0u : 0u;
+        }
+    }
+    // What a score is as an exponent.
+    static __device__ __forceinline__ float exponent(const Rows& w, float s) {
+        if constexpr (kBlocks) return fmaf(s, w.tile.key, w.tile.lift);
+        else return s * w.scale;
+    }
+    // After a tile's terms: their sum, and weights of values that are zero.
+    __device__ __forceinline__ void end_terms(Rows& w, vec8 (&p)[kK]) const {
+        if constexpr (kBlocks) {
+            w.l = fmaf(w.tile.sum, w.tile.unlift, w.l);
+            w.tile.sum = 0.0f;
+#pragma unroll
+            for (int k = 0; k < kK; ++k) {
+                uint4_t x = __builtin_bit_cast(uint4_t, p[k]) & w.tile.keep;
+                p[k] = __builtin_bit_cast(vec8, x);
+            }
+        }
+    }
 
     // The granule of step m for score tile b / of column tile t and token step kk.
     __device__ __forceinline__ vec8 key(const uint8_t* tile, int m, int b) const {
         // which token is row n of the product: token(j) of the lane that gets it
         const int tok = kRows == 32 ? (n & 19) | (n & 4) << 1 | (n & 8) >> 1 : (n >> 2) * 8 + b * 4 + (n & 3);
-        return operand<E, F8>(*reinterpret_cast<const raw*>(tile + ((kGroups * m + g) * 32 + tok) * 8 * kElem));
+        return operand<E, C>(*reinterpret_cast<const raw*>(tile + ((kGroups * m + g) * 32 + tok) * 8 * kElem));
     }
     __device__ __forceinline__ vec8 value(const uint8_t* tile, int t, int kk) const {
-        return operand<E, F8>(
+        return operand<E, C>(
             *reinterpret_cast<const raw*>(tile + ((kGroups * kk + g) * D + t * kRows + n) * 8 * kElem));
     }
     // Token of a lane's score j.
     __device__ __forceinline__ int token(int j) const { return kRows == 32 ? (j & 8) * 2 + g * 8 + (j & 7) : g * 8 + j; }
-
-    struct Nothing {
-        __device__ __forceinline__ void operator()(int) const {}
-    };
 
     // `beside`(step): other work, a part after the matrix instructions of each step.
     static constexpr int kScoreSteps = kM * kB, kValueSteps = kK * kT;
@@ -1003,8 +1072,8 @@ struct Unit {
 
     // The reference follows the rows' largest scores (`largest`: of this lane's).
     __device__ __forceinline__ void follow(Rows& w, float largest) const {
-        if (__builtin_expect(__any(largest * w.scale > w.mx + kRise), 0)) {
-            const float m_new = fmaxf(w.mx, row_max<kRows>(largest) * w.scale - kLift);
+        if (__builtin_expect(__any(exponent(w, largest) > w.mx + kRise), 0)) {
+            const float m_new = fmaxf(w.mx, exponent(w, row_max<kRows>(largest)) - kLift);
             const float shrink = m_new == w.mx ? 1.0f : __builtin_amdgcn_exp2f(w.mx - m_new);
             w.l *= shrink;
 #pragma unroll
@@ -1020,8 +1089,14 @@ struct Unit {
         for (int i = j0; i < j1; ++i) {
             const int j = i;
             const float ref = w.mx == -__builtin_inff() ? 0.0f : w.mx;
-            const float e = __builtin_amdgcn_exp2f(fmaf(s[j / kAcc][j % kAcc], w.scale, -ref));
-            w.l += e;
+            float e;
+            if constexpr (kBlocks) {
+                e = __builtin_amdgcn_exp2f(fmaf(s[j / kAcc][j % kAcc], w.tile.key, w.tile.lift - ref));
+                w.tile.sum += e;
+            } else {
+                e = __builtin_amdgcn_exp2f(fmaf(s[j / kAcc][j % kAcc], w.scale, -ref));
+                w.l += e;
+            }
             p[j / 8][j % 8] = (typename E::elem)e;
         }
     }
@@ -1033,6 +1108,7 @@ struct Unit {
         top = largest(s);
         follow(w, top);
         terms(w, s, p);
+        end_terms(w, p);
     }
 
     template <class F = Nothing>
@@ -1058,7 +1134,7 @@ struct Unit {
     template <bool kShared>
     __device__ __forceinline__ void split_off_infinities(uint8_t* tile, Rows& w, int t0, bool there,
                                                          uint32_t* marks) const {
-        if (__builtin_expect(!__any(not_finite(tile)), 1)) return;
+        if (kFinite || __builtin_expect(!__any(not_finite(tile)), 1)) return;
         mark_infinities(tile, w, t0, there, marks);
         if (kShared) __syncthreads();
         make_finite(tile, kShared ? wave : 0, kShared ? kWaves : 1);
@@ -1076,7 +1152,7 @@ struct Unit {
 #pragma unroll 4
         for (int i = 0; i < kParts; ++i)
             top = __builtin_elementwise_max(
-                top, __builtin_bit_cast(bits_t, operand<E, F8>(*reinterpret_cast<const raw*>(granule(tile, i)))) &
+                top, __builtin_bit_cast(bits_t, operand<E, C>(*reinterpret_cast<const raw*>(granule(tile, i)))) &
                          (short)0x7fff);
         bool bad = false;
 #pragma unroll
@@ -1177,6 +1253,14 @@ struct Unit {
         uint32_t block = ((uint32_t)id * (uint32_t)a.kv_heads + p.h) * a.page_blocks + (b - pi * a.page_blocks);
         asm("" : "+v"(block));  // (a choice of two values, not of two paths)
         p.blocks = (uint32_t)id < a.n_pages ? block : kNoBlock;
+        if constexpr (kBlocks) {  // their scales, a lane's at a time, ahead of their copies
+            typedef const __attribute__((address_space(1))) void global_t;
+            typedef __attribute__((address_space(3))) void lds_t;
+            const uint32_t at = p.blocks == kNoBlock ? 0u : p.blocks;
+            float(&to)[2][64] = sh.scales[wave][i >> 6 & 1];
+            __builtin_amdgcn_global_load_lds((global_t*)(a.k_blocks + at), (lds_t*)to[0], 4, 0, 0);
+            __builtin_amdgcn_global_load_lds((global_t*)(a.v_blocks + at), (lds_t*)to[1], 4, 0, 0);
+        }
     }
     // Tile i, the last looked up or the first of the next 64.
     __device__ __forceinline__ uint32_t block_of(Pages& p, int i) const {
@@ -1276,6 +1360,7 @@ struct Unit {
             const int clear0 = tiles.sink + ((w.all_lo + 31) / 32 > tiles.lo ? (w.all_lo + 31) / 32 - tiles.lo : 0) - pages.first;
             const int clear1 = tiles.sink + w.all_hi / 32 - tiles.lo - pages.first;
             auto see_and_follow = [&](int i) {
+                scale_tile(w, i);
                 if (i < clear0 || i >= clear1 || missing) {
                     const bool there = there_bits >> (loaded - 1 - i) & 1;
                     const int t0 = tiles.at(pages.first + i) * 32;
@@ -1304,6 +1389,7 @@ struct Unit {
                     if (copies && m < kEach) copy_1kb(from, to, m, lane);
                     terms(w, s, p, kScores * m / kScoreSteps, kScores * (m + 1) / kScoreSteps);
                 });
+                end_terms(w, p);
                 top = -__builtin_inff();
                 add_values(ring + (i % kPairs) * 2 * kTile + kTile, w, p, [&](int m) {
 #pragma unroll
@@ -1319,6 +1405,7 @@ struct Unit {
             for (; i + 1 < pages.count; ++i) step(i, std::false_type{});
             see_and_follow(i);
             terms(w, s, p);
+            end_terms(w, p);
             add_values(ring + (i % kPairs) * 2 * kTile + kTile, w, p);
             wait_lds();
         } else {
@@ -1333,6 +1420,7 @@ struct Unit {
                 vec8 p[kK];
                 if (more) wait_vm<kLater>();
                 else wait_vm<0>();
+                scale_tile(w, i);
                 scores(at, w, s);
                 uint32_t block = 0;
                 if (more) {
@@ -1355,7 +1443,7 @@ struct Unit {
         if (__builtin_expect(w.marked, 0)) add_infinities(w, marks);
         w.l = row_sum<kRows>(w.l);
 
-        const float v_scale = F8 && a.v_scale ? a.v_scale[h] : 1.0f;
+        const float v_scale = F8 && !kBlocks && a.v_scale ? a.v_scale[h] : 1.0f;
         static_assert(kRows * D * 4 <= kRing / kWaves, "a wave's sums of a row tile fit its part of the ring");
         if (!kShared && !by_wave) {
             // The waves of a row group join: each leaves its sums in LDS, then
@@ -1483,7 +1571,7 @@ struct Unit {
                 asm volatile("" ::: "memory");  // (eight loads at a time)
             }
         }
-        w.scale = a.scale_log2 * (F8 && a.k_scale ? a.k_scale[h] : 1.0f);
+        w.scale = a.scale_log2 * (F8 && !kBlocks && a.k_scale ? a.k_scale[h] : 1.0f);
     }
 
     __device__ __forceinline__ void use_queries(Rows& w) const {
@@ -1539,6 +1627,7 @@ struct Unit {
         }
         w.mx = -__builtin_inff();
         w.l = 0.0f;
+        if constexpr (kBlocks) w.tile = Blocks{0.0f, 0.0f, 1.0f, 0.0f, ~0u};
 #pragma unroll
         for (int t2 = 0; t2 < kT; ++t2) w.o[t2] = acc{};
         w.all_lo = lane_max(w.all_lo, 0);
@@ -1567,36 +1656,62 @@ struct Unit {
 // kWide: waves share their tiles in some unit of the launch.
 template <int D, class E, bool F8, bool kWide>
 __global__ __launch_bounds__(kThreads, D == 256 ? 1 : 2) void prefix_attention_kernel(AttnArgs a) {
+    constexpr Kind C = F8 ? Kind::e4m3 : Kind::wide;
     extern __shared__ __align__(16) uint8_t lds[];
-    Shared<D>& sh = *reinterpret_cast<Shared<D>*>(lds);
-    uint64_t* const cost = reinterpret_cast<uint64_t*>(lds + sizeof(Shared<D>));
+    shared_of<D, C>& sh = *reinterpret_cast<shared_of<D, C>*>(lds);
+    uint64_t* const cost = reinterpret_cast<uint64_t*>(lds + sizeof(sh));
     uint32_t* const info = reinterpret_cast<uint32_t*>(cost + a.plan.own_entries + 1);
     Line line = build_line(a, cost, info, sh);
     const RowSplit &pre = a.plan.prefix, &own = a.plan.own;
     Job job;
     while (next_prefix(a, line, job, D)) {
         if (job.s0 >= job.s1) continue;
-        if (kWide && pre.shared) Unit<D, E, F8, 32>(a, sh).template run<true>(job, pre, true, false, line.plain);
-        else if (pre.narrow) Unit<D, E, F8, 16>(a, sh).template run<false>(job, pre, true, false, line.plain);
-        else Unit<D, E, F8, 32>(a, sh).template run<false>(job, pre, true, false, line.plain);
+        if (kWide && pre.shared) Unit<D, E, C, 32>(a, sh).template run<true>(job, pre, true, false, line.plain);
+        else if (pre.narrow) Unit<D, E, C, 16>(a, sh).template run<false>(job, pre, true, false, line.plain);
+        else Unit<D, E, C, 32>(a, sh).template run<false>(job, pre, true, false, line.plain);
     }
     while (next_own(a, line, cost, info, sh, job, D)) {
         if (job.s0 >= job.s1) continue;
-        if (kWide && own.shared) Unit<D, E, F8, 32>(a, sh).template run<true>(job, own, false, false, false);
-        else if (own.narrow) Unit<D, E, F8, 16>(a, sh).template run<false>(job, own, false, true, false);
-        else Unit<D, E, F8, 32>(a, sh).template run<false>(job, own, false, true, false);
+        if (kWide && own.shared) Unit<D, E, C, 32>(a, sh).template run<true>(job, own, false, false, false);
+        else if (own.narrow) Unit<D, E, C, 16>(a, sh).template run<false>(job, own, false, true, false);
+        else Unit<D, E, C, 32>(a, sh).template run<false>(job, own, false, true, false);
+    }
+}
+
+// The same of a block-scaled cache.  (A body of both, called from either, has its
+// registers allocated otherwise: the kernel above would no longer be the one measured.)
+template <int D, class E, Kind C, bool kWide>
+__global__ __launch_bounds__(kThreads, D == 256 ? 1 : 2) void block_attention_kernel(AttnArgs a) {
+    extern __shared__ __align__(16) uint8_t lds[];
+    shared_of<D, C>& sh = *reinterpret_cast<shared_of<D, C>*>(lds);
+    uint64_t* const cost = reinterpret_cast<uint64_t*>(lds + sizeof(sh));
+    uint32_t* const info = reinterpret_cast<uint32_t*>(cost + a.plan.own_entries + 1);
+    Line line = build_line(a, cost, info, sh);
+    const RowSplit &pre = a.plan.prefix, &own = a.plan.own;
+    Job job;
+    while (next_prefix(a, line, job, D)) {
+        if (job.s0 >= job.s1) continue;
+        if (kWide && pre.shared) Unit<D, E, C, 32>(a, sh).template run<true>(job, pre, true, false, line.plain);
+        else if (pre.narrow) Unit<D, E, C, 16>(a, sh).template run<false>(job, pre, true, false, line.plain);
+        else Unit<D, E, C, 32>(a, sh).template run<false>(job, pre, true, false, line.plain);
+    }
+    while (next_own(a, line, cost, info, sh, job, D)) {
+        if (job.s0 >= job.s1) continue;
+        if (kWide && own.shared) Unit<D, E, C, 32>(a, sh).template run<true>(job, own, false, false, false);
+        else if (own.narrow) Unit<D, E, C, 16>(a, sh).template run<false>(job, own, false, true, false);
+        else Unit<D, E, C, 32>(a, sh).template run<false>(job, own, false, true, false);
     }
 }
 
 // Dynamic LDS of a launch: the tiles and the line of entries.
-template <int D>
+template <int D, bool kBlocks>
 constexpr size_t lds_bytes(int own_entries) {
-    return sizeof(Shared<D>) + 8 * ((size_t)own_entries + 1) + 4 * (size_t)own_entries;
+    return (kBlocks ? sizeof(SharedBlocks<D>) : sizeof(Shared<D>)) + 8 * ((size_t)own_entries + 1) + 4 * (size_t)own_entries;
 }
 
 template <int D, class E, bool F8, bool kWide>
 hipError_t launch_as(const AttnArgs& a, hipStream_t stream) {
-    prefix_attention_kernel<D, E, F8, kWide><<<dim3(1u << a.plan.log2_workgroups), kThreads, lds_bytes<D>(a.plan.own_entries), stream>>>(a);
+    prefix_attention_kernel<D, E, F8, kWide><<<dim3(1u << a.plan.log2_workgroups), kThreads, lds_bytes<D, false>(a.plan.own_entries), stream>>>(a);
     return hipGetLastError();
 }
 
@@ -1610,6 +1725,22 @@ template <int D>
 hipError_t launch_dim(const AttnArgs& a, bool bf16, bool f8, hipStream_t stream) {
     if (bf16) return f8 ? launch_rows<D, Bf16, true>(a, stream) : launch_rows<D, Bf16, false>(a, stream);
     return f8 ? launch_rows<D, Half, true>(a, stream) : launch_rows<D, Half, false>(a, stream);
+}
+
+template <int D, class E, Kind C>
+hipError_t launch_kind(const AttnArgs& a, hipStream_t stream) {
+    const dim3 grid(1u << a.plan.log2_workgroups);
+    const size_t lds = lds_bytes<D, true>(a.plan.own_entries);
+    if (a.plan.shared) block_attention_kernel<D, E, C, true><<<grid, kThreads, lds, stream>>>(a);
+    else block_attention_kernel<D, E, C, false><<<grid, kThreads, lds, stream>>>(a);
+    return hipGetLastError();
+}
+
+template <int D>
+hipError_t launch_blocks(const AttnArgs& a, bool bf16, bool i8, hipStream_t stream) {
+    if (i8) return launch_kind<D, Half, Kind::i8_blocks>(a, stream);
+    if (bf16) return launch_kind<D, Bf16, Kind::e4m3_blocks>(a, stream);
+    return launch_kind<D, Half, Kind::e4m3_blocks>(a, stream);
 }
 
 }  // namespace attn

@@ -219,12 +219,15 @@ hipError_t launch_join(const AttnArgs& a, hipStream_t stream) {
 
 }  // namespace
 
-int most_own_entries(int dim) {
+int most_own_entries(int dim, bool blocks) {
     constexpr size_t kLds = 160 * 1024, kEntry = 12;
-    static_assert(attn::lds_bytes<64>(1) - attn::lds_bytes<64>(0) == kEntry);
-    const size_t rest = kLds - (dim == 64    ? attn::lds_bytes<64>(0)
-                                : dim == 128 ? attn::lds_bytes<128>(0)
-                                             : attn::lds_bytes<256>(0));
+    static_assert(attn::lds_bytes<64, false>(1) - attn::lds_bytes<64, false>(0) == kEntry);
+    const size_t rest = kLds - (blocks       ? dim == 64    ? attn::lds_bytes<64, true>(0)
+                                               : dim == 128 ? attn::lds_bytes<128, true>(0)
+                                                            : attn::lds_bytes<256, true>(0)
+                                : dim == 64  ? attn::lds_bytes<64, false>(0)
+                                : dim == 128 ? attn::lds_bytes<128, false>(0)
+                                             : attn::lds_bytes<256, false>(0));
     return (int)(rest / kEntry);
 }
 
@@ -260,9 +263,13 @@ AttnPlan plan_attention(const AttnShape& s) {
 hipError_t launch_prefix_attention(const AttnArgs& a, int dim, uint32_t q_dtype, uint32_t cache_dtype,
                                    hipStream_t stream) {
     const bool bf16 = q_dtype == QW35_HIP_DTYPE_BF16, f8 = cache_dtype == QW35_HIP_DTYPE_E4M3;
-    hipError_t e = dim == 64    ? launch_attn_d64(a, bf16, f8, stream)
-                   : dim == 128 ? launch_attn_d128(a, bf16, f8, stream)
-                                : launch_attn_d256(a, bf16, f8, stream);
+    const bool i8 = cache_dtype == QW35_HIP_DTYPE_I8_BLOCKS;
+    hipError_t e = block_scaled(cache_dtype) ? dim == 64    ? launch_attn_blocks_d64(a, bf16, i8, stream)
+                                               : dim == 128 ? launch_attn_blocks_d128(a, bf16, i8, stream)
+                                                            : launch_attn_blocks_d256(a, bf16, i8, stream)
+                   : dim == 64               ? launch_attn_d64(a, bf16, f8, stream)
+                   : dim == 128              ? launch_attn_d128(a, bf16, f8, stream)
+                                             : launch_attn_d256(a, bf16, f8, stream);
     if (e != hipSuccess) return e;
     return dim == 64    ? launch_join<64>(a, stream)
            : dim == 128 ? launch_join<128>(a, stream)
