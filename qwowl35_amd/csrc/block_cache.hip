@@ -36,6 +36,14 @@ struct Codes<Int8> {
         };
         return low(a) | low(b) << 8 | low(c) << 16 | low(d) << 24;
     }
+    // The same of x inv, within the codes and numbers all: one instruction each.
+    static __device__ __forceinline__ uint32_t pack4_fits(const float* x, float inv) {
+        uint32_t b[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) b[i] = __builtin_bit_cast(uint32_t, fmaf(x[i], inv, 12582912.0f));
+        const uint32_t lo = __builtin_amdgcn_perm(b[1], b[0], 0x0c0c0400), hi = __builtin_amdgcn_perm(b[3], b[2], 0x04000c0c);
+        return lo | hi;
+    }
     static __device__ __forceinline__ void unpack4(uint32_t w, float (&v)[4]) {
 #pragma unroll
         for (int i = 0; i < 4; ++i) v[i] = (float)(int8_t)(w >> 8 * i);
@@ -49,6 +57,10 @@ struct Codes<Fp8> {
     static __device__ __forceinline__ uint32_t pack4(float a, float b, float c, float d) {
         return pack4_e4m3(a, b, c, d);
     }
+    static __device__ __forceinline__ uint32_t pack4_fits(const float* x, float inv) {
+        const int w = __builtin_amdgcn_cvt_pk_fp8_f32(x[0] * inv, x[1] * inv, 0, false);
+        return (uint32_t)__builtin_amdgcn_cvt_pk_fp8_f32(x[2] * inv, x[3] * inv, w, true);
+    }
     static __device__ __forceinline__ void unpack4(uint32_t w, float (&v)[4]) {
         const auto lo = __builtin_amdgcn_cvt_pk_f32_fp8((int)w, false), hi = __builtin_amdgcn_cvt_pk_f32_fp8((int)w, true);
         v[0] = lo[0];
@@ -58,6 +70,7 @@ struct Codes<Fp8> {
     }
 };
 
+constexpr int kLeastGroups = 1024;   // workgroups that a launch is not cut below
 constexpr int kLeastExponent = -60;  // of a scale: its reciprocal and log2 stay far inside fp32
 
 // The least power of two s with m <= Q s.
@@ -75,7 +88,7 @@ struct BlockAppend {
     int n_tokens;        // of the positions
     int t0, t1;          // the tokens of this launch
     const int64_t* slots;
-    int per;             // tokens whose blocks a workgroup looks for
+    int per;             // tokens whose blocks a workgroup looks for: 32, or 1 of up to 64
     int heads_per;       // heads of a workgroup
     RopeArgs rope;
 };
@@ -83,10 +96,14 @@ struct BlockAppend {
 // What a workgroup shares.
 template <int D>
 struct BlockShared {
-    int src[32];        // of the block's tokens: which of the call it is (-1: none)
-    float top[2][4];    // the waves' largest magnitudes, of this head and the last
+    int src[4][32];     // of the block's tokens: which of the call it is (-1: none); a list, or a list a wave
+    uint32_t top[2][4];  // the waves' largest magnitudes, of this head and the last
     float before[2];    // the scale before
-    uint2 codes[32][D / 8 + 1];
+    int count[4];       // the waves' counts of a block's tokens
+    union {
+        uint2 codes[32][D / 8 + 1];         // of values, on their way to eight tokens of a column
+        alignas(16) float angles[32][D / 2 + 2][2];  // of keys: cosine and sine of each pair (the pad: rows apart in the banks)
+    };
 };
 
 // The scale of a block, and what its old codes are multiplied by (zero: they are forgotten).
@@ -108,25 +125,34 @@ __device__ __forceinline__ Scale scale_of(float before, bool anew, float m) {
     return s;
 }
 
-// The block's scale from every thread's largest magnitude.
-template <class C, int D>
-__device__ __forceinline__ Scale agree(BlockShared<D>& sh, int parity, const float* at, bool anew, float m) {
-#pragma unroll
-    for (int o = 1; o < 64; o *= 2) m = fmaxf(m, __shfl_xor(m, o));
+// The largest of every thread's magnitudes (as fp32 bits), and thread 0's `before`.
+template <int D>
+__device__ __forceinline__ uint32_t agree(BlockShared<D>& sh, int parity, uint32_t m, float& before) {
+    m = __builtin_bit_cast(uint32_t, wave_max_abs(__builtin_bit_cast(float, m)));
     if ((threadIdx.x & 63) == 0) sh.top[parity][threadIdx.x >> 6] = m;
-    if (threadIdx.x == 0) sh.before[parity] = anew ? 0.0f : *at;
+    if (threadIdx.x == 0) sh.before[parity] = before;
     __syncthreads();
-    m = fmaxf(fmaxf(sh.top[parity][0], sh.top[parity][1]), fmaxf(sh.top[parity][2], sh.top[parity][3]));
-    return scale_of<C>(sh.before[parity], anew, m);
+    before = sh.before[parity];
+    const uint32_t a = dpp_max_u32(sh.top[parity][0], sh.top[parity][1]), b = dpp_max_u32(sh.top[parity][2], sh.top[parity][3]);
+    return dpp_max_u32(a, b);
 }
 
-// The largest finite magnitude of eight numbers; infinities become fp32's largest number (and so the largest code).
-__device__ __forceinline__ float largest(float (&x)[8], float m) {
+constexpr uint32_t kInfinity = 0x7f800000u;
+
+__device__ __forceinline__ uint32_t largest(const float (&x)[8], uint32_t m) {
+#pragma unroll
+    for (int j = 0; j < 8; ++j) m = dpp_max_u32(m, __builtin_bit_cast(uint32_t, x[j]) & 0x7fffffffu);
+    return m;
+}
+
+// For a block with infinities or NaN: the largest of eight numbers that are finite; infinities become fp32's
+// largest number, and so the largest code.
+__device__ __forceinline__ uint32_t largest_finite(float (&x)[8], uint32_t m) {
 #pragma unroll
     for (int j = 0; j < 8; ++j) {
-        const float v = fabsf(x[j]);
-        m = v < __builtin_inff() && v > m ? v : m;
-        if (v == __builtin_inff()) x[j] = copysignf(0x1.fffffep127f, x[j]);
+        const uint32_t v = __builtin_bit_cast(uint32_t, x[j]) & 0x7fffffffu;
+        m = v < kInfinity && v > m ? v : m;
+        if (v == kInfinity) x[j] = copysignf(0x1.fffffep127f, x[j]);
     }
     return m;
 }
@@ -141,7 +167,8 @@ __device__ __forceinline__ uint32_t again(uint32_t w, float shrink) {
 }
 
 template <class C>
-__device__ __forceinline__ uint2 pack8(const float (&x)[8], float inv) {
+__device__ __forceinline__ uint2 pack8(const float (&x)[8], float inv, bool fits) {
+    if (fits) return {Codes<C>::pack4_fits(x, inv), Codes<C>::pack4_fits(x + 4, inv)};
     return {Codes<C>::pack4(x[0] * inv, x[1] * inv, x[2] * inv, x[3] * inv),
             Codes<C>::pack4(x[4] * inv, x[5] * inv, x[6] * inv, x[7] * inv)};
 }
@@ -156,88 +183,270 @@ __device__ __forceinline__ void transpose4(const uint32_t (&w)[4], uint32_t (&r)
     r[3] = __builtin_amdgcn_perm(d, c, 0x07060302);
 }
 
-// A workgroup writes blocks: of `per` tokens of the call those that are the
-// first of theirs look through the call's slots for the block's other tokens (of two
-// with the same slot the last counts), so that every block has one writer, in
-// whatever order the tokens come, and results do not depend on timing.  A
-// thread holds eight columns of D / 64 of the block's tokens.
+// A block of a call: its tokens there (-1: none) in the list, and which they are as bits.
+struct Found {
+    const int* src;
+    uint32_t written;
+    int64_t block;
+};
+
+// The blocks that a workgroup writes: those of which one of its `per` tokens is
+// the call's first.  Each has one writer, in whatever order the tokens come (of two
+// with the same slot the last counts), so results do not depend on timing.
+//   Up to 64 tokens: a lane each, every wave by itself.  More: the first of each run
+// of a block's tokens begins with those in its chunk (`start`), and looks through all
+// of the call's slots meanwhile.  If there are more of the block it gives way to an
+// earlier one, or begins again with all of them.
+template <int D, class S, class W>
+__device__ __forceinline__ void each_block(const BlockAppend& a, BlockShared<D>& sh, S start, W write) {
+    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+    const int64_t n_slots = (int64_t)a.cache.n_pages * a.cache.page_size;
+    // (a prompt's blocks: the first of them may have begun before it)
+    const int base = a.per == 1 ? a.t0 : a.t0 + (int)blockIdx.x * 32 - (int)(a.slots[a.t0] & 31);
+    const int here = base + lane, end = a.per == 1 || base + 32 > a.t1 ? a.t1 : base + 32;
+    const int64_t slot = here >= a.t0 && here < end ? a.slots[here] : -1;
+    const bool valid = slot >= 0 && slot < n_slots;
+    const int64_t mine = valid ? slot >> 5 : -1;
+    int* const src = sh.src[wave];
+    auto of_lane = [](int64_t v, int l) {
+        return (int64_t)((uint64_t)(uint32_t)__builtin_amdgcn_readlane((int)(v >> 32), l) << 32 |
+                         (uint32_t)__builtin_amdgcn_readlane((int)v, l));
+    };
+    auto near = [&](int64_t block) {  // the lanes' tokens of a block
+        if (lane < 32) src[lane] = -1;
+        __builtin_amdgcn_wave_barrier();
+        if (mine == block) atomicMax(&src[slot & 31], here);
+        __builtin_amdgcn_wave_barrier();
+        return Found{src, (uint32_t)__ballot(src[lane & 31] >= 0), block};
+    };
+    if (a.per == 1) {
+        const int first = (int)blockIdx.x;  // below 64
+        const int64_t block = of_lane(mine, first);
+        if (block < 0 || __ballot(mine == block) & ((1ull << first) - 1)) return;
+        const Found f = near(block);
+        start(f);
+        write(f);
+        return;
+    }
+    const int64_t before = (int64_t)((uint64_t)(uint32_t)__shfl_up((int)(mine >> 32), 1) << 32 | (uint32_t)__shfl_up((int)mine, 1));
+    uint32_t runs = (uint32_t)__ballot(valid && (lane == 0 || mine != before));
+    while (runs) {
+        const int l = __builtin_ctz(runs);
+        runs &= runs - 1;
+        const int64_t block = of_lane(mine, l);
+        if (__ballot(mine == block) & ((1ull << l) - 1)) continue;
+        Found f = near(block);
+        start(f);
+        // how many tokens of the block the call has
+        const uint32_t lo = (uint32_t)block << 5, hi = (uint32_t)(block >> 27);
+        int count = 0;
+        typedef uint32_t pair_t __attribute__((ext_vector_type(4), aligned(8)));
+        constexpr int kAhead = 4;  // loads on their way together
+        for (int j0 = a.t0 + 2 * tid; j0 < a.t1; j0 += 512 * kAhead) {
+            pair_t s[kAhead];
+#pragma unroll
+            for (int i = 0; i < kAhead; ++i) {
+                const int j = j0 + 512 * i;
+                s[i] = pair_t{~0u, ~0u, ~0u, ~0u};
+                if (j + 1 < a.t1) s[i] = *reinterpret_cast<const pair_t*>(a.slots + j);
+                else if (j < a.t1) s[i] = pair_t{(uint32_t)a.slots[j], (uint32_t)(a.slots[j] >> 32), ~0u, ~0u};
+            }
+#pragma unroll
+            for (int i = 0; i < kAhead; ++i) {
+                count += ((s[i][0] ^ lo) & ~31u | (s[i][1] ^ hi)) == 0;
+                count += ((s[i][2] ^ lo) & ~31u | (s[i][3] ^ hi)) == 0;
+            }
+        }
+#pragma unroll
+        for (int o = 1; o < 64; o *= 2) count += __shfl_xor(count, o);
+        if (lane == 0) sh.count[wave] = count;
+        __syncthreads();
+        count = sh.count[0] + sh.count[1] + sh.count[2] + sh.count[3];
+        if (count != __popcll(__ballot(mine == block))) {  // some lie elsewhere in the call
+            int* const all = sh.src[0];
+            if (tid < 32) all[tid] = -1;
+            __syncthreads();
+            int earlier = 0;
+            for (int j = a.t0 + tid; j < a.t1; j += 256) {
+                const int64_t s = a.slots[j];
+                if (s >> 5 != block) continue;
+                if (j < base) earlier = 1;
+                else atomicMax(&all[s & 31], j);
+            }
+            if (__syncthreads_or(earlier)) continue;
+            f = Found{all, (uint32_t)__ballot(all[lane & 31] >= 0), block};
+            start(f);
+        }
+        write(f);
+        __syncthreads();  // (the lists are read)
+    }
+}
+
+__device__ __forceinline__ void positions_of(const RopeArgs& r, int n_tokens, int t, int (&pos)[4]) {
+#pragma unroll
+    for (int a = 0; a < 4; ++a) pos[a] = a < r.n_axes ? r.positions[(int64_t)a * n_tokens + t] : 0;
+}
+
+// What turn_of and norm_and_turn (rope_rows.h) compute, of a pair, and of rows with
+// the norm's weights and the angles at hand.
+__device__ __forceinline__ void turn_pair(const RopeArgs& r, const int (&pos)[4], int pair, uint64_t freq, float (&to)[2]) {
+    int p = pos[0];
+    if (r.n_axes > 1) {
+        const int a = axis_of(r, pair);
+        p = a == 0 ? pos[0] : a == 1 ? pos[1] : a == 2 ? pos[2] : pos[3];
+    }
+    const uint64_t turns = (uint64_t)(int64_t)p * freq;
+    sincospif((float)(int32_t)(turns >> 32) * 0x1p-31f, &to[1], &to[0]);
+}
+
+template <int D, int kRows>
+__device__ __forceinline__ void norm_and_turn_rows(const RopeArgs& r, int li, int row0, const float (&weight)[8],
+                                                   const BlockShared<D>& sh, float (&v)[kRows][8]) {
+    constexpr int kLanes = D / 8, kStep = 256 / kLanes;
+    if (r.norm) {
+        float sum[kRows];
+#pragma unroll
+        for (int i = 0; i < kRows; ++i) {
+            sum[i] = 0.0f;
+#pragma unroll
+            for (int j = 0; j < 8; ++j) sum[i] = fmaf(v[i][j], v[i][j], sum[i]);
+        }
+#pragma unroll
+        for (int o = kLanes / 2; o; o >>= 1)
+#pragma unroll
+            for (int i = 0; i < kRows; ++i) sum[i] += __shfl_xor(sum[i], o);
+#pragma unroll
+        for (int i = 0; i < kRows; ++i) {
+            const float inv = 1.0f / sqrtf(sum[i] / (float)(8 * kLanes) + r.eps);
+#pragma unroll
+            for (int j = 0; j < 8; ++j) v[i][j] = v[i][j] * inv * weight[j];
+        }
+    }
+    if (r.freq) {
+        const int step = r.rot_dim / 16;  // lanes from a column to its pair's other half
+        const int lane = threadIdx.x & 63;
+        const bool low = li < step, in = li < 2 * step;
+        const int from = in ? (low ? lane + step : lane - step) : lane, pair = low ? li * 8 : (li - step) * 8;
+#pragma unroll
+        for (int i = 0; i < kRows; ++i) {
+            const float4_t* const angles = reinterpret_cast<const float4_t*>(sh.angles[row0 + i * kStep][in ? pair : 0]);
+#pragma unroll
+            for (int k = 0; k < 4; ++k) {
+                const float4_t two = angles[k];
+#pragma unroll
+                for (int e = 0; e < 2; ++e) {
+                    const float mine = v[i][2 * k + e], other = __shfl(mine, from);
+                    const float cos = two[2 * e], sin = low ? -two[2 * e + 1] : two[2 * e + 1];
+                    if (in) v[i][2 * k + e] = mine * cos + other * sin;
+                }
+            }
+            asm volatile("" ::: "memory");  // (a row's angles at a time)
+        }
+    }
+}
+
+// A thread holds eight columns of D / 64 of the block's tokens; the next head's
+// are on their way while one is written.
 template <class TI, class C, int D, bool kValues>
 __device__ __forceinline__ void append_blocks(const BlockAppend& a, BlockShared<D>& sh) {
     constexpr int kLanes = D / 8, kRows = D / 64, kStep = 256 / kLanes;
     const int tid = threadIdx.x, li = tid % kLanes, row0 = tid / kLanes;
     const int heads = (int)a.cache.kv_heads, blocks = (int)a.cache.page_size / 32;
-    const int64_t n_slots = (int64_t)a.cache.n_pages * a.cache.page_size;
     const int h0 = ((int)blockIdx.y >> 1) * a.heads_per, h1 = h0 + a.heads_per < heads ? h0 + a.heads_per : heads;
     const HeadsView& x_view = kValues ? a.v : a.k;
     uint8_t* const pages = static_cast<uint8_t*>(kValues ? a.cache.v : a.cache.k);
     float* const scales = const_cast<float*>(kValues ? a.cache.v_scale : a.cache.k_scale);  // (the cache's, written here)
-    for (int i = 0; i < a.per; ++i) {
-        const int t = a.t0 + (int)blockIdx.x * a.per + i;
-        if (t >= a.t1) break;
-        const int64_t slot = a.slots[t];
-        if (slot < 0 || slot >= n_slots) continue;
-        const int64_t block = slot / 32;
-        if (t > a.t0) {
-            const int64_t last = a.slots[t - 1];
-            if (last >= 0 && last / 32 == block) continue;
-        }
-        __syncthreads();
-        if (tid < 32) sh.src[tid] = -1;
-        __syncthreads();
-        int earlier = 0;
-        for (int j = a.t0 + tid; j < a.t1; j += 256) {
-            const int64_t s = a.slots[j];
-            if (s < 0 || s / 32 != block) continue;
-            if (j < t) earlier = 1;
-            else atomicMax(&sh.src[s & 31], j);
-        }
-        if (__syncthreads_or(earlier)) continue;
-        const uint32_t written = (uint32_t)__ballot(sh.src[tid & 31] >= 0);
-        const bool anew = written & 1;
-        const int64_t page = block / blocks;
-        const int in_page = (int)(block - page * blocks);
-        int src[kRows];
+    // values: this thread's granules are four columns of eight tokens
+    const int quad = tid % (D / 4), octet = tid / (D / 4);
+    // of the block that is written, and of its next head
+    bool anew = false, merge = false;  // merge: with granules that hold other tokens
+    int64_t tile0 = 0;
+    uint32_t mine = 0;
+    int src[kRows];
+    float next[kRows][8], before_next = 0.0f;
+    uint4_t old_next[2] = {};
+    auto load = [&](int h) {
+        const int64_t tile = tile0 + (int64_t)h * blocks;
 #pragma unroll
-        for (int r = 0; r < kRows; ++r) src[r] = sh.src[row0 + r * kStep];
-        Turn turn[kRows];
+        for (int r = 0; r < kRows; ++r) {
+#pragma unroll
+            for (int j = 0; j < 8; ++j) next[r][j] = 0.0f;
+            if (src[r] >= 0)
+                load8<TI>(x_view.data, src[r] * x_view.token_stride + h * x_view.head_stride + li * 8, x_view.vec, next[r]);
+        }
+        before_next = tid == 0 && !anew ? scales[tile] : 0.0f;
+        if (merge) {
+            const uint4_t* const from = reinterpret_cast<const uint4_t*>(pages + tile * (32 * D) + octet * 8 * D + quad * 32);
+            old_next[0] = from[0];
+            old_next[1] = from[1];
+        }
+    };
+    float weight[8] = {};
+    if (!kValues && a.rope.norm) {
+#pragma unroll
+        for (int j = 0; j < 8; ++j) weight[j] = a.rope.norm[li * 8 + j];
+    }
+    auto start = [&](const Found& f) {
+        anew = f.written & 1;
+        const int64_t page = f.block / blocks;
+        tile0 = page * heads * blocks + (f.block - page * blocks);
+        mine = octet < 4 ? f.written >> octet * 8 & 0xff : 0xff;
+        merge = kValues && !anew && mine != 0xff;
+#pragma unroll
+        for (int r = 0; r < kRows; ++r) src[r] = f.src[row0 + r * kStep];
+        load(h0);
+    };
+    each_block<D>(a, sh, start, [&](const Found& f) {
         if constexpr (!kValues) {
+            // the block's angles, by eight threads a token, four of each on their way together (by the lanes that take
+            // them they are 12 us of a chunk of 249 tokens x 256 columns, of which 64 turn)
+            const int half = a.rope.rot_dim / 2, token = f.src[tid >> 3];
+            if (a.rope.freq && token >= 0) {
+                int pos[4];
+                positions_of(a.rope, a.n_tokens, token, pos);
+                for (int p = tid & 7; p < half; p += 32) {
+                    uint64_t freq[4];
 #pragma unroll
-            for (int r = 0; r < kRows; ++r) {
-                turn[r] = Turn{};
-                if (a.rope.freq && src[r] >= 0 && li * 8 < a.rope.rot_dim) turn[r] = turn_of(a.rope, a.n_tokens, src[r], li * 8);
+                    for (int i = 0; i < 4; ++i) freq[i] = a.rope.freq[p + 8 * i < half ? p + 8 * i : p];
+#pragma unroll
+                    for (int i = 0; i < 4; ++i)
+                        if (p + 8 * i < half) turn_pair(a.rope, pos, p + 8 * i, freq[i], sh.angles[tid >> 3][p + 8 * i]);
+                }
             }
+            __syncthreads();
         }
         for (int h = h0; h < h1; ++h) {
-            const int64_t tile = (page * heads + h) * blocks + in_page;
+            const int64_t tile = tile0 + (int64_t)h * blocks;
             uint8_t* const codes = pages + tile * (32 * D);
-            float x[kRows][8] = {}, m = 0.0f;
+            float x[kRows][8];
+            uint32_t m = 0;
 #pragma unroll
             for (int r = 0; r < kRows; ++r)
-                if (src[r] >= 0)
-                    load8<TI>(x_view.data, src[r] * x_view.token_stride + h * x_view.head_stride + li * 8, x_view.vec, x[r]);
-            if constexpr (!kValues) {
 #pragma unroll
-                for (int r = 0; r < kRows; ++r) norm_and_turn(a.rope, D, kLanes, li, turn[r], x[r]);
-            }
+                for (int j = 0; j < 8; ++j) x[r][j] = next[r][j];
+            float before = before_next;
+            const uint4_t old[2] = {old_next[0], old_next[1]};
+            if (h + 1 < h1) load(h + 1);
+            if constexpr (!kValues) norm_and_turn_rows<D>(a.rope, li, row0, weight, sh, x);
 #pragma unroll
-            for (int r = 0; r < kRows; ++r) m = largest(x[r], m);
-            // (values: this thread's granules, four columns of eight tokens)
-            const int quad = tid % (D / 4), octet = tid / (D / 4);
-            const uint32_t mine = octet < 4 ? written >> octet * 8 & 0xff : 0xff;
-            uint4_t* const granules = reinterpret_cast<uint4_t*>(codes + (octet & 3) * 8 * D + quad * 32);
-            uint4_t old[2] = {};
-            if (kValues && !anew && mine != 0xff) {
-                old[0] = granules[0];
-                old[1] = granules[1];
+            for (int r = 0; r < kRows; ++r) m = src[r] >= 0 ? largest(x[r], m) : m;
+            m = agree<D>(sh, h & 1, m, before);
+            const bool finite = m < kInfinity;
+            if (!finite) {
+                m = 0;
+#pragma unroll
+                for (int r = 0; r < kRows; ++r) m = src[r] >= 0 ? largest_finite(x[r], m) : m;
+                __syncthreads();
+                m = agree<D>(sh, h & 1, m, before);
             }
-            const Scale s = agree<C>(sh, h & 1, scales + tile, anew, m);
+            const Scale s = scale_of<C>(before, anew, __builtin_bit_cast(float, m));
             const float inv = s.now > 0.0f ? 1.0f / s.now : 0.0f;
             const bool rewrite = anew || s.shrink != 1.0f;  // the tokens that the call does not write change too
             if constexpr (!kValues) {
 #pragma unroll
                 for (int r = 0; r < kRows; ++r) {
                     uint2* const at = reinterpret_cast<uint2*>(codes + li * 256 + (row0 + r * kStep) * 8);
-                    uint2 w = pack8<C>(x[r], inv);
+                    uint2 w = pack8<C>(x[r], inv, finite);
                     if (src[r] < 0) {
                         if (!rewrite) continue;
                         w = {0, 0};
@@ -250,7 +459,7 @@ __device__ __forceinline__ void append_blocks(const BlockAppend& a, BlockShared<
                 }
             } else {
 #pragma unroll
-                for (int r = 0; r < kRows; ++r) sh.codes[row0 + r * kStep][li] = pack8<C>(x[r], inv);
+                for (int r = 0; r < kRows; ++r) sh.codes[row0 + r * kStep][li] = pack8<C>(x[r], inv, finite);
                 __syncthreads();
                 if (octet < 4 && (mine || rewrite)) {
                     uint32_t w[2][4], g[2][4];
@@ -260,7 +469,7 @@ __device__ __forceinline__ void append_blocks(const BlockAppend& a, BlockShared<
                     transpose4(w[0], g[0]);
                     transpose4(w[1], g[1]);
                     uint4_t out[2] = {{g[0][0], g[1][0], g[0][1], g[1][1]}, {g[0][2], g[1][2], g[0][3], g[1][3]}};
-                    if (!anew && mine != 0xff) {
+                    if (merge) {
                         uint32_t keep[2];  // bytes of the tokens that the call writes
 #pragma unroll
                         for (int j = 0; j < 2; ++j) keep[j] = ((mine >> 4 * j & 15) * 0x00204081u & 0x01010101u) * 255u;
@@ -271,18 +480,19 @@ __device__ __forceinline__ void append_blocks(const BlockAppend& a, BlockShared<
                             out[j / 4][j % 4] = (out[j / 4][j % 4] & keep[j & 1]) | (o & ~keep[j & 1]);
                         }
                     }
-                    granules[0] = out[0];
-                    granules[1] = out[1];
+                    uint4_t* const to = reinterpret_cast<uint4_t*>(codes + octet * 8 * D + quad * 32);
+                    to[0] = out[0];
+                    to[1] = out[1];
                 }
             }
             if (tid == 0 && s.changed) scales[tile] = s.now;
         }
-    }
+    });
 }
 
 // blockIdx.y: even keys, odd values of a group of heads.
 template <class TI, class C, int D>
-__global__ __launch_bounds__(256) void kv_append_blocks_kernel(BlockAppend a) {
+__global__ __launch_bounds__(256, D == 256 ? 3 : 4) void kv_append_blocks_kernel(BlockAppend a) {
     __shared__ BlockShared<D> sh;
     if (blockIdx.y & 1) append_blocks<TI, C, D, true>(a, sh);
     else append_blocks<TI, C, D, false>(a, sh);
@@ -294,9 +504,13 @@ hipError_t append_dim(BlockAppend a, int n, hipStream_t stream) {
     for (a.t0 = 0; a.t0 < n; a.t0 = a.t1) {
         const int count = n - a.t0 < kAppendSlice ? n - a.t0 : kAppendSlice;
         a.t1 = a.t0 + count;
-        a.per = (int64_t)count * heads > 2048 ? 32 : 1;
+        a.per = count > 64 ? 32 : 1;
+        const int chunks = a.per == 1 ? count : (count + 31 + 31) / 32;  // (the first may begin before the tokens)
+        // (every workgroup of several heads saves one a look through the slots)
         a.heads_per = 1;
-        const dim3 grid((unsigned)((count + a.per - 1) / a.per), (unsigned)((heads + a.heads_per - 1) / a.heads_per * 2));
+        while (a.per > 1 && a.heads_per < heads && (int64_t)chunks * 2 * ((heads + 2 * a.heads_per - 1) / (2 * a.heads_per)) >= kLeastGroups)
+            a.heads_per *= 2;
+        const dim3 grid((unsigned)chunks, (unsigned)((heads + a.heads_per - 1) / a.heads_per * 2));
         kv_append_blocks_kernel<TI, C, D><<<grid, 256, 0, stream>>>(a);
         const hipError_t e = hipGetLastError();
         if (e != hipSuccess) return e;
@@ -329,54 +543,156 @@ struct CacheRead {
     int by_block;  // scales: of a block; else of a head
 };
 
+// Four consecutive elements of a cache, from where they are or out of a word of 8-bit ones.
 template <class C>
-__device__ __forceinline__ float element(const void* cache, int64_t at) {
-    if constexpr (std::is_same_v<C, Int8>) {
-        return (float)static_cast<const int8_t*>(cache)[at];
-    } else if constexpr (std::is_same_v<C, Fp8>) {
+struct Four {
+    typedef C raw __attribute__((ext_vector_type(4)));
+    static __device__ __forceinline__ void unpack(raw w, float (&v)[4]) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) v[i] = (float)w[i];
+    }
+    static __device__ __forceinline__ float one(const void* cache, int64_t at) { return (float)static_cast<const C*>(cache)[at]; }
+};
+template <class C>
+struct Four8 {
+    typedef uint32_t raw;
+    static __device__ __forceinline__ void unpack(raw w, float (&v)[4]) { Codes<C>::unpack4(w, v); }
+    static __device__ __forceinline__ float one(const void* cache, int64_t at) {
         float v[4];
-        Codes<Fp8>::unpack4(static_cast<const uint8_t*>(cache)[at], v);
+        unpack(static_cast<const uint8_t*>(cache)[at], v);
         return v[0];
+    }
+};
+template <>
+struct Four<Int8> : Four8<Int8> {};
+template <>
+struct Four<Fp8> : Four8<Fp8> {};
+
+template <class T>
+__device__ __forceinline__ void store4(void* base, int64_t at, bool vec, const float (&v)[4]) {
+    T* const p = static_cast<T*>(base) + at;
+    typedef T vec_t __attribute__((ext_vector_type(4)));
+    if (vec) {
+        *reinterpret_cast<vec_t*>(p) = vec_t{(T)v[0], (T)v[1], (T)v[2], (T)v[3]};
     } else {
-        return (float)static_cast<const C*>(cache)[at];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) p[i] = (T)v[i];
     }
 }
 
-// A lane has eight columns of a head of a token.
-template <class C, class TO>
+// Bound by bytes.  Of keys a thread has eight columns (a granule of the cache) of
+// D / 64 tokens, a workgroup 32 tokens of a head, so that it uses whole lines of
+// the granules, which lie token by token.  Of values a thread has four columns of
+// eight tokens: where those are the eight of a granule it reads 32 bytes (64 of a
+// 16-bit cache) and writes four elements of each token, a row at a time by its lanes.
+template <class C, class TO, int D>
 __global__ __launch_bounds__(256) void kv_read_kernel(CacheRead a) {
-    const int heads = (int)a.cache.kv_heads, dim = (int)a.cache.head_dim, page_size = (int)a.cache.page_size;
-    const int lanes = dim / 8;
-    const bool values = blockIdx.y != 0;
-    const int64_t item = ((int64_t)blockIdx.x * 256 + threadIdx.x) / lanes;
-    const int li = threadIdx.x % lanes;
-    const int64_t t = item / heads;
-    const int h = (int)(item - t * heads);
-    if (t >= a.n_tokens) return;
-    const int64_t slot = a.slots[t];
-    float x[8] = {};
-    if (slot >= 0 && slot < (int64_t)a.cache.n_pages * page_size) {
-        const int64_t page = slot / page_size, tile0 = (page * heads + h) * (page_size / 32);
-        const int at = (int)(slot - page * page_size);
-        const float* const scales = values ? a.cache.v_scale : a.cache.k_scale;
-        const float scale = !scales ? 1.0f : a.by_block ? scales[tile0 + at / 32] : scales[h];
-        const int64_t base = tile0 * (32 * dim);
+    const int tid = threadIdx.x, h = (int)blockIdx.y >> 1, heads = (int)a.cache.kv_heads;
+    const int64_t n_slots = (int64_t)a.cache.n_pages * a.cache.page_size;
+    const bool small = n_slots <= 0xffffffffll;
+    const float* const scales = blockIdx.y & 1 ? a.cache.v_scale : a.cache.k_scale;
+    struct Place {
+        int64_t tile;  // 32 tokens of the head
+        float scale;
+        int at;        // token of the tile
+        bool live;
+    };
+    auto find = [&](int64_t slot) {
+        Place p = {0, 1.0f, (int)(slot & 31), slot >= 0 && slot < n_slots};
+        const int blocks = (int)a.cache.page_size / 32;
+        const int64_t block = p.live ? slot >> 5 : 0;
+        const int64_t page = small ? (int64_t)((uint32_t)block / (uint32_t)blocks) : block / blocks;
+        p.tile = (page * heads + h) * blocks + (block - page * blocks);
+        if (scales) p.scale = a.by_block ? scales[p.tile] : scales[h];
+        return p;
+    };
+    typedef typename Four<C>::raw raw;
+    if ((blockIdx.y & 1) == 0) {
+        constexpr int kLanes = D / 8, kRows = D / 64, kStep = 256 / kLanes;
+        const int li = tid % kLanes, t0 = (int)blockIdx.x * 32 + tid / kLanes;
+        int64_t slot[kRows];
+        Place p[kRows];
+        raw w[kRows][2];
 #pragma unroll
-        for (int j = 0; j < 8; ++j) {
-            const int64_t e = values ? base + (int64_t)(at / 8) * 8 * dim + (li * 8 + j) * 8 + at % 8
-                                     : base + (int64_t)(at / 32) * 32 * dim + li * 256 + (at % 32) * 8 + j;
-            x[j] = element<C>(values ? a.cache.v : a.cache.k, e) * scale;
+        for (int r = 0; r < kRows; ++r) slot[r] = t0 + r * kStep < a.n_tokens ? a.slots[t0 + r * kStep] : -1;
+#pragma unroll
+        for (int r = 0; r < kRows; ++r) {
+            p[r] = find(slot[r]);
+            const raw* const from = static_cast<const raw*>(a.cache.k) + (p[r].tile * (32 * D) + li * 256 + p[r].at * 8) / 4;
+            w[r][0] = w[r][1] = raw{};
+            if (p[r].live) {
+                w[r][0] = from[0];
+                w[r][1] = from[1];
+            }
         }
+#pragma unroll
+        for (int r = 0; r < kRows; ++r) {
+            const int t = t0 + r * kStep;
+            if (t >= a.n_tokens) continue;
+            float lo[4], hi[4], x[8];
+            Four<C>::unpack(w[r][0], lo);
+            Four<C>::unpack(w[r][1], hi);
+#pragma unroll
+            for (int j = 0; j < 8; ++j) x[j] = p[r].live ? (j < 4 ? lo[j & 3] : hi[j & 3]) * p[r].scale : 0.0f;
+            store8<TO>(a.k.data, t * a.k.token_stride + h * a.k.head_stride + li * 8, a.k.vec, x);
+        }
+    } else {
+        constexpr int kQuads = D / 4, kOctets = 256 / kQuads;
+        const int shift = (int)(a.slots[0] & 7);  // where the first token lies in its granule
+        const int quad = tid % kQuads, t0 = ((int)blockIdx.x * kOctets + tid / kQuads) * 8 - shift;
+        if (t0 >= a.n_tokens) return;
+        int64_t slot[8];
+        bool whole = true;
+#pragma unroll
+        for (int j = 0; j < 8; ++j) slot[j] = t0 + j >= 0 && t0 + j < a.n_tokens ? a.slots[t0 + j] : -1;
+#pragma unroll
+        for (int j = 0; j < 8; ++j) whole &= slot[j] >= 0 && slot[j] < n_slots && slot[j] == slot[0] + j;
+        float x[8][4];
+        if (whole && (slot[0] & 7) == 0) {
+            const Place p = find(slot[0]);
+            const raw* const from = static_cast<const raw*>(a.cache.v) + (p.tile * (32 * D) + p.at * D + quad * 32) / 4;
+            raw w[8];
+#pragma unroll
+            for (int i = 0; i < 8; ++i) w[i] = from[i];
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+                float v[4];
+                Four<C>::unpack(w[i], v);
+#pragma unroll
+                for (int j = 0; j < 4; ++j) x[i % 2 * 4 + j][i / 2] = v[j] * p.scale;
+            }
+        } else {
+#pragma unroll
+            for (int j = 0; j < 8; ++j) {
+                const Place p = find(slot[j]);
+                const int64_t at = p.tile * (32 * D) + p.at / 8 * (8 * D) + quad * 32 + p.at % 8;
+#pragma unroll
+                for (int i = 0; i < 4; ++i) x[j][i] = p.live ? Four<C>::one(a.cache.v, at + i * 8) * p.scale : 0.0f;
+            }
+        }
+#pragma unroll
+        for (int j = 0; j < 8; ++j)
+            if (t0 + j >= 0 && t0 + j < a.n_tokens)
+                store4<TO>(a.v.data, (t0 + j) * a.v.token_stride + h * a.v.head_stride + quad * 4, a.v.vec, x[j]);
     }
-    const HeadsView& y = values ? a.v : a.k;
-    store8<TO>(y.data, t * y.token_stride + h * y.head_stride + li * 8, y.vec, x);
+}
+
+template <class C, class TO, int D>
+hipError_t read_dim(const CacheRead& a, hipStream_t stream) {
+    constexpr int kTokens = 8192 / D;  // of values in a workgroup; the first octet may begin before the tokens
+    const int keys = (a.n_tokens + 31) / 32, values = (a.n_tokens + 7 + kTokens - 1) / kTokens;
+    const dim3 grid((unsigned)(keys > values ? keys : values), a.cache.kv_heads * 2);
+    kv_read_kernel<C, TO, D><<<grid, 256, 0, stream>>>(a);
+    return hipGetLastError();
 }
 
 template <class C, class TO>
 hipError_t read_as(const CacheRead& a, hipStream_t stream) {
-    const int64_t items = (int64_t)a.n_tokens * a.cache.kv_heads * (a.cache.head_dim / 8);
-    kv_read_kernel<C, TO><<<dim3((unsigned)((items + 255) / 256), 2), 256, 0, stream>>>(a);
-    return hipGetLastError();
+    switch (a.cache.head_dim) {
+        case 64: return read_dim<C, TO, 64>(a, stream);
+        case 128: return read_dim<C, TO, 128>(a, stream);
+        default: return read_dim<C, TO, 256>(a, stream);
+    }
 }
 
 template <class C>
