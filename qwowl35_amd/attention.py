@@ -218,6 +218,7 @@ class PagedCache:
         self.view = _ffi.KvCache(k.data_ptr(), v.data_ptr(), at_k, at_v, pages, self.page_size, heads, self.head_dim,
                                  codes[k.dtype], 0)
         self._at, self._device = C.addressof(self.view), device
+        self.number = torch.float16 if k.dtype.itemsize == 1 else k.dtype  # that its elements are read as
 
     @classmethod
     def empty(cls, n_pages: int, kv_heads: int, page_size: int, head_dim: int, dtype: torch.dtype = torch.float16,
@@ -293,18 +294,25 @@ def kv_read(cache: PagedCache, slots: torch.Tensor, dtype: torch.dtype | None = 
             return kv_read(cache, slots, dtype, k, v)
     if slots.dim() != 1:
         raise Qw35Error("slots must be int64 [n_tokens]")
-    n = int(slots.shape[0])
+    n = len(slots)
     where = _index(slots, torch.int64, (n,), device, "slots")
-    if dtype is None:
-        dtype = next((x.dtype for x in (k, v) if x is not None), cache.k.dtype)
-        dtype = torch.float16 if dtype.itemsize == 1 else dtype
-    shape = (n, cache.kv_heads, cache.head_dim)
-    k, v = (torch.empty(shape, dtype=dtype, device=cache.k.device) if x is None else x for x in (k, v))
-    for name, x in (("k", k), ("v", v)):
-        if x.shape != shape or x.dtype != dtype or x.get_device() != device:
-            raise Qw35Error(f"{name} must be a {dtype} {list(shape)} tensor on {cache.k.device}, got {x.dtype} "
-                            f"{list(x.shape)} on {x.device}")
-    hk, hv = _heads(k, "k"), _heads(v, "v")
+    heads, dim = cache.kv_heads, cache.head_dim
+    shape = (n, heads, dim)
+    if k is None and v is None:  # (rows of its own: what there is to check is the type)
+        dtype = dtype or cache.number
+        code = _FLOAT.get(dtype)
+        if code is None:
+            raise Qw35Error(f"dtype must be fp32, bf16 or fp16, got {dtype}")
+        k, v = (torch.empty(shape, dtype=dtype, device=cache.k.device) for _ in range(2))
+        hk, hv = ((x.data_ptr(), heads * dim, dim, code, 0) for x in (k, v))
+    else:
+        dtype = dtype or (v if k is None else k).dtype
+        k, v = (torch.empty(shape, dtype=dtype, device=cache.k.device) if x is None else x for x in (k, v))
+        for name, x in (("k", k), ("v", v)):
+            if x.shape != shape or x.dtype != dtype or x.get_device() != device:
+                raise Qw35Error(f"{name} must be a {dtype} {list(shape)} tensor on {cache.k.device}, got {x.dtype} "
+                                f"{list(x.shape)} on {x.device}")
+        hk, hv = _heads(k, "k"), _heads(v, "v")
     if n:
         _call("qw35_hip_kv_read", cache._at, _HEADS.pack(*hk), _HEADS.pack(*hv), n, where, rt._raw_stream(device))
     return k, v

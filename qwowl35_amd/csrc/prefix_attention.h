@@ -850,10 +850,35 @@ __device__ __forceinline__ void wait_lds() {
     __builtin_amdgcn_s_waitcnt(0xF | (3 << 14) | (0x7 << 4));
 }
 
+// One such copy (kOffset on both sides) as an instruction that the compiler does not know: behind its own it waits
+// for all LDS reads at a time, at every fifth matrix instruction, since it takes a copy for an access of either
+// memory (256 tokens x 16 heads of 256 over 16001, int8: 136 us with those, 128 without).  Its counts of operations
+// in flight are then too small and its waits too long, never the other way.
+template <int kOffset, int kBytes = 16>
+__device__ __forceinline__ void copy_apart(const void* from, void* to) {
+    typedef __attribute__((address_space(3))) void lds_t;
+    const int at = uniform((int)(uint32_t)(uintptr_t)(lds_t*)to);
+    if constexpr (kBytes == 16)
+        asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, off offset:%2" ::"s"(at), "v"(from), "n"(kOffset) : "m0");
+    else
+        asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dword %1, off offset:%2" ::"s"(at), "v"(from), "n"(kOffset) : "m0");
+}
+
 // Copies kCount KB from global memory to LDS without registers: each
 // instruction moves 1 KB, lane i's 16 bytes to base + 16 i.
-template <int kCount>
+template <int kCount, bool kApart = false>
 __device__ __forceinline__ void copy_kb(const uint8_t* from, uint8_t* to, int lane) {
+    if constexpr (kApart) {
+#pragma unroll
+        for (int i = 0; i < kCount; i += 4) {
+            const uint8_t* const g = from + i * 1024 + lane * 16;
+            copy_apart<0>(g, to + i * 1024);
+            if (i + 1 < kCount) copy_apart<1024>(g, to + i * 1024);
+            if (i + 2 < kCount) copy_apart<2048>(g, to + i * 1024);
+            if (i + 3 < kCount) copy_apart<3072>(g, to + i * 1024);
+        }
+        return;
+    }
     typedef const __attribute__((address_space(1))) void global_t;
     typedef __attribute__((address_space(3))) void lds_t;
 #pragma unroll
@@ -868,8 +893,9 @@ __device__ __forceinline__ void copy_kb(const uint8_t* from, uint8_t* to, int la
 }
 
 // KB i of such a copy.
+template <bool kApart = false>
 __device__ __forceinline__ void copy_1kb(const uint8_t* from, uint8_t* to, int i, int lane) {
-    copy_kb<1>(from + i * 1024, to + i * 1024, lane);
+    copy_kb<1, kApart>(from + i * 1024, to + i * 1024, lane);
 }
 
 template <int D>
@@ -900,12 +926,14 @@ template <int D, Kind C>
 using shared_of = std::conditional_t<(C >= Kind::e4m3_blocks), SharedBlocks<D>, Shared<D>>;
 
 // Raw granules of a tile: 16 bytes of a 16-bit cache, 8 of an 8-bit one.
+typedef uint32_t uint2_t __attribute__((ext_vector_type(2)));
 template <Kind C>
-using raw8 = std::conditional_t<C != Kind::wide, uint2, uint4_t>;
+using raw8 = std::conditional_t<C == Kind::wide, uint4_t, std::conditional_t<C == Kind::e4m3, uint2, uint2_t>>;
 
 template <class E, Kind C>
 __device__ __forceinline__ typename E::vec8 operand(raw8<C> w) {
-    if constexpr (C == Kind::i8_blocks) return E::from_i8(w);
+    if constexpr (C == Kind::i8_blocks) return E::from_i8(uint2{w.x, w.y});
+    else if constexpr (C == Kind::e4m3_blocks) return E::from_e4m3(uint2{w.x, w.y});
     else if constexpr (C != Kind::wide) return E::from_e4m3(w);
     else return __builtin_bit_cast(typename E::vec8, w);
 }
@@ -976,19 +1004,28 @@ struct Unit {
         std::conditional_t<kBlocks, Blocks, Nothing> tile;
     };
 
-    // Tile i's, whose scales came with its copies.
+    // Of tile i, whose scales came with its copies; `last` is the tile before.
+    struct Scales {
+        float k, v;
+    };
+    __device__ __forceinline__ Scales scales_of(int i) const {
+        const float(&from)[2][64] = sh.scales[wave][i >> 6 & 1];
+        return {from[0][i & 63], from[1][i & 63]};
+    }
+    static __device__ __forceinline__ Blocks blocks_of(const Rows& w, Scales s, const Blocks& last) {
+        Blocks b;
+        // (zero: every finite score alike; a missing tile's may be anything, and its scores are masked)
+        b.key = fminf(fmaxf(w.scale * s.k, 2e-38f), 3e38f);
+        const bool some = s.v > 0.0f;
+        const float lift = __builtin_amdgcn_logf(s.v);
+        b.lift = some ? lift : last.lift;
+        b.unlift = __builtin_amdgcn_exp2f(-b.lift);
+        b.keep = some ? ~0u : 0u;
+        b.sum = 0.0f;
+        return b;
+    }
     __device__ __forceinline__ void scale_tile(Rows& w, int i) const {
-        if constexpr (kBlocks) {
-            const float(&from)[2][64] = sh.scales[wave][i >> 6 & 1];
-            const float v = from[1][i & 63];
-            // (zero: every finite score alike; a missing tile's may be anything, and its scores are masked)
-            w.tile.key = fminf(fmaxf(w.scale * from[0][i & 63], 2e-38f), 3e38f);
-            const bool some = v > 0.0f;
-            const float lift = __builtin_amdgcn_logf(v);
-            w.tile.lift = some ? lift : w.tile.lift;
-            w.tile.unlift = __builtin_amdgcn_exp2f(-w.tile.lift);
-            w.tile.keep = some ? ~0u : 0u;
-        }
+        if constexpr (kBlocks) w.tile = blocks_of(w, scales_of(i), w.tile);
     }
     // What a score is as an exponent.
     static __device__ __forceinline__ float exponent(const Rows& w, float s) {
@@ -1023,8 +1060,9 @@ struct Unit {
 
     // `beside`(step): other work, a part after the matrix instructions of each step.
     static constexpr int kScoreSteps = kM * kB, kValueSteps = kK * kT;
-    template <class F = Nothing>
-    __device__ __forceinline__ void scores(const uint8_t* keys, const Rows& w, acc (&s)[kB], F beside = {}) const {
+    // (w: a wave's Rows, this unit's or those of the block-scaled one that unpacked the tile for it)
+    template <class F = Nothing, class R>
+    __device__ __forceinline__ void scores(const uint8_t* keys, const R& w, acc (&s)[kB], F beside = {}) const {
         constexpr int kSteps = kScoreSteps, kAhead = kSteps < 4 ? kSteps : 4;
         vec8 k[kAhead];
 #pragma unroll
@@ -1048,7 +1086,7 @@ struct Unit {
         __builtin_amdgcn_sched_group_barrier(0x100, kAhead, 0);
 #pragma unroll
         for (int m = 0; m < kSteps; ++m) {
-            if (F8) __builtin_amdgcn_sched_group_barrier(0x002, 4, 0);
+            if (F8) __builtin_amdgcn_sched_group_barrier(0x002, C == Kind::i8_blocks ? 10 : 4, 0);
             __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
             if (m + kAhead < kSteps) __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);
         }
@@ -1111,13 +1149,20 @@ struct Unit {
         end_terms(w, p);
     }
 
-    template <class F = Nothing>
-    __device__ __forceinline__ void add_values(const uint8_t* values, Rows& w, const vec8 (&p)[kK],
+    static constexpr int kValuesAhead = kValueSteps < 4 ? kValueSteps : 4;
+    template <class F = Nothing, class R>
+    __device__ __forceinline__ void add_values(const uint8_t* values, R& w, const vec8 (&p)[kK],
                                                F beside = {}) const {
-        constexpr int kSteps = kValueSteps, kAhead = kSteps < 4 ? kSteps : 4;
-        vec8 v[kAhead];
+        vec8 v[kValuesAhead];
 #pragma unroll
-        for (int i = 0; i < kAhead; ++i) v[i] = value(values, i / kK, i % kK);
+        for (int i = 0; i < kValuesAhead; ++i) v[i] = value(values, i / kK, i % kK);
+        add_values_from(v, values, w, p, beside);
+    }
+    // v: the first operands.
+    template <class F = Nothing, class R>
+    __device__ __forceinline__ void add_values_from(vec8 (&v)[kValuesAhead], const uint8_t* values, R& w,
+                                                    const vec8 (&p)[kK], F beside = {}) const {
+        constexpr int kSteps = kValueSteps, kAhead = kValuesAhead;
 #pragma unroll
         for (int i = 0; i < kSteps; ++i) {
             const vec8 vv = v[i % kAhead];
@@ -1131,8 +1176,8 @@ struct Unit {
 
     // Keeps infinities and NaN of a tile's values, of which some rows see only
     // a part, from the product (all waves of a shared tile come here together).
-    template <bool kShared>
-    __device__ __forceinline__ void split_off_infinities(uint8_t* tile, Rows& w, int t0, bool there,
+    template <bool kShared, class R>
+    __device__ __forceinline__ void split_off_infinities(uint8_t* tile, R& w, int t0, bool there,
                                                          uint32_t* marks) const {
         if (kFinite || __builtin_expect(!__any(not_finite(tile)), 1)) return;
         mark_infinities(tile, w, t0, there, marks);
@@ -1183,7 +1228,8 @@ struct Unit {
     //   marks: [t][sign][kRows], bits of the tile's kRows columns; a lane
     // keeps sign g % 2 of row n.  (No branch here or in the tile loop depends on
     // the lane: the paths would keep copies of the accumulators where they meet.)
-    __device__ __forceinline__ void mark_infinities(const uint8_t* tile, Rows& w, int t0, bool there,
+    template <class R>
+    __device__ __forceinline__ void mark_infinities(const uint8_t* tile, R& w, int t0, bool there,
                                                     uint32_t* marks) const {
         const int mine = (g & 1) * kRows + n;
         if (!w.marked) {
@@ -1254,12 +1300,10 @@ struct Unit {
         asm("" : "+v"(block));  // (a choice of two values, not of two paths)
         p.blocks = (uint32_t)id < a.n_pages ? block : kNoBlock;
         if constexpr (kBlocks) {  // their scales, a lane's at a time, ahead of their copies
-            typedef const __attribute__((address_space(1))) void global_t;
-            typedef __attribute__((address_space(3))) void lds_t;
             const uint32_t at = p.blocks == kNoBlock ? 0u : p.blocks;
             float(&to)[2][64] = sh.scales[wave][i >> 6 & 1];
-            __builtin_amdgcn_global_load_lds((global_t*)(a.k_blocks + at), (lds_t*)to[0], 4, 0, 0);
-            __builtin_amdgcn_global_load_lds((global_t*)(a.v_blocks + at), (lds_t*)to[1], 4, 0, 0);
+            copy_apart<0, 4>(a.k_blocks + at, to[0]);
+            copy_apart<0, 4>(a.v_blocks + at, to[1]);
         }
     }
     // Tile i, the last looked up or the first of the next 64.
@@ -1299,7 +1343,9 @@ struct Unit {
 
         if (!by_wave) __syncthreads();  // the ring is free
         else wait_lds();
-        constexpr int kFit = kShared ? kRing / (2 * kTile) : kRing / kWaves / (2 * kTile);
+        // (shared tiles of a block-scaled cache are unpacked in LDS: two of keys and two of values besides those on their way)
+        constexpr int kUnpacked = 32 * D * 2, kRaw = kShared && kBlocks ? kRing - 4 * kUnpacked : kRing;
+        constexpr int kFit = kShared ? kRaw / (2 * kTile) : kRing / kWaves / (2 * kTile);
         static_assert(kRows * D / 4 <= sizeof(sh.marks[0]), "room for the marks");
         constexpr int kMost = kShared ? 6 : 4;
         constexpr int kPairs = kFit < kMost ? kFit : kMost;
@@ -1325,25 +1371,137 @@ struct Unit {
         load_queries(w, sq, h, row0, row_end);
         int loaded = 0;
         if constexpr (kShared) {
-            for (; loaded < kPairs - 1 && loaded < pages.count; ++loaded) {
+            for (; loaded < kPairs - (kBlocks ? 0 : 1) && loaded < pages.count; ++loaded) {
                 const uint8_t* from;
                 uint8_t* to;
                 quarter_of(loaded, from, to);
-                copy_kb<kKb / 2>(from, to, lane);
+                copy_kb<kKb / 2, kBlocks>(from, to, lane);
             }
         } else {
             for (; loaded < kPairs && loaded < pages.count; ++loaded) {
                 const uint32_t block = block_of(pages, loaded);
                 note(block);
                 uint8_t* const to = ring + loaded * 2 * kTile;
-                copy_kb<kKb>(kbase + bytes_at(block), to, lane);
-                copy_kb<kKb>(vbase + bytes_at(block), to + kTile, lane);
+                copy_kb<kKb, kBlocks>(kbase + bytes_at(block), to, lane);
+                copy_kb<kKb, kBlocks>(vbase + bytes_at(block), to + kTile, lane);
             }
         }
         start_rows<kShared>(w, sq, prefix, plain, row0, row_end);
         use_queries(w);  // (here the queries are waited for, not in the tile loop)
 
-        if constexpr (kShared) {
+        if constexpr (kShared && kBlocks) {
+            // As below, over tiles that the four waves unpack together, a quarter each, into the queries' type: each
+            // of them by itself took 151 us for 256 tokens x 16 heads of 256 over 16001, int8, this 136 (and 128 with
+            // copies apart).  A step unpacks the keys of the tile after the next and the values of the next among
+            // its matrix instructions; its barrier is also theirs.  Over longer contexts a tile takes what one of a
+            // 16-bit cache does (32002 tokens more: 162 us, fp16 155).
+            typedef Unit<D, E, Kind::wide, kRows> Wide;
+            const Wide wide(a, sh);
+            constexpr int kEach = kKb / 2;       // a wave's copies of a pair
+            constexpr int kQuarter = D / 64;     // granules of a tile that a lane unpacks
+            constexpr int kStride = kScoreSteps / kQuarter;
+            static_assert(kScoreSteps == kValueSteps && kStride * kQuarter == kScoreSteps && kPairs >= 4);
+            auto raw_keys = [&](int i) { return ring + (i % kPairs) * 2 * kTile; };
+            auto keys = [&](int i) { return ring + kRaw + (i & 1) * kUnpacked; };
+            auto values = [&](int i) { return ring + kRaw + (2 + (i & 1)) * kUnpacked; };
+            raw packed;
+            // Of a quarter's granules one every kStride matrix instructions, read two of those ahead.
+            auto unpack = [&](const uint8_t* from, uint8_t* to, int m) {
+                const int at = (wave * kQuarter + m / kStride) * 64 + lane;
+                if (m % kStride == 0) packed = *reinterpret_cast<const raw*>(from + at * 8);
+                if (m % kStride == 2) *reinterpret_cast<vec8*>(to + at * 16) = operand<E, C>(packed);
+            };
+            auto unpack_all = [&](const uint8_t* from, uint8_t* to) {
+                raw all[kQuarter];
+#pragma unroll
+                for (int j = 0; j < kQuarter; ++j)
+                    all[j] = *reinterpret_cast<const raw*>(from + ((wave * kQuarter + j) * 64 + lane) * 8);
+#pragma unroll
+                for (int j = 0; j < kQuarter; ++j)
+                    *reinterpret_cast<vec8*>(to + ((wave * kQuarter + j) * 64 + lane) * 16) = operand<E, C>(all[j]);
+            };
+            acc s[kB];
+            float top;
+            if (kPairs <= pages.count) wait_vm<(kPairs - 2) * kEach>();  // (a job has a step, and a step a tile)
+            else wait_vm<0>();
+            __builtin_amdgcn_s_barrier();  // tiles 0 and 1 are there
+            asm volatile("" ::: "memory");
+            unpack_all(raw_keys(0), keys(0));
+            unpack_all(raw_keys(1), keys(1));
+            unpack_all(raw_keys(0) + kTile, values(0));
+            wait_lds();
+            __builtin_amdgcn_s_barrier();
+            asm volatile("" ::: "memory");
+            wide.scores(keys(0), w, s);
+            top = largest(s);
+            const int clear0 = tiles.sink + ((w.all_lo + 31) / 32 > tiles.lo ? (w.all_lo + 31) / 32 - tiles.lo : 0) - pages.first;
+            const int clear1 = tiles.sink + w.all_hi / 32 - tiles.lo - pages.first;
+            scale_tile(w, 0);
+            auto see_and_follow = [&](int i) {
+                if (i < clear0 || i >= clear1 || missing) {
+                    const bool there = there_bits >> (loaded - 1 - i) & 1;
+                    const int t0 = tiles.at(pages.first + i) * 32;
+                    if constexpr (!kFinite) {
+                        __syncthreads();  // (all of the tile is unpacked)
+                        wide.template split_off_infinities<true>(values(i), w, t0, there, marks);
+                    }
+                    mask(w, s, t0, there);
+                    top = largest(s);
+                }
+                follow(w, top);
+            };
+            vec8 p[kK];
+            auto step = [&](int i, auto copies) {
+                see_and_follow(i);
+                if (copies) wait_vm<(kPairs - 3) * kEach>();
+                else wait_vm<0>();
+                // tile i + 2 is there, and keys i + 1 and values i unpacked; the raw tile i has been read by all, and
+                // the keys i and values i - 1
+                __builtin_amdgcn_s_barrier();
+                asm volatile("" ::: "memory");
+                const uint8_t* from = nullptr;
+                uint8_t* to = nullptr;
+                if (copies) quarter_of(loaded++, from, to);
+                __builtin_amdgcn_sched_barrier(0);
+                acc next[kB];
+                static_assert(kEach <= kScoreSteps, "a copy a step");
+                // (past the last tile: what lies there, for nobody)
+                const uint8_t* const more_keys = raw_keys(i + 2);
+                const uint8_t* const more_values = raw_keys(i + 1) + kTile;
+                const Scales coming = scales_of(i + 1);
+                vec8 first[Wide::kValuesAhead];  // of the values, on their way while the last scores are made
+                wide.scores(keys(i + 1), w, next, [&](int m) {
+                    if (copies && m < kEach) copy_1kb<true>(from, to, m, lane);
+                    unpack(more_keys, keys(i), m);
+                    terms(w, s, p, kScores * m / kScoreSteps, kScores * (m + 1) / kScoreSteps);
+                    const int v = m - (kScoreSteps - Wide::kValuesAhead);
+                    if (v >= 0) first[v] = wide.value(values(i), v / kK, v % kK);
+                });
+                end_terms(w, p);
+                top = -__builtin_inff();
+                Blocks after;
+                wide.add_values_from(first, values(i), w, p, [&](int m) {
+                    unpack(more_values, values(i + 1), m);
+                    if (m == 1) after = blocks_of(w, coming, w.tile);
+#pragma unroll
+                    for (int j = kScores * m / kValueSteps; j < kScores * (m + 1) / kValueSteps; ++j) {
+                        top = fmaxf(top, next[j / kAcc][j % kAcc]);
+                        s[j / kAcc][j % kAcc] = next[j / kAcc][j % kAcc];
+                    }
+                });
+                w.tile = after;
+                wait_lds();
+            };
+            int i = 0;
+            for (; i + kPairs < pages.count; ++i) step(i, std::true_type{});
+            for (; i + 1 < pages.count; ++i) step(i, std::false_type{});
+            see_and_follow(i);
+            __syncthreads();  // (values i are unpacked)
+            terms(w, s, p);
+            end_terms(w, p);
+            wide.add_values(values(i), w, p);
+            wait_lds();
+        } else if constexpr (kShared) {
             // In one step the matrix unit makes the next tile's scores while
             // the vector unit turns this one's into the softmax' terms, then
             // the values' product while it looks for the largest of the next.
@@ -1360,7 +1518,6 @@ struct Unit {
             const int clear0 = tiles.sink + ((w.all_lo + 31) / 32 > tiles.lo ? (w.all_lo + 31) / 32 - tiles.lo : 0) - pages.first;
             const int clear1 = tiles.sink + w.all_hi / 32 - tiles.lo - pages.first;
             auto see_and_follow = [&](int i) {
-                scale_tile(w, i);
                 if (i < clear0 || i >= clear1 || missing) {
                     const bool there = there_bits >> (loaded - 1 - i) & 1;
                     const int t0 = tiles.at(pages.first + i) * 32;
@@ -1428,7 +1585,7 @@ struct Unit {
                     block = block_of(pages, loaded);
                     note(block);
                     ++loaded;
-                    copy_kb<kKb>(kbase + bytes_at(block), at, lane);
+                    copy_kb<kKb, kBlocks>(kbase + bytes_at(block), at, lane);
                 }
                 softmax(w, s, t0, masked, there, p);
                 if (more) wait_vm<kLater>();
@@ -1436,7 +1593,7 @@ struct Unit {
                 add_values(at + kTile, w, p);
                 if (more) {
                     wait_lds();
-                    copy_kb<kKb>(vbase + bytes_at(block), at + kTile, lane);
+                    copy_kb<kKb, kBlocks>(vbase + bytes_at(block), at + kTile, lane);
                 }
             }
         }
