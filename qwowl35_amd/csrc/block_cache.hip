@@ -70,7 +70,8 @@ struct Codes<Fp8> {
     }
 };
 
-constexpr int kLeastGroups = 1024;   // workgroups that a launch is not cut below
+constexpr int kLeastGroups = 1024;  // workgroups that a launch is not cut below
+constexpr int kMostLooks = 128;     // places of a call whose blocks are looked for apart
 constexpr int kLeastExponent = -60;  // of a scale: its reciprocal and log2 stay far inside fp32
 
 // The least power of two s with m <= Q s.
@@ -88,7 +89,7 @@ struct BlockAppend {
     int n_tokens;        // of the positions
     int t0, t1;          // the tokens of this launch
     const int64_t* slots;
-    int per;             // tokens whose blocks a workgroup looks for: 32, or 1 of up to 64
+    int per;             // tokens whose blocks a workgroup looks for (a power of two up to 32)
     int heads_per;       // heads of a workgroup
     RopeArgs rope;
 };
@@ -190,52 +191,68 @@ struct Found {
     int64_t block;
 };
 
+__device__ __forceinline__ int64_t of_lane(int64_t v, int l) {
+    return (int64_t)((uint64_t)(uint32_t)__builtin_amdgcn_readlane((int)(v >> 32), l) << 32 |
+                     (uint32_t)__builtin_amdgcn_readlane((int)v, l));
+}
+
+// A token of the call in a lane.
+struct Near {
+    int token;
+    int64_t slot, block;  // -1: none
+};
+__device__ __forceinline__ Near near(const BlockAppend& a, int token) {
+    Near x = {token, token >= a.t0 && token < a.t1 ? a.slots[token] : -1, -1};
+    if (x.slot >= 0 && x.slot < (int64_t)a.cache.n_pages * a.cache.page_size) x.block = x.slot >> 5;
+    return x;
+}
+
+// The lanes' tokens of a block, in a wave's list.
+__device__ __forceinline__ Found found(int* src, const Near& x, int64_t block) {
+    const int lane = threadIdx.x & 63;
+    if (lane < 32) src[lane] = -1;
+    __builtin_amdgcn_wave_barrier();
+    if (x.block == block) atomicMax(&src[x.slot & 31], x.token);
+    __builtin_amdgcn_wave_barrier();
+    return {src, (uint32_t)__ballot(src[lane & 31] >= 0), block};
+}
+
 // The blocks that a workgroup writes: those of which one of its `per` tokens is
 // the call's first.  Each has one writer, in whatever order the tokens come (of two
 // with the same slot the last counts), so results do not depend on timing.
-//   Up to 64 tokens: a lane each, every wave by itself.  More: the first of each run
-// of a block's tokens begins with those in its chunk (`start`), and looks through all
-// of the call's slots meanwhile.  If there are more of the block it gives way to an
-// earlier one, or begins again with all of them.
-template <int D, class S, class W>
+//   kFew, of up to 64 tokens: every wave has them all, a lane each, and a workgroup
+// one.  (In the general form, whose paths wait for what they have loaded where they
+// meet, 8 tokens took 8.0 us for 6.7.)
+//   Else a wave has the 64 tokens before the workgroup's and the 64 from them on, two
+// a lane.  A block whose first token there is the workgroup's begins with those
+// (`start`), and all slots are looked through meanwhile; if there are more of the
+// block it gives way to an earlier one, or begins again with all of them.
+template <bool kFew, int D, class S, class W>
 __device__ __forceinline__ void each_block(const BlockAppend& a, BlockShared<D>& sh, S start, W write) {
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
-    const int64_t n_slots = (int64_t)a.cache.n_pages * a.cache.page_size;
-    // (a prompt's blocks: the first of them may have begun before it)
-    const int base = a.per == 1 ? a.t0 : a.t0 + (int)blockIdx.x * 32 - (int)(a.slots[a.t0] & 31);
-    const int here = base + lane, end = a.per == 1 || base + 32 > a.t1 ? a.t1 : base + 32;
-    const int64_t slot = here >= a.t0 && here < end ? a.slots[here] : -1;
-    const bool valid = slot >= 0 && slot < n_slots;
-    const int64_t mine = valid ? slot >> 5 : -1;
     int* const src = sh.src[wave];
-    auto of_lane = [](int64_t v, int l) {
-        return (int64_t)((uint64_t)(uint32_t)__builtin_amdgcn_readlane((int)(v >> 32), l) << 32 |
-                         (uint32_t)__builtin_amdgcn_readlane((int)v, l));
-    };
-    auto near = [&](int64_t block) {  // the lanes' tokens of a block
-        if (lane < 32) src[lane] = -1;
-        __builtin_amdgcn_wave_barrier();
-        if (mine == block) atomicMax(&src[slot & 31], here);
-        __builtin_amdgcn_wave_barrier();
-        return Found{src, (uint32_t)__ballot(src[lane & 31] >= 0), block};
-    };
-    if (a.per == 1) {
-        const int first = (int)blockIdx.x;  // below 64
-        const int64_t block = of_lane(mine, first);
-        if (block < 0 || __ballot(mine == block) & ((1ull << first) - 1)) return;
-        const Found f = near(block);
+    if constexpr (kFew) {
+        const Near mine = near(a, a.t0 + lane);
+        const int first = (int)blockIdx.x;
+        const int64_t block = of_lane(mine.block, first);
+        if (block < 0 || __ballot(mine.block == block) & ((1ull << first) - 1)) return;
+        const Found f = found(src, mine, block);
         start(f);
         write(f);
         return;
     }
-    const int64_t before = (int64_t)((uint64_t)(uint32_t)__shfl_up((int)(mine >> 32), 1) << 32 | (uint32_t)__shfl_up((int)mine, 1));
-    uint32_t runs = (uint32_t)__ballot(valid && (lane == 0 || mine != before));
+    // (workgroups begin where a prompt's blocks do: the first may have begun before it)
+    const int base = a.t0 + (int)blockIdx.x * a.per - (a.per > 1 ? (int)(a.slots[a.t0] & (a.per - 1)) : 0);
+    const Near below = near(a, base - 64 + lane), here = near(a, base + lane);
+    const int64_t last = (int64_t)((uint64_t)(uint32_t)__shfl_up((int)(here.block >> 32), 1) << 32 | (uint32_t)__shfl_up((int)here.block, 1));
+    uint32_t runs = (uint32_t)__ballot(lane < a.per && here.block >= 0 && (lane == 0 || here.block != last));
     while (runs) {
         const int l = __builtin_ctz(runs);
         runs &= runs - 1;
-        const int64_t block = of_lane(mine, l);
-        if (__ballot(mine == block) & ((1ull << l) - 1)) continue;
-        Found f = near(block);
+        const int64_t block = of_lane(here.block, l);
+        const uint64_t before = __ballot(below.block == block), from = __ballot(here.block == block);
+        if (before || from & ((1ull << l) - 1)) continue;
+        Found f = found(src, here, block);
         start(f);
         // how many tokens of the block the call has
         const uint32_t lo = (uint32_t)block << 5, hi = (uint32_t)(block >> 27);
@@ -262,7 +279,7 @@ __device__ __forceinline__ void each_block(const BlockAppend& a, BlockShared<D>&
         if (lane == 0) sh.count[wave] = count;
         __syncthreads();
         count = sh.count[0] + sh.count[1] + sh.count[2] + sh.count[3];
-        if (count != __popcll(__ballot(mine == block))) {  // some lie elsewhere in the call
+        if (count != __popcll(from)) {  // some lie elsewhere in the call
             int* const all = sh.src[0];
             if (tid < 32) all[tid] = -1;
             __syncthreads();
@@ -347,7 +364,7 @@ __device__ __forceinline__ void norm_and_turn_rows(const RopeArgs& r, int li, in
 
 // A thread holds eight columns of D / 64 of the block's tokens; the next head's
 // are on their way while one is written.
-template <class TI, class C, int D, bool kValues>
+template <class TI, class C, int D, bool kFew, bool kValues>
 __device__ __forceinline__ void append_blocks(const BlockAppend& a, BlockShared<D>& sh) {
     constexpr int kLanes = D / 8, kRows = D / 64, kStep = 256 / kLanes;
     const int tid = threadIdx.x, li = tid % kLanes, row0 = tid / kLanes;
@@ -396,7 +413,7 @@ __device__ __forceinline__ void append_blocks(const BlockAppend& a, BlockShared<
         for (int r = 0; r < kRows; ++r) src[r] = f.src[row0 + r * kStep];
         load(h0);
     };
-    each_block<D>(a, sh, start, [&](const Found& f) {
+    each_block<kFew, D>(a, sh, start, [&](const Found& f) {
         if constexpr (!kValues) {
             // the block's angles, by eight threads a token, four of each on their way together (by the lanes that take
             // them they are 12 us of a chunk of 249 tokens x 256 columns, of which 64 turn)
@@ -491,11 +508,11 @@ __device__ __forceinline__ void append_blocks(const BlockAppend& a, BlockShared<
 }
 
 // blockIdx.y: even keys, odd values of a group of heads.
-template <class TI, class C, int D>
+template <class TI, class C, int D, bool kFew>
 __global__ __launch_bounds__(256, D == 256 ? 3 : 4) void kv_append_blocks_kernel(BlockAppend a) {
     __shared__ BlockShared<D> sh;
-    if (blockIdx.y & 1) append_blocks<TI, C, D, true>(a, sh);
-    else append_blocks<TI, C, D, false>(a, sh);
+    if (blockIdx.y & 1) append_blocks<TI, C, D, kFew, true>(a, sh);
+    else append_blocks<TI, C, D, kFew, false>(a, sh);
 }
 
 template <class TI, class C, int D>
@@ -504,14 +521,18 @@ hipError_t append_dim(BlockAppend a, int n, hipStream_t stream) {
     for (a.t0 = 0; a.t0 < n; a.t0 = a.t1) {
         const int count = n - a.t0 < kAppendSlice ? n - a.t0 : kAppendSlice;
         a.t1 = a.t0 + count;
-        a.per = count > 64 ? 32 : 1;
-        const int chunks = a.per == 1 ? count : (count + 31 + 31) / 32;  // (the first may begin before the tokens)
+        // A prompt has a block for every 32 tokens, a decode step one for each: workgroups for up to kMostLooks places
+        // keep both apart enough.
+        a.per = 1;
+        while (a.per < 32 && count > kMostLooks * a.per) a.per *= 2;
+        const int chunks = (count + 2 * (a.per - 1)) / a.per;  // (the first may begin before the tokens)
         // (every workgroup of several heads saves one a look through the slots)
         a.heads_per = 1;
-        while (a.per > 1 && a.heads_per < heads && (int64_t)chunks * 2 * ((heads + 2 * a.heads_per - 1) / (2 * a.heads_per)) >= kLeastGroups)
+        while (count > 64 && a.heads_per < heads && (int64_t)chunks * 2 * ((heads + 2 * a.heads_per - 1) / (2 * a.heads_per)) >= kLeastGroups)
             a.heads_per *= 2;
         const dim3 grid((unsigned)chunks, (unsigned)((heads + a.heads_per - 1) / a.heads_per * 2));
-        kv_append_blocks_kernel<TI, C, D><<<grid, 256, 0, stream>>>(a);
+        if (count <= 64) kv_append_blocks_kernel<TI, C, D, true><<<grid, 256, 0, stream>>>(a);
+        else kv_append_blocks_kernel<TI, C, D, false><<<grid, 256, 0, stream>>>(a);
         const hipError_t e = hipGetLastError();
         if (e != hipSuccess) return e;
     }

@@ -77,6 +77,36 @@ def test_append_of_many_tokens(cuda, kind, n, heads):
     blk.same(c, want)
 
 
+MANY = {  # slots of n tokens, of pages of 64
+    "step": lambda n: torch.arange(n) * 64 + 5,                                     # a decode step: a block for each
+    "prompts": lambda n: torch.cat([p * 1024 + torch.arange(37 * p % 50, 37 * p % 50 + m)
+                                    for p, m in enumerate((n // 3, n // 4 + 7, n - n // 3 - n // 4 - 7))]),
+    "apart": lambda n: torch.arange(n) // 2 + torch.arange(n) % 2 * 2048,            # two sequences token by token
+    "late": lambda n: torch.cat([torch.arange(n - 3), torch.tensor([7, 40, 7])]),    # a block's tokens at either end
+    "shuffled": lambda n: torch.randperm(n, generator=torch.Generator().manual_seed(n)),
+    "padded": lambda n: torch.where(torch.arange(n) % 40 < 33, torch.arange(n), -1),
+    "one": lambda n: torch.arange(n) % 32 + 96,                                      # every token in one block
+}
+
+
+@pytest.mark.parametrize("kind", [I8, E4M3])
+@pytest.mark.parametrize("many", MANY)
+@pytest.mark.parametrize("n", [64, 65, 130, 300, 700])
+def test_append_wherever_the_tokens_go(cuda, kind, many, n):
+    """Every block has one writer, which finds all of its tokens in the call."""
+    from qwowl35_amd import attention as at
+
+    slots = MANY[many](n)
+    c = _blocks(cuda, int(slots.max()) // 64 + 2, 2, 64, 64, kind)
+    want = blk.decode(c)
+    randn = _gen(cuda, n)
+    k, v = randn(n, 2, 64), randn(n, 2, 64)
+    at.kv_append(c, k, v, slots.to(cuda))
+    for state, x in zip(want, (k, v)):
+        blk.append(state, x.double().cpu(), slots, kind)
+    blk.same(c, want, many)
+
+
 @pytest.mark.parametrize("kind", [I8, E4M3])
 @pytest.mark.parametrize("dim,rot,sections,normed", [(256, 64, [11, 11, 10], True), (64, 64, [], False), (128, 32, [], True)])
 def test_append_of_rotated_keys(cuda, kind, dim, rot, sections, normed):
