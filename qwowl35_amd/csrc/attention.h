@@ -114,7 +114,7 @@ struct AttnShape {
     bool single;
     int most_entries;  // the plan counts no more own entries than these
 };
-int most_own_entries(int dim, bool blocks);  // that a compute unit's LDS lists
+int most_own_entries(int dim, uint32_t cache_dtype);  // that a compute unit's LDS lists
 AttnPlan plan_attention(const AttnShape& s);
 hipError_t launch_prefix_attention(const AttnArgs& a, int dim, uint32_t q_dtype, uint32_t cache_dtype,
                                    hipStream_t stream);

@@ -282,7 +282,7 @@ uint64_t qw35_hip_prefix_attention_workspace_size(const qw35_hip_kv_cache* cache
     const uint32_t most[] = {1, 16 / group, 32 / group, 64 / group, 64 / group + 1, n_tokens};
     // A division whose row tiles the list does not hold is refused for this
     // batch, but smaller ones may take it: its size then is that of a full list.
-    const int room = qw35::most_own_entries((int)cache->head_dim, qw35::block_scaled(cache->dtype));
+    const int room = qw35::most_own_entries((int)cache->head_dim, cache->dtype);
     uint64_t need = 256;
     bool served = n_tokens == 0;
     if (n_seqs == n_tokens)
@@ -358,7 +358,7 @@ int qw35_hip_prefix_attention(const qw35_hip_attention* op, const qw35_hip_kv_ca
     a.plan = plan_of(cache, op->n_heads, op->n_seqs, op->n_tokens, max_new, op->prefix_len, op->pages_per_seq,
                      !op->starts, INT_MAX);
     const bool blocks = qw35::block_scaled(cache->dtype);
-    const int room = qw35::most_own_entries((int)cache->head_dim, blocks);
+    const int room = qw35::most_own_entries((int)cache->head_dim, cache->dtype);
     if (a.plan.own_entries > room) {
         set_err(err, err_len, "%s: %d row tiles in a call are %d over the list's room; give it fewer tokens or sequences",
                 what, a.plan.own_entries, a.plan.own_entries - room);

@@ -913,17 +913,20 @@ struct Shared {
     int lane_line[5][64];  // of a line in lanes: cost before, cost, and q0, n, length
 };
 
-// The block scales of a wave's tiles, keys' and values': of the 64 looked up last and of the 64 before.
+// The block scales of a wave's tiles, keys' and values': of the 32 fetched last and of the 32 before.  (int8 keeps them
+// in the place of `marks`, of which it needs none: 64 columns have room for two workgroups a compute unit up to 592
+// sequences then, and 400 with 64 tiles at a time beside them, over which 400 sequences of 400 tokens took 83 us for 67.)
+typedef float scales_t[2][2][32];
 template <int D>
 struct SharedBlocks : Shared<D> {
-    float scales[kWaves][2][2][64];
+    scales_t scales[kWaves];
 };
 
 // What a cache holds: 16-bit numbers of the queries' type, e4m3 with a scale of the
 // head, or e4m3 or int8 with a scale for each 32 tokens of a head.
 enum class Kind { wide, e4m3, e4m3_blocks, i8_blocks };
 template <int D, Kind C>
-using shared_of = std::conditional_t<(C >= Kind::e4m3_blocks), SharedBlocks<D>, Shared<D>>;
+using shared_of = std::conditional_t<C == Kind::e4m3_blocks, SharedBlocks<D>, Shared<D>>;
 
 // Raw granules of a tile: 16 bytes of a 16-bit cache, 8 of an 8-bit one.
 typedef uint32_t uint2_t __attribute__((ext_vector_type(2)));
@@ -1008,15 +1011,20 @@ struct Unit {
     struct Scales {
         float k, v;
     };
+    __device__ __forceinline__ scales_t& scales() const {
+        static_assert(sizeof(scales_t) <= sizeof(sh.marks[0]), "room in the place of the marks");
+        if constexpr (kFinite) return *reinterpret_cast<scales_t*>(sh.marks[wave]);
+        else return sh.scales[wave];
+    }
     __device__ __forceinline__ Scales scales_of(int i) const {
-        const float(&from)[2][64] = sh.scales[wave][i >> 6 & 1];
-        return {from[0][i & 63], from[1][i & 63]};
+        const float(&from)[2][32] = scales()[i >> 5 & 1];
+        return {from[0][i & 31], from[1][i & 31]};
     }
     static __device__ __forceinline__ Blocks blocks_of(const Rows& w, Scales s, const Blocks& last) {
         Blocks b;
         // (zero: every finite score alike; a missing tile's may be anything, and its scores are masked)
         b.key = fminf(fmaxf(w.scale * s.k, 2e-38f), 3e38f);
-        const bool some = s.v > 0.0f;
+        const bool some = s.v > 0.0f && s.v < __builtin_inff();
         const float lift = __builtin_amdgcn_logf(s.v);
         b.lift = some ? lift : last.lift;
         b.unlift = __builtin_amdgcn_exp2f(-b.lift);
@@ -1299,16 +1307,20 @@ struct Unit {
         uint32_t block = ((uint32_t)id * (uint32_t)a.kv_heads + p.h) * a.page_blocks + (b - pi * a.page_blocks);
         asm("" : "+v"(block));  // (a choice of two values, not of two paths)
         p.blocks = (uint32_t)id < a.n_pages ? block : kNoBlock;
-        if constexpr (kBlocks) {  // their scales, a lane's at a time, ahead of their copies
-            const uint32_t at = p.blocks == kNoBlock ? 0u : p.blocks;
-            float(&to)[2][64] = sh.scales[wave][i >> 6 & 1];
-            copy_apart<0, 4>(a.k_blocks + at, to[0]);
-            copy_apart<0, 4>(a.v_blocks + at, to[1]);
-        }
     }
     // Tile i, the last looked up or the first of the next 64.
     __device__ __forceinline__ uint32_t block_of(Pages& p, int i) const {
         if (i && (i & 63) == 0) look_up(p, i);
+        if constexpr (kBlocks) {
+            // the scales of tiles i .. i + 31, keys' by the lower lanes and values' by the upper, ahead of their copies
+            if ((i & 31) == 0) {
+                int l = lane;
+                asm volatile("" : "+v"(l));  // (what follows from it is made here, not kept)
+                const uint32_t block = (uint32_t)__shfl((int)p.blocks, (i & 32) + (l & 31));
+                const float* const from = l < 32 ? a.k_blocks : a.v_blocks;
+                copy_apart<0, 4>(from + (block == kNoBlock ? 0u : block), scales()[i >> 5 & 1]);
+            }
+        }
         return (uint32_t)__builtin_amdgcn_readlane((int)p.blocks, i & 63);
     }
     static __device__ __forceinline__ int64_t bytes_at(uint32_t block) {
@@ -1861,9 +1873,9 @@ __global__ __launch_bounds__(kThreads, D == 256 ? 1 : 2) void block_attention_ke
 }
 
 // Dynamic LDS of a launch: the tiles and the line of entries.
-template <int D, bool kBlocks>
+template <int D, bool kScales>
 constexpr size_t lds_bytes(int own_entries) {
-    return (kBlocks ? sizeof(SharedBlocks<D>) : sizeof(Shared<D>)) + 8 * ((size_t)own_entries + 1) + 4 * (size_t)own_entries;
+    return (kScales ? sizeof(SharedBlocks<D>) : sizeof(Shared<D>)) + 8 * ((size_t)own_entries + 1) + 4 * (size_t)own_entries;
 }
 
 template <int D, class E, bool F8, bool kWide>
@@ -1887,7 +1899,7 @@ hipError_t launch_dim(const AttnArgs& a, bool bf16, bool f8, hipStream_t stream)
 template <int D, class E, Kind C>
 hipError_t launch_kind(const AttnArgs& a, hipStream_t stream) {
     const dim3 grid(1u << a.plan.log2_workgroups);
-    const size_t lds = lds_bytes<D, true>(a.plan.own_entries);
+    const size_t lds = lds_bytes<D, C == Kind::e4m3_blocks>(a.plan.own_entries);
     if (a.plan.shared) block_attention_kernel<D, E, C, true><<<grid, kThreads, lds, stream>>>(a);
     else block_attention_kernel<D, E, C, false><<<grid, kThreads, lds, stream>>>(a);
     return hipGetLastError();

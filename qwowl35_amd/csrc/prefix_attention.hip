@@ -219,10 +219,11 @@ hipError_t launch_join(const AttnArgs& a, hipStream_t stream) {
 
 }  // namespace
 
-int most_own_entries(int dim, bool blocks) {
+int most_own_entries(int dim, uint32_t cache_dtype) {
+    const bool scales = cache_dtype == QW35_HIP_DTYPE_E4M3_BLOCKS;
     constexpr size_t kLds = 160 * 1024, kEntry = 12;
     static_assert(attn::lds_bytes<64, false>(1) - attn::lds_bytes<64, false>(0) == kEntry);
-    const size_t rest = kLds - (blocks       ? dim == 64    ? attn::lds_bytes<64, true>(0)
+    const size_t rest = kLds - (scales       ? dim == 64    ? attn::lds_bytes<64, true>(0)
                                                : dim == 128 ? attn::lds_bytes<128, true>(0)
                                                             : attn::lds_bytes<256, true>(0)
                                 : dim == 64  ? attn::lds_bytes<64, false>(0)

@@ -83,15 +83,17 @@ def test_query_types():
             attend(c=blocks(dtype), q=heads(q), workspace=None)
 
 
+@pytest.mark.parametrize("dtype", BLOCKS)
 @pytest.mark.parametrize("dim", [64, 128, 256])
-def test_the_workspace_is_a_16_bit_caches_or_none(dim):
-    """The scales take room from the list of row tiles: larger batches than that has are refused, by size and call."""
+def test_the_workspace_is_a_16_bit_caches_or_none(dim, dtype):
+    """Scales beside the marks take room from the list of row tiles: larger batches than that has are refused, by size
+    and call."""
     lib = _ffi.load()
-    like, mine = cache(head_dim=dim), blocks(head_dim=dim)
+    like, mine = cache(head_dim=dim), blocks(dtype, head_dim=dim)
     size = lambda c, n: lib.qw35_hip_prefix_attention_workspace_size(C.byref(c), 2, n, n)  # noqa: E731
     assert size(mine, 8) == size(like, 8)
     last = max(n for n in range(1000, 9000) if size(mine, n))
-    assert size(mine, last + 1) == 0
+    assert size(mine, last + 1) == 0 and bool(size(like, last + 1)) == (dtype == _ffi.DTYPE_E4M3_BLOCKS)
     with pytest.raises(Qw35Error, match="row tiles in a call"):
         attend(c=mine, n_heads=2, n_seqs=last + 1, n_tokens=last + 1)
     with pytest.raises(Qw35Error, match="needs a 256-byte aligned workspace"):
