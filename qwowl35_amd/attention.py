@@ -294,7 +294,7 @@ def kv_read(cache: PagedCache, slots: torch.Tensor, dtype: torch.dtype | None = 
             return kv_read(cache, slots, dtype, k, v)
     if slots.dim() != 1:
         raise Qw35Error("slots must be int64 [n_tokens]")
-    n = len(slots)
+    n = slots.shape[0]
     where = _index(slots, torch.int64, (n,), device, "slots")
     heads, dim = cache.kv_heads, cache.head_dim
     shape = (n, heads, dim)
@@ -303,7 +303,8 @@ def kv_read(cache: PagedCache, slots: torch.Tensor, dtype: torch.dtype | None = 
         code = _FLOAT.get(dtype)
         if code is None:
             raise Qw35Error(f"dtype must be fp32, bf16 or fp16, got {dtype}")
-        k, v = (torch.empty(shape, dtype=dtype, device=cache.k.device) for _ in range(2))
+        k = torch.empty(shape, dtype=dtype, device=cache.k.device)
+        v = torch.empty_like(k)
         hk, hv = ((x.data_ptr(), heads * dim, dim, code, 0) for x in (k, v))
     else:
         dtype = dtype or (v if k is None else k).dtype
@@ -348,6 +349,9 @@ def prefix_attention(q: torch.Tensor, cache: PagedCache, pages: torch.Tensor, le
     1 / sqrt(head_dim)), zeros where nothing is seen, times sigmoid(``gate``), in
     ``out_dtype`` (default q's type); the softmax' weights have q's precision in the
     product with v whatever ``out_dtype`` is, everything else is fp32.
+
+    q has the cache's type; over an e4m3 cache either 16-bit type, over an int8 one
+    fp16.
 
     ``max_new``: the most new tokens of a sequence, where it is known: it chooses
     how rows are divided, not what is computed.  All lengths live on the device, so
@@ -415,8 +419,9 @@ class GatedAttention:
     ``HipWeight``.  Up to 8 tokens run the decode GEMVs, more the prefill matmul
     (fp32 activations).  Nothing of a call is kept but the cache, workspaces
     included (torch's allocator serves them): calls of one layer may overlap on
-    several streams as far as their slots differ, and a call can be recorded into a
-    graph, with lengths, slots, positions and pages on the device."""
+    several streams as far as their slots differ (their blocks of 32, of a
+    block-scaled cache), and a call can be recorded into a graph, with lengths, slots,
+    positions and pages on the device."""
 
     def __init__(self, weights: dict, cache: PagedCache, heads: int, rope: Rotary | None,
                  q_norm: torch.Tensor | None = None, k_norm: torch.Tensor | None = None, eps: float = 1e-6,

@@ -71,6 +71,16 @@ def test_long_chunks(cuda, dim, dtype, kind):
     close(b.run(window=700, sink=33), want, bound, "under a window")
 
 
+@pytest.mark.parametrize("dim,dtype,kind", [(64, F16, I8), (64, BF16, E4M3), (256, F16, I8)])
+def test_many_sequences(cuda, dim, dtype, kind):
+    """More sequences than a line of lanes, and than are kept in LDS, with a prefix and without."""
+    for seqs, prefix in ((70, 40), (300, 33), (300, 0)):
+        b = BlockBatch(cuda, [1 + (s % 90 == 0) for s in range(seqs)], [2 + 7 * s % 95 for s in range(seqs)], prefix, 2, 1,
+                       dim, 32, dtype, kind, seed=seqs + prefix)
+        want, bound = b.want()
+        close(b.run(), want, bound, f"{seqs} sequences after {prefix}")
+
+
 @pytest.mark.parametrize("dtype,kind", KINDS)
 @pytest.mark.parametrize("shape", ["prefix", "chunk", "chunk_long"])
 def test_scales_far_apart(cuda, dtype, kind, shape):

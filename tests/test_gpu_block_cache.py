@@ -107,6 +107,25 @@ def test_append_wherever_the_tokens_go(cuda, kind, many, n):
     blk.same(c, want, many)
 
 
+@pytest.mark.parametrize("dtype,kind", [(F32, I8), (BF16, E4M3)])
+def test_append_of_unaligned_rows(cuda, dtype, kind):
+    """Rows at odd element offsets, heads first, and no token at all."""
+    from qwowl35_amd import attention as at
+
+    c = _blocks(cuda, 3, 2, 64, 128, kind)
+    want = blk.decode(c)
+    randn = _gen(cuda, 6)
+    slots = torch.arange(70) + 20
+    k, v = randn(70, 2, 129).to(dtype)[..., 1:], randn(2, 70, 131).to(dtype).transpose(0, 1)[..., 2:130]
+    at.kv_append(c, k, v, slots.to(cuda))
+    for state, x in zip(want, (k, v)):
+        blk.append(state, x.double().cpu(), slots, kind)
+    blk.same(c, want)
+    at.kv_append(c, k[:0], v[:0], slots[:0].to(cuda))
+    at.kv_append(c, k[:3], v[:3], torch.tensor([-1, 192, -7], device=cuda))
+    blk.same(c, want, "nothing to write")
+
+
 @pytest.mark.parametrize("kind", [I8, E4M3])
 @pytest.mark.parametrize("dim,rot,sections,normed", [(256, 64, [11, 11, 10], True), (64, 64, [], False), (128, 32, [], True)])
 def test_append_of_rotated_keys(cuda, kind, dim, rot, sections, normed):
