@@ -305,7 +305,8 @@ __device__ __forceinline__ void positions_of(const RopeArgs& r, int n_tokens, in
 }
 
 // What turn_of and norm_and_turn (rope_rows.h) compute, of a pair, and of rows with
-// the norm's weights and the angles at hand.
+// the norm's weights and the angles at hand.  An angle's bits past fp32's are added to
+// first order, since every error of a key is a chance of the code beside the right one.
 __device__ __forceinline__ void turn_pair(const RopeArgs& r, const int (&pos)[4], int pair, uint64_t freq, float (&to)[2]) {
     int p = pos[0];
     if (r.n_axes > 1) {
@@ -313,7 +314,11 @@ __device__ __forceinline__ void turn_pair(const RopeArgs& r, const int (&pos)[4]
         p = a == 0 ? pos[0] : a == 1 ? pos[1] : a == 2 ? pos[2] : pos[3];
     }
     const uint64_t turns = (uint64_t)(int64_t)p * freq;
-    sincospif((float)(int32_t)(turns >> 32) * 0x1p-31f, &to[1], &to[0]);
+    float sin, cos;
+    sincospif((float)((int32_t)(turns >> 32) & ~0x7f) * 0x1p-31f, &sin, &cos);  // (24 bits and a sign: exact)
+    const float rest = (float)(uint32_t)(turns >> 7) * (3.14159265f * 0x1p-56f);
+    to[0] = fmaf(-rest, sin, cos);
+    to[1] = fmaf(rest, cos, sin);
 }
 
 template <int D, int kRows>
