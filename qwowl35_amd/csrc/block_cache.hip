@@ -70,9 +70,22 @@ struct Codes<Fp8> {
     }
 };
 
-constexpr int kLeastGroups = 1024;  // workgroups that a launch is not cut below
-constexpr int kMostLooks = 128;     // places of a call whose blocks are looked for apart
 constexpr int kLeastExponent = -60;  // of a scale: its reciprocal and log2 stay far inside fp32
+
+// Workgroups that a launch is not cut below by giving each more heads: a workgroup
+// of several looks through the slots once for them and has the next head's rows on
+// their way, and needs others beside it.  8192 tokens x 8 heads x 128, bf16, took 27.5 us at
+// 256 workgroups, 27.4 at 512, 22.0 at 1024, 29.0 at 2048 and 41.8 at 4096.
+constexpr int kLeastGroups = 1024;
+// Places of a call, up to 32 tokens each, whose blocks are looked for apart: a
+// prompt has a block for every 32 tokens, a decode step one for each.  A prompt's
+// tokens / as many scattered ones, 4 heads x 256, us:
+//   places       64           128 (taken)   256           512
+//   128 tokens   7.4 / 12     10 / 10       10 / 10       10 / 10
+//   256          7.4 / 22     8.1 / 18      12 / 12       12 / 12
+//   512          7.8 / 39     8.4 / 32      10 / 24       21 / 19
+//   4096         18 / 286     18 / 285      17 / 164      21 / 127
+constexpr int kMostLooks = 128;
 
 // The least power of two s with m <= Q s.
 template <class C>
@@ -513,6 +526,13 @@ __device__ __forceinline__ void append_blocks(const BlockAppend& a, BlockShared<
 }
 
 // blockIdx.y: even keys, odd values of a group of heads.
+//   Bytes are the least of it: a call of few tokens is one chain of slots, rows, angles,
+// the largest, codes (8 tokens x 4 heads of 256, int8: 6.8 us, of 249: 9.7), and one of
+// many the chain of a head after the other (8192 x 8 heads of 128, bf16: 21.6 us, 50 MB
+// at 2.3 TB/s).  So a workgroup is a block, whose 32 rows of a head are all in
+// registers between the reading, the largest and the codes, each read and written
+// once; registers allow four of them a compute unit (three of 256 columns, without
+// spills).
 template <class TI, class C, int D, bool kFew>
 __global__ __launch_bounds__(256, D == 256 ? 3 : 4) void kv_append_blocks_kernel(BlockAppend a) {
     __shared__ BlockShared<D> sh;
@@ -606,7 +626,8 @@ __device__ __forceinline__ void store4(void* base, int64_t at, bool vec, const f
     }
 }
 
-// Bound by bytes.  Of keys a thread has eight columns (a granule of the cache) of
+// Bound by bytes (20011 tokens x 8 heads of 128, e4m3 to bf16: 23.1 us, 123 MB at
+// 5.3 TB/s, where a copy of 1 GiB has 5.1; a byte a load took 91).  Of keys a thread has eight columns (a granule of the cache) of
 // D / 64 tokens, a workgroup 32 tokens of a head, so that it uses whole lines of
 // the granules, which lie token by token.  Of values a thread has four columns of
 // eight tokens: where those are the eight of a granule it reads 32 bytes (64 of a

@@ -915,7 +915,7 @@ struct Shared {
 
 // The block scales of a wave's tiles, keys' and values': of the 32 fetched last and of the 32 before.  (int8 keeps them
 // in the place of `marks`, of which it needs none: 64 columns have room for two workgroups a compute unit up to 592
-// sequences then, and 400 with 64 tiles at a time beside them, over which 400 sequences of 400 tokens took 83 us for 67.)
+// sequences then, and 400 with 64 tiles at a time beside them, over which 400 sequences of 400 tokens took 83 us for 62.)
 typedef float scales_t[2][2][32];
 template <int D>
 struct SharedBlocks : Shared<D> {
@@ -1847,8 +1847,12 @@ __global__ __launch_bounds__(kThreads, D == 256 ? 1 : 2) void prefix_attention_k
     }
 }
 
-// The same of a block-scaled cache.  (A body of both, called from either, has its
-// registers allocated otherwise: the kernel above would no longer be the one measured.)
+// The same of a block-scaled cache: half the bytes of a 16-bit one.  They are what
+// bounds decode steps over long ones (5 sequences that share 100003 tokens, 4 heads of
+// 256, int8: 52 us at 4.1 TB/s, of which 8 are the beginning), and the one wave of a
+// SIMD, which unpacks besides, chunks (256 tokens x 16 heads of 256 over 16001: 125 us,
+// fp16 111).  (A body of both, called from either, has its registers allocated
+// otherwise: the kernel above would no longer be the one measured.)
 template <int D, class E, Kind C, bool kWide>
 __global__ __launch_bounds__(kThreads, D == 256 ? 1 : 2) void block_attention_kernel(AttnArgs a) {
     extern __shared__ __align__(16) uint8_t lds[];
