@@ -80,12 +80,13 @@ constexpr int kLeastGroups = 1024;
 // Places of a call, up to 32 tokens each, whose blocks are looked for apart: a
 // prompt has a block for every 32 tokens, a decode step one for each.  A prompt's
 // tokens / as many scattered ones, 4 heads x 256, us:
-//   places       64           128 (taken)   256           512
-//   128 tokens   7.4 / 12     10 / 10       10 / 10       10 / 10
-//   256          7.4 / 22     8.1 / 18      12 / 12       12 / 12
-//   512          7.8 / 39     8.4 / 32      10 / 24       21 / 19
-//   4096         18 / 286     18 / 285      17 / 164      21 / 127
-constexpr int kMostLooks = 128;
+//   places       16           32            64 (taken)    128
+//   128 tokens   7.5 / 9.3    7.6 / 7.1     7.6 / 7.4     11 / 11
+//   256          7.6 / 16     7.6 / 9.9     7.7 / 8.0     8.5 / 12
+//   512          7.9 / 29     7.8 / 17      8.2 / 12      8.8 / 13
+//   1024         8.2 / 32     8.2 / 32      8.2 / 20      9.1 / 21
+//   8192         30 / 134     30 / 134      30 / 133      30 / 134
+constexpr int kMostLooks = 64;
 
 // The least power of two s with m <= Q s.
 template <class C>
@@ -113,7 +114,7 @@ struct BlockShared {
     int src[4][32];     // of the block's tokens: which of the call it is (-1: none); a list, or a list a wave
     uint32_t top[2][4];  // the waves' largest magnitudes, of this head and the last
     float before[2];    // the scale before
-    int count[4];       // the waves' counts of a block's tokens
+    uint32_t count[4][2];  // the waves' counts of the tokens of a block, or of four by halves
     union {
         uint2 codes[32][D / 8 + 1];         // of values, on their way to eight tokens of a column
         alignas(16) float angles[32][D / 2 + 2][2];  // of keys: cosine and sine of each pair (the pad: rows apart in the banks)
@@ -230,6 +231,33 @@ __device__ __forceinline__ Found found(int* src, const Near& x, int64_t block) {
     return {src, (uint32_t)__ballot(src[lane & 31] >= 0), block};
 }
 
+// How many tokens of each of some blocks (as the halves of slots) the call has: this thread's share.
+template <int kBlocks>
+__device__ __forceinline__ void look(const BlockAppend& a, const uint32_t (&lo)[kBlocks], const uint32_t (&hi)[kBlocks],
+                                     int (&count)[kBlocks]) {
+    typedef uint32_t pair_t __attribute__((ext_vector_type(4), aligned(8)));
+    constexpr int kAhead = 4;  // loads on their way together
+#pragma unroll
+    for (int b = 0; b < kBlocks; ++b) count[b] = 0;
+    for (int j0 = a.t0 + 2 * (int)threadIdx.x; j0 < a.t1; j0 += 512 * kAhead) {
+        pair_t s[kAhead];
+#pragma unroll
+        for (int i = 0; i < kAhead; ++i) {
+            const int j = j0 + 512 * i;
+            s[i] = pair_t{~0u, ~0u, ~0u, ~0u};
+            if (j + 1 < a.t1) s[i] = *reinterpret_cast<const pair_t*>(a.slots + j);
+            else if (j < a.t1) s[i] = pair_t{(uint32_t)a.slots[j], (uint32_t)(a.slots[j] >> 32), ~0u, ~0u};
+        }
+#pragma unroll
+        for (int i = 0; i < kAhead; ++i)
+#pragma unroll
+            for (int b = 0; b < kBlocks; ++b) {
+                count[b] += ((s[i][0] ^ lo[b]) & ~31u | (s[i][1] ^ hi[b])) == 0;
+                count[b] += ((s[i][2] ^ lo[b]) & ~31u | (s[i][3] ^ hi[b])) == 0;
+            }
+    }
+}
+
 // The blocks that a workgroup writes: those of which one of its `per` tokens is
 // the call's first.  Each has one writer, in whatever order the tokens come (of two
 // with the same slot the last counts), so results do not depend on timing.
@@ -240,8 +268,13 @@ __device__ __forceinline__ Found found(int* src, const Near& x, int64_t block) {
 // a lane.  A block whose first token there is the workgroup's begins with those
 // (`start`), and all slots are looked through meanwhile; if there are more of the
 // block it gives way to an earlier one, or begins again with all of them.
-template <bool kFew, int D, class S, class W>
-__device__ __forceinline__ void each_block(const BlockAppend& a, BlockShared<D>& sh, S start, W write) {
+//   Several blocks of one token, as of a batch's decode step, are looked for and
+// written four at a time, a wave each (`start_one`, `write_one`): 512 sequences x 4
+// heads of 256 take 12 us, and 32 one after the other by the workgroup, prompts
+// 0.4 us more for it.
+template <bool kFew, int D, class S, class W, class S1, class W1>
+__device__ __forceinline__ void each_block(const BlockAppend& a, BlockShared<D>& sh, S start, W write, S1 start_one,
+                                           W1 write_one) {
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
     int* const src = sh.src[wave];
     if constexpr (kFew) {
@@ -259,6 +292,55 @@ __device__ __forceinline__ void each_block(const BlockAppend& a, BlockShared<D>&
     const Near below = near(a, base - 64 + lane), here = near(a, base + lane);
     const int64_t last = (int64_t)((uint64_t)(uint32_t)__shfl_up((int)(here.block >> 32), 1) << 32 | (uint32_t)__shfl_up((int)here.block, 1));
     uint32_t runs = (uint32_t)__ballot(lane < a.per && here.block >= 0 && (lane == 0 || here.block != last));
+    uint32_t ones = 0;
+    if (runs & (runs - 1))
+        for (uint32_t left = runs; left; left &= left - 1) {
+            const int l = __builtin_ctz(left);
+            const int64_t block = of_lane(here.block, l);
+            if (!__ballot(below.block == block) && __ballot(here.block == block) == 1ull << l) ones |= 1u << l;
+        }
+    if (ones & (ones - 1)) {
+        runs &= ~ones;
+        while (ones) {
+            const int w = __builtin_amdgcn_readfirstlane(wave);
+            int at[4], n[4], mine = -1;
+            uint32_t lo[4], hi[4];
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                at[i] = ones ? __builtin_ctz(ones) : -1;
+                ones &= ones - 1;
+                const int64_t block = at[i] >= 0 ? of_lane(here.block, at[i]) : -1;
+                lo[i] = (uint32_t)block << 5;
+                hi[i] = (uint32_t)(block >> 27);
+                if (i == w) mine = at[i];
+            }
+            const int64_t slot = mine >= 0 ? of_lane(here.slot, mine) : -1;
+            if (mine >= 0) start_one(base + mine, slot);
+            look<4>(a, lo, hi, n);
+            static_assert(kAppendSlice + 2048 < 1 << 16, "a count, and of no block negative slots and those past the end");
+            uint32_t halves[2] = {(uint32_t)(n[0] | n[1] << 16), (uint32_t)(n[2] | n[3] << 16)};
+#pragma unroll
+            for (int o = 1; o < 64; o *= 2) {
+                halves[0] += __shfl_xor(halves[0], o);
+                halves[1] += __shfl_xor(halves[1], o);
+            }
+            if (lane < 2) sh.count[wave][lane] = halves[lane];
+            __syncthreads();
+            uint32_t all[2] = {0, 0};
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                all[0] += sh.count[i][0];
+                all[1] += sh.count[i][1];
+            }
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                const bool one = (all[i / 2] >> i % 2 * 16 & 0xffff) == 1;
+                if (at[i] >= 0 && !one) runs |= 1u << at[i];  // others lie elsewhere in the call
+                if (i == w && one && mine >= 0) write_one(base + mine, slot);
+            }
+            __syncthreads();  // (the counts are read, and what the waves shared)
+        }
+    }
     while (runs) {
         const int l = __builtin_ctz(runs);
         runs &= runs - 1;
@@ -268,30 +350,14 @@ __device__ __forceinline__ void each_block(const BlockAppend& a, BlockShared<D>&
         Found f = found(src, here, block);
         start(f);
         // how many tokens of the block the call has
-        const uint32_t lo = (uint32_t)block << 5, hi = (uint32_t)(block >> 27);
-        int count = 0;
-        typedef uint32_t pair_t __attribute__((ext_vector_type(4), aligned(8)));
-        constexpr int kAhead = 4;  // loads on their way together
-        for (int j0 = a.t0 + 2 * tid; j0 < a.t1; j0 += 512 * kAhead) {
-            pair_t s[kAhead];
-#pragma unroll
-            for (int i = 0; i < kAhead; ++i) {
-                const int j = j0 + 512 * i;
-                s[i] = pair_t{~0u, ~0u, ~0u, ~0u};
-                if (j + 1 < a.t1) s[i] = *reinterpret_cast<const pair_t*>(a.slots + j);
-                else if (j < a.t1) s[i] = pair_t{(uint32_t)a.slots[j], (uint32_t)(a.slots[j] >> 32), ~0u, ~0u};
-            }
-#pragma unroll
-            for (int i = 0; i < kAhead; ++i) {
-                count += ((s[i][0] ^ lo) & ~31u | (s[i][1] ^ hi)) == 0;
-                count += ((s[i][2] ^ lo) & ~31u | (s[i][3] ^ hi)) == 0;
-            }
-        }
+        int counts[1];
+        look<1>(a, {(uint32_t)block << 5}, {(uint32_t)(block >> 27)}, counts);
+        int count = counts[0];
 #pragma unroll
         for (int o = 1; o < 64; o *= 2) count += __shfl_xor(count, o);
-        if (lane == 0) sh.count[wave] = count;
+        if (lane == 0) sh.count[wave][0] = (uint32_t)count;
         __syncthreads();
-        count = sh.count[0] + sh.count[1] + sh.count[2] + sh.count[3];
+        count = (int)(sh.count[0][0] + sh.count[1][0] + sh.count[2][0] + sh.count[3][0]);
         if (count != __popcll(from)) {  // some lie elsewhere in the call
             int* const all = sh.src[0];
             if (tid < 32) all[tid] = -1;
@@ -431,6 +497,84 @@ __device__ __forceinline__ void append_blocks(const BlockAppend& a, BlockShared<
         for (int r = 0; r < kRows; ++r) src[r] = f.src[row0 + r * kStep];
         load(h0);
     };
+    // The token of a block that the call has no other of, by a wave: as many heads at a time as its lanes have room for,
+    // eight columns a lane.
+    constexpr int kHeads = 64 / kLanes;
+    const int lane = tid & 63, wave = tid >> 6, group = lane / kLanes;
+    int64_t one_tile = 0;
+    float one[8], one_before = 0.0f;
+    auto load_one = [&](int token, int h) {
+        const bool in = h < h1;
+#pragma unroll
+        for (int j = 0; j < 8; ++j) one[j] = 0.0f;
+        if (in) load8<TI>(x_view.data, token * x_view.token_stride + h * x_view.head_stride + li * 8, x_view.vec, one);
+        one_before = in ? scales[one_tile + (int64_t)h * blocks] : 0.0f;
+    };
+    auto start_one = [&](int token, int64_t slot) {
+        const int64_t block = slot >> 5, page = block / blocks;
+        one_tile = page * heads * blocks + (block - page * blocks);
+        load_one(token, h0 + group);
+    };
+    auto write_one = [&](int token, int64_t slot) {
+        if (!kValues && a.rope.freq) {
+            int pos[4];
+            positions_of(a.rope, a.n_tokens, token, pos);
+            for (int p = lane; p < a.rope.rot_dim / 2; p += 64) turn_pair(a.rope, pos, p, a.rope.freq[p], sh.angles[wave][p]);
+            __builtin_amdgcn_wave_barrier();
+        }
+        const int row = (int)slot & 31;
+        for (int hb = h0; hb < h1; hb += kHeads) {
+            const int h = hb + group;
+            if (hb != h0) load_one(token, h);
+            float x[1][8];
+#pragma unroll
+            for (int j = 0; j < 8; ++j) x[0][j] = one[j];
+            if constexpr (!kValues) norm_and_turn_rows<D>(a.rope, li, wave, weight, sh, x);
+            uint32_t m = largest(x[0], 0);
+            for (int o = kLanes / 2; o; o >>= 1) m = dpp_max_u32(m, (uint32_t)__shfl_xor((int)m, o));
+            const bool finite = m < kInfinity;
+            if (__any(!finite)) {
+                uint32_t f = finite ? m : largest_finite(x[0], 0);
+                for (int o = kLanes / 2; o; o >>= 1) f = dpp_max_u32(f, (uint32_t)__shfl_xor((int)f, o));
+                m = f;
+            }
+            if (h >= h1) continue;
+            const int64_t tile = one_tile + (int64_t)h * blocks;
+            uint8_t* const codes = pages + tile * (32 * D);
+            const bool first = row == 0;
+            const Scale s = scale_of<C>(first ? 0.0f : one_before, first, __builtin_bit_cast(float, m));
+            const float inv = s.now > 0.0f ? 1.0f / s.now : 0.0f;
+            const bool rewrite = first || s.shrink != 1.0f;
+            const uint2 w = pack8<C>(x[0], inv, finite);
+            // the lane's columns of the block: of keys a granule a token, of values a granule a column and eight tokens
+            if (rewrite) {
+                uint4_t* const at = reinterpret_cast<uint4_t*>(codes + li * (kValues ? 64 : 256));
+                constexpr int kStep = kValues ? D / 2 : 4;  // (of values from one octet to the next, in four)
+                for (int i = 0; i < 4; ++i) {
+                    uint4_t* const to = at + i * (kValues ? kStep : 4);
+                    uint4_t old[4] = {};
+                    if (s.shrink > 0.0f) {
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) old[e] = to[e];
+                    }
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) {
+#pragma unroll
+                        for (int c = 0; c < 4; ++c) old[e][c] = again<C>(old[e][c], s.shrink);
+                        to[e] = old[e];
+                    }
+                }
+            }
+            if constexpr (!kValues) {
+                *reinterpret_cast<uint2*>(codes + li * 256 + row * 8) = w;
+            } else {
+                uint8_t* const to = codes + row / 8 * (8 * D) + li * 64 + row % 8;
+#pragma unroll
+                for (int j = 0; j < 8; ++j) to[j * 8] = (uint8_t)((j < 4 ? w.x : w.y) >> j % 4 * 8);
+            }
+            if (li == 0 && s.changed) scales[tile] = s.now;
+        }
+    };
     each_block<kFew, D>(a, sh, start, [&](const Found& f) {
         if constexpr (!kValues) {
             // the block's angles, by eight threads a token, four of each on their way together (by the lanes that take
@@ -522,7 +666,7 @@ __device__ __forceinline__ void append_blocks(const BlockAppend& a, BlockShared<
             }
             if (tid == 0 && s.changed) scales[tile] = s.now;
         }
-    });
+    }, start_one, write_one);
 }
 
 // blockIdx.y: even keys, odd values of a group of heads.

@@ -107,6 +107,73 @@ def test_append_wherever_the_tokens_go(cuda, kind, many, n):
     blk.same(c, want, many)
 
 
+def _steps(n, step):
+    """Slots of a step of n sequences, a page of 64 each, at different places; some without a token, some with two."""
+    i = torch.arange(n)
+    slots = i * 64 + (i * 7) % 31 + step
+    slots[i % 23 == 5] = -1
+    slots[n - 1] = slots[3] + (-1 if slots[3] % 32 else 1)   # block 3's other token, behind all
+    slots[n // 2] = slots[10]                                # the last of two counts
+    return slots
+
+
+@pytest.mark.parametrize("n,dim,heads,dtype,kind", [
+    (65, 256, 4, F32, I8), (129, 64, 3, BF16, E4M3), (200, 128, 5, F16, I8), (260, 256, 3, F32, E4M3),
+    (400, 256, 1, BF16, I8), (513, 64, 9, F32, I8), (600, 128, 2, F32, E4M3), (1100, 256, 1, F16, E4M3),
+])
+def test_append_of_a_step_of_many_sequences(cuda, n, dim, heads, dtype, kind):
+    """Blocks that get one token: growing, beginning anew, with infinities and NaN, unaligned rows."""
+    from qwowl35_amd import attention as at
+
+    c = _blocks(cuda, n + 1, heads, 64, dim, kind)
+    want = blk.decode(c)
+    randn = _gen(cuda, n)
+    for step in range(3):
+        slots = _steps(n, step)
+        k = (randn(n, heads, dim + 1) * 6.0 ** step).to(dtype)[..., 1:]
+        v = (randn(heads, n, dim) * 4.0 ** step).to(dtype).transpose(0, 1)
+        k[20, 0, 3], k[21, heads - 1, 0], v[22, 0, dim - 1], v[24] = math.inf, math.nan, -math.inf, 0.0
+        at.kv_append(c, k, v, slots.to(cuda))
+        for state, x in zip(want, (k, v)):
+            blk.append(state, x.double().cpu(), slots, kind)
+        blk.same(c, want, f"step {step}")
+
+
+@pytest.mark.parametrize("kind", [I8, E4M3])
+@pytest.mark.parametrize("dim,rot,sections,normed", [(256, 64, [11, 11, 10], True), (64, 64, [], False), (128, 128, [], True)])
+def test_a_step_of_many_is_what_steps_of_few_make(cuda, kind, dim, rot, sections, normed):
+    """The keys' rotation and norm, bit for bit, whichever way the step is cut into calls; and in a graph."""
+    from qwowl35_amd import attention as at
+
+    n, heads = 333, 3
+    randn = _gen(cuda, dim)
+    k, v = randn(n, heads, dim), randn(n, heads, dim)
+    norm = randn(dim).abs() + 0.5 if normed else None
+    rope = at.Rotary(rot, 1e7, sections, True, device=cuda)
+    pos = torch.randint(0, 100000, (rope.axes, n), device=cuda, dtype=torch.int32)
+    pos = pos if rope.axes > 1 else pos[0]
+    i = torch.arange(n, device=cuda)
+    slots = i * 32 + (i * 5) % 32
+    few, many, graphed = (_blocks(cuda, n, heads, 32, dim, kind) for _ in range(3))
+    for a in range(0, n, 37):
+        at.kv_append(few, k[a:a + 37], v[a:a + 37], slots[a:a + 37], rope=rope,
+                     positions=pos[..., a:a + 37].contiguous(), norm=norm)
+    at.kv_append(many, k, v, slots, rope=rope, positions=pos, norm=norm)
+    start = [x.clone() for x in (graphed.k.view(torch.uint8), graphed.v.view(torch.uint8), graphed.k_scale, graphed.v_scale)]
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        at.kv_append(graphed, k, v, slots, rope=rope, positions=pos, norm=norm)
+    for _ in range(3):
+        for x, was in zip((graphed.k.view(torch.uint8), graphed.v.view(torch.uint8), graphed.k_scale, graphed.v_scale), start):
+            x.copy_(was)
+        g.replay()
+        torch.cuda.synchronize()
+        for c in (many, graphed):
+            for x, y in ((c.k, few.k), (c.v, few.v)):
+                assert torch.equal(x.view(torch.uint8), y.view(torch.uint8))
+            assert torch.equal(c.k_scale, few.k_scale) and torch.equal(c.v_scale, few.v_scale)
+
+
 @pytest.mark.parametrize("dtype,kind", [(F32, I8), (BF16, E4M3)])
 def test_append_of_unaligned_rows(cuda, dtype, kind):
     """Rows at odd element offsets, heads first, and no token at all."""
