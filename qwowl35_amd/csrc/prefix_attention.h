@@ -873,9 +873,9 @@ __device__ __forceinline__ void copy_kb(const uint8_t* from, uint8_t* to, int la
         for (int i = 0; i < kCount; i += 4) {
             const uint8_t* const g = from + i * 1024 + lane * 16;
             copy_apart<0>(g, to + i * 1024);
-            if (i + 1 < kCount) copy_apart<1024>(g, to + i * 1024);
-            if (i + 2 < kCount) copy_apart<2048>(g, to + i * 1024);
-            if (i + 3 < kCount) copy_apart<3072>(g, to + i * 1024);
+            if (i + 1 < kCount) copy_apart<1 * 1024>(g, to + i * 1024);
+            if (i + 2 < kCount) copy_apart<2 * 1024>(g, to + i * 1024);
+            if (i + 3 < kCount) copy_apart<3 * 1024>(g, to + i * 1024);
         }
         return;
     }
