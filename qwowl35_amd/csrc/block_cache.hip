@@ -671,8 +671,8 @@ __device__ __forceinline__ void append_blocks(const BlockAppend& a, BlockShared<
 
 // blockIdx.y: even keys, odd values of a group of heads.
 //   Bytes are the least of it: a call of few tokens is one chain of slots, rows, angles,
-// the largest, codes (8 tokens x 4 heads of 256, int8: 6.8 us, of 249: 9.7), and one of
-// many the chain of a head after the other (8192 x 8 heads of 128, bf16: 21.6 us, 50 MB
+// the largest, codes (8 tokens x 4 heads of 256, int8: 6.8 us, of 249: 9.5), and one of
+// many the chain of a head after the other (8192 x 8 heads of 128, bf16: 21.7 us, 50 MB
 // at 2.3 TB/s).  So a workgroup is a block, whose 32 rows of a head are all in
 // registers between the reading, the largest and the codes, each read and written
 // once; registers allow four of them a compute unit (three of 256 columns, without
