@@ -986,20 +986,24 @@ struct Unit {
         __device__ __forceinline__ void operator()(int) const {}
     };
 
-    // A block-scaled tile: with keys s^k c and values s^v c a term is 2^(scale s^k q.c - m) s^v c.  The values'
-    // scale goes into the exponent, u = scale s^k q.c + log2 s^v, and the reference m follows the largest u: the
-    // product's weights 2^(u - m) take what a row's values weigh, whatever the scales, and the sum of the
-    // softmax' terms gets the tile's back at once, by 2^-log2 s^v.  Four instructions a tile and none an element.
+    // A block-scaled tile: with z = scale s^k q.c and values s^v c the product needs 2^z s^v c, the softmax' sum
+    // 2^z.  The values' scale goes into the exponent, u = z + log2 s^v, and the reference m follows the largest u: the
+    // product's weights 2^(u - m) take what a row's values weigh.  The sum counts from a reference of its own, ml, which
+    // follows the largest z: a tile's weights come to it times 2^(m - log2 s^v - ml).  A tile whose values are zero has
+    // none, and must not raise m (one that did, by its scores alone, left the others' weights to fp16's subnormals and
+    // below): its terms are 2^(z - ml).  A dozen instructions a tile and none an element.
     struct Blocks {
-        float key, lift, unlift;  // scale s^k, log2 s^v, 2^-log2 s^v
-        float sum;                // of the tile's weights
-        uint32_t keep;            // all ones; zero where the values are, by a scale of zero
+        float key, lift;   // scale s^k, log2 s^v (minus infinity: values of zero)
+        float bias, back;  // of the exponents; what the sum of the terms is worth beside the others
+        float sum;         // of the tile's terms
+        uint32_t keep;     // all ones; zero where the values are
     };
     // What a wave carries through its tiles.
     struct Rows {
         vec8 q[kM];
         acc o[kT];
         float mx, l;
+        float ml;  // (block scales: what l counts from)
         Limits lim;
         int all_lo, all_hi, all_sink;  // what every row of the wave sees
         float scale;
@@ -1007,7 +1011,7 @@ struct Unit {
         std::conditional_t<kBlocks, Blocks, Nothing> tile;
     };
 
-    // Of tile i, whose scales came with its copies; `last` is the tile before.
+    // Of tile i, whose scales came with its copies.
     struct Scales {
         float k, v;
     };
@@ -1020,30 +1024,30 @@ struct Unit {
         const float(&from)[2][32] = scales()[i >> 5 & 1];
         return {from[0][i & 31], from[1][i & 31]};
     }
-    static __device__ __forceinline__ Blocks blocks_of(const Rows& w, Scales s, const Blocks& last) {
-        Blocks b;
+    static __device__ __forceinline__ Blocks blocks_of(const Rows& w, Scales s) {
+        Blocks b = {};
         // (zero: every finite score alike; a missing tile's may be anything, and its scores are masked)
         b.key = fminf(fmaxf(w.scale * s.k, 2e-38f), 3e38f);
         const bool some = s.v > 0.0f && s.v < __builtin_inff();
         const float lift = __builtin_amdgcn_logf(s.v);
-        b.lift = some ? lift : last.lift;
-        b.unlift = __builtin_amdgcn_exp2f(-b.lift);
-        b.keep = some ? ~0u : 0u;
-        b.sum = 0.0f;
+        b.lift = some ? lift : -__builtin_inff();
         return b;
     }
     __device__ __forceinline__ void scale_tile(Rows& w, int i) const {
-        if constexpr (kBlocks) w.tile = blocks_of(w, scales_of(i), w.tile);
+        if constexpr (kBlocks) w.tile = blocks_of(w, scales_of(i));
     }
-    // What a score is as an exponent.
-    static __device__ __forceinline__ float exponent(const Rows& w, float s) {
-        if constexpr (kBlocks) return fmaf(s, w.tile.key, w.tile.lift);
-        else return s * w.scale;
+    // Before a tile's terms, after the references followed its scores.
+    __device__ __forceinline__ void begin_terms(Rows& w) const {
+        const float m = w.mx == -__builtin_inff() ? 0.0f : w.mx, ml = w.ml == -__builtin_inff() ? 0.0f : w.ml;
+        const bool none = w.tile.lift == -__builtin_inff();
+        w.tile.bias = none ? -ml : w.tile.lift - m;
+        w.tile.back = none ? 1.0f : __builtin_amdgcn_exp2f(m - w.tile.lift - ml);
+        w.tile.keep = none ? 0u : ~0u;
     }
-    // After a tile's terms: their sum, and weights of values that are zero.
+    // After them: their sum, and no weights of values that are zero.
     __device__ __forceinline__ void end_terms(Rows& w, vec8 (&p)[kK]) const {
         if constexpr (kBlocks) {
-            w.l = fmaf(w.tile.sum, w.tile.unlift, w.l);
+            w.l = fmaf(w.tile.sum, w.tile.back, w.l);
             w.tile.sum = 0.0f;
 #pragma unroll
             for (int k = 0; k < kK; ++k) {
@@ -1118,8 +1122,23 @@ struct Unit {
 
     // The reference follows the rows' largest scores (`largest`: of this lane's).
     __device__ __forceinline__ void follow(Rows& w, float largest) const {
-        if (__builtin_expect(__any(exponent(w, largest) > w.mx + kRise), 0)) {
-            const float m_new = fmaxf(w.mx, exponent(w, row_max<kRows>(largest)) - kLift);
+        if constexpr (kBlocks) {
+            const float z = largest * w.tile.key;
+            if (__builtin_expect(__any(z + w.tile.lift > w.mx + kRise || z > w.ml + kRise), 0)) {
+                const float top = row_max<kRows>(largest) * w.tile.key;
+                const float m_new = fmaxf(w.mx, top + w.tile.lift - kLift), ml_new = fmaxf(w.ml, top);
+                const float shrink = m_new == w.mx ? 1.0f : __builtin_amdgcn_exp2f(w.mx - m_new);
+                w.l *= ml_new == w.ml ? 1.0f : __builtin_amdgcn_exp2f(w.ml - ml_new);
+#pragma unroll
+                for (int t = 0; t < kT; ++t) scale_in_place<kAgpr>(w.o[t], shrink);
+                w.mx = m_new;
+                w.ml = ml_new;
+            }
+            begin_terms(w);
+            return;
+        }
+        if (__builtin_expect(__any(largest * w.scale > w.mx + kRise), 0)) {
+            const float m_new = fmaxf(w.mx, row_max<kRows>(largest) * w.scale - kLift);
             const float shrink = m_new == w.mx ? 1.0f : __builtin_amdgcn_exp2f(w.mx - m_new);
             w.l *= shrink;
 #pragma unroll
@@ -1134,12 +1153,12 @@ struct Unit {
 #pragma unroll
         for (int i = j0; i < j1; ++i) {
             const int j = i;
-            const float ref = w.mx == -__builtin_inff() ? 0.0f : w.mx;
             float e;
             if constexpr (kBlocks) {
-                e = __builtin_amdgcn_exp2f(fmaf(s[j / kAcc][j % kAcc], w.tile.key, w.tile.lift - ref));
+                e = __builtin_amdgcn_exp2f(fmaf(s[j / kAcc][j % kAcc], w.tile.key, w.tile.bias));
                 w.tile.sum += e;
             } else {
+                const float ref = w.mx == -__builtin_inff() ? 0.0f : w.mx;
                 e = __builtin_amdgcn_exp2f(fmaf(s[j / kAcc][j % kAcc], w.scale, -ref));
                 w.l += e;
             }
@@ -1281,6 +1300,24 @@ struct Unit {
                 }
                 __builtin_amdgcn_sched_barrier(0);
             }
+    }
+
+    // Both sums count from one reference: the values', or, where that is over 2^90 from the terms' (values of zero
+    // or far from one), one between them, so that neither leaves fp32's range.
+    __device__ __forceinline__ void one_reference(Rows& w) const {
+        const bool none = w.mx == -__builtin_inff();  // (nothing but zeros)
+        float ref = w.mx;
+        if (!(fabsf(w.mx - w.ml) <= 90.0f)) ref = none ? w.ml : fmaxf(0.5f * (w.mx + w.ml), w.ml - 90.0f);
+        if (__builtin_expect(__any(ref != w.mx), 0)) {
+            const float f = none || ref == w.mx ? 1.0f : __builtin_amdgcn_exp2f(w.mx - ref);
+#pragma unroll
+            for (int t = 0; t < kT; ++t) {
+                w.o[t] *= f;
+                __builtin_amdgcn_sched_barrier(0);
+            }
+        }
+        w.l *= ref == w.ml ? 1.0f : __builtin_amdgcn_exp2f(w.ml - ref);
+        w.mx = ref;
     }
 
     __device__ __forceinline__ bool partly(const Rows& w, int t0, bool there) const {
@@ -1494,7 +1531,7 @@ struct Unit {
                 Blocks after;
                 wide.add_values_from(first, values(i), w, p, [&](int m) {
                     unpack(more_values, values(i + 1), m);
-                    if (m == 1) after = blocks_of(w, coming, w.tile);
+                    if (m == 1) after = blocks_of(w, coming);
 #pragma unroll
                     for (int j = kScores * m / kValueSteps; j < kScores * (m + 1) / kValueSteps; ++j) {
                         top = fmaxf(top, next[j / kAcc][j % kAcc]);
@@ -1611,6 +1648,7 @@ struct Unit {
         }
         if (__builtin_expect(w.marked, 0)) add_infinities(w, marks);
         w.l = row_sum<kRows>(w.l);
+        if constexpr (kBlocks) one_reference(w);
 
         const float v_scale = F8 && !kBlocks && a.v_scale ? a.v_scale[h] : 1.0f;
         static_assert(kRows * D * 4 <= kRing / kWaves, "a wave's sums of a row tile fit its part of the ring");
@@ -1796,7 +1834,10 @@ struct Unit {
         }
         w.mx = -__builtin_inff();
         w.l = 0.0f;
-        if constexpr (kBlocks) w.tile = Blocks{0.0f, 0.0f, 1.0f, 0.0f, ~0u};
+        if constexpr (kBlocks) {
+            w.ml = -__builtin_inff();
+            w.tile = Blocks{};
+        }
 #pragma unroll
         for (int t2 = 0; t2 < kT; ++t2) w.o[t2] = acc{};
         w.all_lo = lane_max(w.all_lo, 0);
