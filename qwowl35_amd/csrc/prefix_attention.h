@@ -836,6 +836,14 @@ __device__ __forceinline__ float part_weight(float m, float top) {
     // (never zero otherwise: an infinity in a part that hardly counts stays one)
     return m == -__builtin_inff() ? 0.0f : fmaxf(__builtin_amdgcn_exp2f(m - top), 1e-37f);
 }
+// The weight of such a part's sum of terms, which with block scales may be up to 2^118 and count for something where
+// the part's values hardly do: the smaller exponential's rest goes to the sum, and nothing is put in the place of zero.
+__device__ __forceinline__ float sum_weight(float m, float top, float& sum) {
+    const float x = m - top;
+    const bool far = x < -100.0f;
+    if (far) sum *= 0x1p-100f;
+    return m == -__builtin_inff() ? 0.0f : __builtin_amdgcn_exp2f(far ? x + 100.0f : x);
+}
 
 // Waits until at most n of this wave's vector memory operations are in flight.
 template <int N>
@@ -991,12 +999,15 @@ struct Unit {
     // product's weights 2^(u - m) take what a row's values weigh.  The sum counts from a reference of its own, ml, which
     // follows the largest z: a tile's weights come to it times 2^(m - log2 s^v - ml).  A tile whose values are zero has
     // none, and must not raise m (one that did, by its scores alone, left the others' weights to fp16's subnormals and
-    // below): its terms are 2^(z - ml).  A dozen instructions a tile and none an element.
+    // below).  One whose weights are all under 2^-kFar has none that fp16 holds, or bf16 beside the largest of the
+    // tile, but may have the sum's largest terms, if its scale is far below another's (2^-60 and 2^122 may meet).
+    // There the terms are 2^(z - ml).  A dozen instructions a tile and none an element.
+    static constexpr float kFar = std::is_same_v<E, Half> ? 60.0f : 100.0f;  // (terms of a tile: 2^-26 of its largest are held)
     struct Blocks {
         float key, lift;   // scale s^k, log2 s^v (minus infinity: values of zero)
         float bias, back;  // of the exponents; what the sum of the terms is worth beside the others
         float sum;         // of the tile's terms
-        uint32_t keep;     // all ones; zero where the values are
+        uint32_t keep;     // all ones; zero where no weight is kept
     };
     // What a wave carries through its tiles.
     struct Rows {
@@ -1036,15 +1047,15 @@ struct Unit {
     __device__ __forceinline__ void scale_tile(Rows& w, int i) const {
         if constexpr (kBlocks) w.tile = blocks_of(w, scales_of(i));
     }
-    // Before a tile's terms, after the references followed its scores.
-    __device__ __forceinline__ void begin_terms(Rows& w) const {
-        const float m = w.mx == -__builtin_inff() ? 0.0f : w.mx, ml = w.ml == -__builtin_inff() ? 0.0f : w.ml;
-        const bool none = w.tile.lift == -__builtin_inff();
-        w.tile.bias = none ? -ml : w.tile.lift - m;
-        w.tile.back = none ? 1.0f : __builtin_amdgcn_exp2f(m - w.tile.lift - ml);
-        w.tile.keep = none ? 0u : ~0u;
+    // Before a tile's terms, after the references followed its scores; z: the largest of this lane's, scaled.
+    __device__ __forceinline__ void begin_terms(Rows& w, float z) const {
+        const bool far = !(z + w.tile.lift > w.mx - kFar);  // (as long as m is minus infinity too)
+        const float ml = w.ml == -__builtin_inff() ? 0.0f : w.ml;
+        w.tile.bias = far ? -ml : w.tile.lift - w.mx;
+        w.tile.back = far ? 1.0f : __builtin_amdgcn_exp2f(w.mx - w.tile.lift - ml);
+        w.tile.keep = far ? 0u : ~0u;
     }
-    // After them: their sum, and no weights of values that are zero.
+    // After them: their sum, and no weights where none are kept.
     __device__ __forceinline__ void end_terms(Rows& w, vec8 (&p)[kK]) const {
         if constexpr (kBlocks) {
             w.l = fmaf(w.tile.sum, w.tile.back, w.l);
@@ -1134,7 +1145,7 @@ struct Unit {
                 w.mx = m_new;
                 w.ml = ml_new;
             }
-            begin_terms(w);
+            begin_terms(w, z);
             return;
         }
         if (__builtin_expect(__any(largest * w.scale > w.mx + kRise), 0)) {
@@ -1302,14 +1313,12 @@ struct Unit {
             }
     }
 
-    // Both sums count from one reference: the values', or, where that is over 2^90 from the terms' (values of zero
-    // or far from one), one between them, so that neither leaves fp32's range.
+    // Both sums count from one reference: the values', or 2^90 from the terms' where it is further from those (values
+    // of zero, or far from one), so that neither leaves fp32's range.
     __device__ __forceinline__ void one_reference(Rows& w) const {
-        const bool none = w.mx == -__builtin_inff();  // (nothing but zeros)
-        float ref = w.mx;
-        if (!(fabsf(w.mx - w.ml) <= 90.0f)) ref = none ? w.ml : fmaxf(0.5f * (w.mx + w.ml), w.ml - 90.0f);
+        const float ref = fminf(fmaxf(w.mx, w.ml - 90.0f), w.ml + 90.0f);
         if (__builtin_expect(__any(ref != w.mx), 0)) {
-            const float f = none || ref == w.mx ? 1.0f : __builtin_amdgcn_exp2f(w.mx - ref);
+            const float f = ref == w.mx ? 1.0f : __builtin_amdgcn_exp2f(w.mx - ref);
 #pragma unroll
             for (int t = 0; t < kT; ++t) {
                 w.o[t] *= f;
@@ -1734,8 +1743,10 @@ struct Unit {
         }
 #pragma unroll
         for (int v = 0; v < kStep; ++v) {
+            float l = sh.l[rg + v * kRg][n];
+            const float of_sum = sum_weight(weight[v], top, l);
             weight[v] = part_weight(weight[v], top);
-            sum += weight[v] * sh.l[rg + v * kRg][n];
+            sum += of_sum * l;
         }
         const int row = row0 + n;
         if (row >= row_end) return;

@@ -142,13 +142,13 @@ __global__ __launch_bounds__(256) void prefix_attention_join(AttnArgs a, int wav
         vec_t v[kBatch];
         load(0, v);  // (on their way while the weights are made)
         const float now = fmaxf(top, over_lanes(pm, [](float x, float y) { return fmaxf(x, y); }));
-        const float shrink = attn::part_weight(top, now);
+        const float shrink = attn::part_weight(top, now), sum_shrink = attn::sum_weight(top, now, sum);
         top = now;
-        sum *= shrink;
+        sum *= sum_shrink;
 #pragma unroll
         for (int j = 0; j < N; ++j) acc[j] *= shrink;
-        const float weight = attn::part_weight(pm, now);
-        sum += weight * pl;
+        const float weight = attn::part_weight(pm, now), of_sum = attn::sum_weight(pm, now, pl);
+        sum += of_sum * pl;
         for (int i = 0; i < count; i += kBatch) {
             if (i) load(i, v);
 #pragma unroll
@@ -176,8 +176,9 @@ __global__ __launch_bounds__(256) void prefix_attention_join(AttnArgs a, int wav
         for (int c = 0; c < N; ++c) acc[c] = 0.0f;
 #pragma unroll
         for (int w = 0; w < 4; ++w) {
-            const float weight = attn::part_weight(sh_m[w], all);
-            sum += weight * sh_l[w];
+            float l = sh_l[w];
+            const float weight = attn::part_weight(sh_m[w], all), of_sum = attn::sum_weight(sh_m[w], all, l);
+            sum += of_sum * l;
 #pragma unroll
             for (int c = 0; c < N; ++c) acc[c] += weight * sh_o[w][lane * N + c];
         }

@@ -24,7 +24,12 @@ PATHS = [(64, "many"), (64, "shared"), (128, "prefix"), (128, "chunk_long"), (12
 
 def _batch(cuda, shape, dim, dtype, kind, seed, **kw):
     new, lens, prefix, heads, kv_heads, page = (SHAPES | LONG)[shape]
-    return BlockBatch(cuda, new, lens, prefix, heads, kv_heads, dim, page, dtype, kind, seed=seed, **kw)
+    b = BlockBatch(cuda, new, lens, prefix, heads, kv_heads, dim, page, dtype, kind, seed=seed, **kw)
+    if kind == E4M3:  # (no code past 448, which is NaN: rows that are numbers)
+        for codes, scale in ((b.cache.k, b.cache.k_scale), (b.cache.v, b.cache.v_scale)):
+            held = ~scale.isnan()[..., None].expand(-1, -1, -1, codes[0, 0].numel() // scale.shape[2]).reshape(codes.shape)
+            codes.copy_(codes.float().masked_fill_(codes.isnan() & held, 416.0))
+    return b
 
 
 def _order(b):
@@ -53,3 +58,55 @@ def test_blocks_of_zero_values_beside_small_ones(cuda, dtype, kind, dim, shape, 
         b.cache.k_scale[page[zero], :, at[zero]] *= 2.0
     want, bound = b.want()
     close(b.run(out_dtype=F32), want, bound, f"{shape}, the others 2^-{less}")
+
+
+APART = {  # log2 of the values' scale of block i of n of a sequence, and how much higher its logits' spread is
+    "any": lambda i, n, g: (torch.randint(-60, 113, (n,), generator=g), torch.ones(n)),
+    "ends": lambda i, n, g: (torch.where(torch.rand(n, generator=g) < 0.5, -60, 112), torch.ones(n)),
+    "small_first": lambda i, n, g: (torch.where(i <= n // 2, -60, 112), torch.ones(n)),
+    "large_first": lambda i, n, g: (torch.where(i <= n // 2, 112, -60), torch.ones(n)),
+    # small values at the softmax' large terms, so that either decides about a part of the result
+    "small_louder": lambda i, n, g: ((e := torch.randint(-60, 113, (n,), generator=g)), torch.where(e < 20, 16.0, 1.0)),
+    "zeros_too": lambda i, n, g: (torch.where(torch.rand(n, generator=g) < 0.3, -1000,
+                                              torch.randint(-60, 113, (n,), generator=g)), torch.ones(n)),
+}
+
+
+def _wider(bound):
+    """want()'s bound for scales so far apart.
+
+    Six sums of exponents below 2^8 and the logarithm of a scale below 2^7 within two steps: 2^-14 of a row's sum of
+    magnitudes, of which the bound has 2^-11 and more.
+
+    And beside a row's largest value what fp32 does not hold (a column may have nothing else: codes of zero).  bf16
+    weights under 2^-100 of the largest are dropped, and a part of a row counts 2^-123 at least, with sums of up to 2^33
+    (the reference 90 from the terms', scales up to 2^123) 2^8 (a rise it does not follow) 4 (the largest code to a
+    token's largest) 2^13 tokens: 2^-67 of the largest.  The bound has 2^-8 of that in the column that holds it."""
+    return bound * (1 + 2.0 ** -3) + bound.nan_to_num(0.0).amax(-1, keepdim=True) * 2.0 ** -59
+
+
+@pytest.mark.parametrize("dtype,kind", KINDS)
+@pytest.mark.parametrize("dim,shape", PATHS)
+@pytest.mark.parametrize("apart", APART)
+def test_scales_from_one_end_of_the_range_to_the_other(cuda, dtype, kind, dim, shape, apart):
+    """A block of small values counts in the softmax' sum whatever the values beside it weigh."""
+    b = _batch(cuda, shape, dim, dtype, kind, seed=len(apart), spread=(-5, -4))
+    g = torch.Generator().manual_seed(dim)
+    for page, at in _order(b):
+        e, louder = APART[apart](torch.arange(len(page)), len(page), g)
+        b.cache.v_scale[page, :, at] = torch.exp2(e.float()).to(cuda)[:, None].expand(-1, b.cache.kv_heads)
+        b.cache.k_scale[page, :, at] *= louder.to(cuda)[:, None]
+    want, bound = b.want()
+    close(b.run(out_dtype=F32), want, _wider(bound), f"{shape}, {apart}")
+
+
+@pytest.mark.parametrize("dtype,kind", KINDS)
+def test_a_prefix_and_own_tokens_at_either_end(cuda, dtype, kind):
+    """Parts of a row whose references are far apart: what hardly counts in the values does in the sum."""
+    for less, more in ((-60, 112), (112, -60), (-60, -1000), (-1000, 112)):
+        for shape in ("prefix", "rows_60", "pieces"):
+            b = _batch(cuda, shape, 128, dtype, kind, seed=more + 1100, spread=(-5, -4))
+            for i, (page, at) in enumerate(_order(b)):
+                b.cache.v_scale[page, :, at] = 2.0 ** (more if i else less)
+            want, bound = b.want()
+            close(b.run(out_dtype=F32), want, _wider(bound), f"{shape}, 2^{less} before 2^{more}")
