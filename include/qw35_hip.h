@@ -630,7 +630,8 @@ typedef struct qw35_hip_kv_cache {
  * call's are stored as their multiples of s, rounded to nearest even.  A block
  * begins anew when a call writes its first token, or when its scale is zero: its
  * scale is then the least power of two with m <= Q s (2^-60 at least; zero if m is),
- * and its other tokens are zero.  Infinities become the largest code, NaN zero in
+ * and its other tokens are zero.  Infinities become the largest code (zero in a
+ * block whose scale is zero, for want of a number that gives it one), NaN zero in
  * I8_BLOCKS and NaN in E4M3_BLOCKS.  Of tokens with one slot the last counts; more
  * than 16384 tokens are written as calls of 16384 would. */
 int qw35_hip_kv_append(const qw35_hip_kv_cache *cache, const qw35_hip_heads *k, const qw35_hip_heads *v,

@@ -161,7 +161,7 @@ __device__ __forceinline__ uint32_t largest(const float (&x)[8], uint32_t m) {
 }
 
 // For a block with infinities or NaN: the largest of eight numbers that are finite; infinities become fp32's
-// largest number, and so the largest code.
+// largest number, and so the largest code (and zero under a scale of zero, which a block without a number but zeros has).
 __device__ __forceinline__ uint32_t largest_finite(float (&x)[8], uint32_t m) {
 #pragma unroll
     for (int j = 0; j < 8; ++j) {
