@@ -110,3 +110,14 @@ def test_a_prefix_and_own_tokens_at_either_end(cuda, dtype, kind):
                 b.cache.v_scale[page, :, at] = 2.0 ** (more if i else less)
             want, bound = b.want()
             close(b.run(out_dtype=F32), want, _wider(bound), f"{shape}, 2^{less} before 2^{more}")
+
+
+@pytest.mark.parametrize("dtype,kind", KINDS)
+@pytest.mark.parametrize("dim,shape", [(64, "prefix"), (128, "chunk_long"), (256, "shared"), (256, "rows_60")])
+def test_a_softmax_scale_of_zero(cuda, dtype, kind, dim, shape):
+    """Every token that a row sees weighs the same, whatever the queries and the keys' scales."""
+    b = _batch(cuda, shape, dim, dtype, kind, seed=dim, spread=(-9, -1), q_spread=3.0)
+    want, bound = b.want(scale=0.0)
+    other, _ = b.want()
+    assert (want - other).abs().max() > 100 * bound.max()  # (another scale would be noticed)
+    close(b.run(scale=0.0, out_dtype=F32), want, bound, shape)
