@@ -121,3 +121,19 @@ def test_a_softmax_scale_of_zero(cuda, dtype, kind, dim, shape):
     other, _ = b.want()
     assert (want - other).abs().max() > 100 * bound.max()  # (another scale would be noticed)
     close(b.run(scale=0.0, out_dtype=F32), want, bound, shape)
+
+
+@pytest.mark.parametrize("dtype,kind", KINDS)
+@pytest.mark.parametrize("dim,shape", [(64, "many"), (128, "pieces"), (256, "shared"), (256, "rows_60")])
+@pytest.mark.parametrize("share", [1.0, 0.5])
+def test_values_up_to_fp32s_largest(cuda, dtype, kind, dim, shape, share):
+    """Values of up to 2^127, all or beside the smallest: nothing in between leaves fp32."""
+    b = _batch(cuda, shape, dim, dtype, kind, seed=dim, spread=(-5, -4))
+    g = torch.Generator().manual_seed(dim)
+    for page, at in _order(b):
+        e = torch.where(torch.rand(len(page), generator=g) < share, 120.0 if kind == I8 else 118.0, -60.0)
+        b.cache.v_scale[page, :, at] = torch.exp2(e).to(cuda)[:, None].expand(-1, b.cache.kv_heads)
+    want, bound = b.want()
+    got = b.run(out_dtype=F32)
+    assert got.isfinite().all()
+    close(got, want, _wider(bound), shape)
