@@ -661,7 +661,7 @@ int qw35_hip_kv_read(const qw35_hip_kv_cache *cache, const qw35_hip_heads *k, co
  * weight.  Scores, sums and results are fp32; the weights exp(..) are rounded once
  * to q's type on their way to the product with v, whatever out's type is.
  *   q: F16 or BF16, the cache's type (either for an E4M3 or E4M3_BLOCKS cache, F16
- * for an I8_BLOCKS one, whose codes it takes exactly); out and gate:
+ * for an I8_BLOCKS one); out and gate:
  * F32, BF16 or F16.  n_heads a multiple of the cache's kv_heads: query head h
  * reads kv head h / (n_heads / kv_heads).
  *   max_new: the most new tokens of a sequence (0: n_tokens; without starts

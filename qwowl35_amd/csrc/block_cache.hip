@@ -74,8 +74,16 @@ constexpr int kLeastExponent = -60;  // of a scale: its reciprocal and log2 stay
 
 // Workgroups that a launch is not cut below by giving each more heads: a workgroup
 // of several looks through the slots once for them and has the next head's rows on
-// their way, and needs others beside it.  8192 tokens x 8 heads x 128, bf16, took 27.5 us at
-// 256 workgroups, 27.4 at 512, 22.0 at 1024, 29.0 at 2048 and 41.8 at 4096.
+// their way, and needs others beside it.  Which number is best depends on how the
+// workgroups of a shape fill the compute units; 1024 is within 28% of it here.  Prompts from
+// a block's beginning / from its middle, int8, us:
+//   tokens x heads x columns       512           1024          2048
+//   8192 x 8 x 128, bf16           26.6 / 26.9   21.2 / 28.3   26.4 / 28.1
+//   8192 x 4 x 256, bf16           23.8 / 23.7   24.4 / 25.8   28.5 / 28.9
+//   8192 x 4 x 256, fp32           26.8 / 25.7   29.7 / 30.3   37.0 / 33.8
+//   16384 x 8 x 128, bf16          34.0 / 49.3   33.9 / 49.3   45.3 / 54.8
+//   4096 x 8 x 128, bf16           16.2 / 15.5   14.5 / 14.5   17.9 / 17.9
+//   5000 x 8 x 64, bf16            11.7 / 11.5   14.7 / 14.7   18.5 / 18.6
 constexpr int kLeastGroups = 1024;
 // Places of a call, up to 32 tokens each, whose blocks are looked for apart: a
 // prompt has a block for every 32 tokens, a decode step one for each.  A prompt's
@@ -671,9 +679,9 @@ __device__ __forceinline__ void append_blocks(const BlockAppend& a, BlockShared<
 
 // blockIdx.y: even keys, odd values of a group of heads.
 //   Bytes are the least of it: a call of few tokens is one chain of slots, rows, angles,
-// the largest, codes (8 tokens x 4 heads of 256, int8: 6.8 us, of 249: 9.5), and one of
-// many the chain of a head after the other (8192 x 8 heads of 128, bf16: 21.7 us, 50 MB
-// at 2.3 TB/s).  So a workgroup is a block, whose 32 rows of a head are all in
+// the largest, codes (8 tokens x 4 heads of 256, int8: 6.8 us, of 249: 9.6), and one of
+// many the chain of a head after the other (8192 x 8 heads of 128, bf16: 22.7 us, 50 MB
+// at 2.2 TB/s).  So a workgroup is a block, whose 32 rows of a head are all in
 // registers between the reading, the largest and the codes, each read and written
 // once; registers allow four of them a compute unit (three of 256 columns, without
 // spills).
@@ -776,6 +784,9 @@ __device__ __forceinline__ void store4(void* base, int64_t at, bool vec, const f
 // the granules, which lie token by token.  Of values a thread has four columns of
 // eight tokens: where those are the eight of a granule it reads 32 bytes (64 of a
 // 16-bit cache) and writes four elements of each token, a row at a time by its lanes.
+// The eights are counted from the first token's place in its granule: the values of
+// another sequence of the call that does not lie so (seven of eight) are read a byte a
+// load (20 sequences of 1000 tokens x 4 heads of 256, int8: 20 us if all lie alike, 53).
 template <class C, class TO, int D>
 __global__ __launch_bounds__(256) void kv_read_kernel(CacheRead a) {
     const int tid = threadIdx.x, h = (int)blockIdx.y >> 1, heads = (int)a.cache.kv_heads;

@@ -836,8 +836,8 @@ __device__ __forceinline__ float part_weight(float m, float top) {
     // (never zero otherwise: an infinity in a part that hardly counts stays one)
     return m == -__builtin_inff() ? 0.0f : fmaxf(__builtin_amdgcn_exp2f(m - top), 1e-37f);
 }
-// The weight of such a part's sum of terms, which with block scales may be up to 2^118 and count for something where
-// the part's values hardly do: the smaller exponential's rest goes to the sum, and nothing is put in the place of zero.
+// The weight of such a part's sum of terms.  With block scales a sum may be up to 2^118 and count where the part's
+// values no longer do: nothing takes the place of zero, and of an exponent under -100 the sum itself takes 2^-100.
 __device__ __forceinline__ float sum_weight(float m, float top, float& sum) {
     const float x = m - top;
     const bool far = x < -100.0f;
@@ -1451,8 +1451,8 @@ struct Unit {
             // As below, over tiles that the four waves unpack together, a quarter each, into the queries' type: each
             // of them by itself took 151 us for 256 tokens x 16 heads of 256 over 16001, int8, this 136 (and 128 with
             // copies apart).  A step unpacks the keys of the tile after the next and the values of the next among
-            // its matrix instructions; its barrier is also theirs.  Over longer contexts a tile takes what one of a
-            // 16-bit cache does (32002 tokens more: 162 us, fp16 155).
+            // its matrix instructions; its barrier is also theirs.  Over longer contexts a tile takes 13% more than
+            // one of a 16-bit cache, e4m3's 9% (32002 tokens more: 169 and 163 us, fp16 150).
             typedef Unit<D, E, Kind::wide, kRows> Wide;
             const Wide wide(a, sh);
             constexpr int kEach = kKb / 2;       // a wave's copies of a pair
@@ -1901,9 +1901,10 @@ __global__ __launch_bounds__(kThreads, D == 256 ? 1 : 2) void prefix_attention_k
 
 // The same of a block-scaled cache: half the bytes of a 16-bit one.  They are what
 // bounds decode steps over long ones (5 sequences that share 100003 tokens, 4 heads of
-// 256, int8: 52 us at 4.1 TB/s, of which 8 are the beginning), and the one wave of a
-// SIMD, which unpacks besides, chunks (256 tokens x 16 heads of 256 over 16001: 125 us,
-// fp16 111).  (A body of both, called from either, has its registers allocated
+// 256, int8: 53 us at 4.1 TB/s, of which 8 are the beginning), and the one wave of a
+// SIMD, which unpacks besides, chunks (256 tokens x 16 heads of 256 over 16001: 127 to
+// 138 us with the join, fp16 112 to 118; 5.3 and 4.6 us for 1000 tokens, and what does
+// not depend on them).  (A body of both, called from either, has its registers allocated
 // otherwise: the kernel above would no longer be the one measured.)
 template <int D, class E, Kind C, bool kWide>
 __global__ __launch_bounds__(kThreads, D == 256 ? 1 : 2) void block_attention_kernel(AttnArgs a) {
