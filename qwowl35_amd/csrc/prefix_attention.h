@@ -836,7 +836,7 @@ __device__ __forceinline__ float part_weight(float m, float top) {
     // (never zero otherwise: an infinity in a part that hardly counts stays one)
     return m == -__builtin_inff() ? 0.0f : fmaxf(__builtin_amdgcn_exp2f(m - top), 1e-37f);
 }
-// The weight of such a part's sum of terms.  With block scales a sum may be up to 2^118 and count where the part's
+// The weight of such a part's sum of terms.  With block scales a sum may be up to 2^110 and count where the part's
 // values no longer do: nothing takes the place of zero, and of an exponent under -100 the sum itself takes 2^-100.
 __device__ __forceinline__ float sum_weight(float m, float top, float& sum) {
     const float x = m - top;
@@ -1313,10 +1313,11 @@ struct Unit {
             }
     }
 
-    // Both sums count from one reference: the values', or 2^90 from the terms' where it is further from those (values
-    // of zero, or far from one), so that neither leaves fp32's range.
+    // Both sums count from one reference: the values', or one 2^-70 or 2^90 from the terms' where it is further from
+    // those (values of zero, or far from one), so that neither leaves fp32's range: the terms' sum is below 2^127 for
+    // 2^42 of them, and what values lose below 2^-126 is 2^-196 of a row's largest term, past any result's last bit.
     __device__ __forceinline__ void one_reference(Rows& w) const {
-        const float ref = fminf(fmaxf(w.mx, w.ml - 90.0f), w.ml + 90.0f);
+        const float ref = fminf(fmaxf(w.mx, w.ml - 70.0f), w.ml + 90.0f);
         if (__builtin_expect(__any(ref != w.mx), 0)) {
             const float f = ref == w.mx ? 1.0f : __builtin_amdgcn_exp2f(w.mx - ref);
 #pragma unroll
